@@ -112,8 +112,6 @@ def draw(rng):
         most = 16384 * 1024 * 4096 // (4 if dtype == "f32" else 1)
         while case["rows"] * case["n_in"] * case["n_out"] > most:
             case["rows"] = (case["rows"] + 1) // 2
-        if mode == "train":
-            case["rows"] = max(2, case["rows"])
     else:
         case["cols"] = _width(rng, 64, 8192)
         while case["rows"] * case["cols"] * (2 if dtype == "f32" else 1) > 32768 * 4096:
@@ -122,6 +120,7 @@ def draw(rng):
             case["affine"] = rng.random() < 0.85
         else:
             case.update(p=round(rng.uniform(0.02, 0.5), 3), res=rng.random() < 0.5)
+    case["rows"] += case["rows"] == SKIPPED
     return case
 
 
