@@ -39,6 +39,16 @@ pub const DRH_CFG_NON_POSITIVE_SIGMA: c_int = 2;
 pub const DRH_CFG_SIGMA_NOT_DECREASING: c_int = 3;
 pub const DRH_CFG_NON_POSITIVE_LEARNING_RATE: c_int = 4;
 
+pub const DRH_F32: c_int = 0;
+pub const DRH_BF16: c_int = 1;
+pub const DRH_F16: c_int = 2;
+
+pub const DRH_ACT_NONE: c_int = 0;
+pub const DRH_ACT_RELU: c_int = 1;
+pub const DRH_ACT_GELU: c_int = 2;
+pub const DRH_ACT_GELU_TANH: c_int = 3;
+pub const DRH_ACT_SILU: c_int = 4;
+
 /// `drh_ctx`: a device, its buffer pool and its timing state.
 #[repr(C)]
 pub struct drh_ctx {
@@ -317,6 +327,110 @@ extern "C" {
         dst: *mut u8,
         new_h: i64,
         new_w: i64,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+
+    pub fn drh_layer_norm(
+        ctx: *mut drh_ctx,
+        x: *const c_void,
+        weight: *const c_void,
+        bias: *const c_void,
+        rows: i64,
+        cols: i64,
+        x_stride: i64,
+        dtype: c_int,
+        weight_dtype: c_int,
+        eps: f32,
+        y: *mut c_void,
+        mean: *mut f32,
+        rstd: *mut f32,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_layer_norm_backward_bytes(
+        rows: i64,
+        cols: i64,
+        out_bytes: *mut u64,
+    ) -> c_int;
+    pub fn drh_layer_norm_backward(
+        ctx: *mut drh_ctx,
+        x: *const c_void,
+        weight: *const c_void,
+        mean: *const f32,
+        rstd: *const f32,
+        grad_y: *const c_void,
+        rows: i64,
+        cols: i64,
+        x_stride: i64,
+        grad_stride: i64,
+        dtype: c_int,
+        weight_dtype: c_int,
+        grad_x: *mut c_void,
+        grad_weight: *mut c_void,
+        grad_bias: *mut c_void,
+        workspace: *mut c_void,
+        workspace_bytes: u64,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_linear(
+        ctx: *mut drh_ctx,
+        x: *const c_void,
+        weight: *const c_void,
+        bias: *const c_void,
+        residual: *const c_void,
+        rows: i64,
+        n_out: i64,
+        n_in: i64,
+        x_stride: i64,
+        weight_stride: i64,
+        dtype: c_int,
+        activation: c_int,
+        y: *mut c_void,
+        kept: *mut c_void,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_linear_backward_bytes(
+        rows: i64,
+        n_out: i64,
+        n_in: i64,
+        dtype: c_int,
+        activation: c_int,
+        out_bytes: *mut u64,
+    ) -> c_int;
+    pub fn drh_linear_backward(
+        ctx: *mut drh_ctx,
+        x: *const c_void,
+        weight: *const c_void,
+        kept: *const c_void,
+        grad_y: *const c_void,
+        rows: i64,
+        n_out: i64,
+        n_in: i64,
+        x_stride: i64,
+        weight_stride: i64,
+        dtype: c_int,
+        activation: c_int,
+        grad_x: *mut c_void,
+        grad_weight: *mut c_void,
+        grad_bias: *mut c_void,
+        workspace: *mut c_void,
+        workspace_bytes: u64,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_dropout(
+        ctx: *mut drh_ctx,
+        x: *const c_void,
+        residual: *const c_void,
+        n: i64,
+        dtype: c_int,
+        p: f64,
+        seed: u64,
+        offset: u64,
+        y: *mut c_void,
         stream: *mut c_void,
         flags: u32,
     ) -> c_int;

@@ -10,6 +10,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -18,8 +20,9 @@ CSRC = HERE / "csrc"
 LIB = HERE / "libdiffrast_hip.so"
 ARCH = os.environ.get("DIFFRAST_OFFLOAD_ARCH", "gfx950")
 
-SOURCES = [CSRC / "kernels.hip", CSRC / "runtime.hip", CSRC / "fit.hip", CSRC / "scratch.hip", CSRC / "resize.hip"]
-HEADERS = [CSRC / "kernels.h", CSRC / "runtime.h", ROOT / "include" / "diffrast_hip.h"]
+SOURCES = [CSRC / "kernels.hip", CSRC / "runtime.hip", CSRC / "fit.hip", CSRC / "scratch.hip", CSRC / "resize.hip",
+           CSRC / "layers.hip", CSRC / "layer_norm.hip", CSRC / "linear.hip", CSRC / "dropout.hip"]
+HEADERS = [CSRC / "kernels.h", CSRC / "runtime.h", CSRC / "layers.h", ROOT / "include" / "diffrast_hip.h"]
 
 # -ffp-contract=off: the kernels state every FMA explicitly; plain a*b+c must
 # round twice, as the reference's arithmetic does.
@@ -34,7 +37,6 @@ FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-mllvm", "-structurizecfg-skip-uniform-regions=true",
@@ -51,9 +53,7 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found")
 
 
-def build(verbose: bool = False) -> Path:
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [hipcc(), *FLAGS, *map(str, SOURCES), "-o", str(tmp)]
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -63,6 +63,16 @@ def build(verbose: bool = False) -> Path:
         raise RuntimeError(f"hipcc failed ({res.returncode}):\n{err}")
     if verbose and err.strip():
         print(err)
+
+
+def build(verbose: bool = False) -> Path:
+    """Compiles each source (several at a time), then links them."""
+    cc, tmp = hipcc(), LIB.with_suffix(".so.tmp")
+    with tempfile.TemporaryDirectory() as objdir:
+        objs = [str(Path(objdir) / f"{src.stem}.o") for src in SOURCES]
+        with ThreadPoolExecutor(min(4, os.cpu_count() or 1)) as pool:
+            list(pool.map(lambda so: _run([cc, *FLAGS, "-c", str(so[0]), "-o", so[1]], verbose), zip(SOURCES, objs)))
+        _run([cc, f"--offload-arch={ARCH}", "-fPIC", "-shared", *objs, "-o", str(tmp)], verbose)
     os.replace(tmp, LIB)
     return LIB
 

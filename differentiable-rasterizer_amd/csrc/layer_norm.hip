@@ -1,0 +1,408 @@
+// Layer norm over the last dimension, forward and backward.
+//
+//   mu = mean(x), v = mean((x - mu)^2), r = 1 / sqrt(v + eps), h = (x - mu) r
+//   y  = h w + b
+//   dx = r (g w - mean(g w) - h mean(g w h)),  dw = sum over rows of g h,  db = sum over rows of g
+//
+// Every sum, mean, variance and reciprocal is held in 32 bits; the variance is taken
+// about the mean in a second sum over the row's registers, so it does not cancel where
+// the mean is large. All of it is bound by memory: the forward pass reads a row once and
+// writes it once, the backward pass reads two and writes one.
+
+#include "layers.h"
+
+using namespace drh_rt;
+
+namespace drh_nn {
+namespace {
+
+// A row is held in the registers of TPR threads, EPT elements each: a wave up to 2048
+// elements, then four waves up to LN_MAX_COLS. Thread t's vectors are t, t + TPR, ...
+constexpr int LN_MAX_COLS = 256 * 32;
+
+template <int VEC>
+__device__ inline void load_weight(const void* w, bool wf32, int is_bf16, int64_t c, float (&out)[VEC]) {
+    // weights may stand in 32 bits beside activations in 16
+    if (wf32)
+        for (int i = 0; i < VEC; i++) out[i] = ((const float*)w)[c + i];
+    else if (is_bf16)
+        for (int i = 0; i < VEC; i++) out[i] = (float)((const bf16*)w)[c + i];
+    else
+        for (int i = 0; i < VEC; i++) out[i] = (float)((const f16*)w)[c + i];
+}
+
+// Sums of a and b over a row's threads, in all of them. `slot` alternates between
+// calls, so that one barrier a call is enough.
+template <int TPR, int THREADS>
+__device__ inline void row_sums(float& a, float& b, int slot) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (TPR > 64) {
+        __shared__ float2 part[2][THREADS / 64];
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) part[slot & 1][w] = make_float2(a, b);
+        __syncthreads();
+        const int first = w & ~(TPR / 64 - 1);
+        a = b = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; i++) {
+            const float2 p = part[slot & 1][first + i];
+            a += p.x;
+            b += p.y;
+        }
+    }
+}
+
+struct LnArgs {
+    const void *x, *w, *b, *g;
+    void *y, *dx;
+    float *mean, *rstd, *part;
+    int64_t rows, xs, gs;
+    int cols, wf32;
+    float eps;
+};
+
+template <class T, int VEC, int EPT, int TPR>
+__global__ __launch_bounds__(256) void ln_forward(LnArgs p) {
+    constexpr int NV = EPT / VEC, RPB = 256 / TPR;
+    const int t = threadIdx.x % TPR, D = p.cols;
+    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    if (TPR <= 64 && row >= p.rows) return;
+    const T* x = (const T*)p.x + row * p.xs;
+    float v[NV][VEC];
+    float s = 0.0f, q = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int c = (j * TPR + t) * VEC;
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[j][i] = 0.0f;
+        if (c < D) load<VEC>(x + c, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) s += v[j][i];
+    row_sums<TPR, 256>(s, q, 0);
+    const float mu = s / (float)D;
+    q = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+        if ((j * TPR + t) * VEC < D)
+#pragma unroll
+            for (int i = 0; i < VEC; i++) q = fmaf(v[j][i] - mu, v[j][i] - mu, q);
+    s = 0.0f;
+    row_sums<TPR, 256>(q, s, 1);
+    const float r = 1.0f / sqrtf(q / (float)D + p.eps);
+    if (t == 0 && p.mean) {
+        p.mean[row] = mu;
+        p.rstd[row] = r;
+    }
+    T* y = (T*)p.y + row * D;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int c = (j * TPR + t) * VEC;
+        if (c >= D) continue;
+        float o[VEC], w[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; i++) o[i] = (v[j][i] - mu) * r;
+        if (p.w) {
+            load_weight<VEC>(p.w, p.wf32, std::is_same_v<T, bf16>, c, w);
+#pragma unroll
+            for (int i = 0; i < VEC; i++) o[i] *= w[i];
+        }
+        if (p.b) {
+            load_weight<VEC>(p.b, p.wf32, std::is_same_v<T, bf16>, c, w);
+#pragma unroll
+            for (int i = 0; i < VEC; i++) o[i] += w[i];
+        }
+        store<VEC>(y + c, o);
+    }
+}
+
+// One workgroup takes every gridDim-th group of THREADS / TPR rows and keeps its
+// columns' sums of g h and g in registers; at the end its row groups are added through
+// LDS in order and go to the workgroup's own row of p.part, which reduce_columns adds up.
+template <class T, int VEC, int EPT, int TPR, int THREADS>
+__global__ __launch_bounds__(THREADS) void ln_backward(LnArgs p) {
+    constexpr int NV = EPT / VEC, GROUPS = THREADS / TPR;
+    const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR, D = p.cols;
+    float w[NV][VEC], aw[NV][VEC], ab[NV][VEC];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int c = (j * TPR + t) * VEC;
+#pragma unroll
+        for (int i = 0; i < VEC; i++) w[j][i] = 1.0f, aw[j][i] = ab[j][i] = 0.0f;
+        if (p.w && c < D) load_weight<VEC>(p.w, p.wf32, std::is_same_v<T, bf16>, c, w[j]);
+    }
+    const float inv = 1.0f / (float)D;
+    int slot = 0;
+    for (int64_t row0 = (int64_t)blockIdx.x * GROUPS; row0 < p.rows; row0 += (int64_t)gridDim.x * GROUPS, slot++) {
+        const int64_t row = row0 + grp;
+        const bool live = row < p.rows;
+        const float mu = live ? p.mean[row] : 0.0f, r = live ? p.rstd[row] : 0.0f;
+        float h[NV][VEC], g[NV][VEC];
+        float sg = 0.0f, sh = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int c = (j * TPR + t) * VEC;
+#pragma unroll
+            for (int i = 0; i < VEC; i++) h[j][i] = mu, g[j][i] = 0.0f;
+            if (live && c < D) {
+                load<VEC>((const T*)p.x + row * p.xs + c, h[j]);
+                load<VEC>((const T*)p.g + row * p.gs + c, g[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                h[j][i] = (h[j][i] - mu) * r;
+                aw[j][i] = fmaf(g[j][i], h[j][i], aw[j][i]);
+                ab[j][i] += g[j][i];
+                g[j][i] *= w[j][i];
+                sg += g[j][i];
+                sh = fmaf(g[j][i], h[j][i], sh);
+            }
+        row_sums<TPR, THREADS>(sg, sh, slot);
+        sg *= inv;
+        sh *= inv;
+        if (live && p.dx) {
+            T* dx = (T*)p.dx + row * D;
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int c = (j * TPR + t) * VEC;
+                float o[VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; i++) o[i] = r * (g[j][i] - sg - h[j][i] * sh);
+                if (c < D) store<VEC>(dx + c, o);
+            }
+        }
+    }
+    if (!p.part) return;
+    __shared__ float sums[GROUPS][TPR * VEC];
+    float* out = p.part + (int64_t)blockIdx.x * 2 * D;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+        for (int which = 0; which < 2; which++) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < VEC; i++) sums[grp][t * VEC + i] = which ? ab[j][i] : aw[j][i];
+            __syncthreads();
+            for (int k = threadIdx.x; k < TPR * VEC; k += THREADS) {
+                const int c = j * TPR * VEC + k;
+                if (c >= D) break;
+                float s = 0.0f;
+                for (int i = 0; i < GROUPS; i++) s += sums[i][k];
+                out[which * D + c] = s;
+            }
+        }
+}
+
+// Rows wider than the registers hold: a workgroup a row, the row read again from the
+// caches for each sum.
+constexpr int WIDE = 1024;
+
+template <class T>
+__global__ __launch_bounds__(WIDE) void ln_forward_wide(LnArgs p) {
+    const int64_t row = blockIdx.x;
+    const int D = p.cols;
+    const T* x = (const T*)p.x + row * p.xs;
+    T* y = (T*)p.y + row * D;
+    float s = 0.0f, q = 0.0f;
+    for (int c = threadIdx.x; c < D; c += WIDE) s += (float)x[c];
+    row_sums<WIDE, WIDE>(s, q, 0);
+    const float mu = s / (float)D;
+    q = 0.0f;
+    for (int c = threadIdx.x; c < D; c += WIDE) q = fmaf((float)x[c] - mu, (float)x[c] - mu, q);
+    s = 0.0f;
+    row_sums<WIDE, WIDE>(q, s, 1);
+    const float r = 1.0f / sqrtf(q / (float)D + p.eps);
+    if (threadIdx.x == 0 && p.mean) {
+        p.mean[row] = mu;
+        p.rstd[row] = r;
+    }
+    for (int c = threadIdx.x; c < D; c += WIDE) {
+        float o[1] = {((float)x[c] - mu) * r}, w[1];
+        if (p.w) load_weight<1>(p.w, p.wf32, std::is_same_v<T, bf16>, c, w), o[0] *= w[0];
+        if (p.b) load_weight<1>(p.b, p.wf32, std::is_same_v<T, bf16>, c, w), o[0] += w[0];
+        store<1>(y + c, o);
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(WIDE) void ln_backward_wide(LnArgs p) {
+    const int64_t row = blockIdx.x;
+    const int D = p.cols;
+    const T* x = (const T*)p.x + row * p.xs;
+    const T* g = (const T*)p.g + row * p.gs;
+    const float mu = p.mean[row], r = p.rstd[row];
+    float sg = 0.0f, sh = 0.0f, w[1] = {1.0f};
+    for (int c = threadIdx.x; c < D; c += WIDE) {
+        if (p.w) load_weight<1>(p.w, p.wf32, std::is_same_v<T, bf16>, c, w);
+        const float gw = (float)g[c] * w[0];
+        sg += gw;
+        sh = fmaf(gw, ((float)x[c] - mu) * r, sh);
+    }
+    row_sums<WIDE, WIDE>(sg, sh, 0);
+    sg /= (float)D;
+    sh /= (float)D;
+    for (int c = threadIdx.x; c < D; c += WIDE) {
+        if (p.w) load_weight<1>(p.w, p.wf32, std::is_same_v<T, bf16>, c, w);
+        ((T*)p.dx)[row * D + c] = (T)(r * ((float)g[c] * w[0] - sg - ((float)x[c] - mu) * r * sh));
+    }
+}
+
+// The wide rows' column sums: a wave owns 64 columns of every gridDim.y-th row.
+template <class T>
+__global__ __launch_bounds__(64) void ln_columns_wide(LnArgs p) {
+    const int c = blockIdx.x * 64 + threadIdx.x;
+    if (c >= p.cols) return;
+    float sw = 0.0f, sb = 0.0f;
+    for (int64_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
+        const float g = (float)((const T*)p.g)[row * p.gs + c];
+        sw = fmaf(g, ((float)((const T*)p.x)[row * p.xs + c] - p.mean[row]) * p.rstd[row], sw);
+        sb += g;
+    }
+    float* out = p.part + (int64_t)blockIdx.y * 2 * p.cols;
+    out[c] = sw;
+    out[p.cols + c] = sb;
+}
+
+// f(threads per row, elements per thread) as constants, for rows of D elements.
+template <class F>
+void with_row(int64_t D, F&& f) {
+    using std::integral_constant;
+    auto ept = [&](auto tpr, int64_t per) {
+        if (per <= 8) f(tpr, integral_constant<int, 8>());
+        else if (per <= 16) f(tpr, integral_constant<int, 16>());
+        else f(tpr, integral_constant<int, 32>());
+    };
+    if (D <= 2048) ept(integral_constant<int, 64>(), (D + 63) / 64);
+    else ept(integral_constant<int, 256>(), (D + 255) / 256);
+}
+
+template <class T, class F>
+void with_vec(int vec, F&& f) {
+    using std::integral_constant;
+    if (vec == 1) f(integral_constant<int, 1>());
+    else if (sizeof(T) == 2 && vec == 2) f(integral_constant<int, 2>());
+    else f(integral_constant<int, 16 / (int)sizeof(T)>());
+}
+
+// Workgroups of the backward pass, each with a row of partial sums.
+constexpr int LN_GROUPS = 512;
+
+// Threads of a backward workgroup: the accumulators of 32 elements a thread need the
+// registers of eight waves a workgroup, smaller rows fit sixteen.
+constexpr int ln_threads(int ept) { return ept == 32 ? 512 : 1024; }
+
+int64_t ln_backward_groups(int64_t rows, int64_t cols) {
+    if (cols > LN_MAX_COLS) return rows < 64 ? rows : 64;
+    int64_t per = 1;
+    with_row(cols, [&](auto tpr, auto ept) { per = ln_threads(ept.value) / tpr.value; });
+    const int64_t need = (rows + per - 1) / per;
+    return need < LN_GROUPS ? need : LN_GROUPS;
+}
+
+int check_ln(drh_ctx* ctx, int64_t rows, int64_t cols, int dtype, int weight_dtype, uint32_t flags) {
+    int rc = check_call(ctx, dtype, flags);
+    if (rc) return rc;
+    if (weight_dtype != dtype && weight_dtype != DRH_F32)
+        return fail(DRH_ERR_INVALID_ARG, "weight and bias stand in the input's element type or in 32 bits");
+    if (rows < 0 || cols <= 0) return fail(DRH_ERR_INVALID_ARG, "rows must not be negative and cols positive");
+    if (rows > INT32_MAX || cols > (1 << 30)) return fail(DRH_ERR_TOO_LARGE, "more than 2^31 - 1 rows or 2^30 columns");
+    return DRH_OK;
+}
+
+}  // namespace
+}  // namespace drh_nn
+
+using namespace drh_nn;
+
+extern "C" {
+
+int drh_layer_norm(drh_ctx* ctx, const void* x, const void* weight, const void* bias, int64_t rows, int64_t cols,
+                   int64_t x_stride, int dtype, int weight_dtype, float eps, void* y, float* mean, float* rstd,
+                   void* stream, uint32_t flags) {
+    int rc = check_ln(ctx, rows, cols, dtype, weight_dtype, flags);
+    if (rc) return rc;
+    if (!(eps >= 0.0f)) return fail(DRH_ERR_INVALID_ARG, "eps must not be negative");
+    if (rows == 0) return DRH_OK;
+    if (!x || !y || !mean != !rstd)
+        return fail(DRH_ERR_INVALID_ARG, "x and y must not be NULL; mean and rstd come together");
+    if (rows > 1 && x_stride < 0) return fail(DRH_ERR_INVALID_ARG, "x_stride must not be negative");
+    DeviceGuard dg(ctx->device);
+    hipStream_t s = (hipStream_t)stream;
+    LnArgs p{};
+    p.x = x, p.w = weight, p.b = bias, p.y = y, p.mean = mean, p.rstd = rstd;
+    p.rows = rows, p.cols = (int)cols, p.xs = x_stride, p.eps = eps, p.wf32 = weight_dtype == DRH_F32;
+    const int vec = vector_width(dtype, {cols, rows > 1 ? x_stride : 0}, {x, y});
+    with_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        if (cols > LN_MAX_COLS) {
+            ln_forward_wide<T><<<dim3((unsigned)rows), WIDE, 0, s>>>(p);
+            return DRH_OK;
+        }
+        with_vec<T>(vec, [&](auto v) {
+            with_row(cols, [&](auto tpr, auto ept) {
+                constexpr int RPB = 256 / tpr.value;
+                ln_forward<T, v.value, ept.value, tpr.value><<<dim3((unsigned)((rows + RPB - 1) / RPB)), 256, 0, s>>>(p);
+            });
+        });
+        return DRH_OK;
+    });
+    return finish_call(s, flags, "layer norm");
+}
+
+int drh_layer_norm_backward_bytes(int64_t rows, int64_t cols, uint64_t* out_bytes) {
+    if (!out_bytes || rows < 0 || cols <= 0) return fail(DRH_ERR_INVALID_ARG, "bad sizes, or out_bytes is NULL");
+    *out_bytes = up256((size_t)ln_backward_groups(rows, cols) * 2 * (size_t)cols * sizeof(float));
+    return DRH_OK;
+}
+
+int drh_layer_norm_backward(drh_ctx* ctx, const void* x, const void* weight, const float* mean, const float* rstd,
+                            const void* grad_y, int64_t rows, int64_t cols, int64_t x_stride, int64_t grad_stride,
+                            int dtype, int weight_dtype, void* grad_x, void* grad_weight, void* grad_bias,
+                            void* workspace, uint64_t workspace_bytes, void* stream, uint32_t flags) {
+    int rc = check_ln(ctx, rows, cols, dtype, weight_dtype, flags);
+    if (rc) return rc;
+    const bool sums = grad_weight || grad_bias;
+    if (rows > 0 && (!x || !mean || !rstd || !grad_y)) return fail(DRH_ERR_INVALID_ARG, "an input pointer is NULL");
+    if (rows > 1 && (x_stride < 0 || grad_stride < 0)) return fail(DRH_ERR_INVALID_ARG, "strides must not be negative");
+    uint64_t need = 0;
+    if (sums) drh_layer_norm_backward_bytes(rows, cols, &need);
+    if (sums && (workspace_bytes < need || (need && !workspace)))
+        return fail(DRH_ERR_INVALID_ARG, "the weight's gradient needs " + std::to_string(need) + " bytes of workspace");
+    if ((uintptr_t)workspace % 16) return fail(DRH_ERR_INVALID_ARG, "the workspace must be 16-byte aligned");
+    DeviceGuard dg(ctx->device);
+    hipStream_t s = (hipStream_t)stream;
+    const int64_t groups = ln_backward_groups(rows, cols);
+    LnArgs p{};
+    p.x = x, p.w = weight, p.g = grad_y, p.dx = grad_x, p.mean = (float*)mean, p.rstd = (float*)rstd;
+    p.part = sums ? (float*)workspace : nullptr;
+    p.rows = rows, p.cols = (int)cols, p.xs = x_stride, p.gs = grad_stride, p.wf32 = weight_dtype == DRH_F32;
+    const int vec = vector_width(dtype, {cols, rows > 1 ? x_stride : 0, rows > 1 ? grad_stride : 0}, {x, grad_y, grad_x});
+    if (rows > 0 && (grad_x || sums))
+        with_type(dtype, [&](auto t) {
+            using T = decltype(t);
+            if (cols > LN_MAX_COLS) {
+                if (grad_x) ln_backward_wide<T><<<dim3((unsigned)rows), WIDE, 0, s>>>(p);
+                if (sums)
+                    ln_columns_wide<T><<<dim3((unsigned)((cols + 63) / 64), (unsigned)groups), 64, 0, s>>>(p);
+                return DRH_OK;
+            }
+            with_vec<T>(vec, [&](auto v) {
+                with_row(cols, [&](auto tpr, auto ept) {
+                    constexpr int THREADS = ln_threads(ept.value);
+                    ln_backward<T, v.value, ept.value, tpr.value, THREADS><<<dim3((unsigned)groups), THREADS, 0, s>>>(p);
+                });
+            });
+            return DRH_OK;
+        });
+    if (sums)
+        reduce_columns((const float*)workspace, groups, 2 * cols, cols, grad_weight, grad_bias, weight_dtype, s);
+    return finish_call(s, flags, "layer norm backward");
+}
+
+}  // extern "C"

@@ -32,6 +32,9 @@ DETERMINISTIC = 0x8
 CHANNELS_FIRST = 0x10
 PHASES = 0x20
 
+# Element types of the network layers
+F32, BF16, F16 = 0, 1, 2
+
 STOP_REASONS = {0: "Completed", 1: "Converged", 2: "Diverged"}
 CONFIG_ERRORS = {1: "NoTriangles", 2: "NonPositiveSigma", 3: "SigmaNotDecreasing",
                  4: "NonPositiveLearningRate"}
@@ -40,6 +43,8 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _F32 = ctypes.c_float
 _U32 = ctypes.c_uint32
+_U64 = ctypes.c_uint64
+_INT = ctypes.c_int
 
 
 class DiffrastError(RuntimeError):
@@ -150,6 +155,13 @@ SIGNATURES = {
     "drh_encode_srgb": ([_P, _P, _I64, _P, _P, _U32], ctypes.c_int),
     "drh_decode_srgb": ([_P, _P, _I64, _P, _P, _U32], ctypes.c_int),
     "drh_resize_lanczos3": ([_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _U32], ctypes.c_int),
+    "drh_layer_norm": ([_P, _P, _P, _P, _I64, _I64, _I64, _INT, _INT, _F32, _P, _P, _P, _P, _U32], ctypes.c_int),
+    "drh_layer_norm_backward_bytes": ([_I64, _I64, ctypes.POINTER(_U64)], ctypes.c_int),
+    "drh_layer_norm_backward": ([_P] * 6 + [_I64] * 4 + [_INT, _INT, _P, _P, _P, _P, _U64, _P, _U32], ctypes.c_int),
+    "drh_linear": ([_P] * 5 + [_I64] * 5 + [_INT, _INT, _P, _P, _P, _U32], ctypes.c_int),
+    "drh_linear_backward_bytes": ([_I64, _I64, _I64, _INT, _INT, ctypes.POINTER(_U64)], ctypes.c_int),
+    "drh_linear_backward": ([_P] * 5 + [_I64] * 5 + [_INT, _INT, _P, _P, _P, _P, _U64, _P, _U32], ctypes.c_int),
+    "drh_dropout": ([_P, _P, _P, _I64, _INT, ctypes.c_double, _U64, _U64, _P, _P, _U32], ctypes.c_int),
 }
 
 _lib = None

@@ -331,6 +331,80 @@ int drh_decode_srgb(drh_ctx *ctx, const uint8_t *bytes, int64_t n, float *out, v
 int drh_resize_lanczos3(drh_ctx *ctx, const uint8_t *src, int64_t H, int64_t W, int64_t C, uint8_t *dst,
                         int64_t new_H, int64_t new_W, void *stream, uint32_t flags);
 
+/* ---- Layers of a network whose output is a scene's parameters ----
+ *
+ * The reference trains such a network through its PyTorch op with PyTorch's own
+ * layers (python/diffrast/model.py); these have no counterpart there. Arrays are
+ * device pointers, row-major; DRH_SYNC is the only flag (others are refused with
+ * DRH_ERR_INVALID_ARG). The calls allocate nothing, so a HIP graph may capture
+ * them: what they need besides their inputs and outputs is the caller's workspace
+ * (16-byte aligned, of the bytes that the *_bytes function gives; no content is
+ * expected in it or kept). Sums, statistics and activations are held in 32 bits
+ * and rounded to the arrays' element type once; results do not depend on timing. */
+
+/* Element types. */
+enum { DRH_F32 = 0, DRH_BF16 = 1, DRH_F16 = 2 };
+
+/* Layer norm of `rows` rows of `cols` elements:
+ *   y = (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias
+ * x_stride elements lie between the starts of x's rows; y is contiguous. weight and
+ * bias (cols elements, of weight_dtype: dtype or DRH_F32) may each be NULL. mean
+ * and rstd (rows floats each, both or neither) keep the statistics for the
+ * backward pass. */
+int drh_layer_norm(drh_ctx *ctx, const void *x, const void *weight, const void *bias, int64_t rows,
+                   int64_t cols, int64_t x_stride, int dtype, int weight_dtype, float eps, void *y,
+                   float *mean, float *rstd, void *stream, uint32_t flags);
+
+/* Workspace of drh_layer_norm_backward; none is needed (NULL, 0) without grad_weight and grad_bias. */
+int drh_layer_norm_backward_bytes(int64_t rows, int64_t cols, uint64_t *out_bytes);
+
+/* Gradients of drh_layer_norm from its x, weight, mean and rstd and from grad_y
+ * (rows grad_stride elements apart). grad_x (contiguous), grad_weight and grad_bias
+ * (of weight_dtype) may each be NULL: not computed. */
+int drh_layer_norm_backward(drh_ctx *ctx, const void *x, const void *weight, const float *mean,
+                            const float *rstd, const void *grad_y, int64_t rows, int64_t cols,
+                            int64_t x_stride, int64_t grad_stride, int dtype, int weight_dtype,
+                            void *grad_x, void *grad_weight, void *grad_bias, void *workspace,
+                            uint64_t workspace_bytes, void *stream, uint32_t flags);
+
+/* Activations of drh_linear. GELU is z Phi(z); GELU_TANH is its form by tanh(sqrt(2 /
+ * pi) (z + 0.044715 z^3)). */
+enum { DRH_ACT_NONE = 0, DRH_ACT_RELU = 1, DRH_ACT_GELU = 2, DRH_ACT_GELU_TANH = 3, DRH_ACT_SILU = 4 };
+
+/* Linear layer: y = activation(x weight^T + bias) + residual, x rows x n_in (rows
+ * x_stride elements apart), weight n_out x n_in (rows weight_stride apart), y and
+ * residual rows x n_out, contiguous. bias (n_out) and residual may be NULL. kept, if
+ * not NULL, receives what the backward pass needs of an activation's argument: rows x
+ * n_out floats for DRH_F32, 16-bit elements for the other types; nothing is written
+ * with DRH_ACT_NONE. */
+int drh_linear(drh_ctx *ctx, const void *x, const void *weight, const void *bias, const void *residual,
+               int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride,
+               int dtype, int activation, void *y, void *kept, void *stream, uint32_t flags);
+
+/* Workspace of drh_linear_backward. */
+int drh_linear_backward_bytes(int64_t rows, int64_t n_out, int64_t n_in, int dtype, int activation,
+                              uint64_t *out_bytes);
+
+/* Gradients of drh_linear from grad_y (rows x n_out, contiguous), its x and weight,
+ * and `kept` (NULL with DRH_ACT_NONE). grad_x (rows x n_in), grad_weight (n_out x
+ * n_in) and grad_bias (n_out), contiguous, may each be NULL: not computed. The
+ * residual's gradient is grad_y. */
+int drh_linear_backward(drh_ctx *ctx, const void *x, const void *weight, const void *kept,
+                        const void *grad_y, int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride,
+                        int64_t weight_stride, int dtype, int activation, void *grad_x,
+                        void *grad_weight, void *grad_bias, void *workspace, uint64_t workspace_bytes,
+                        void *stream, uint32_t flags);
+
+/* Dropout of n elements: y = x * keep / (1 - p') + residual (NULL: 0). The mask is
+ * not stored: element i is dropped where its 16 random bits, as a number, are below
+ * round(p * 65536), and p' is that over 65536 (at most 65535 / 65536). The bits are
+ * half i % 2 of word (i % 8) / 2 of Philox4x32-10 with key `seed` and counter (i / 8,
+ * offset), 64 bits each, so (seed, offset) names the mask: a program that counts
+ * `offset` up draws a new one each call. The backward pass is the same call on the
+ * gradient, without residual. 0 <= p < 1. */
+int drh_dropout(drh_ctx *ctx, const void *x, const void *residual, int64_t n, int dtype, double p,
+                uint64_t seed, uint64_t offset, void *y, void *stream, uint32_t flags);
+
 #ifdef __cplusplus
 }
 #endif
