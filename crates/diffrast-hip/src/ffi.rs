@@ -389,13 +389,26 @@ extern "C" {
         activation: c_int,
         y: *mut c_void,
         kept: *mut c_void,
+        workspace: *mut c_void,
+        workspace_bytes: u64,
         stream: *mut c_void,
         flags: u32,
+    ) -> c_int;
+    pub fn drh_linear_bytes(
+        rows: i64,
+        n_out: i64,
+        n_in: i64,
+        x_stride: i64,
+        weight_stride: i64,
+        dtype: c_int,
+        out_bytes: *mut u64,
     ) -> c_int;
     pub fn drh_linear_backward_bytes(
         rows: i64,
         n_out: i64,
         n_in: i64,
+        x_stride: i64,
+        weight_stride: i64,
         dtype: c_int,
         activation: c_int,
         out_bytes: *mut u64,

@@ -1,0 +1,359 @@
+// The matrix product of the linear layer on gfx950's matrix cores:
+//   out[m][n] = epilogue(sum over k of A(m, k) B(n, k)),
+// each operand with either k or its rows contiguous in memory.
+//
+// Operands go from memory to LDS without passing registers (buffer loads with LDS as their
+// destination, 16 bytes a lane) in units of 128 rows by 128 bytes of k. The buffer's bounds
+// check fills rows and k past the end with zeros, so no shape needs a case of its own as long
+// as 16-byte chunks do not straddle an edge. In LDS a unit keeps its layout in memory, with
+// its 16-byte chunks permuted by an exclusive or that spreads a wave's reads over the banks;
+// the permutation is made on the loads' addresses, since a wave's load writes LDS linearly.
+#pragma once
+
+#include "layers.h"
+
+namespace drh_nn {
+
+using floatx4 = vec<float, 4>;
+
+struct Operand {
+    const void* ptr;
+    int64_t ld;    // elements between rows (k contiguous) or between values of k (rows contiguous)
+    int64_t rows;  // M or N; with rows contiguous up to the end of the last 16-byte chunk
+};
+
+struct Gemm {
+    Operand a, b;
+    int64_t M, N, K;
+    const void *bias, *res;  // N; M x N
+    void* kept;              // M x N of Kept<T>, or null
+    void* out;               // M x N
+    float* partial;          // splits x M x N sums instead of `out`, or null
+    int act;
+    int splits;              // the k range in this many parts, grid.y
+    int tiles_per_split;     // tiles of k in each
+    bool wide_out;           // N and the epilogue's pointers allow 16-byte accesses
+};
+
+// D = A B + C on a wave: lane l gives row l % 16 of A and of B, the 16 bytes of k that
+// l / 16 picks, and holds D[4 (l / 16) + i][l % 16]. In 32 bits the four k of a lane go
+// through one instruction each: any order of k will do that A and B share.
+__device__ inline floatx4 mma(vec<bf16, 8> a, vec<bf16, 8> b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx4 mma(vec<f16, 8> a, vec<f16, 8> b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx4 mma(vec<float, 4> a, vec<float, 4> b, floatx4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+}
+
+constexpr int UNIT_BYTES = 16384;
+constexpr uint32_t PAST_END = 0x7ffffff0u;  // an offset that no buffer here reaches
+
+using lds_char = __attribute__((address_space(3))) char;
+
+// Which of a wave's fragments of 16 rows hold which rows of a unit. Fragments of A take
+// 16 rows in order. Those of B are interleaved by fours, so that a lane's results (four
+// rows of each of NF fragments) are 4 NF neighbours in the output.
+template <bool B, int NF>
+__device__ inline int frag_row(int f, int r) {
+    return B ? (r >> 2) * (4 * NF) + f * 4 + (r & 3) : f * 16 + r;
+}
+
+// The chunk permutation: by row where k is contiguous (eight chunks a row), by k where the
+// rows are (sixteen chunks a value of k, 32 in 32 bits).
+template <class T, bool KC, bool B, int NF>
+__device__ inline int swizzle(int i) {
+    if constexpr (KC) {
+        return B ? (i & 3) | ((i / (4 * NF)) & 1) << 2 : i & 7;
+    } else if constexpr (sizeof(T) == 2) {
+        return B ? 4 * (i & 3) : 2 * ((i & 3) | ((i >> 3) & 1) << 2);
+    } else {
+        return B ? 8 * ((i >> 2) & 1) + ((i >> 3) & 1) : 4 * ((i >> 2) & 3);
+    }
+}
+
+// One operand of a workgroup's tile: UNITS units of 128 rows; row R of unit u is row
+// u * 128 + R of the tile, or with UNITS == 2 on B's side (R / 32) * 64 + u * 32 + R % 32,
+// which puts a wave's 32 rows of both units side by side.
+template <class T, bool KC, bool B, int UNITS, int NF, int WAVES>
+struct Loader {
+    static constexpr int CH = 16 / sizeof(T), BK = 8 * CH, LOADS = 16 / WAVES;
+    const char* base;
+    uint64_t step;          // bytes per tile of k
+    uint64_t span;          // KC: bytes from the base to the end of the tile's last row
+    int64_t K;
+    uint32_t row_bytes, tail_bytes;  // rows contiguous: bytes between values of k; from a row's start to its end
+    uint32_t off[UNITS][LOADS];
+    int kc;                 // KC: first k of the lane's chunk in a tile
+
+    __device__ void init(const Operand& o, int64_t row0, int64_t K_) {
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+        K = K_;
+        const int64_t ld = o.ld;
+        const int64_t valid = o.rows - row0 < 128 * UNITS ? o.rows - row0 : 128 * UNITS;
+        if constexpr (KC) {
+            base = (const char*)o.ptr + row0 * ld * (int64_t)sizeof(T);
+            step = 128;
+            span = ((valid - 1) * ld + (K + CH - 1) / CH * CH) * (int64_t)sizeof(T);  // whole chunks
+        } else {
+            base = (const char*)o.ptr + row0 * (int64_t)sizeof(T);
+            step = BK * ld * (int64_t)sizeof(T);
+            row_bytes = (uint32_t)(ld * sizeof(T));
+            const int64_t tail = (o.rows - row0 < 512 ? o.rows - row0 : 512) * (int64_t)sizeof(T);
+            tail_bytes = (uint32_t)tail;
+        }
+        kc = 0;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int pos = (i * WAVES + w) * 64 + lane;  // chunk of the unit that this load fills
+#pragma unroll
+            for (int u = 0; u < UNITS; u++) {
+                if constexpr (KC) {
+                    const int R = pos >> 3, chunk = (pos & 7) ^ swizzle<T, KC, B, NF>(R);
+                    off[u][i] = (uint32_t)(tile_row(u, R) * ld * sizeof(T)) + chunk * 16;
+                    kc = chunk * CH;
+                } else {
+                    constexpr int PER = 128 / CH;
+                    const int k = pos / PER, R = ((pos % PER) ^ swizzle<T, KC, B, NF>(k)) * CH;
+                    const int64_t row = tile_row(u, R);
+                    off[u][i] = row0 + row < o.rows ? (uint32_t)(k * ld * sizeof(T) + row * sizeof(T)) : PAST_END;
+                }
+            }
+        }
+    }
+
+    static __device__ int64_t tile_row(int u, int R) {
+        return B && UNITS == 2 ? (R / 32) * 64 + u * 32 + R % 32 : u * 128 + R;
+    }
+
+    // Starts the loads of unit u of k tile kt into LDS at `lds`; past the last tile they
+    // fill it with zeros and touch no memory, so that every tile has the same loads.
+    __device__ void issue(int u, int64_t kt, uint32_t lds) const {
+        const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int64_t left = K - kt * BK;
+        const char* p = base + kt * step;
+        uint32_t bytes;
+        if constexpr (KC) {
+            bytes = left > 0 ? (uint32_t)(span - kt * 128) : 0u;
+        } else {
+            const int rows = left >= BK ? BK : left > 0 ? (int)left : 0;
+            bytes = rows ? (uint32_t)(rows - 1) * row_bytes + tail_bytes : 0u;
+        }
+        vec<uint32_t, 4> rsrc = {(uint32_t)(uintptr_t)p, (uint32_t)((uintptr_t)p >> 32) & 0xffffu, bytes, 0x00020000u};
+#pragma unroll
+        for (int i = 0; i < 4; i++) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const uint32_t dst = __builtin_amdgcn_readfirstlane(lds + (i * WAVES + w) * 1024);
+            uint32_t o = off[u][i];
+            if constexpr (KC) o = kc < left ? o : PAST_END;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(o),
+                         "s"(rsrc)
+                         : "memory");
+        }
+    }
+};
+
+template <int N>
+__device__ inline void wait_vm() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
+__device__ inline void wg_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+// A wave's fragments of one unit, NFR of 16 rows from row r0 on, both halves of the k tile.
+template <class T, bool KC, bool B, int NF>
+struct Frags {
+    static constexpr int CH = 16 / sizeof(T);
+    using F = vec<T, CH>;
+    F f[NF][2];
+
+    // unit: the unit in LDS
+    __device__ void read(const char* unit, int r0) {
+        const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < NF; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if constexpr (KC) {
+                    const int R = r0 + frag_row<B, NF>(i, r);
+                    f[i][h] = *(const F*)(unit + R * 128 + (((h * 4 + q) ^ swizzle<T, KC, B, NF>(R)) * 16));
+                } else if constexpr (sizeof(T) == 2) {
+                    // A transposing read: sixteen lanes give the addresses of four rows' pieces
+                    // for four values of k, and each gets its row's four values.
+                    using S4 = vec<short, 4>;
+                    union {
+                        S4 s[2];
+                        F v;
+                    } x;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int k = h * 32 + q * 8 + e * 4 + (r >> 2), R = r0 + frag_row<B, NF>(i, (r & 3) * 4);
+                        const char* p = unit + k * 256 + (((R >> 3) ^ swizzle<T, KC, B, NF>(k)) * 16) + (R & 7) * 2;
+                        x.s[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)p);
+                    }
+                    f[i][h] = x.v;
+                } else {
+                    const int R = r0 + frag_row<B, NF>(i, r);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int k = h * 16 + q * 4 + e;
+                        f[i][h][e] = *(const float*)(unit + k * 512 + (((R >> 2) ^ swizzle<T, KC, B, NF>(k)) * 16) + (R & 3) * 4);
+                    }
+                }
+            }
+    }
+};
+
+template <class T, bool AK, bool BK_, int NA, int NB>
+__device__ inline void multiply(const Frags<T, AK, false, NA>& a, const Frags<T, BK_, true, NB>& b, floatx4 (&acc)[NA][NB]) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < NA; i++)
+#pragma unroll
+            for (int j = 0; j < NB; j++) acc[i][j] = mma(b.f[j][h], a.f[i][h], acc[i][j]);
+}
+
+// The tile that a workgroup takes. Workgroups go to the eight XCDs in turn and each XCD
+// has an L2 of its own: an XCD gets a run of neighbouring tiles, in bands eight tiles high.
+__device__ inline void pick_tile(int64_t tiles_m, int64_t tiles_n, int64_t& tm, int64_t& tn) {
+    const uint32_t total = gridDim.x, b = blockIdx.x, xcd = b & 7, in = b >> 3;
+    const uint32_t per = total >> 3, extra = total & 7;
+    const uint32_t id = xcd * per + (xcd < extra ? xcd : extra) + in;
+    constexpr uint32_t BAND = 8;
+    const uint32_t band = id / (uint32_t)(BAND * tiles_n), first = band * BAND;
+    const uint32_t high = tiles_m - first < BAND ? (uint32_t)tiles_m - first : BAND;
+    const uint32_t rest = id - band * (uint32_t)(BAND * tiles_n);
+    tm = first + rest % high;
+    tn = rest / high;
+}
+
+// 256 x 256 of the output by eight waves, 128 x 64 each, in quarters of 64 x 32: one unit
+// of A by one of B. LDS holds two k tiles (128 KiB), so one workgroup fills a CU, two waves
+// a SIMD. The waves of a SIMD are of two groups that run half a step apart: while one reads
+// its fragments and starts loads, the other has the matrix cores. A k tile is four steps, each
+// reading at most one unit's fragments and starting one unit's loads, six steps ahead of
+// their use (five units in flight). A unit is overwritten two steps after both groups have
+// read it at the earliest.
+template <class T, bool AK, bool BK_, class Epilogue>
+__device__ inline void gemm_256(const Gemm& p, Epilogue& epilogue) {
+    __shared__ __align__(1024) char lds[8 * UNIT_BYTES];
+    using LA = Loader<T, AK, false, 2, 4, 8>;
+    using LB = Loader<T, BK_, true, 2, 2, 8>;
+    int64_t tm, tn;
+    pick_tile((p.M + 255) / 256, (p.N + 255) / 256, tm, tn);
+    const int64_t m0 = tm * 256, n0 = tn * 256;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w >> 2, wn = w & 3;
+    const int64_t tiles = (p.K + LA::BK - 1) / LA::BK, first = (int64_t)blockIdx.y * p.tiles_per_split;
+    const int64_t last = first + p.tiles_per_split < tiles ? first + p.tiles_per_split : tiles;
+    LA la;
+    LB lb;
+    la.init(p.a, m0, p.K);
+    lb.init(p.b, n0, p.K);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)lds;
+    // units of a buffer: A0, A1, B0, B1
+    auto at = [&](int64_t kt, int unit) { return (uint32_t)(((kt - first) & 1) * 4 + unit) * UNIT_BYTES; };
+    auto load_a = [&](int u, int64_t kt) { la.issue(u, kt, lds0 + at(kt, u)); };
+    auto load_b = [&](int u, int64_t kt) { lb.issue(u, kt, lds0 + at(kt, 2 + u)); };
+
+    floatx4 acc[2][2][4][2] = {};
+    Frags<T, AK, false, 4> fa;
+    Frags<T, BK_, true, 2> fb[2];
+
+    load_b(0, first);
+    load_a(0, first);
+    load_b(1, first);
+    load_a(1, first);
+    load_b(0, first + 1);
+    load_a(0, first + 1);
+    load_b(1, first + 1);
+    wait_vm<10>();
+    wg_barrier();
+    fb[0].read(lds + at(first, 2), wn * 32);
+    if (wm == 1) wg_barrier();
+
+    auto step = [&](int ua, int ub) {
+        wait_vm<10>();
+        __builtin_amdgcn_sched_barrier(0);
+        wg_barrier();
+        __builtin_amdgcn_s_setprio(1);
+        multiply<T, AK, BK_, 4, 2>(fa, fb[ub], acc[ua][ub]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        wg_barrier();
+    };
+    for (int64_t kt = first; kt < last; kt++) {
+        fa.read(lds + at(kt, 0), wm * 64);
+        load_a(1, kt + 1);
+        step(0, 0);
+        fb[1].read(lds + at(kt, 3), wn * 32);
+        load_b(0, kt + 2);
+        step(0, 1);
+        fa.read(lds + at(kt, 1), wm * 64);
+        load_a(0, kt + 2);
+        step(1, 0);
+        fb[0].read(lds + at(kt + 1, 2), wn * 32);
+        load_b(1, kt + 2);
+        step(1, 1);
+    }
+    if (wm == 0) wg_barrier();
+    wait_vm<0>();  // LDS is given up with no load on its way there
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int ub = 0; ub < 2; ub++) {
+        epilogue.columns(p, n0 + wn * 64 + ub * 32 + q * 8);
+#pragma unroll
+        for (int ua = 0; ua < 2; ua++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) epilogue.row(p, m0 + ua * 128 + wm * 64 + i * 16 + r, acc[ua][ub][i]);
+    }
+}
+
+// 128 x 128 by four waves, 64 x 64 each, two k tiles in LDS (64 KiB): two workgroups a CU,
+// each covering the other's waits.
+template <class T, bool AK, bool BK_, class Epilogue>
+__device__ inline void gemm_128(const Gemm& p, Epilogue& epilogue) {
+    __shared__ __align__(1024) char lds[4 * UNIT_BYTES];
+    using LA = Loader<T, AK, false, 1, 4, 4>;
+    using LB = Loader<T, BK_, true, 1, 4, 4>;
+    int64_t tm, tn;
+    pick_tile((p.M + 127) / 128, (p.N + 127) / 128, tm, tn);
+    const int64_t m0 = tm * 128, n0 = tn * 128;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w >> 1, wn = w & 1;
+    const int64_t tiles = (p.K + LA::BK - 1) / LA::BK, first = (int64_t)blockIdx.y * p.tiles_per_split;
+    const int64_t last = first + p.tiles_per_split < tiles ? first + p.tiles_per_split : tiles;
+    LA la;
+    LB lb;
+    la.init(p.a, m0, p.K);
+    lb.init(p.b, n0, p.K);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)lds;
+    auto load = [&](int64_t kt) {
+        const uint32_t b = (uint32_t)((kt - first) & 1) * 2 * UNIT_BYTES;
+        la.issue(0, kt, lds0 + b);
+        lb.issue(0, kt, lds0 + b + UNIT_BYTES);
+    };
+    floatx4 acc[4][4] = {};
+    load(first);
+    for (int64_t kt = first; kt < last; kt++) {
+        const char* b = lds + ((kt - first) & 1) * 2 * UNIT_BYTES;
+        wait_vm<0>();
+        wg_barrier();  // this tile is there, and the other buffer read by every wave
+        load(kt + 1);
+        Frags<T, AK, false, 4> fa;
+        Frags<T, BK_, true, 4> fb;
+        fa.read(b, wm * 64);
+        fb.read(b + UNIT_BYTES, wn * 64);
+        multiply<T, AK, BK_, 4, 4>(fa, fb, acc);
+    }
+    wait_vm<0>();
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    epilogue.columns(p, n0 + wn * 64 + q * 16);
+#pragma unroll
+    for (int i = 0; i < 4; i++) epilogue.row(p, m0 + wm * 64 + i * 16 + r, acc[i]);
+}
+
+}  // namespace drh_nn

@@ -9,7 +9,7 @@
 // bfloat16's 8 would, and act' has its limit long before float16 ends, so larger values
 // are kept as its largest.
 
-#include "layers.h"
+#include "gemm.h"
 
 using namespace drh_rt;
 
@@ -90,68 +90,147 @@ __device__ inline Kept<T> keep(float z) {
     }
 }
 
-// ---------------------------------------------------------------- the product
+// ---------------------------------------------------------------- the product's epilogue
 
-// out[m][n] = epilogue(sum over k of A(m, k) B(n, k)); A(m, k) = a[m * am + k * ak], one of
-// am and ak being 1, and B likewise.
-struct Gemm {
-    const void *a, *b;
-    int64_t am, ak, bn, bk;
-    int64_t M, N, K;
-    const void *bias, *res;  // N; M x N
-    void* z;                 // M x N of Kept<T>, or null
-    void* out;               // M x N
-    int act;
+// One lane's 4 NV neighbouring outputs of a row: columns() is called before the rows that
+// share them.
+template <class T, int ACT, int NV>
+struct Epilogue {
+    static constexpr bool EXACT = sizeof(T) == 4;
+    static constexpr int CH = 16 / sizeof(T), W = 4 * NV;
+    int64_t n = 0;
+    float bias[W];
+
+    __device__ void columns(const Gemm& p, int64_t n_) {
+        n = n_;
+#pragma unroll
+        for (int i = 0; i < W; i++) bias[i] = p.bias && !p.partial && n + i < p.N ? (float)((const T*)p.bias)[n + i] : 0.0f;
+    }
+
+    __device__ void row(const Gemm& p, int64_t m, const floatx4 (&v)[NV]) const {
+        if (m >= p.M) return;
+        const int64_t at = m * p.N + n;
+        if (p.partial) {
+            float* out = p.partial + (int64_t)blockIdx.y * p.M * p.N + at;
+#pragma unroll
+            for (int j = 0; j < NV; j++)
+                if (p.wide_out && n + 4 * j < p.N) {
+                    *(floatx4*)(out + 4 * j) = v[j];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (n + 4 * j + i < p.N) out[4 * j + i] = v[j][i];
+                }
+            return;
+        }
+        if (W % CH == 0 && p.wide_out) {
+#pragma unroll
+            for (int g = 0; g + CH <= W; g += CH)
+                if (n + g < p.N) group<CH>(p, at + g, v, g);
+        } else {
+#pragma unroll
+            for (int g = 0; g < W; g++)
+                if (n + g < p.N) group<1>(p, at + g, v, g);
+        }
+    }
+
+    template <int C>
+    __device__ void group(const Gemm& p, int64_t at, const floatx4 (&v)[NV], int g) const {
+        float o[C];
+#pragma unroll
+        for (int i = 0; i < C; i++) o[i] = v[(g + i) / 4][(g + i) % 4] + bias[g + i];
+        apply<C>(p, at, o);
+    }
+
+    // From z on: keeps it, activates, adds the residual, stores.
+    template <int C>
+    static __device__ void apply(const Gemm& p, int64_t at, float (&o)[C]) {
+        if (ACT != DRH_ACT_NONE) {
+            if (p.kept) {
+                Kept<T>* kept = (Kept<T>*)p.kept + at;
+                vec<Kept<T>, C> k;
+#pragma unroll
+                for (int i = 0; i < C; i++) k[i] = keep<T>(o[i]);
+                *(vec<Kept<T>, C>*)kept = k;
+            }
+#pragma unroll
+            for (int i = 0; i < C; i++) o[i] = act<EXACT>(ACT, o[i]);
+        }
+        if (p.res) {
+            float r[C];
+            load<C>((const T*)p.res + at, r);
+#pragma unroll
+            for (int i = 0; i < C; i++) o[i] += r[i];
+        }
+        store<C>((T*)p.out + at, o);
+    }
 };
 
-template <class T>
-using frag16 = std::conditional_t<std::is_same_v<T, bf16>, vec<bf16, 8>, vec<f16, 8>>;
-using floatx4 = vec<float, 4>;
+// ---------------------------------------------------------------- the products
 
-// D = A B + C on a wave: lane l gives row l % 16 of A and of B, the 16 bytes of k that
-// l / 16 picks, and holds D[4 (l / 16) + i][l % 16]. In 32 bits the four k of a lane go
-// through one instruction each: any order of k will do that A and B share.
-__device__ inline floatx4 mma(vec<bf16, 8> a, vec<bf16, 8> b, floatx4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+template <class T, bool AK, bool BK, int ACT>
+__global__ __launch_bounds__(512, 2) void gemm_256_kernel(Gemm p) {
+    Epilogue<T, ACT, 2> e;
+    gemm_256<T, AK, BK>(p, e);
 }
-__device__ inline floatx4 mma(vec<f16, 8> a, vec<f16, 8> b, floatx4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+
+template <class T, bool AK, bool BK, int ACT>
+__global__ __launch_bounds__(256, 2) void gemm_128_kernel(Gemm p) {
+    Epilogue<T, ACT, 4> e;
+    gemm_128<T, AK, BK>(p, e);
 }
-__device__ inline floatx4 mma(vec<float, 4> a, vec<float, 4> b, floatx4 c) {
+
+// The parts of a split product added in order, and the epilogue.
+template <class T, int ACT, int VEC>
+__global__ __launch_bounds__(256) void join_splits(Gemm p) {
+    const int64_t n_all = p.M * p.N;
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
+    if (at >= n_all) return;
+    float o[VEC] = {};
+    for (int s = 0; s < p.splits; s++) {
+        float v[VEC];
+        const float* part = p.partial + s * n_all + at;
 #pragma unroll
-    for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-    return c;
+        for (int i = 0; i < VEC; i += VEC < 4 ? VEC : 4) {
+            float4 q;
+            if constexpr (VEC >= 4) {
+                q = *(const float4*)(part + i);
+                v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+            } else {
+                v[i] = part[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; i++) o[i] += v[i];
+    }
+    if (p.bias) {
+        const int64_t n = at % p.N;
+#pragma unroll
+        for (int i = 0; i < VEC; i++) o[i] += (float)((const T*)p.bias)[n + i];
+    }
+    Epilogue<T, ACT, 2>::template apply<VEC>(p, at, o);
 }
 
-template <class T>
-__device__ inline void finish_element(const Gemm& p, int64_t m, int64_t n, float v) {
-    constexpr bool EXACT = sizeof(T) == 4;
-    const int64_t i = m * p.N + n;
-    if (p.bias) v += (float)((const T*)p.bias)[n];
-    if (p.z) ((Kept<T>*)p.z)[i] = keep<T>(v);
-    v = act<EXACT>(p.act, v);
-    if (p.res) v += (float)((const T*)p.res)[i];
-    ((T*)p.out)[i] = (T)v;
-}
-
-// 64 x 64 of the output a workgroup, a quarter each of its four waves; 16-byte chunks of
-// k staged through LDS by guarded loads.
-template <class T>
-__global__ __launch_bounds__(256) void gemm_simple(Gemm p) {
+// Any strides and sizes: 64 x 64 of the output a workgroup, a quarter each of its four
+// waves, 16-byte chunks of k staged through LDS by guarded loads. Takes what the kernels
+// above do not: operands that are not 16-byte aligned or too large for their offsets.
+template <class T, int ACT>
+__global__ __launch_bounds__(256) void gemm_any_kernel(Gemm p, bool a_kc, bool b_kc) {
     constexpr int CH = 16 / sizeof(T), BK = 4 * CH, LD = BK + CH;
     __shared__ __align__(16) T sa[64][LD], sb[64][LD];
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
     const int64_t tiles_n = (p.N + 63) / 64;
     const int64_t m0 = blockIdx.x / tiles_n * 64, n0 = blockIdx.x % tiles_n * 64;
     const int wm = (w & 1) * 32, wn = (w >> 1) * 32;
+    const int64_t am = a_kc ? p.a.ld : 1, ak = a_kc ? 1 : p.a.ld, bn = b_kc ? p.b.ld : 1, bk = b_kc ? 1 : p.b.ld;
     floatx4 acc[2][2] = {};
     for (int64_t k0 = 0; k0 < p.K; k0 += BK) {
         for (int i = t; i < 64 * BK; i += 256) {
             // consecutive threads along the contiguous dimension
-            const int ra = p.ak == 1 ? i / BK : i % 64, ka = p.ak == 1 ? i % BK : i / 64;
-            const int rb = p.bk == 1 ? i / BK : i % 64, kb = p.bk == 1 ? i % BK : i / 64;
-            sa[ra][ka] = m0 + ra < p.M && k0 + ka < p.K ? ((const T*)p.a)[(m0 + ra) * p.am + (k0 + ka) * p.ak] : (T)0.0f;
-            sb[rb][kb] = n0 + rb < p.N && k0 + kb < p.K ? ((const T*)p.b)[(n0 + rb) * p.bn + (k0 + kb) * p.bk] : (T)0.0f;
+            const int ra = a_kc ? i / BK : i % 64, ka = a_kc ? i % BK : i / 64;
+            const int rb = b_kc ? i / BK : i % 64, kb = b_kc ? i % BK : i / 64;
+            sa[ra][ka] = m0 + ra < p.M && k0 + ka < p.K ? ((const T*)p.a.ptr)[(m0 + ra) * am + (k0 + ka) * ak] : (T)0.0f;
+            sb[rb][kb] = n0 + rb < p.N && k0 + kb < p.K ? ((const T*)p.b.ptr)[(n0 + rb) * bn + (k0 + kb) * bk] : (T)0.0f;
         }
         __syncthreads();
         using F = vec<T, CH>;
@@ -168,39 +247,177 @@ __global__ __launch_bounds__(256) void gemm_simple(Gemm p) {
         __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int j = 0; j < 2; j++) {
+        Epilogue<T, ACT, 1> e;
+        e.columns(p, n0 + wn + 16 * j + 4 * (lane / 16));
 #pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int64_t m = m0 + wm + 16 * i + lane % 16, n = n0 + wn + 16 * j + 4 * (lane / 16) + e;
-                if (m < p.M && n < p.N) finish_element<T>(p, m, n, acc[i][j][e]);
-            }
+        for (int i = 0; i < 2; i++) {
+            const floatx4 v[1] = {acc[i][j]};
+            e.row(p, m0 + wm + 16 * i + lane % 16, v);
+        }
+    }
 }
 
-int gemm(int dtype, const Gemm& p, hipStream_t s) {
-    const int64_t tiles = (p.M + 63) / 64 * ((p.N + 63) / 64);
-    if (tiles == 0) return DRH_OK;
-    if (tiles > INT32_MAX) return fail(DRH_ERR_TOO_LARGE, "more than 2^31 - 1 tiles of 64 x 64 outputs");
+// ---------------------------------------------------------------- which kernel
+
+enum Layout { KK, KN, MN };  // A's and B's contiguous dimension: forward, dx, dW
+
+struct GemmPlan {
+    int tile = 0;    // 256, 128, or 0: any
+    int splits = 1;
+    size_t bytes = 0;  // of partial sums
+};
+
+constexpr int CUS = 256;
+
+// Whether an operand's sizes suit the kernels that load 16-byte chunks through buffers.
+bool chunked(int dtype, bool kc, int64_t ld, int64_t rows, int64_t K) {
+    const int64_t size = type_size(dtype), ch = 16 / size;
+    if (ld % ch || (kc ? K : rows) % ch) return false;
+    return kc ? 256 * ld * size < PAST_END : 64 * ld * size < PAST_END;
+}
+
+GemmPlan plan_gemm(int dtype, int64_t M, int64_t N, int64_t K, bool fits) {
+    GemmPlan g;
+    if (!fits || K == 0) return g;
+    const int64_t bk = 128 / (int64_t)type_size(dtype), kt = (K + bk - 1) / bk;
+    double best = 1e30;
+    for (int tile : {256, 128}) {
+        const int64_t tiles = (M + tile - 1) / tile * ((N + tile - 1) / tile);
+        const int64_t slots = tile == 256 ? CUS : 2 * CUS;
+        if (tiles > INT32_MAX) continue;
+        for (int s = 1; s <= 64 && s <= kt; s++) {
+            const int64_t per = (kt + s - 1) / s;
+            if ((kt + per - 1) / per != s) continue;
+            if (s > 1 && (size_t)s * M * N * 4 > ((size_t)1 << 30)) break;
+            const int64_t rounds = (tiles * s + slots - 1) / slots;
+            // microseconds of a k tile, and of a tile's start and end
+            const double step = (dtype == DRH_F32 ? 7.0 : 1.0) * (tile == 256 ? 1.25 : 0.9);
+            double t = rounds * (per * step + 4.0);
+            if (s > 1) t += 4.0 + s * (double)M * N * 8 / 4e6;
+            if (t < best) best = t, g.tile = tile, g.splits = s;
+        }
+    }
+    if (g.splits > 1) g.bytes = up256((size_t)g.splits * M * N * sizeof(float));
+    return g;
+}
+
+template <class F>
+int with_act(int act, F&& f) {
+    using std::integral_constant;
+    switch (act) {
+        case DRH_ACT_RELU: return f(integral_constant<int, DRH_ACT_RELU>());
+        case DRH_ACT_GELU: return f(integral_constant<int, DRH_ACT_GELU>());
+        case DRH_ACT_GELU_TANH: return f(integral_constant<int, DRH_ACT_GELU_TANH>());
+        case DRH_ACT_SILU: return f(integral_constant<int, DRH_ACT_SILU>());
+        default: return f(integral_constant<int, DRH_ACT_NONE>());
+    }
+}
+
+// p without its plan's fields; `partial` has plan.bytes bytes.
+int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial, hipStream_t s) {
+    if (p.M == 0 || p.N == 0) return DRH_OK;
+    const int64_t ch = 16 / (int64_t)type_size(dtype);
+    auto aligned = [](const void* q) { return (uintptr_t)q % 16 == 0; };
+    p.wide_out = p.N % ch == 0 && aligned(p.out) && aligned(p.res) && aligned(p.kept);
+    const bool fast = plan.tile && aligned(p.a.ptr) && aligned(p.b.ptr);
+    const int tile = fast ? plan.tile : 64;
+    const int64_t tiles = (p.M + tile - 1) / tile * ((p.N + tile - 1) / tile);
+    if (tiles > INT32_MAX) return fail(DRH_ERR_TOO_LARGE, "more than 2^31 - 1 tiles of the output");
+    p.splits = fast ? plan.splits : 1;
+    const int64_t bk = 128 / (int64_t)type_size(dtype), kt = (p.K + bk - 1) / bk;
+    p.tiles_per_split = (int)((kt + p.splits - 1) / p.splits);
+    p.partial = p.splits > 1 ? partial : nullptr;
+    const dim3 grid((unsigned)tiles, (unsigned)p.splits);
     return with_type(dtype, [&](auto t) {
-        gemm_simple<decltype(t)><<<dim3((unsigned)tiles), 256, 0, s>>>(p);
+        using T = decltype(t);
+        if (!fast) {
+            p.wide_out = false;  // a lane has four neighbouring outputs there
+            return with_act(p.act, [&](auto a) {
+                gemm_any_kernel<T, a.value><<<grid, 256, 0, s>>>(p, layout != MN, layout == KK);
+                return DRH_OK;
+            });
+        }
+        auto go = [&](auto a) {
+            constexpr int ACT = a.value;
+            if (layout == KK) {
+                if (tile == 256) gemm_256_kernel<T, true, true, ACT><<<grid, 512, 0, s>>>(p);
+                else gemm_128_kernel<T, true, true, ACT><<<grid, 256, 0, s>>>(p);
+            } else if constexpr (ACT == DRH_ACT_NONE) {
+                if (layout == KN) {
+                    if (tile == 256) gemm_256_kernel<T, true, false, ACT><<<grid, 512, 0, s>>>(p);
+                    else gemm_128_kernel<T, true, false, ACT><<<grid, 256, 0, s>>>(p);
+                } else {
+                    if (tile == 256) gemm_256_kernel<T, false, false, ACT><<<grid, 512, 0, s>>>(p);
+                    else gemm_128_kernel<T, false, false, ACT><<<grid, 256, 0, s>>>(p);
+                }
+            }
+            return DRH_OK;
+        };
+        if (!p.partial) return with_act(p.act, go);
+        go(std::integral_constant<int, DRH_ACT_NONE>());
+        return with_act(p.act, [&](auto a) {
+            const int64_t n = p.M * p.N;
+            constexpr int V = 16 / sizeof(T);
+            if (p.wide_out) join_splits<T, a.value, V><<<dim3((unsigned)((n / V + 255) / 256)), 256, 0, s>>>(p);
+            else join_splits<T, a.value, 1><<<dim3((unsigned)((n + 255) / 256)), 256, 0, s>>>(p);
+            return DRH_OK;
+        });
+    });
+}
+
+// An M x K operand copied to rows of K elements rounded up to 16 bytes, zeros behind K.
+template <class T>
+__global__ __launch_bounds__(256) void pad_rows(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t K,
+                                                T* __restrict__ dst) {
+    constexpr int CH = 16 / sizeof(T);
+    const int64_t per = (K + CH - 1) / CH, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * per) return;
+    const int64_t row = i / per, c = i % per * CH;
+    vec<T, CH> v;
+#pragma unroll
+    for (int e = 0; e < CH; e++) v[e] = c + e < K ? src[row * ld + c + e] : (T)0.0f;
+    *(vec<T, CH>*)(dst + row * per * CH + c) = v;
+}
+
+// A row-major operand as the fast kernels take it: as it stands, or copied to `space`.
+struct Rows {
+    int64_t ld;
+    size_t bytes = 0;  // of the copy, 0: none
+};
+
+Rows rows_for(int dtype, int64_t rows, int64_t K, int64_t ld) {
+    const int64_t ch = 16 / (int64_t)type_size(dtype);
+    if (K % ch == 0 && ld % ch == 0) return {ld};
+    const int64_t padded = (K + ch - 1) / ch * ch;
+    return {padded, up256((size_t)rows * padded * type_size(dtype))};
+}
+
+const void* place_rows(int dtype, const Rows& r, const void* src, int64_t ld, int64_t rows, int64_t K, void* space,
+                       hipStream_t s) {
+    if (!r.bytes) return src;
+    with_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        const int64_t chunks = rows * (r.ld / (16 / (int64_t)sizeof(T)));
+        pad_rows<T><<<dim3((unsigned)((chunks + 255) / 256)), 256, 0, s>>>((const T*)src, ld, rows, K, (T*)space);
         return DRH_OK;
     });
+    return space;
 }
 
 // ---------------------------------------------------------------- dz and the bias gradient
 
-// dz = dy act'(z), rounded to its type for the products, and the column sums of the
-// unrounded values: a workgroup owns 64 VEC columns of every gridDim.y-th slab of rows,
-// its four waves a row each, added in order at the end.
+// dz = dy act'(z), rounded to its type for the products, in rows of ldz elements with zeros
+// behind N, and the column sums of the unrounded values: a workgroup owns 64 VEC columns of
+// every gridDim.y-th slab of rows, its four waves a row each, added in order at the end.
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const Kept<T>* __restrict__ z, int kind,
-                                                    int64_t M, int64_t N, T* __restrict__ dz, float* part) {
+                                                    int64_t M, int64_t N, int64_t ldz, T* __restrict__ dz, float* part) {
     constexpr bool EXACT = sizeof(T) == 4;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * VEC;
     float sum[VEC] = {};
-    if (c < N)
+    if (c < N) {
         for (int64_t row = (int64_t)blockIdx.y * 4 + w; row < M; row += (int64_t)gridDim.y * 4) {
             float g[VEC];
             load<VEC>(dy + row * N + c, g);
@@ -209,11 +426,16 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
                 load<VEC>(z + row * N + c, zz);
 #pragma unroll
                 for (int i = 0; i < VEC; i++) g[i] *= act_slope<EXACT>(kind, zz[i]);
-                store<VEC>(dz + row * N + c, g);
             }
+            if (dz) store<VEC>(dz + row * ldz + c, g);
 #pragma unroll
             for (int i = 0; i < VEC; i++) sum[i] += g[i];
         }
+    } else if (dz && c < ldz) {
+        const float zero[VEC] = {};
+        for (int64_t row = (int64_t)blockIdx.y * 4 + w; row < M; row += (int64_t)gridDim.y * 4)
+            store<VEC>(dz + row * ldz + c, zero);
+    }
     if (!part) return;
     __shared__ float sums[4][64 * VEC];
 #pragma unroll
@@ -230,18 +452,56 @@ int64_t slope_groups(int64_t M) {
     return need < 256 ? need : 256;
 }
 
-struct BackwardPlan {
-    size_t dz = 0, part = 0, total = 0;
+struct ForwardPlan {
+    Rows x, w;
+    GemmPlan y;
+    size_t x_at = 0, w_at = 0, part_at = 0, total = 0;
 };
 
-BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int dtype, int act) {
+ForwardPlan forward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype) {
+    ForwardPlan f;
+    f.x = rows_for(dtype, M, K, xs);
+    f.w = rows_for(dtype, N, K, ws);
+    const int64_t ch = 16 / (int64_t)type_size(dtype), K_pad = (K + ch - 1) / ch * ch;
+    f.y = plan_gemm(dtype, M, N, K, chunked(dtype, true, f.x.ld, M, K_pad) && chunked(dtype, true, f.w.ld, N, K_pad));
+    if (!f.y.tile) f.x = {xs}, f.w = {ws};
+    f.x_at = 0;
+    f.w_at = f.x_at + f.x.bytes;
+    f.part_at = f.w_at + f.w.bytes;
+    f.total = f.part_at + f.y.bytes;
+    return f;
+}
+
+// x and W padded where dW and dx need them, dz where it is not dy itself or dy needs
+// padding, the bias gradient's partial sums, and the larger of the products' partial sums.
+struct BackwardPlan {
+    Rows x, w;
+    bool dz = false;
+    int64_t ldz = 0;
+    GemmPlan dx, dw;
+    size_t x_at = 0, w_at = 0, dz_at = 0, sums_at = 0, part_at = 0, total = 0;
+};
+
+BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype, int act) {
     BackwardPlan b;
-    size_t off = 0;
-    b.dz = off;
-    if (act != DRH_ACT_NONE) off = up256(off + (size_t)M * N * type_size(dtype));
-    b.part = off;
-    off = up256(off + (size_t)slope_groups(M) * N * sizeof(float));
-    b.total = off;
+    const int64_t ch = 16 / (int64_t)type_size(dtype), N_pad = (N + ch - 1) / ch * ch, K_pad = (K + ch - 1) / ch * ch;
+    b.x = rows_for(dtype, M, K, xs);
+    b.w = rows_for(dtype, N, K, ws);
+    b.ldz = N_pad;
+    b.dz = act != DRH_ACT_NONE || N_pad != N;
+    b.dx = plan_gemm(dtype, M, K, N, chunked(dtype, true, b.ldz, M, N_pad) && chunked(dtype, false, b.w.ld, K_pad, N));
+    b.dw = plan_gemm(dtype, N, K, M, chunked(dtype, false, b.ldz, N_pad, M) && chunked(dtype, false, b.x.ld, K_pad, M));
+    if (!b.dx.tile) b.w = {ws};
+    if (!b.dw.tile) b.x = {xs};
+    size_t off = b.x.bytes;
+    b.w_at = off;
+    off += b.w.bytes;
+    b.dz_at = off;
+    if (b.dz) off += up256((size_t)M * b.ldz * type_size(dtype));
+    b.sums_at = off;
+    off += up256((size_t)slope_groups(M) * N * sizeof(float));
+    b.part_at = off;
+    b.total = off + (b.dx.bytes > b.dw.bytes ? b.dx.bytes : b.dw.bytes);
     return b;
 }
 
@@ -257,6 +517,13 @@ int check_linear(drh_ctx* ctx, int64_t M, int64_t N, int64_t K, int64_t xs, int6
     return DRH_OK;
 }
 
+int check_workspace(size_t need, const void* workspace, uint64_t bytes) {
+    if (bytes < need || (need && !workspace))
+        return fail(DRH_ERR_INVALID_ARG, "the call needs " + std::to_string(need) + " bytes of workspace");
+    if ((uintptr_t)workspace % 16) return fail(DRH_ERR_INVALID_ARG, "the workspace must be 16-byte aligned");
+    return DRH_OK;
+}
+
 }  // namespace
 }  // namespace drh_nn
 
@@ -264,28 +531,42 @@ using namespace drh_nn;
 
 extern "C" {
 
+int drh_linear_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride, int dtype,
+                     uint64_t* out_bytes) {
+    if (!out_bytes || !known_type(dtype) || rows < 0 || n_out <= 0 || n_in < 0)
+        return fail(DRH_ERR_INVALID_ARG, "bad sizes or type, or out_bytes is NULL");
+    *out_bytes = forward_plan(rows, n_out, n_in, x_stride, weight_stride, dtype).total;
+    return DRH_OK;
+}
+
 int drh_linear(drh_ctx* ctx, const void* x, const void* weight, const void* bias, const void* residual, int64_t rows,
                int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride, int dtype, int activation, void* y,
-               void* kept, void* stream, uint32_t flags) {
+               void* kept, void* workspace, uint64_t workspace_bytes, void* stream, uint32_t flags) {
     int rc = check_linear(ctx, rows, n_out, n_in, x_stride, weight_stride, dtype, activation, flags);
     if (rc) return rc;
     if (rows == 0) return DRH_OK;
     if (!y || (n_in > 0 && (!x || !weight))) return fail(DRH_ERR_INVALID_ARG, "x, weight and y must not be NULL");
+    const ForwardPlan plan = forward_plan(rows, n_out, n_in, x_stride, weight_stride, dtype);
+    rc = check_workspace(plan.total, workspace, workspace_bytes);
+    if (rc) return rc;
     DeviceGuard dg(ctx->device);
     hipStream_t s = (hipStream_t)stream;
+    char* ws = (char*)workspace;
     Gemm p{};
-    p.a = x, p.am = x_stride, p.ak = 1, p.b = weight, p.bn = weight_stride, p.bk = 1;
+    p.a = {place_rows(dtype, plan.x, x, x_stride, rows, n_in, ws + plan.x_at, s), plan.x.ld, rows};
+    p.b = {place_rows(dtype, plan.w, weight, weight_stride, n_out, n_in, ws + plan.w_at, s), plan.w.ld, n_out};
     p.M = rows, p.N = n_out, p.K = n_in;
     p.bias = bias, p.res = residual, p.out = y, p.act = activation;
-    p.z = activation != DRH_ACT_NONE ? kept : nullptr;
-    rc = gemm(dtype, p, s);
+    p.kept = activation != DRH_ACT_NONE ? kept : nullptr;
+    rc = gemm(dtype, KK, p, plan.y, (float*)(ws + plan.part_at), s);
     return rc ? rc : finish_call(s, flags, "linear");
 }
 
-int drh_linear_backward_bytes(int64_t rows, int64_t n_out, int64_t n_in, int dtype, int activation, uint64_t* out_bytes) {
+int drh_linear_backward_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride,
+                              int dtype, int activation, uint64_t* out_bytes) {
     if (!out_bytes || !known_type(dtype) || rows < 0 || n_out <= 0 || n_in < 0)
         return fail(DRH_ERR_INVALID_ARG, "bad sizes or type, or out_bytes is NULL");
-    *out_bytes = backward_plan(rows, n_out, n_in, dtype, activation).total;
+    *out_bytes = backward_plan(rows, n_out, n_in, x_stride, weight_stride, dtype, activation).total;
     return DRH_OK;
 }
 
@@ -300,45 +581,48 @@ int drh_linear_backward(drh_ctx* ctx, const void* x, const void* weight, const v
     if (M > 0 && (!grad_y || (slope && !kept))) return fail(DRH_ERR_INVALID_ARG, "grad_y and kept must not be NULL");
     if (M > 0 && K > 0 && ((grad_x && !weight) || (grad_weight && !x)))
         return fail(DRH_ERR_INVALID_ARG, "an input pointer is NULL");
-    const BackwardPlan plan = backward_plan(M, N, K, dtype, activation);
-    if (workspace_bytes < plan.total || (plan.total && !workspace))
-        return fail(DRH_ERR_INVALID_ARG, "the backward pass needs " + std::to_string(plan.total) + " bytes of workspace");
-    if ((uintptr_t)workspace % 16) return fail(DRH_ERR_INVALID_ARG, "the workspace must be 16-byte aligned");
+    const BackwardPlan plan = backward_plan(M, N, K, x_stride, weight_stride, dtype, activation);
+    rc = check_workspace(plan.total, workspace, workspace_bytes);
+    if (rc) return rc;
     DeviceGuard dg(ctx->device);
     hipStream_t s = (hipStream_t)stream;
-    const void* dz = grad_y;
-    float* part = grad_bias ? (float*)((char*)workspace + plan.part) : nullptr;
-    const int64_t groups = slope_groups(M);
-    if (M > 0 && (slope || grad_bias)) {
-        void* out = slope ? (char*)workspace + plan.dz : nullptr;
+    char* ws = (char*)workspace;
+    const bool products = K > 0 && M > 0 && (grad_x || grad_weight), dz_made = plan.dz && products;
+    float* sums = grad_bias ? (float*)(ws + plan.sums_at) : nullptr;
+    const int64_t groups = slope_groups(M), ldz = plan.ldz;
+    const void* dz = dz_made ? ws + plan.dz_at : grad_y;
+    if (M > 0 && (dz_made || grad_bias))
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
-            const int vec = vector_width(dtype, {N}, {grad_y, kept});
             auto go = [&](auto v) {
                 const int64_t cols = 64 * v.value;
-                slope_kernel<T, v.value><<<dim3((unsigned)((N + cols - 1) / cols), (unsigned)groups), 256, 0, s>>>(
-                    (const T*)grad_y, slope ? (const Kept<T>*)kept : nullptr, activation, M, N, (T*)out, part);
+                slope_kernel<T, v.value><<<dim3((unsigned)((ldz + cols - 1) / cols), (unsigned)groups), 256, 0, s>>>(
+                    (const T*)grad_y, slope ? (const Kept<T>*)kept : nullptr, activation, M, N, ldz,
+                    dz_made ? (T*)dz : nullptr, sums);
             };
+            const int vec = vector_width(dtype, {N}, {grad_y, kept});
             if (vec == 1) go(std::integral_constant<int, 1>());
             else if (sizeof(T) == 2 && vec == 2) go(std::integral_constant<int, 2>());
             else go(std::integral_constant<int, 16 / (int)sizeof(T)>());
             return DRH_OK;
         });
-        if (slope) dz = out;
-    }
-    if (grad_bias) reduce_columns(part, M > 0 ? groups : 0, N, N, grad_bias, nullptr, dtype, s);
+    if (grad_bias) reduce_columns(sums, M > 0 ? groups : 0, N, N, grad_bias, nullptr, dtype, s);
+    const int64_t ch = 16 / (int64_t)type_size(dtype), N_pad = (N + ch - 1) / ch * ch, K_pad = (K + ch - 1) / ch * ch;
+    float* part = (float*)(ws + plan.part_at);
     if (grad_x && M > 0 && K > 0) {
         Gemm p{};
-        p.a = dz, p.am = N, p.ak = 1, p.b = weight, p.bn = 1, p.bk = weight_stride;
+        const void* w = place_rows(dtype, plan.w, weight, weight_stride, N, K, ws + plan.w_at, s);
+        p.a = {dz, ldz, M}, p.b = {w, plan.w.ld, plan.w.bytes ? K_pad : K};
         p.M = M, p.N = K, p.K = N, p.out = grad_x, p.act = DRH_ACT_NONE;
-        rc = gemm(dtype, p, s);
+        rc = gemm(dtype, KN, p, plan.dx, part, s);
         if (rc) return rc;
     }
     if (grad_weight && K > 0) {
         Gemm p{};
-        p.a = dz, p.am = 1, p.ak = N, p.b = x, p.bn = 1, p.bk = x_stride;
+        const void* xp = M > 0 ? place_rows(dtype, plan.x, x, x_stride, M, K, ws + plan.x_at, s) : x;
+        p.a = {dz, ldz, dz_made ? N_pad : N}, p.b = {xp, plan.x.ld, plan.x.bytes ? K_pad : K};
         p.M = N, p.N = K, p.K = M, p.out = grad_weight, p.act = DRH_ACT_NONE;
-        rc = gemm(dtype, p, s);
+        rc = gemm(dtype, MN, p, plan.dw, part, s);
         if (rc) return rc;
     }
     return finish_call(s, flags, "linear backward");

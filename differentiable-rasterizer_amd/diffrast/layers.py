@@ -53,6 +53,11 @@ def _rows(x: Tensor) -> Tensor:
     return v
 
 
+def _stride(v: Tensor) -> int:
+    """Elements between the rows of _rows' view; one row has no stride of its own."""
+    return v.stride(0) if v.shape[0] > 1 else v.shape[1]
+
+
 def _flat(t: Tensor | None) -> Tensor | None:
     return t if t is None or t.is_contiguous() else t.contiguous()
 
@@ -181,10 +186,14 @@ def _linear_forward(x, weight, bias, act, residual, keep):
     kept = None
     if keep and act:
         kept = torch.empty((rows, n_out), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=dev)
+    xs, wst, code = _stride(xv), _stride(weight), DTYPES[x.dtype]
+    L = _lib.lib()
+    n = _bytes(L.drh_linear_bytes, rows, n_out, n_in, xs, wst, code)
+    ws = _workspace(n, dev)
     handle, stream = _enter(dev)
-    _lib.check(_lib.lib().drh_linear(
-        handle, xv.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), rows, n_out, n_in, xv.stride(0),
-        weight.stride(0), DTYPES[x.dtype], act, y.data_ptr(), _ptr(kept), stream, 0))
+    _lib.check(L.drh_linear(
+        handle, xv.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), rows, n_out, n_in, xs, wst, code, act,
+        y.data_ptr(), _ptr(kept), _ptr(ws), n, stream, 0))
     return y, xv, kept
 
 
@@ -212,12 +221,13 @@ class _Linear(torch.autograd.Function):
         if want_x or want_w or want_b:
             g = g.contiguous()
             L = _lib.lib()
-            n = _bytes(L.drh_linear_backward_bytes, rows, n_out, n_in, DTYPES[dt], ctx.act)
+            xs, wst, code = _stride(xv), _stride(weight), DTYPES[dt]
+            n = _bytes(L.drh_linear_backward_bytes, rows, n_out, n_in, xs, wst, code, ctx.act)
             ws = _workspace(n, dev)
             handle, stream = _enter(dev)
             _lib.check(L.drh_linear_backward(
-                handle, xv.data_ptr(), weight.data_ptr(), _ptr(kept), g.data_ptr(), rows, n_out, n_in, xv.stride(0),
-                weight.stride(0), DTYPES[dt], ctx.act, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n, stream, 0))
+                handle, xv.data_ptr(), weight.data_ptr(), _ptr(kept), g.data_ptr(), rows, n_out, n_in, xs, wst, code,
+                ctx.act, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n, stream, 0))
         return dx, dw, db, None, g if want_r else None
 
 

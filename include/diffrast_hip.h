@@ -379,11 +379,14 @@ enum { DRH_ACT_NONE = 0, DRH_ACT_RELU = 1, DRH_ACT_GELU = 2, DRH_ACT_GELU_TANH =
  * with DRH_ACT_NONE. */
 int drh_linear(drh_ctx *ctx, const void *x, const void *weight, const void *bias, const void *residual,
                int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride,
-               int dtype, int activation, void *y, void *kept, void *stream, uint32_t flags);
+               int dtype, int activation, void *y, void *kept, void *workspace, uint64_t workspace_bytes,
+               void *stream, uint32_t flags);
 
-/* Workspace of drh_linear_backward. */
-int drh_linear_backward_bytes(int64_t rows, int64_t n_out, int64_t n_in, int dtype, int activation,
-                              uint64_t *out_bytes);
+/* Workspace of drh_linear (0 for many sizes) and of drh_linear_backward. */
+int drh_linear_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride,
+                     int dtype, uint64_t *out_bytes);
+int drh_linear_backward_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride,
+                              int64_t weight_stride, int dtype, int activation, uint64_t *out_bytes);
 
 /* Gradients of drh_linear from grad_y (rows x n_out, contiguous), its x and weight,
  * and `kept` (NULL with DRH_ACT_NONE). grad_x (rows x n_in), grad_weight (n_out x
