@@ -17,6 +17,7 @@ ValueError, and there is no CPU path. The calls may be captured into a HIP graph
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 from torch import Tensor
@@ -34,21 +35,16 @@ def _dtype(t: Tensor) -> int:
     return code
 
 
-def _device(x: Tensor) -> torch.device:
-    """Where the call runs: the GPU that x is on, or the current one."""
-    return x.device if x.is_cuda else torch_layer._gpu()
-
-
 def _rows(x: Tensor) -> Tensor:
     """x as (rows, features) with contiguous features: a view where x's strides allow."""
-    D = x.shape[-1]
     if x.dim() == 2:
+        if x.is_contiguous():
+            return x
         v = x
-    elif x.is_contiguous():
-        v = x.view(x.numel() // D if D else 0, D) if D else x.reshape(-1, 0)
     else:
-        v = x.reshape(-1, D)
-    if v.stride(1) != 1 or (v.shape[0] > 1 and v.stride(0) < D):
+        D = x.shape[-1]
+        v = x.reshape(x.numel() // D if D else math.prod(x.shape[:-1]), D)
+    if v.stride(1) != 1 or (v.shape[0] > 1 and v.stride(0) < v.shape[1]):
         v = v.contiguous()
     return v
 
@@ -67,12 +63,13 @@ def _ptr(t: Tensor | None):
 
 
 def _enter(dev: torch.device):
-    """(context handle, stream handle) of a call on `dev`."""
+    """(context handle, stream handle) of a call on `dev`. The stream is torch's current
+    one, without the Stream object around it, which costs 2 us a call."""
     ctx = torch_layer._contexts.get(dev.index)
     if ctx is None:
         ctx = torch_layer._context(dev)
     torch_layer._note_gpu()
-    return ctx.handle, torch.cuda.current_stream(dev).cuda_stream
+    return ctx.handle, torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _bytes(fn, *sizes) -> int:
@@ -85,12 +82,31 @@ def _workspace(n: int, dev: torch.device) -> Tensor | None:
     return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
 
 
-def _to(dev: torch.device, *tensors):
-    return [t if t is None or t.device == dev else t.to(dev) for t in tensors]
+def _elsewhere(x: Tensor, *others: Tensor | None) -> bool:
+    """Whether a tensor is not on the GPU that x is on (or x on none)."""
+    if not x.is_cuda:
+        return True
+    for t in others:
+        if t is not None and t.device != x.device:
+            return True
+    return False
 
 
-def _grads_wanted(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _moved(x: Tensor, *others: Tensor | None):
+    """The tensors on the GPU that x is on, or on the current one."""
+    dev = x.device if x.is_cuda else torch_layer._gpu()
+    return [t if t is None else t.to(dev) for t in (x, *others)]
+
+
+def _once(backward):
+    """`backward`, differentiable once. torch's own wrapper for that is entered only where a
+    graph of the backward pass is asked for, since it costs 4 us a call."""
+    wrapped = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return wrapped(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 # ---------------------------------------------------------------- layer norm
@@ -100,46 +116,51 @@ def _layer_norm_forward(x, weight, bias, eps, keep):
     dev = x.device
     xv = _rows(x)
     rows, cols = xv.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=dev) if keep else None
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if keep:
+        stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
+    else:
+        stats = mean = rstd = None
     code = DTYPES[x.dtype]
-    wcode = code if weight is None and bias is None else DTYPES[(bias if weight is None else weight).dtype]
-    mean = _ptr(stats)
+    wcode = DTYPES[weight.dtype] if weight is not None else DTYPES[bias.dtype] if bias is not None else code
     handle, stream = _enter(dev)
     _lib.check(_lib.lib().drh_layer_norm(
-        handle, xv.data_ptr(), _ptr(weight), _ptr(bias), rows, cols, xv.stride(0), code, wcode, eps, y.data_ptr(),
-        mean, mean + 4 * rows if mean else mean, stream, 0))
-    return y, xv, stats, wcode
+        handle, xv.data_ptr(), _ptr(weight), _ptr(bias), rows, cols, _stride(xv), code, wcode, eps, y.data_ptr(),
+        mean, rstd, stream, 0))
+    return y, xv, stats
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         weight, bias = _flat(weight), _flat(bias)
-        y, xv, stats, ctx.wcode = _layer_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(xv, weight, stats)
-        ctx.wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else None
+        y, xv, stats = _layer_norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(xv, weight, bias, stats)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
-        xv, weight, stats = ctx.saved_tensors
+        xv, weight, bias, stats = ctx.saved_tensors
         dev = xv.device
         rows, cols = xv.shape
         gv = _rows(g)
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(g.shape, dtype=xv.dtype, device=dev) if want_x else None
-        dw = torch.empty(cols, dtype=ctx.wdtype, device=dev) if want_w else None
-        db = torch.empty(cols, dtype=ctx.wdtype, device=dev) if want_b else None
+        want_x, want_w, want_b, _ = ctx.needs_input_grad
+        dx = torch.empty_like(g, memory_format=torch.contiguous_format) if want_x else None
+        dw = torch.empty_like(weight) if want_w else None
+        db = torch.empty_like(bias) if want_b else None
+        code = DTYPES[xv.dtype]
+        wcode = DTYPES[weight.dtype] if weight is not None else DTYPES[bias.dtype] if bias is not None else code
         L = _lib.lib()
         n = _bytes(L.drh_layer_norm_backward_bytes, rows, cols) if want_w or want_b else 0
         ws = _workspace(n, dev)
         mean = stats.data_ptr()
         handle, stream = _enter(dev)
         _lib.check(L.drh_layer_norm_backward(
-            handle, xv.data_ptr(), _ptr(weight), mean, mean + 4 * rows, gv.data_ptr(), rows, cols, xv.stride(0),
-            gv.stride(0), DTYPES[xv.dtype], ctx.wcode, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n, stream, 0))
+            handle, xv.data_ptr(), _ptr(weight), mean, mean + 4 * rows, gv.data_ptr(), rows, cols, _stride(xv),
+            _stride(gv), code, wcode, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n, stream, 0))
         return dx, dw, db, None
 
 
@@ -152,24 +173,24 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
         eps: added to the variance, which is the mean of squares about the mean.
     """
     _dtype(x)
-    if x.dim() < 1 or x.shape[-1] == 0:
+    D = x.shape[-1] if x.dim() else 0
+    if D == 0:
         raise ValueError(f"expected x of shape (..., D), got {tuple(x.shape)}")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
-        if t.shape != x.shape[-1:]:
-            raise ValueError(f"expected {name} of shape ({x.shape[-1]},), got {tuple(t.shape)}")
+        if t.dim() != 1 or t.shape[0] != D:
+            raise ValueError(f"expected {name} of shape ({D},), got {tuple(t.shape)}")
         if t.dtype != x.dtype and t.dtype != torch.float32:
             raise ValueError(f"expected {name} in {x.dtype} or float32, got {t.dtype}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"weight is {weight.dtype} but bias {bias.dtype}")
-    home, dev = x.device, _device(x)
-    if home != dev:
-        return layer_norm(*_to(dev, x, weight, bias), eps=eps).to(home)
-    weight, bias = _to(dev, weight, bias)
-    if _grads_wanted(x, weight, bias):
+    if _elsewhere(x, weight, bias):
+        return layer_norm(*_moved(x, weight, bias), eps=eps).to(x.device)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps)
     return _layer_norm_forward(x, _flat(weight), _flat(bias), eps, False)[0]
 
@@ -182,7 +203,7 @@ def _linear_forward(x, weight, bias, act, residual, keep):
     xv = _rows(x)
     rows, n_in = xv.shape
     n_out = weight.shape[0]
-    y = torch.empty((*x.shape[:-1], n_out), dtype=x.dtype, device=dev)
+    y = x.new_empty((rows, n_out) if x.dim() == 2 else (*x.shape[:-1], n_out))
     kept = None
     if keep and act:
         kept = torch.empty((rows, n_out), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=dev)
@@ -208,16 +229,16 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
         xv, weight, kept = ctx.saved_tensors
         dev, dt = xv.device, xv.dtype
         rows, n_in = xv.shape
         n_out = weight.shape[0]
         want_x, want_w, want_b, _, want_r = ctx.needs_input_grad
-        dx = torch.empty(ctx.x_shape, dtype=dt, device=dev) if want_x else None
-        dw = torch.empty((n_out, n_in), dtype=dt, device=dev) if want_w else None
-        db = torch.empty(n_out, dtype=dt, device=dev) if want_b else None
+        dx = xv.new_empty(ctx.x_shape) if want_x else None
+        dw = xv.new_empty((n_out, n_in)) if want_w else None
+        db = xv.new_empty(n_out) if want_b else None
         if want_x or want_w or want_b:
             g = g.contiguous()
             L = _lib.lib()
@@ -257,13 +278,12 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: st
     for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
         if t is not None and t.dtype != x.dtype:
             raise ValueError(f"x is {x.dtype} but {name} {t.dtype}")
-    home, dev = x.device, _device(x)
-    if home != dev:
-        xd, wd, bd, rd = _to(dev, x, weight, bias, residual)
-        return linear(xd, wd, bd, activation, rd).to(home)
-    weight, bias, residual = _to(dev, weight, bias, residual)
+    if _elsewhere(x, weight, bias, residual):
+        xd, wd, bd, rd = _moved(x, weight, bias, residual)
+        return linear(xd, wd, bd, activation, rd).to(x.device)
     act = ACTIVATIONS[activation]
-    if _grads_wanted(x, weight, bias, residual):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, act, residual)
     return _linear_forward(x, _rows(weight), _flat(bias), act, _flat(residual), False)[0]
 
@@ -273,7 +293,7 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: st
 
 def _dropout(x, residual, p, seed, offset):
     x = x.contiguous()
-    y = torch.empty_like(x)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     handle, stream = _enter(x.device)
     _lib.check(_lib.lib().drh_dropout(handle, x.data_ptr(), _ptr(residual), x.numel(), DTYPES[x.dtype], p, seed, offset,
                                       y.data_ptr(), stream, 0))
@@ -287,7 +307,7 @@ class _Dropout(torch.autograd.Function):
         return _dropout(x, _flat(residual), p, seed, offset)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
         dx = _dropout(g, None, *ctx.draw) if ctx.needs_input_grad[0] else None
         return dx, None, None, None, g if ctx.needs_input_grad[4] else None
@@ -315,11 +335,9 @@ def dropout(x: Tensor, p: float, *, seed: int, offset: int = 0, residual: Tensor
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"expected a residual of shape {tuple(x.shape)} in {x.dtype}, got "
                          f"{tuple(residual.shape)} in {residual.dtype}")
-    home, dev = x.device, _device(x)
-    if home != dev:
-        xd, rd = _to(dev, x, residual)
-        return dropout(xd, p, seed=seed, offset=offset, residual=rd).to(home)
-    (residual,) = _to(dev, residual)
-    if _grads_wanted(x, residual):
+    if _elsewhere(x, residual):
+        xd, rd = _moved(x, residual)
+        return dropout(xd, p, seed=seed, offset=offset, residual=rd).to(x.device)
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return _Dropout.apply(x, p, seed, offset, residual)
     return _dropout(x, _flat(residual), p, seed, offset)
