@@ -77,8 +77,9 @@ __device__ inline int swizzle(int i) {
 }
 
 // One operand of a workgroup's tile: UNITS units of 128 rows; row R of unit u is row
-// u * 128 + R of the tile, or with UNITS == 2 on B's side (R / 32) * 64 + u * 32 + R % 32,
-// which puts a wave's 32 rows of both units side by side.
+// u * 128 + R of the tile. On B's side with two units and k contiguous it is (R / 32) * 64
+// + u * 32 + R % 32 instead, so that a wave's 32 rows of both units are neighbours in the
+// output; with rows contiguous that would read half lines.
 template <class T, bool KC, bool B, int UNITS, int NF, int WAVES>
 struct Loader {
     static constexpr int CH = 16 / sizeof(T), BK = 8 * CH, LOADS = 16 / WAVES;
@@ -127,7 +128,7 @@ struct Loader {
     }
 
     static __device__ int64_t tile_row(int u, int R) {
-        return B && UNITS == 2 ? (R / 32) * 64 + u * 32 + R % 32 : u * 128 + R;
+        return B && KC && UNITS == 2 ? (R / 32) * 64 + u * 32 + R % 32 : u * 128 + R;
     }
 
     // Starts the loads of unit u of k tile kt into LDS at `lds`; past the last tile they
@@ -240,7 +241,7 @@ __device__ inline void pick_tile(int64_t tiles_m, int64_t tiles_n, int64_t& tm, 
 // their use (five units in flight). A unit is overwritten two steps after both groups have
 // read it at the earliest.
 template <class T, bool AK, bool BK_, class Epilogue>
-__device__ inline void gemm_256(const Gemm& p, Epilogue& epilogue) {
+__device__ inline void gemm_256(const Gemm& p) {
     __shared__ __align__(1024) char lds[8 * UNIT_BYTES];
     using LA = Loader<T, AK, false, 2, 4, 8>;
     using LB = Loader<T, BK_, true, 2, 2, 8>;
@@ -303,20 +304,24 @@ __device__ inline void gemm_256(const Gemm& p, Epilogue& epilogue) {
     if (wm == 0) wg_barrier();
     wait_vm<0>();  // LDS is given up with no load on its way there
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int nu = BK_ ? 32 : 128;
+    Epilogue e0, e1;
+    e0.columns(p, n0 + wn * (BK_ ? 64 : 32) + q * 8);
+    e1.columns(p, n0 + wn * (BK_ ? 64 : 32) + nu + q * 8);
 #pragma unroll
-    for (int ub = 0; ub < 2; ub++) {
-        epilogue.columns(p, n0 + wn * 64 + ub * 32 + q * 8);
+    for (int ua = 0; ua < 2; ua++)
 #pragma unroll
-        for (int ua = 0; ua < 2; ua++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) epilogue.row(p, m0 + ua * 128 + wm * 64 + i * 16 + r, acc[ua][ub][i]);
-    }
+        for (int i = 0; i < 4; i++) {
+            const int64_t m = m0 + ua * 128 + wm * 64 + i * 16 + r;
+            e0.row(p, m, acc[ua][0][i]);
+            e1.row(p, m, acc[ua][1][i]);
+        }
 }
 
 // 128 x 128 by four waves, 64 x 64 each, two k tiles in LDS (64 KiB): two workgroups a CU,
 // each covering the other's waits.
 template <class T, bool AK, bool BK_, class Epilogue>
-__device__ inline void gemm_128(const Gemm& p, Epilogue& epilogue) {
+__device__ inline void gemm_128(const Gemm& p) {
     __shared__ __align__(1024) char lds[4 * UNIT_BYTES];
     using LA = Loader<T, AK, false, 1, 4, 4>;
     using LB = Loader<T, BK_, true, 1, 4, 4>;
@@ -351,6 +356,7 @@ __device__ inline void gemm_128(const Gemm& p, Epilogue& epilogue) {
     }
     wait_vm<0>();
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    Epilogue epilogue;
     epilogue.columns(p, n0 + wn * 64 + q * 16);
 #pragma unroll
     for (int i = 0; i < 4; i++) epilogue.row(p, m0 + wm * 64 + i * 16 + r, acc[i]);

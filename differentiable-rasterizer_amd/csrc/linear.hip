@@ -170,14 +170,12 @@ struct Epilogue {
 
 template <class T, bool AK, bool BK, int ACT>
 __global__ __launch_bounds__(512, 2) void gemm_256_kernel(Gemm p) {
-    Epilogue<T, ACT, 2> e;
-    gemm_256<T, AK, BK>(p, e);
+    gemm_256<T, AK, BK, Epilogue<T, ACT, 2>>(p);
 }
 
 template <class T, bool AK, bool BK, int ACT>
 __global__ __launch_bounds__(256, 2) void gemm_128_kernel(Gemm p) {
-    Epilogue<T, ACT, 4> e;
-    gemm_128<T, AK, BK>(p, e);
+    gemm_128<T, AK, BK, Epilogue<T, ACT, 4>>(p);
 }
 
 // The parts of a split product added in order, and the epilogue.
