@@ -1,7 +1,8 @@
-"""Builds libdiffrast_hip.so (gfx950) in-tree with hipcc.
+"""Builds libdiffrast_hip.so (gfx950) in-tree with hipcc, and the native torch
+operations of diffrast.layers over it with the host compiler.
 
 Usage: python build.py [--verbose]. The library lands next to this file, where
-`diffrast._lib` loads it from.
+`diffrast._lib` loads it from, the torch operations in diffrast/.
 """
 
 from __future__ import annotations
@@ -10,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
@@ -18,6 +20,8 @@ HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libdiffrast_hip.so"
+TORCH_SOURCE = CSRC / "torch_layers.cpp"
+TORCH_LIB = HERE / "diffrast" / "_torch_layers.so"
 ARCH = os.environ.get("DIFFRAST_OFFLOAD_ARCH", "gfx950")
 
 SOURCES = [CSRC / "kernels.hip", CSRC / "runtime.hip", CSRC / "fit.hip", CSRC / "scratch.hip", CSRC / "resize.hip",
@@ -60,7 +64,7 @@ def _run(cmd: list[str], verbose: bool) -> None:
     noise = "packed-fp32-ops"
     err = "\n".join(l for l in (res.stderr or "").splitlines() if noise not in l)
     if res.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({res.returncode}):\n{err}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed ({res.returncode}):\n{err}")
     if verbose and err.strip():
         print(err)
 
@@ -77,5 +81,27 @@ def build(verbose: bool = False) -> Path:
     return LIB
 
 
+def build_torch(verbose: bool = False) -> Path | None:
+    """The native torch operations (host code alone), linked to LIB; None without PyTorch."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    pkg = Path(torch.__file__).resolve().parent
+    rocm = Path(hipcc()).resolve().parents[1]
+    tmp = TORCH_LIB.with_suffix(".so.tmp")
+    _run([shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-sign-compare",
+          "-Wno-unknown-pragmas", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-DTORCH_EXTENSION_NAME=_torch_layers",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *(f"-isystem{d}" for d in (pkg / "include", pkg / "include" / "torch" / "csrc" / "api" / "include",
+                                     rocm / "include", sysconfig.get_paths()["include"])),
+          f"-I{ROOT / 'include'}", str(TORCH_SOURCE), "-o", str(tmp), f"-L{pkg / 'lib'}", f"-L{HERE}",
+          "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-ltorch_python", "-ldiffrast_hip",
+          "-Wl,-rpath,$ORIGIN/.."], verbose)
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
+
+
 if __name__ == "__main__":
     print(build(verbose="--verbose" in sys.argv))
+    print(build_torch(verbose="--verbose" in sys.argv))
