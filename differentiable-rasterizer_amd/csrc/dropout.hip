@@ -35,33 +35,30 @@ __device__ inline void philox(uint64_t block, uint64_t offset, uint64_t seed, ui
     out[0] = c0, out[1] = c1, out[2] = c2, out[3] = c3;
 }
 
-// A thread takes the eight elements of one counter; `vec` of them a load.
-template <class T, int VEC>
+// A thread takes the eight elements of one counter.
+template <class T>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, const T* __restrict__ res, int64_t n,
                                                       uint32_t threshold, float scale, uint64_t seed, uint64_t offset,
                                                       T* __restrict__ y) {
+    constexpr int VEC = 16 / sizeof(T);
     const int64_t block = (int64_t)blockIdx.x * 256 + threadIdx.x, i0 = block * 8;
     if (i0 >= n) return;
     uint32_t w[4];
     philox((uint64_t)block, offset, seed, w);
-    auto value = [&](int i, float xv, float rv) {
-        const uint32_t bits = (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
-        const float kept = bits >= threshold ? xv * scale : 0.0f;
-        return res ? kept + rv : kept;
-    };
-    if (i0 + 8 <= n) {
 #pragma unroll
-        for (int j = 0; j < 8; j += VEC) {
-            float a[VEC], r[VEC] = {};
-            load<VEC>(x + i0 + j, a);
-            if (res) load<VEC>(res + i0 + j, r);
+    for (int j = 0; j < 8; j += VEC) {
+        if (i0 + j >= n) break;
+        float a[VEC] = {}, r[VEC] = {};
+        load_some<VEC>(x + i0 + j, n - i0 - j, a);
+        if (res) load_some<VEC>(res + i0 + j, n - i0 - j, r);
 #pragma unroll
-            for (int i = 0; i < VEC; i++) a[i] = value(j + i, a[i], r[i]);
-            store<VEC>(y + i0 + j, a);
+        for (int i = 0; i < VEC; i++) {
+            const int e = i + j;
+            const uint32_t bits = (e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
+            a[i] = bits >= threshold ? a[i] * scale : 0.0f;
+            if (res) a[i] += r[i];
         }
-    } else {
-        for (int j = 0; j < 8; j++)
-            if (i0 + j < n) y[i0 + j] = (T)value(j, (float)x[i0 + j], res ? (float)res[i0 + j] : 0.0f);
+        store_some<VEC>(y + i0 + j, n - i0 - j, a);
     }
 }
 
@@ -86,14 +83,9 @@ extern "C" int drh_dropout(drh_ctx* ctx, const void* x, const void* residual, in
     DeviceGuard dg(ctx->device);
     hipStream_t s = (hipStream_t)stream;
     const dim3 grid((unsigned)((n + 2047) / 2048));
-    const bool wide = ((uintptr_t)x | (uintptr_t)y | (uintptr_t)residual) % 16 == 0;
     with_type(dtype, [&](auto ty) {
         using T = decltype(ty);
-        constexpr int V = 16 / sizeof(T);
-        if (wide)
-            dropout_kernel<T, V><<<grid, 256, 0, s>>>((const T*)x, (const T*)residual, n, t, scale, seed, offset, (T*)y);
-        else
-            dropout_kernel<T, 1><<<grid, 256, 0, s>>>((const T*)x, (const T*)residual, n, t, scale, seed, offset, (T*)y);
+        dropout_kernel<T><<<grid, 256, 0, s>>>((const T*)x, (const T*)residual, n, t, scale, seed, offset, (T*)y);
         return DRH_OK;
     });
     return finish_call(s, flags, "dropout");

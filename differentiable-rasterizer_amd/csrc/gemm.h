@@ -26,13 +26,12 @@ struct Gemm {
     Operand a, b;
     int64_t M, N, K;
     const void *bias, *res;  // N; M x N
-    void* kept;              // M x N of Kept<T>, or null
+    void* kept;              // M x N of Kept<T>: the activation's slopes; or null
     void* out;               // M x N
     float* partial;          // splits x M x N sums instead of `out`, or null
     int act;
     int splits;              // the k range in this many parts, grid.y
     int tiles_per_split;     // tiles of k in each
-    bool wide_out;           // N and the epilogue's pointers allow 16-byte accesses
 };
 
 // D = A B + C on a wave: lane l gives row l % 16 of A and of B, the 16 bytes of k that

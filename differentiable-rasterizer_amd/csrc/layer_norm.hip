@@ -20,15 +20,13 @@ namespace {
 // elements, then four waves up to LN_MAX_COLS. Thread t's vectors are t, t + TPR, ...
 constexpr int LN_MAX_COLS = 256 * 32;
 
-template <int VEC>
-__device__ inline void load_weight(const void* w, bool wf32, int is_bf16, int64_t c, float (&out)[VEC]) {
-    // weights may stand in 32 bits beside activations in 16
+// Weights from column c on; they may stand in 32 bits beside activations in 16.
+template <class T, int VEC>
+__device__ inline void load_weight(const void* w, bool wf32, int c, int D, float (&out)[VEC]) {
     if (wf32)
-        for (int i = 0; i < VEC; i++) out[i] = ((const float*)w)[c + i];
-    else if (is_bf16)
-        for (int i = 0; i < VEC; i++) out[i] = (float)((const bf16*)w)[c + i];
+        load_some<VEC>((const float*)w + c, D - c, out);
     else
-        for (int i = 0; i < VEC; i++) out[i] = (float)((const f16*)w)[c + i];
+        load_some<VEC>((const T*)w + c, D - c, out);
 }
 
 // Sums of a and b over a row's threads, in all of them. `slot` alternates between
@@ -62,9 +60,9 @@ struct LnArgs {
     float eps;
 };
 
-template <class T, int VEC, int EPT, int TPR>
+template <class T, int EPT, int TPR>
 __global__ __launch_bounds__(256) void ln_forward(LnArgs p) {
-    constexpr int NV = EPT / VEC, RPB = 256 / TPR;
+    constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC, RPB = 256 / TPR;
     const int t = threadIdx.x % TPR, D = p.cols;
     const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
     if (TPR <= 64 && row >= p.rows) return;
@@ -76,7 +74,7 @@ __global__ __launch_bounds__(256) void ln_forward(LnArgs p) {
         const int c = (j * TPR + t) * VEC;
 #pragma unroll
         for (int i = 0; i < VEC; i++) v[j][i] = 0.0f;
-        if (c < D) load<VEC>(x + c, v[j]);
+        if (c < D) load_some<VEC>(x + c, D - c, v[j]);
     }
 #pragma unroll
     for (int j = 0; j < NV; j++)
@@ -86,10 +84,17 @@ __global__ __launch_bounds__(256) void ln_forward(LnArgs p) {
     const float mu = s / (float)D;
     q = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-        if ((j * TPR + t) * VEC < D)
+    for (int j = 0; j < NV; j++) {
+        const int left = D - (j * TPR + t) * VEC;
+        if (left >= VEC) {
 #pragma unroll
             for (int i = 0; i < VEC; i++) q = fmaf(v[j][i] - mu, v[j][i] - mu, q);
+        } else if (left > 0) {
+#pragma unroll
+            for (int i = 0; i < VEC; i++)
+                if (i < left) q = fmaf(v[j][i] - mu, v[j][i] - mu, q);
+        }
+    }
     s = 0.0f;
     row_sums<TPR, 256>(q, s, 1);
     const float r = 1.0f / sqrtf(q / (float)D + p.eps);
@@ -102,29 +107,29 @@ __global__ __launch_bounds__(256) void ln_forward(LnArgs p) {
     for (int j = 0; j < NV; j++) {
         const int c = (j * TPR + t) * VEC;
         if (c >= D) continue;
-        float o[VEC], w[VEC];
+        float o[VEC], w[VEC] = {};
 #pragma unroll
         for (int i = 0; i < VEC; i++) o[i] = (v[j][i] - mu) * r;
         if (p.w) {
-            load_weight<VEC>(p.w, p.wf32, std::is_same_v<T, bf16>, c, w);
+            load_weight<T, VEC>(p.w, p.wf32, c, D, w);
 #pragma unroll
             for (int i = 0; i < VEC; i++) o[i] *= w[i];
         }
         if (p.b) {
-            load_weight<VEC>(p.b, p.wf32, std::is_same_v<T, bf16>, c, w);
+            load_weight<T, VEC>(p.b, p.wf32, c, D, w);
 #pragma unroll
             for (int i = 0; i < VEC; i++) o[i] += w[i];
         }
-        store<VEC>(y + c, o);
+        store_some<VEC>(y + c, D - c, o);
     }
 }
 
 // One workgroup takes every gridDim-th group of THREADS / TPR rows and keeps its
 // columns' sums of g h and g in registers; at the end its row groups are added through
 // LDS in order and go to the workgroup's own row of p.part, which reduce_columns adds up.
-template <class T, int VEC, int EPT, int TPR, int THREADS>
+template <class T, int EPT, int TPR, int THREADS>
 __global__ __launch_bounds__(THREADS) void ln_backward(LnArgs p) {
-    constexpr int NV = EPT / VEC, GROUPS = THREADS / TPR;
+    constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC, GROUPS = THREADS / TPR;
     const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR, D = p.cols;
     float w[NV][VEC], aw[NV][VEC], ab[NV][VEC];
 #pragma unroll
@@ -132,7 +137,7 @@ __global__ __launch_bounds__(THREADS) void ln_backward(LnArgs p) {
         const int c = (j * TPR + t) * VEC;
 #pragma unroll
         for (int i = 0; i < VEC; i++) w[j][i] = 1.0f, aw[j][i] = ab[j][i] = 0.0f;
-        if (p.w && c < D) load_weight<VEC>(p.w, p.wf32, std::is_same_v<T, bf16>, c, w[j]);
+        if (p.w && c < D) load_weight<T, VEC>(p.w, p.wf32, c, D, w[j]);
     }
     const float inv = 1.0f / (float)D;
     int slot = 0;
@@ -148,8 +153,8 @@ __global__ __launch_bounds__(THREADS) void ln_backward(LnArgs p) {
 #pragma unroll
             for (int i = 0; i < VEC; i++) h[j][i] = mu, g[j][i] = 0.0f;
             if (live && c < D) {
-                load<VEC>((const T*)p.x + row * p.xs + c, h[j]);
-                load<VEC>((const T*)p.g + row * p.gs + c, g[j]);
+                load_some<VEC>((const T*)p.x + row * p.xs + c, D - c, h[j]);
+                load_some<VEC>((const T*)p.g + row * p.gs + c, D - c, g[j]);
             }
         }
 #pragma unroll
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(THREADS) void ln_backward(LnArgs p) {
                 float o[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; i++) o[i] = r * (g[j][i] - sg - h[j][i] * sh);
-                if (c < D) store<VEC>(dx + c, o);
+                if (c < D) store_some<VEC>(dx + c, D - c, o);
             }
         }
     }
@@ -224,8 +229,8 @@ __global__ __launch_bounds__(WIDE) void ln_forward_wide(LnArgs p) {
     }
     for (int c = threadIdx.x; c < D; c += WIDE) {
         float o[1] = {((float)x[c] - mu) * r}, w[1];
-        if (p.w) load_weight<1>(p.w, p.wf32, std::is_same_v<T, bf16>, c, w), o[0] *= w[0];
-        if (p.b) load_weight<1>(p.b, p.wf32, std::is_same_v<T, bf16>, c, w), o[0] += w[0];
+        if (p.w) load_weight<T, 1>(p.w, p.wf32, c, D, w), o[0] *= w[0];
+        if (p.b) load_weight<T, 1>(p.b, p.wf32, c, D, w), o[0] += w[0];
         store<1>(y + c, o);
     }
 }
@@ -239,7 +244,7 @@ __global__ __launch_bounds__(WIDE) void ln_backward_wide(LnArgs p) {
     const float mu = p.mean[row], r = p.rstd[row];
     float sg = 0.0f, sh = 0.0f, w[1] = {1.0f};
     for (int c = threadIdx.x; c < D; c += WIDE) {
-        if (p.w) load_weight<1>(p.w, p.wf32, std::is_same_v<T, bf16>, c, w);
+        if (p.w) load_weight<T, 1>(p.w, p.wf32, c, D, w);
         const float gw = (float)g[c] * w[0];
         sg += gw;
         sh = fmaf(gw, ((float)x[c] - mu) * r, sh);
@@ -248,7 +253,7 @@ __global__ __launch_bounds__(WIDE) void ln_backward_wide(LnArgs p) {
     sg /= (float)D;
     sh /= (float)D;
     for (int c = threadIdx.x; c < D; c += WIDE) {
-        if (p.w) load_weight<1>(p.w, p.wf32, std::is_same_v<T, bf16>, c, w);
+        if (p.w) load_weight<T, 1>(p.w, p.wf32, c, D, w);
         ((T*)p.dx)[row * D + c] = (T)(r * ((float)g[c] * w[0] - sg - ((float)x[c] - mu) * r * sh));
     }
 }
@@ -280,14 +285,6 @@ void with_row(int64_t D, F&& f) {
     };
     if (D <= 2048) ept(integral_constant<int, 64>(), (D + 63) / 64);
     else ept(integral_constant<int, 256>(), (D + 255) / 256);
-}
-
-template <class T, class F>
-void with_vec(int vec, F&& f) {
-    using std::integral_constant;
-    if (vec == 1) f(integral_constant<int, 1>());
-    else if (sizeof(T) == 2 && vec == 2) f(integral_constant<int, 2>());
-    else f(integral_constant<int, 16 / (int)sizeof(T)>());
 }
 
 // Workgroups of the backward pass, each with a row of partial sums.
@@ -337,18 +334,15 @@ int drh_layer_norm(drh_ctx* ctx, const void* x, const void* weight, const void* 
     LnArgs p{};
     p.x = x, p.w = weight, p.b = bias, p.y = y, p.mean = mean, p.rstd = rstd;
     p.rows = rows, p.cols = (int)cols, p.xs = x_stride, p.eps = eps, p.wf32 = weight_dtype == DRH_F32;
-    const int vec = vector_width(dtype, {cols, rows > 1 ? x_stride : 0}, {x, y});
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
         if (cols > LN_MAX_COLS) {
             ln_forward_wide<T><<<dim3((unsigned)rows), WIDE, 0, s>>>(p);
             return DRH_OK;
         }
-        with_vec<T>(vec, [&](auto v) {
-            with_row(cols, [&](auto tpr, auto ept) {
-                constexpr int RPB = 256 / tpr.value;
-                ln_forward<T, v.value, ept.value, tpr.value><<<dim3((unsigned)((rows + RPB - 1) / RPB)), 256, 0, s>>>(p);
-            });
+        with_row(cols, [&](auto tpr, auto ept) {
+            constexpr int RPB = 256 / tpr.value;
+            ln_forward<T, ept.value, tpr.value><<<dim3((unsigned)((rows + RPB - 1) / RPB)), 256, 0, s>>>(p);
         });
         return DRH_OK;
     });
@@ -382,7 +376,6 @@ int drh_layer_norm_backward(drh_ctx* ctx, const void* x, const void* weight, con
     p.x = x, p.w = weight, p.g = grad_y, p.dx = grad_x, p.mean = (float*)mean, p.rstd = (float*)rstd;
     p.part = sums ? (float*)workspace : nullptr;
     p.rows = rows, p.cols = (int)cols, p.xs = x_stride, p.gs = grad_stride, p.wf32 = weight_dtype == DRH_F32;
-    const int vec = vector_width(dtype, {cols, rows > 1 ? x_stride : 0, rows > 1 ? grad_stride : 0}, {x, grad_y, grad_x});
     if (rows > 0 && (grad_x || sums))
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
@@ -392,11 +385,9 @@ int drh_layer_norm_backward(drh_ctx* ctx, const void* x, const void* weight, con
                     ln_columns_wide<T><<<dim3((unsigned)((cols + 63) / 64), (unsigned)groups), 64, 0, s>>>(p);
                 return DRH_OK;
             }
-            with_vec<T>(vec, [&](auto v) {
-                with_row(cols, [&](auto tpr, auto ept) {
-                    constexpr int THREADS = ln_threads(ept.value);
-                    ln_backward<T, v.value, ept.value, tpr.value, THREADS><<<dim3((unsigned)groups), THREADS, 0, s>>>(p);
-                });
+            with_row(cols, [&](auto tpr, auto ept) {
+                constexpr int THREADS = ln_threads(ept.value);
+                ln_backward<T, ept.value, tpr.value, THREADS><<<dim3((unsigned)groups), THREADS, 0, s>>>(p);
             });
             return DRH_OK;
         });

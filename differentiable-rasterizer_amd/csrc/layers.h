@@ -5,7 +5,6 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
-#include <initializer_list>
 #include <string>
 #include <type_traits>
 
@@ -20,28 +19,50 @@ using f16 = _Float16;
 template <class T, int N>
 using vec = T __attribute__((ext_vector_type(N)));
 
-// N elements at p, aligned to their whole size where N > 1.
+// The same vector at any address that suits one element: global memory takes 16 bytes a
+// lane from and to any of them, at no cost where the address is a multiple of 16.
+template <class T, int N>
+struct Anywhere {
+    typedef vec<T, N> type __attribute__((aligned(sizeof(T))));
+};
+
+// N elements at p.
 template <int N, class T>
 __device__ inline void load(const T* p, float (&out)[N]) {
-    if constexpr (N == 1) {
-        out[0] = (float)*p;
-    } else {
-        const vec<T, N> v = *reinterpret_cast<const vec<T, N>*>(p);
+    const vec<T, N> v = *reinterpret_cast<const typename Anywhere<T, N>::type*>(p);
 #pragma unroll
-        for (int i = 0; i < N; i++) out[i] = (float)v[i];
+    for (int i = 0; i < N; i++) out[i] = (float)v[i];
+}
+
+// The first `left` of N elements at p; the others keep their values.
+template <int N, class T>
+__device__ inline void load_some(const T* p, int64_t left, float (&out)[N]) {
+    if (left >= N) {
+        load<N>(p, out);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i < left) out[i] = (float)p[i];
     }
 }
 
 // Rounds to T once, to nearest even.
 template <int N, class T>
 __device__ inline void store(T* p, const float (&v)[N]) {
-    if constexpr (N == 1) {
-        *p = (T)v[0];
-    } else {
-        vec<T, N> r;
+    vec<T, N> r;
 #pragma unroll
-        for (int i = 0; i < N; i++) r[i] = (T)v[i];
-        *reinterpret_cast<vec<T, N>*>(p) = r;
+    for (int i = 0; i < N; i++) r[i] = (T)v[i];
+    *reinterpret_cast<typename Anywhere<T, N>::type*>(p) = r;
+}
+
+template <int N, class T>
+__device__ inline void store_some(T* p, int64_t left, const float (&v)[N]) {
+    if (left >= N) {
+        store<N>(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i < left) p[i] = (T)v[i];
     }
 }
 
@@ -62,20 +83,6 @@ int with_type(int dtype, F&& f) {
 inline size_t type_size(int dtype) { return dtype == DRH_F32 ? 4 : 2; }
 inline bool known_type(int dtype) { return dtype == DRH_F32 || dtype == DRH_BF16 || dtype == DRH_F16; }
 inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
-
-// The widest vector (16 bytes, then 4, then one element) that divides every one
-// of the strides and addresses given.
-inline int vector_width(int dtype, std::initializer_list<int64_t> strides, std::initializer_list<const void*> ptrs) {
-    const int size = (int)type_size(dtype);
-    for (int bytes : {16, 4}) {
-        if (bytes < size) break;
-        bool ok = true;
-        for (int64_t s : strides) ok = ok && s % (bytes / size) == 0;
-        for (const void* p : ptrs) ok = ok && (uintptr_t)p % bytes == 0;
-        if (ok) return bytes / size;
-    }
-    return 1;
-}
 
 // Checks that every layer call makes; the flags a layer knows are DRH_SYNC alone.
 int check_call(drh_ctx* ctx, int dtype, uint32_t flags);

@@ -4,10 +4,10 @@
 //   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz,  dresidual = dy
 //
 // Products run on the matrix cores with 32-bit sums. Each result is rounded to its type
-// once, from 32 bits. What the backward pass needs of z is kept in 16 bits for the 16-bit
-// types, in float16 whatever the type is: its 11 bits keep act'(z) four times nearer than
-// bfloat16's 8 would, and act' has its limit long before float16 ends, so larger values
-// are kept as its largest.
+// once, from 32 bits. The backward pass needs act'(z) alone, so the forward pass, which has
+// act's exponential at hand, keeps that and not z: in 16 bits beside the 16-bit types, in
+// float16 whatever the type is, since slopes are within [-0.13, 1.13] and its 11 bits keep
+// them eight times nearer than bfloat16's 8 would.
 
 #include "gemm.h"
 
@@ -18,21 +18,15 @@ namespace {
 
 // ---------------------------------------------------------------- activations
 
-// erf for values that are rounded to 16 bits afterwards: Abramowitz and Stegun 7.1.26,
-// within 1.5e-7. Results in 32 bits take the library's.
-template <bool EXACT>
-__device__ inline float erf_of(float x) {
-    if constexpr (EXACT) return erff(x);
-    const float a = fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.0f));
-    float s = fmaf(t, 1.061405429f, -1.453152027f);
-    s = fmaf(t, s, 1.421413741f);
-    s = fmaf(t, s, -0.284496736f);
-    s = fmaf(t, s, 0.254829592f) * t;
-    return copysignf(1.0f - s * __expf(-a * a), x);
-}
-
 constexpr float SQRT_HALF = 0.70710678118654752f, INV_SQRT_2PI = 0.39894228040143268f;
 constexpr float TANH_C = 0.79788456080286536f, TANH_A = 0.044715f;
+
+// EXACT: for results in 32 bits, with the library's functions; else for values that are
+// rounded to 16 bits afterwards.
+template <bool EXACT>
+__device__ inline float exp_of(float x) {
+    return EXACT ? expf(x) : __expf(x);
+}
 
 // 1 / (1 + exp(-v))
 template <bool EXACT>
@@ -40,55 +34,53 @@ __device__ inline float logistic(float v) {
     return EXACT ? 1.0f / (1.0f + expf(-v)) : __builtin_amdgcn_rcpf(1.0f + __expf(-v));
 }
 
-// Far below zero every smooth activation is zero in 32 bits; the bound keeps infinity
-// times zero out of the product there. NaN passes.
-__device__ inline float not_below(float z, float lo) { return z < lo ? lo : z; }
+__device__ inline float not_below(float z, float lo) { return z < lo ? lo : z; }  // NaN passes
 __device__ inline float not_above(float z, float hi) { return z > hi ? hi : z; }
 
-template <bool EXACT>
-__device__ inline float act(int kind, float z) {
-    switch (kind) {
-        case DRH_ACT_RELU: return z < 0.0f ? 0.0f : z;
-        case DRH_ACT_SILU: z = not_below(z, -200.0f); return z * logistic<EXACT>(z);
-        case DRH_ACT_GELU: z = not_below(z, -64.0f); return 0.5f * z * (1.0f + erf_of<EXACT>(z * SQRT_HALF));
-        case DRH_ACT_GELU_TANH: {
-            z = not_below(z, -64.0f);
-            const float c = not_above(z, 64.0f);  // (1 + tanh u) / 2 = logistic(2 u)
-            return z * logistic<EXACT>(2.0f * TANH_C * fmaf(TANH_A * c * c, c, c));
+// act(z), and act'(z) in `slope`. Below -128 every value and slope is 0 in 32 bits, above 64
+// every value z and slope 1; the bounds keep infinity times zero out of the products there.
+template <bool EXACT, int ACT>
+__device__ inline float act(float z, float& slope) {
+    if constexpr (ACT == DRH_ACT_NONE) {
+        slope = 1.0f;
+        return z;
+    } else if constexpr (ACT == DRH_ACT_RELU) {
+        slope = z > 0.0f ? 1.0f : 0.0f;
+        return z < 0.0f ? 0.0f : z;
+    } else {
+        z = not_below(z, -128.0f);
+        const float c = not_above(z, 64.0f);
+        if constexpr (ACT == DRH_ACT_SILU) {
+            const float s = logistic<EXACT>(c);
+            slope = s * fmaf(c, 1.0f - s, 1.0f);
+            return z * s;
+        } else if constexpr (ACT == DRH_ACT_GELU_TANH) {
+            const float u = TANH_A * c * c, s = logistic<EXACT>(2.0f * TANH_C * fmaf(u, c, c));  // (1 + tanh) / 2
+            slope = fmaf(2.0f * TANH_C * c * s * (1.0f - s), fmaf(3.0f, u, 1.0f), s);
+            return z * s;
+        } else {
+            const float x = c * SQRT_HALF, e = exp_of<EXACT>(-x * x);
+            float erf;
+            if constexpr (EXACT) {
+                erf = erff(x);
+            } else {  // Abramowitz and Stegun 7.1.26, within 1.5e-7
+                const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, fabsf(x), 1.0f));
+                float q = fmaf(t, 1.061405429f, -1.453152027f);
+                q = fmaf(t, q, 1.421413741f);
+                q = fmaf(t, q, -0.284496736f);
+                q = fmaf(t, q, 0.254829592f);
+                erf = copysignf(fmaf(-q * t, e, 1.0f), x);
+            }
+            const float phi = fmaf(0.5f, erf, 0.5f);
+            slope = fmaf(c * INV_SQRT_2PI, e, phi);
+            return z * phi;
         }
-        default: return z;
     }
 }
 
-template <bool EXACT>
-__device__ inline float act_slope(int kind, float z) {
-    if (kind == DRH_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    if (kind == DRH_ACT_NONE) return 1.0f;
-    z = not_above(not_below(z, -64.0f), 64.0f);
-    if (kind == DRH_ACT_SILU) {
-        const float s = logistic<EXACT>(z);
-        return s * (1.0f + z * (1.0f - s));
-    }
-    if (kind == DRH_ACT_GELU)
-        return 0.5f * (1.0f + erf_of<EXACT>(z * SQRT_HALF)) + z * INV_SQRT_2PI * (EXACT ? expf(-0.5f * z * z) : __expf(-0.5f * z * z));
-    const float s = logistic<EXACT>(2.0f * TANH_C * fmaf(TANH_A * z * z, z, z));
-    return s + 2.0f * TANH_C * z * s * (1.0f - s) * (1.0f + 3.0f * TANH_A * z * z);
-}
-
-// The type that z is kept in, and its value there: in float16 clamped to the range, and a
-// value above zero never becomes zero, where relu's slope turns.
+// The type that slopes are kept in.
 template <class T>
 using Kept = std::conditional_t<sizeof(T) == 4, float, f16>;
-
-template <class T>
-__device__ inline Kept<T> keep(float z) {
-    if constexpr (sizeof(T) == 4) {
-        return z;
-    } else {
-        const f16 h = (f16)not_above(not_below(z, -65504.0f), 65504.0f);
-        return (z > 0.0f && h == (f16)0.0f) ? (f16)5.9604645e-8f : h;
-    }
-}
 
 // ---------------------------------------------------------------- the product's epilogue
 
@@ -96,15 +88,18 @@ __device__ inline Kept<T> keep(float z) {
 // share them.
 template <class T, int ACT, int NV>
 struct Epilogue {
-    static constexpr bool EXACT = sizeof(T) == 4;
-    static constexpr int CH = 16 / sizeof(T), W = 4 * NV;
+    static constexpr int W = 4 * NV, CH = 16 / sizeof(T) < W ? 16 / sizeof(T) : W;
     int64_t n = 0;
     float bias[W];
 
     __device__ void columns(const Gemm& p, int64_t n_) {
         n = n_;
 #pragma unroll
-        for (int i = 0; i < W; i++) bias[i] = p.bias && !p.partial && n + i < p.N ? (float)((const T*)p.bias)[n + i] : 0.0f;
+        for (int i = 0; i < W; i++) bias[i] = 0.0f;
+        if (p.bias && !p.partial)
+#pragma unroll
+            for (int i = 0; i < W; i++)
+                if (n + i < p.N) bias[i] = (float)((const T*)p.bias)[n + i];
     }
 
     __device__ void row(const Gemm& p, int64_t m, const floatx4 (&v)[NV]) const {
@@ -113,56 +108,38 @@ struct Epilogue {
         if (p.partial) {
             float* out = p.partial + (int64_t)blockIdx.y * p.M * p.N + at;
 #pragma unroll
-            for (int j = 0; j < NV; j++)
-                if (p.wide_out && n + 4 * j < p.N) {
-                    *(floatx4*)(out + 4 * j) = v[j];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (n + 4 * j + i < p.N) out[4 * j + i] = v[j][i];
-                }
+            for (int j = 0; j < NV; j++) {
+                const float o[4] = {v[j][0], v[j][1], v[j][2], v[j][3]};
+                if (n + 4 * j < p.N) store_some<4>(out + 4 * j, p.N - n - 4 * j, o);
+            }
             return;
         }
-        if (W % CH == 0 && p.wide_out) {
 #pragma unroll
-            for (int g = 0; g + CH <= W; g += CH)
-                if (n + g < p.N) group<CH>(p, at + g, v, g);
-        } else {
+        for (int g = 0; g < W; g += CH) {
+            if (n + g >= p.N) break;
+            float o[CH];
 #pragma unroll
-            for (int g = 0; g < W; g++)
-                if (n + g < p.N) group<1>(p, at + g, v, g);
+            for (int i = 0; i < CH; i++) o[i] = v[(g + i) / 4][(g + i) % 4] + bias[g + i];
+            apply<CH>(p, at + g, p.N - n - g, o);
         }
     }
 
+    // From z on: activates, keeps the slope, adds the residual, stores the first `left`.
     template <int C>
-    __device__ void group(const Gemm& p, int64_t at, const floatx4 (&v)[NV], int g) const {
-        float o[C];
+    static __device__ void apply(const Gemm& p, int64_t at, int64_t left, float (&o)[C]) {
+        if constexpr (ACT != DRH_ACT_NONE) {
+            float slope[C];
 #pragma unroll
-        for (int i = 0; i < C; i++) o[i] = v[(g + i) / 4][(g + i) % 4] + bias[g + i];
-        apply<C>(p, at, o);
-    }
-
-    // From z on: keeps it, activates, adds the residual, stores.
-    template <int C>
-    static __device__ void apply(const Gemm& p, int64_t at, float (&o)[C]) {
-        if (ACT != DRH_ACT_NONE) {
-            if (p.kept) {
-                Kept<T>* kept = (Kept<T>*)p.kept + at;
-                vec<Kept<T>, C> k;
-#pragma unroll
-                for (int i = 0; i < C; i++) k[i] = keep<T>(o[i]);
-                *(vec<Kept<T>, C>*)kept = k;
-            }
-#pragma unroll
-            for (int i = 0; i < C; i++) o[i] = act<EXACT>(ACT, o[i]);
+            for (int i = 0; i < C; i++) o[i] = act<sizeof(T) == 4, ACT>(o[i], slope[i]);
+            if (p.kept) store_some<C>((Kept<T>*)p.kept + at, left, slope);
         }
         if (p.res) {
-            float r[C];
-            load<C>((const T*)p.res + at, r);
+            float r[C] = {};
+            load_some<C>((const T*)p.res + at, left, r);
 #pragma unroll
             for (int i = 0; i < C; i++) o[i] += r[i];
         }
-        store<C>((T*)p.out + at, o);
+        store_some<C>((T*)p.out + at, left, o);
     }
 };
 
@@ -178,35 +155,95 @@ __global__ __launch_bounds__(256, 2) void gemm_128_kernel(Gemm p) {
     gemm_128<T, AK, BK, Epilogue<T, ACT, 4>>(p);
 }
 
-// The parts of a split product added in order, and the epilogue.
-template <class T, int ACT, int VEC>
+// The parts of a split product added in order, and the epilogue: a thread a 16-byte chunk of
+// a row of the output.
+template <class T, int ACT>
 __global__ __launch_bounds__(256) void join_splits(Gemm p) {
-    const int64_t n_all = p.M * p.N;
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
-    if (at >= n_all) return;
-    float o[VEC] = {};
+    constexpr int CH = 16 / sizeof(T);
+    const uint32_t per = (uint32_t)((p.N + CH - 1) / CH), id = blockIdx.x * 256 + threadIdx.x;
+    const int64_t m = id / per, n = (int64_t)(id % per) * CH, at = m * p.N + n, left = p.N - n;
+    if (m >= p.M) return;
+    float o[CH] = {};
+    const int64_t size = p.M * p.N;
     for (int s = 0; s < p.splits; s++) {
-        float v[VEC];
-        const float* part = p.partial + s * n_all + at;
+        float v[CH] = {};
+        load_some<CH>(p.partial + s * size + at, left, v);
 #pragma unroll
-        for (int i = 0; i < VEC; i += VEC < 4 ? VEC : 4) {
-            float4 q;
-            if constexpr (VEC >= 4) {
-                q = *(const float4*)(part + i);
-                v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
-            } else {
-                v[i] = part[i];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < VEC; i++) o[i] += v[i];
+        for (int i = 0; i < CH; i++) o[i] += v[i];
     }
     if (p.bias) {
-        const int64_t n = at % p.N;
+        float b[CH] = {};
+        load_some<CH>((const T*)p.bias + n, left, b);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) o[i] += (float)((const T*)p.bias)[n + i];
+        for (int i = 0; i < CH; i++) o[i] += b[i];
     }
-    Epilogue<T, ACT, 2>::template apply<VEC>(p, at, o);
+    Epilogue<T, ACT, 2>::template apply<CH>(p, at, left, o);
+}
+
+// Few rows of x (up to 16 MT): the weights are read once and that is what it costs, so
+// nothing is staged. A workgroup takes 16 outputs; its eight waves take an eighth of k each,
+// straight from memory to the matrix cores (a lane 16 bytes of row l % 16, four lanes 64
+// contiguous bytes), and are added through LDS in order. Rows may start anywhere.
+template <class T, int MT, int ACT>
+__global__ __launch_bounds__(512) void gemm_rows_kernel(Gemm p) {
+    constexpr int CH = 16 / sizeof(T), WAVES = 8;
+    using F = vec<T, CH>;
+    using FU = typename Anywhere<T, CH>::type;
+    __shared__ __align__(16) floatx4 part[WAVES][MT][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16, K = p.K;
+    const int steps = (int)((K + 4 * CH - 1) / (4 * CH)), s0 = (int)((int64_t)steps * w / WAVES),
+              s1 = (int)((int64_t)steps * (w + 1) / WAVES);
+    // rows past the end read the last one's values and are not stored
+    const T* bp = (const T*)p.b.ptr + (n0 + r < p.N ? n0 + r : p.N - 1) * p.b.ld;
+    const T* ap[MT];
+#pragma unroll
+    for (int t = 0; t < MT; t++) ap[t] = (const T*)p.a.ptr + (16 * t + r < p.M ? 16 * t + r : p.M - 1) * p.a.ld;
+    floatx4 acc[MT] = {};
+    // eight (four with more rows) steps' loads at once: a wave has little else to wait with
+    constexpr int AT_ONCE = MT == 1 ? 8 : 4;
+    const int whole = (int)(K / (4 * CH)) < s1 ? (int)(K / (4 * CH)) : s1;
+    int s = s0;
+    for (; s + AT_ONCE <= whole; s += AT_ONCE) {
+        F b[AT_ONCE], a[AT_ONCE][MT];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) {
+            const int64_t k = ((int64_t)(s + u) * 4 + q) * CH;
+            b[u] = *(const FU*)(bp + k);
+#pragma unroll
+            for (int t = 0; t < MT; t++) a[u][t] = *(const FU*)(ap[t] + k);
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++)
+#pragma unroll
+            for (int t = 0; t < MT; t++) acc[t] = mma(b[u], a[u][t], acc[t]);
+    }
+    auto chunk = [&](const T* row, int64_t k) {
+        F v;
+        if (k + CH <= K) {
+            v = *(const FU*)(row + k);
+        } else {
+#pragma unroll
+            for (int i = 0; i < CH; i++) v[i] = k + i < K ? row[k + i] : (T)0.0f;
+        }
+        return v;
+    };
+    for (; s < s1; s++) {
+        const int64_t k = ((int64_t)s * 4 + q) * CH;
+        const F b = chunk(bp, k);
+#pragma unroll
+        for (int t = 0; t < MT; t++) acc[t] = mma(b, chunk(ap[t], k), acc[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; t++) part[w][t][lane] = acc[t];
+    __syncthreads();
+    if (w >= MT) return;
+    floatx4 v[1] = {part[0][w][lane]};
+#pragma unroll
+    for (int i = 1; i < WAVES; i++) v[0] += part[i][w][lane];
+    Epilogue<T, ACT, 1> e;
+    e.columns(p, n0 + 4 * q);
+    e.row(p, 16 * w + r, v);
 }
 
 // Any strides and sizes: 64 x 64 of the output a workgroup, a quarter each of its four
@@ -262,11 +299,13 @@ enum Layout { KK, KN, MN };  // A's and B's contiguous dimension: forward, dx, d
 
 struct GemmPlan {
     int tile = 0;    // 256, 128, or 0: any
+    bool rows = false;  // gemm_rows_kernel
     int splits = 1;
     size_t bytes = 0;  // of partial sums
 };
 
 constexpr int CUS = 256;
+constexpr int64_t ROWS_MOST = 64;  // gemm_rows_kernel
 
 // Whether an operand's sizes suit the kernels that load 16-byte chunks through buffers.
 bool chunked(int dtype, bool kc, int64_t ld, int64_t rows, int64_t K) {
@@ -317,7 +356,6 @@ int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial,
     if (p.M == 0 || p.N == 0) return DRH_OK;
     const int64_t ch = 16 / (int64_t)type_size(dtype);
     auto aligned = [](const void* q) { return (uintptr_t)q % 16 == 0; };
-    p.wide_out = p.N % ch == 0 && aligned(p.out) && aligned(p.res) && aligned(p.kept);
     const bool fast = plan.tile && aligned(p.a.ptr) && aligned(p.b.ptr);
     const int tile = fast ? plan.tile : 64;
     const int64_t tiles = (p.M + tile - 1) / tile * ((p.N + tile - 1) / tile);
@@ -329,13 +367,19 @@ int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial,
     const dim3 grid((unsigned)tiles, (unsigned)p.splits);
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        if (!fast) {
-            p.wide_out = false;  // a lane has four neighbouring outputs there
+        if (plan.rows)
+            return with_act(p.act, [&](auto a) {
+                const dim3 groups((unsigned)((p.N + 15) / 16));
+                if (p.M <= 16) gemm_rows_kernel<T, 1, a.value><<<groups, 512, 0, s>>>(p);
+                else if (p.M <= 32) gemm_rows_kernel<T, 2, a.value><<<groups, 512, 0, s>>>(p);
+                else gemm_rows_kernel<T, 4, a.value><<<groups, 512, 0, s>>>(p);
+                return DRH_OK;
+            });
+        if (!fast)
             return with_act(p.act, [&](auto a) {
                 gemm_any_kernel<T, a.value><<<grid, 256, 0, s>>>(p, layout != MN, layout == KK);
                 return DRH_OK;
             });
-        }
         auto go = [&](auto a) {
             constexpr int ACT = a.value;
             if (layout == KK) {
@@ -355,10 +399,8 @@ int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial,
         if (!p.partial) return with_act(p.act, go);
         go(std::integral_constant<int, DRH_ACT_NONE>());
         return with_act(p.act, [&](auto a) {
-            const int64_t n = p.M * p.N;
-            constexpr int V = 16 / sizeof(T);
-            if (p.wide_out) join_splits<T, a.value, V><<<dim3((unsigned)((n / V + 255) / 256)), 256, 0, s>>>(p);
-            else join_splits<T, a.value, 1><<<dim3((unsigned)((n + 255) / 256)), 256, 0, s>>>(p);
+            const int64_t chunks = p.M * ((p.N + ch - 1) / ch);
+            join_splits<T, a.value><<<dim3((unsigned)((chunks + 255) / 256)), 256, 0, s>>>(p);
             return DRH_OK;
         });
     });
@@ -406,41 +448,36 @@ const void* place_rows(int dtype, const Rows& r, const void* src, int64_t ld, in
 // ---------------------------------------------------------------- dz and the bias gradient
 
 // dz = dy act'(z), rounded to its type for the products, in rows of ldz elements with zeros
-// behind N, and the column sums of the unrounded values: a workgroup owns 64 VEC columns of
-// every gridDim.y-th slab of rows, its four waves a row each, added in order at the end.
-template <class T, int VEC>
-__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const Kept<T>* __restrict__ z, int kind,
-                                                    int64_t M, int64_t N, int64_t ldz, T* __restrict__ dz, float* part) {
-    constexpr bool EXACT = sizeof(T) == 4;
+// behind N, and the column sums of the unrounded values: a workgroup owns 64 chunks of every
+// gridDim.y-th slab of rows, its four waves a row each, added in order at the end.
+template <class T>
+__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const Kept<T>* __restrict__ slope, int64_t M,
+                                                    int64_t N, int64_t ldz, T* __restrict__ dz, float* part) {
+    constexpr int CH = 16 / sizeof(T);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * VEC;
-    float sum[VEC] = {};
-    if (c < N) {
+    const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * CH;
+    float sum[CH] = {};
+    if (c < N)
         for (int64_t row = (int64_t)blockIdx.y * 4 + w; row < M; row += (int64_t)gridDim.y * 4) {
-            float g[VEC];
-            load<VEC>(dy + row * N + c, g);
-            if (z) {
-                float zz[VEC];
-                load<VEC>(z + row * N + c, zz);
+            float g[CH] = {};
+            load_some<CH>(dy + row * N + c, N - c, g);
+            if (slope) {
+                float d[CH] = {};
+                load_some<CH>(slope + row * N + c, N - c, d);
 #pragma unroll
-                for (int i = 0; i < VEC; i++) g[i] *= act_slope<EXACT>(kind, zz[i]);
+                for (int i = 0; i < CH; i++) g[i] *= d[i];
             }
-            if (dz) store<VEC>(dz + row * ldz + c, g);
+            if (dz) store<CH>(dz + row * ldz + c, g);  // ldz is whole chunks
 #pragma unroll
-            for (int i = 0; i < VEC; i++) sum[i] += g[i];
+            for (int i = 0; i < CH; i++) sum[i] += g[i];
         }
-    } else if (dz && c < ldz) {
-        const float zero[VEC] = {};
-        for (int64_t row = (int64_t)blockIdx.y * 4 + w; row < M; row += (int64_t)gridDim.y * 4)
-            store<VEC>(dz + row * ldz + c, zero);
-    }
     if (!part) return;
-    __shared__ float sums[4][64 * VEC];
+    __shared__ float sums[4][64 * CH];
 #pragma unroll
-    for (int i = 0; i < VEC; i++) sums[w][lane * VEC + i] = sum[i];
+    for (int i = 0; i < CH; i++) sums[w][lane * CH + i] = sum[i];
     __syncthreads();
-    for (int k = threadIdx.x; k < 64 * VEC; k += 256) {
-        const int64_t col = (int64_t)blockIdx.x * 64 * VEC + k;
+    for (int k = threadIdx.x; k < 64 * CH; k += 256) {
+        const int64_t col = (int64_t)blockIdx.x * 64 * CH + k;
         if (col < N) part[(int64_t)blockIdx.y * N + col] = sums[0][k] + sums[1][k] + sums[2][k] + sums[3][k];
     }
 }
@@ -458,6 +495,10 @@ struct ForwardPlan {
 
 ForwardPlan forward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype) {
     ForwardPlan f;
+    if (M <= ROWS_MOST && K > 0) {
+        f.x = {xs}, f.w = {ws}, f.y.rows = true;
+        return f;
+    }
     f.x = rows_for(dtype, M, K, xs);
     f.w = rows_for(dtype, N, K, ws);
     const int64_t ch = 16 / (int64_t)type_size(dtype), K_pad = (K + ch - 1) / ch * ch;
@@ -592,16 +633,9 @@ int drh_linear_backward(drh_ctx* ctx, const void* x, const void* weight, const v
     if (M > 0 && (dz_made || grad_bias))
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
-            auto go = [&](auto v) {
-                const int64_t cols = 64 * v.value;
-                slope_kernel<T, v.value><<<dim3((unsigned)((ldz + cols - 1) / cols), (unsigned)groups), 256, 0, s>>>(
-                    (const T*)grad_y, slope ? (const Kept<T>*)kept : nullptr, activation, M, N, ldz,
-                    dz_made ? (T*)dz : nullptr, sums);
-            };
-            const int vec = vector_width(dtype, {N}, {grad_y, kept});
-            if (vec == 1) go(std::integral_constant<int, 1>());
-            else if (sizeof(T) == 2 && vec == 2) go(std::integral_constant<int, 2>());
-            else go(std::integral_constant<int, 16 / (int)sizeof(T)>());
+            const int64_t cols = 64 * (16 / (int64_t)sizeof(T));
+            slope_kernel<T><<<dim3((unsigned)((N + cols - 1) / cols), (unsigned)groups), 256, 0, s>>>(
+                (const T*)grad_y, slope ? (const Kept<T>*)kept : nullptr, M, N, ldz, dz_made ? (T*)dz : nullptr, sums);
             return DRH_OK;
         });
     if (grad_bias) reduce_columns(sums, M > 0 ? groups : 0, N, N, grad_bias, nullptr, dtype, s);

@@ -50,7 +50,7 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: st
         activation: None, "relu", "gelu" (z Phi(z)), "gelu_tanh" or "silu".
         residual: `(..., N)` or None, added after the activation.
 
-    The backward pass rounds dz = dy act'(z) to x's type for its two products, and keeps z
+    The backward pass rounds dz = dy act'(z) to x's type for its two products; act'(z) is kept
     for it in float16 beside 16-bit types (in float32 otherwise), where there is an activation.
     """
     act = ACTIVATIONS.get(activation)

@@ -78,12 +78,13 @@ def linear(x, w, b, kind, res, g, check_fwd=None):
     if kind is None:
         dz, edz = G, torch.zeros_like(G)
     else:
-        # z is kept in 32 bits, or in float16's 11; no slope changes faster than 1.13 per unit
-        kept = (2.0**-24 if dt == torch.float32 else 2.0**-11) * z.abs() + 2.0**-25
-        ds = 1.13 * (ez + kept) + es
+        # no slope changes faster than 1.13 per unit of z; it is kept in 32 bits, or in float16
+        d = slope(kind, z)
+        ds = 1.13 * ez + es
+        ds = ds + (E if dt == torch.float32 else 2.0**-11) * (d.abs() + ds) + 2.0**-25
         if kind == "relu":  # its slope turns at zero alone
             ds = torch.where(z.abs() <= ez, torch.ones_like(z), torch.zeros_like(z))
-        dz = G * slope(kind, z)
+        dz = G * d
         edz = G.abs() * ds + E * dz.abs()
     # dz is rounded to its type for the products, not for the bias gradient
     er = edz + (U[dt] * (dz.abs() + edz) + TINY[dt] if kind is not None else 0.0)
