@@ -208,15 +208,80 @@ struct Frags {
     }
 };
 
-template <class T, bool AK, bool BK_, int NA, int NB>
-__device__ inline void multiply(const Frags<T, AK, false, NA>& a, const Frags<T, BK_, true, NB>& b, floatx4 (&acc)[NA][NB]) {
+// How a k tile's fragments are multiplied.
+//
+// Straight: with the instructions of the operands' own type.
+//
+// Thirds, for 32 bits: v = v1 + v2 + v3 in bfloat16, each the nearest to what is left, is
+// exact (3 x 8 bits; signs fill the gaps), and a b is a1 b1 + a1 b2 + a2 b1 + a2 b2 + a1 b3 +
+// a3 b1 to within 2^-23 |a b|, of either sign. Six bfloat16 products take 96 cycles of the
+// matrix core where the 32-bit instructions take 256, and splitting costs 5.5 vector
+// operations an element, which the other wave of the SIMD hides. Values past bfloat16's
+// range and infinities come out as NaN: see gemm_128's second pass.
+struct Straight {
+    template <class F, int NF>
+    using Held = F;
+    template <class F>
+    static __device__ inline void hold(F& to, const F& from) {
+        to = from;
+    }
+    template <class FA, class FB, int NA, int NB>
+    static __device__ inline void multiply(const FA& a, const FB& b, floatx4 (&acc)[NA][NB]) {
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int i = 0; i < NA; i++)
+            for (int i = 0; i < NA; i++)
 #pragma unroll
-            for (int j = 0; j < NB; j++) acc[i][j] = mma(b.f[j][h], a.f[i][h], acc[i][j]);
-}
+                for (int j = 0; j < NB; j++) acc[i][j] = mma(b.f[j][h], a.f[i][h], acc[i][j]);
+    }
+};
+
+struct Thirds {
+    template <class F, int NF>
+    struct Held {
+        vec<bf16, 8> f[3][NF];
+    };
+    template <class H, class F>
+    static __device__ inline void hold(H& to, const F& from) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(from.f) / sizeof(from.f[0])); i++) {
+            split(from.f[i], to.f[0][i], to.f[1][i], to.f[2][i]);
+        }
+    }
+    // Pairs are converted by one instruction; their values come back by a shift and a mask.
+    static __device__ inline void split(const vec<float, 4> (&v)[2], vec<bf16, 8>& t0, vec<bf16, 8>& t1, vec<bf16, 8>& t2) {
+        using F2 = vec<float, 2>;
+        using B2 = vec<bf16, 2>;
+        vec<uint32_t, 4> o[3];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            F2 r = {v[i / 2][2 * (i % 2)], v[i / 2][2 * (i % 2) + 1]};
+#pragma unroll
+            for (int third = 0; third < 3; third++) {
+                const uint32_t pair = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, B2));
+                o[third][i] = pair;
+                if (third < 2) {
+                    r[0] -= __builtin_bit_cast(float, pair << 16);
+                    r[1] -= __builtin_bit_cast(float, pair & 0xffff0000u);
+                }
+            }
+        }
+        t0 = __builtin_bit_cast(vec<bf16, 8>, o[0]);
+        t1 = __builtin_bit_cast(vec<bf16, 8>, o[1]);
+        t2 = __builtin_bit_cast(vec<bf16, 8>, o[2]);
+    }
+    template <class HA, class HB, int NA, int NB>
+    static __device__ inline void multiply(const HA& a, const HB& b, floatx4 (&acc)[NA][NB]) {
+        // the smallest terms first
+        constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+        for (int t = 0; t < 6; t++)
+#pragma unroll
+            for (int i = 0; i < NA; i++)
+#pragma unroll
+                for (int j = 0; j < NB; j++) acc[i][j] = mma(b.f[PB[t]][j], a.f[PA[t]][i], acc[i][j]);
+    }
+};
 
 // The tile that a workgroup takes. Workgroups go to the eight XCDs in turn and each XCD
 // has an L2 of its own: an XCD gets a run of neighbouring tiles, in bands eight tiles high.
@@ -263,7 +328,6 @@ __device__ inline void gemm_256(const Gemm& p) {
     floatx4 acc[2][2][4][2] = {};
     Frags<T, AK, false, 4> fa;
     Frags<T, BK_, true, 2> fb[2];
-
     load_b(0, first);
     load_a(0, first);
     load_b(1, first);
@@ -281,7 +345,7 @@ __device__ inline void gemm_256(const Gemm& p) {
         __builtin_amdgcn_sched_barrier(0);
         wg_barrier();
         __builtin_amdgcn_s_setprio(1);
-        multiply<T, AK, BK_, 4, 2>(fa, fb[ub], acc[ua][ub]);
+        Straight::multiply(fa, fb[ub], acc[ua][ub]);
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
         wg_barrier();
@@ -319,7 +383,7 @@ __device__ inline void gemm_256(const Gemm& p) {
 
 // 128 x 128 by four waves, 64 x 64 each, two k tiles in LDS (64 KiB): two workgroups a CU,
 // each covering the other's waits.
-template <class T, bool AK, bool BK_, class Epilogue>
+template <class T, bool AK, bool BK_, class Epilogue, class Math>
 __device__ inline void gemm_128(const Gemm& p) {
     __shared__ __align__(1024) char lds[4 * UNIT_BYTES];
     using LA = Loader<T, AK, false, 1, 4, 4>;
@@ -340,20 +404,42 @@ __device__ inline void gemm_128(const Gemm& p) {
         la.issue(0, kt, lds0 + b);
         lb.issue(0, kt, lds0 + b + UNIT_BYTES);
     };
-    floatx4 acc[4][4] = {};
-    load(first);
-    for (int64_t kt = first; kt < last; kt++) {
-        const char* b = lds + ((kt - first) & 1) * 2 * UNIT_BYTES;
+    floatx4 acc[4][4];
+    auto product = [&](auto math) {
+        using How = decltype(math);
+        using FA = Frags<T, AK, false, 4>;
+        using FB = Frags<T, BK_, true, 4>;
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[i >> 2][i & 3] = floatx4{};
+        load(first);
+        for (int64_t kt = first; kt < last; kt++) {
+            const char* b = lds + ((kt - first) & 1) * 2 * UNIT_BYTES;
+            wait_vm<0>();
+            wg_barrier();  // this tile is there, and the other buffer read by every wave
+            load(kt + 1);
+            FA ra;
+            FB rb;
+            ra.read(b, wm * 64);
+            rb.read(b + UNIT_BYTES, wn * 64);
+            typename How::template Held<FA, 4> fa;
+            typename How::template Held<FB, 4> fb;
+            How::hold(fa, ra);
+            How::hold(fb, rb);
+            How::multiply(fa, fb, acc);
+        }
         wait_vm<0>();
-        wg_barrier();  // this tile is there, and the other buffer read by every wave
-        load(kt + 1);
-        Frags<T, AK, false, 4> fa;
-        Frags<T, BK_, true, 4> fb;
-        fa.read(b, wm * 64);
-        fb.read(b + UNIT_BYTES, wn * 64);
-        multiply<T, AK, BK_, 4, 4>(fa, fb, acc);
+    };
+    product(Math());
+    if constexpr (std::is_same_v<Math, Thirds>) {
+        // A result that is not finite comes from an infinity, a NaN or an overflow. The thirds turn
+        // the first and the last into NaN, so the tile is made again with instructions that do not.
+        float zero = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) zero = fmaf(acc[i >> 2][i & 3][e], 0.0f, zero);
+        if (__syncthreads_or(!(zero == 0.0f))) product(Straight());
     }
-    wait_vm<0>();
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     Epilogue epilogue;
     epilogue.columns(p, n0 + wn * 64 + q * 16);

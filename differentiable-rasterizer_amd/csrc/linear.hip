@@ -9,6 +9,9 @@
 // float16 whatever the type is, since slopes are within [-0.13, 1.13] and its 11 bits keep
 // them eight times nearer than bfloat16's 8 would.
 
+#include <algorithm>
+#include <cmath>
+
 #include "gemm.h"
 
 using namespace drh_rt;
@@ -150,9 +153,9 @@ __global__ __launch_bounds__(512, 2) void gemm_256_kernel(Gemm p) {
     gemm_256<T, AK, BK, Epilogue<T, ACT, 2>>(p);
 }
 
-template <class T, bool AK, bool BK, int ACT>
+template <class T, bool AK, bool BK, int ACT, class Math>
 __global__ __launch_bounds__(256, 2) void gemm_128_kernel(Gemm p) {
-    gemm_128<T, AK, BK, Epilogue<T, ACT, 4>>(p);
+    gemm_128<T, AK, BK, Epilogue<T, ACT, 4>, Math>(p);
 }
 
 // The parts of a split product added in order, and the epilogue: a thread a 16-byte chunk of
@@ -306,6 +309,9 @@ struct GemmPlan {
 
 constexpr int CUS = 256;
 constexpr int64_t ROWS_MOST = 64;  // gemm_rows_kernel
+// Products in 32 bits are split in thirds from this k on: their error, 2^-23 of a term, is
+// then below that of the sum, and shorter products are bound by memory either way.
+constexpr int64_t THIRDS_LEAST = 64;
 
 // Whether an operand's sizes suit the kernels that load 16-byte chunks through buffers.
 bool chunked(int dtype, bool kc, int64_t ld, int64_t rows, int64_t K) {
@@ -314,25 +320,40 @@ bool chunked(int dtype, bool kc, int64_t ld, int64_t rows, int64_t K) {
     return kc ? 256 * ld * size < PAST_END : 64 * ld * size < PAST_END;
 }
 
+// Microseconds of a product by tiles of 128 or 256 with k in `splits` parts, from what the
+// kernels took on an MI355X at 1024^2 to 8192 x 4096 outputs and k of 256 to 8192: a tile's start
+// and end, and its k tiles of 128 bytes. A CU takes one large tile or two small ones, which
+// are faster alone (the first figures) than two at a time. Joining is bound by the sums' way
+// to memory and back.
+double gemm_time(int dtype, int tile, double tiles, int splits, double steps, double outputs) {
+    const double wgs = tiles * splits;
+    double t;
+    if (tile == 256) {
+        t = std::ceil(wgs / CUS) * (11.0 + steps * (1.12 + 0.45 * std::min(1.0, wgs / CUS)));
+    } else {
+        const bool f32 = dtype == DRH_F32;
+        const double alone = f32 ? 7.0 + 1.7 * steps : 5.5 + 0.62 * steps, both = f32 ? 13.0 + 2.75 * steps : 8.0 + 0.91 * steps;
+        const double full = std::floor(wgs / (2 * CUS)), rest = wgs - full * 2 * CUS;
+        t = full * both + (rest > CUS ? both : rest > 0 ? alone : 0.0);
+    }
+    return splits > 1 ? t + 3.0 + splits * outputs * 1.45e-6 : t;
+}
+
 GemmPlan plan_gemm(int dtype, int64_t M, int64_t N, int64_t K, bool fits) {
     GemmPlan g;
-    if (!fits || K == 0) return g;
+    if (!fits || K == 0 || M == 0) return g;
     const int64_t bk = 128 / (int64_t)type_size(dtype), kt = (K + bk - 1) / bk;
     double best = 1e30;
     for (int tile : {256, 128}) {
+        if (tile == 256 && dtype == DRH_F32) continue;
         const int64_t tiles = (M + tile - 1) / tile * ((N + tile - 1) / tile);
-        const int64_t slots = tile == 256 ? CUS : 2 * CUS;
         if (tiles > INT32_MAX) continue;
-        for (int s = 1; s <= 64 && s <= kt; s++) {
+        for (int64_t s = 1; s <= 64 && s <= kt; s++) {
             const int64_t per = (kt + s - 1) / s;
             if ((kt + per - 1) / per != s) continue;
-            if (s > 1 && (size_t)s * M * N * 4 > ((size_t)1 << 30)) break;
-            const int64_t rounds = (tiles * s + slots - 1) / slots;
-            // microseconds of a k tile, and of a tile's start and end
-            const double step = (dtype == DRH_F32 ? 7.0 : 1.0) * (tile == 256 ? 1.25 : 0.9);
-            double t = rounds * (per * step + 4.0);
-            if (s > 1) t += 4.0 + s * (double)M * N * 8 / 4e6;
-            if (t < best) best = t, g.tile = tile, g.splits = s;
+            if (s > 1 && (double)s * M * N * 4 > 1e9) break;
+            const double t = gemm_time(dtype, tile, (double)tiles, (int)s, (double)per, (double)M * N);
+            if (t < best) best = t, g.tile = tile, g.splits = (int)s;
         }
     }
     if (g.splits > 1) g.bytes = up256((size_t)g.splits * M * N * sizeof(float));
@@ -380,21 +401,29 @@ int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial,
                 gemm_any_kernel<T, a.value><<<grid, 256, 0, s>>>(p, layout != MN, layout == KK);
                 return DRH_OK;
             });
-        auto go = [&](auto a) {
+        auto with = [&](auto a, auto math) {
             constexpr int ACT = a.value;
-            if (layout == KK) {
-                if (tile == 256) gemm_256_kernel<T, true, true, ACT><<<grid, 512, 0, s>>>(p);
-                else gemm_128_kernel<T, true, true, ACT><<<grid, 256, 0, s>>>(p);
-            } else if constexpr (ACT == DRH_ACT_NONE) {
-                if (layout == KN) {
-                    if (tile == 256) gemm_256_kernel<T, true, false, ACT><<<grid, 512, 0, s>>>(p);
-                    else gemm_128_kernel<T, true, false, ACT><<<grid, 256, 0, s>>>(p);
-                } else {
-                    if (tile == 256) gemm_256_kernel<T, false, false, ACT><<<grid, 512, 0, s>>>(p);
-                    else gemm_128_kernel<T, false, false, ACT><<<grid, 256, 0, s>>>(p);
-                }
+            using Math = decltype(math);
+            // 32 bits have no large tile: with thirds one of 256 x 128 in gemm_256's manner was no
+            // faster (4096^3 699 us, 684 with this one), and 256 x 256 needs more registers
+            constexpr bool LARGE = sizeof(T) == 2;
+            auto launch = [&](auto ak, auto bk) {
+                constexpr bool AK = ak.value, BK = bk.value;
+                if constexpr (LARGE)
+                    if (tile == 256) gemm_256_kernel<T, AK, BK, ACT><<<grid, 512, 0, s>>>(p);
+                if (tile == 128) gemm_128_kernel<T, AK, BK, ACT, Math><<<grid, 256, 0, s>>>(p);
+            };
+            if (layout == KK) launch(std::true_type(), std::true_type());
+            else if constexpr (ACT == DRH_ACT_NONE) {
+                if (layout == KN) launch(std::true_type(), std::false_type());
+                else launch(std::false_type(), std::false_type());
             }
             return DRH_OK;
+        };
+        auto go = [&](auto a) {
+            if constexpr (sizeof(T) == 4)
+                if (p.K >= THIRDS_LEAST) return with(a, Thirds());
+            return with(a, Straight());
         };
         if (!p.partial) return with_act(p.act, go);
         go(std::integral_constant<int, DRH_ACT_NONE>());
