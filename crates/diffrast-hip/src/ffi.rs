@@ -351,6 +351,7 @@ extern "C" {
     pub fn drh_layer_norm_backward_bytes(
         rows: i64,
         cols: i64,
+        dtype: c_int,
         out_bytes: *mut u64,
     ) -> c_int;
     pub fn drh_layer_norm_backward(

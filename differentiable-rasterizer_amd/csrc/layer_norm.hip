@@ -16,17 +16,17 @@ using namespace drh_rt;
 namespace drh_nn {
 namespace {
 
-// A row is held in the registers of TPR threads, EPT elements each: a wave up to 2048
-// elements, then four waves up to LN_MAX_COLS. Thread t's vectors are t, t + TPR, ...
+// A row is held in the registers of TPR threads, EPT elements each (with_row), up to
+// LN_MAX_COLS elements. Thread t's vectors are t, t + TPR, ...
 constexpr int LN_MAX_COLS = 256 * 32;
 
 // Weights from column c on; they may stand in 32 bits beside activations in 16.
-template <class T, int VEC>
+template <class T, bool WHOLE, int VEC>
 __device__ inline void load_weight(const void* w, bool wf32, int c, int D, float (&out)[VEC]) {
     if (wf32)
-        load_some<VEC>((const float*)w + c, D - c, out);
+        load_some<VEC>((const float*)w + c, WHOLE ? VEC : D - c, out);
     else
-        load_some<VEC>((const T*)w + c, D - c, out);
+        load_some<VEC>((const T*)w + c, WHOLE ? VEC : D - c, out);
 }
 
 // Sums of a and b over a row's threads, in all of them. `slot` alternates between
@@ -60,11 +60,12 @@ struct LnArgs {
     float eps;
 };
 
-template <class T, int EPT, int TPR>
-__global__ __launch_bounds__(256) void ln_forward(LnArgs p) {
-    constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC, RPB = 256 / TPR;
+// WHOLE: the columns are whole vectors.
+template <class T, int EPT, int TPR, int THREADS, bool WHOLE>
+__global__ __launch_bounds__(THREADS) void ln_forward(LnArgs p) {
+    constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC, RPB = THREADS / TPR;
     const int t = threadIdx.x % TPR, D = p.cols;
-    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    const int64_t row = (int64_t)blockIdx.x * RPB + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
     if (TPR <= 64 && row >= p.rows) return;
     const T* x = (const T*)p.x + row * p.xs;
     float v[NV][VEC];
@@ -72,31 +73,28 @@ __global__ __launch_bounds__(256) void ln_forward(LnArgs p) {
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int c = (j * TPR + t) * VEC;
+        Raw raw = {};
+        if (c < D) raw = load_raw<WHOLE>(x + c, D - c);
+        const Elements<T> e = __builtin_bit_cast(Elements<T>, raw);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) v[j][i] = 0.0f;
-        if (c < D) load_some<VEC>(x + c, D - c, v[j]);
+        for (int i = 0; i < VEC; i++) v[j][i] = (float)e[i];
     }
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
         for (int i = 0; i < VEC; i++) s += v[j][i];
-    row_sums<TPR, 256>(s, q, 0);
+    row_sums<TPR, THREADS>(s, q, 0);
     const float mu = s / (float)D;
     q = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int left = D - (j * TPR + t) * VEC;
-        if (left >= VEC) {
 #pragma unroll
-            for (int i = 0; i < VEC; i++) q = fmaf(v[j][i] - mu, v[j][i] - mu, q);
-        } else if (left > 0) {
-#pragma unroll
-            for (int i = 0; i < VEC; i++)
-                if (i < left) q = fmaf(v[j][i] - mu, v[j][i] - mu, q);
-        }
+        for (int i = 0; i < VEC; i++)
+            if (WHOLE ? left > 0 : i < left) q = fmaf(v[j][i] - mu, v[j][i] - mu, q);
     }
     s = 0.0f;
-    row_sums<TPR, 256>(q, s, 1);
+    row_sums<TPR, THREADS>(q, s, 1);
     const float r = 1.0f / sqrtf(q / (float)D + p.eps);
     if (t == 0 && p.mean) {
         p.mean[row] = mu;
@@ -111,77 +109,100 @@ __global__ __launch_bounds__(256) void ln_forward(LnArgs p) {
 #pragma unroll
         for (int i = 0; i < VEC; i++) o[i] = (v[j][i] - mu) * r;
         if (p.w) {
-            load_weight<T, VEC>(p.w, p.wf32, c, D, w);
+            load_weight<T, WHOLE>(p.w, p.wf32, c, D, w);
 #pragma unroll
             for (int i = 0; i < VEC; i++) o[i] *= w[i];
         }
         if (p.b) {
-            load_weight<T, VEC>(p.b, p.wf32, c, D, w);
+            load_weight<T, WHOLE>(p.b, p.wf32, c, D, w);
 #pragma unroll
             for (int i = 0; i < VEC; i++) o[i] += w[i];
         }
-        store_some<VEC>(y + c, D - c, o);
+        store_some<VEC>(y + c, WHOLE ? VEC : D - c, o);
     }
 }
 
-// One workgroup takes every gridDim-th group of THREADS / TPR rows and keeps its
-// columns' sums of g h and g in registers; at the end its row groups are added through
-// LDS in order and go to the workgroup's own row of p.part, which reduce_columns adds up.
-template <class T, int EPT, int TPR, int THREADS>
-__global__ __launch_bounds__(THREADS) void ln_backward(LnArgs p) {
+// A workgroup takes every gridDim-th group of THREADS / TPR rows and keeps its columns' sums
+// of g h and g in registers; at the end its row groups are added through LDS in order and go
+// to the workgroup's own row of p.part, which reduce_columns adds up. A group's next rows are
+// on their way while it works on the present ones: the sums over a row wait for all of it, so
+// without that a wave's loads and its arithmetic would take turns.
+template <class T, int EPT, int TPR, int THREADS, int PER_SIMD, bool WHOLE>
+__global__ __launch_bounds__(THREADS, PER_SIMD) void ln_backward(LnArgs p) {
     constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC, GROUPS = THREADS / TPR;
-    const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR, D = p.cols;
+    const int t = threadIdx.x % TPR, D = p.cols;
+    const int grp = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);  // a wave's: rows are addressed by scalars
     float w[NV][VEC], aw[NV][VEC], ab[NV][VEC];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int c = (j * TPR + t) * VEC;
 #pragma unroll
         for (int i = 0; i < VEC; i++) w[j][i] = 1.0f, aw[j][i] = ab[j][i] = 0.0f;
-        if (p.w && c < D) load_weight<T, VEC>(p.w, p.wf32, c, D, w[j]);
+        if (p.w && c < D) load_weight<T, WHOLE>(p.w, p.wf32, c, D, w[j]);
     }
     const float inv = 1.0f / (float)D;
-    int slot = 0;
-    for (int64_t row0 = (int64_t)blockIdx.x * GROUPS; row0 < p.rows; row0 += (int64_t)gridDim.x * GROUPS, slot++) {
-        const int64_t row = row0 + grp;
+    // A row as it stands in memory; it is widened where it is used, which costs an operation
+    // an element and saves the registers of the next row's loads.
+    struct Row {
+        Raw x[NV], g[NV];
+        float mu, r;
+    };
+    auto fetch = [&](Row& to, int64_t row) {  // past the last row zeros: no term of a sum
         const bool live = row < p.rows;
-        const float mu = live ? p.mean[row] : 0.0f, r = live ? p.rstd[row] : 0.0f;
-        float h[NV][VEC], g[NV][VEC];
-        float sg = 0.0f, sh = 0.0f;
+        to.mu = live ? p.mean[row] : 0.0f;
+        to.r = live ? p.rstd[row] : 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const int c = (j * TPR + t) * VEC;
-#pragma unroll
-            for (int i = 0; i < VEC; i++) h[j][i] = mu, g[j][i] = 0.0f;
+            to.x[j] = to.g[j] = Raw{};
             if (live && c < D) {
-                load_some<VEC>((const T*)p.x + row * p.xs + c, D - c, h[j]);
-                load_some<VEC>((const T*)p.g + row * p.gs + c, D - c, g[j]);
+                to.x[j] = load_raw<WHOLE>((const T*)p.x + row * p.xs + c, D - c);
+                to.g[j] = load_raw<WHOLE>((const T*)p.g + row * p.gs + c, D - c);
             }
         }
+    };
+    const int64_t stride = (int64_t)gridDim.x * GROUPS;
+    int slot = 0;
+    Row now, next;
+    fetch(now, (int64_t)blockIdx.x * GROUPS + grp);
+    for (int64_t row0 = (int64_t)blockIdx.x * GROUPS; row0 < p.rows; row0 += stride, slot++) {
+        const int64_t row = row0 + grp;
+        fetch(next, row + stride);
+        float sg = 0.0f, sh = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NV; j++)
+        for (int j = 0; j < NV; j++) {
+            const Elements<T> xe = __builtin_bit_cast(Elements<T>, now.x[j]), ge = __builtin_bit_cast(Elements<T>, now.g[j]);
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
-                h[j][i] = (h[j][i] - mu) * r;
-                aw[j][i] = fmaf(g[j][i], h[j][i], aw[j][i]);
-                ab[j][i] += g[j][i];
-                g[j][i] *= w[j][i];
-                sg += g[j][i];
-                sh = fmaf(g[j][i], h[j][i], sh);
+                // past the row's end g is zero, and with it every term
+                const float h = ((float)xe[i] - now.mu) * now.r, g = (float)ge[i], u = g * w[j][i];
+                aw[j][i] = fmaf(g, h, aw[j][i]);
+                ab[j][i] += g;
+                sg += u;
+                sh = fmaf(u, h, sh);
             }
+        }
         row_sums<TPR, THREADS>(sg, sh, slot);
         sg *= inv;
         sh *= inv;
-        if (live && p.dx) {
+        if (row < p.rows && p.dx) {
             T* dx = (T*)p.dx + row * D;
 #pragma unroll
             for (int j = 0; j < NV; j++) {
                 const int c = (j * TPR + t) * VEC;
                 float o[VEC];
+                // what was computed from them above is forgotten, so that it holds no registers
+                asm volatile("" : "+v"(now.x[j]), "+v"(now.g[j]));
+                const Elements<T> xe = __builtin_bit_cast(Elements<T>, now.x[j]), ge = __builtin_bit_cast(Elements<T>, now.g[j]);
 #pragma unroll
-                for (int i = 0; i < VEC; i++) o[i] = r * (g[j][i] - sg - h[j][i] * sh);
-                if (c < D) store_some<VEC>(dx + c, D - c, o);
+                for (int i = 0; i < VEC; i++) {
+                    const float h = ((float)xe[i] - now.mu) * now.r, u = (float)ge[i] * w[j][i];
+                    o[i] = now.r * (u - sg - h * sh);
+                }
+                if (c < D) store_some<VEC>(dx + c, WHOLE ? VEC : D - c, o);
             }
         }
+        now = next;
     }
     if (!p.part) return;
     __shared__ float sums[GROUPS][TPR * VEC];
@@ -229,8 +250,8 @@ __global__ __launch_bounds__(WIDE) void ln_forward_wide(LnArgs p) {
     }
     for (int c = threadIdx.x; c < D; c += WIDE) {
         float o[1] = {((float)x[c] - mu) * r}, w[1];
-        if (p.w) load_weight<T, 1>(p.w, p.wf32, c, D, w), o[0] *= w[0];
-        if (p.b) load_weight<T, 1>(p.b, p.wf32, c, D, w), o[0] += w[0];
+        if (p.w) load_weight<T, true>(p.w, p.wf32, c, D, w), o[0] *= w[0];
+        if (p.b) load_weight<T, true>(p.b, p.wf32, c, D, w), o[0] += w[0];
         store<1>(y + c, o);
     }
 }
@@ -244,7 +265,7 @@ __global__ __launch_bounds__(WIDE) void ln_backward_wide(LnArgs p) {
     const float mu = p.mean[row], r = p.rstd[row];
     float sg = 0.0f, sh = 0.0f, w[1] = {1.0f};
     for (int c = threadIdx.x; c < D; c += WIDE) {
-        if (p.w) load_weight<T, 1>(p.w, p.wf32, c, D, w);
+        if (p.w) load_weight<T, true>(p.w, p.wf32, c, D, w);
         const float gw = (float)g[c] * w[0];
         sg += gw;
         sh = fmaf(gw, ((float)x[c] - mu) * r, sh);
@@ -253,7 +274,7 @@ __global__ __launch_bounds__(WIDE) void ln_backward_wide(LnArgs p) {
     sg /= (float)D;
     sh /= (float)D;
     for (int c = threadIdx.x; c < D; c += WIDE) {
-        if (p.w) load_weight<T, 1>(p.w, p.wf32, c, D, w);
+        if (p.w) load_weight<T, true>(p.w, p.wf32, c, D, w);
         ((T*)p.dx)[row * D + c] = (T)(r * ((float)g[c] * w[0] - sg - ((float)x[c] - mu) * r * sh));
     }
 }
@@ -274,32 +295,52 @@ __global__ __launch_bounds__(64) void ln_columns_wide(LnArgs p) {
     out[p.cols + c] = sb;
 }
 
-// f(threads per row, elements per thread) as constants, for rows of D elements.
-template <class F>
+// f(threads per row, elements per thread) as constants, for rows of D elements of T: a wave a
+// row as far as it goes, then two, four, and eight for the longest of 32 bits. Few threads with
+// much to load each: 4096 of bfloat16 in 128 threads took the backward pass 170 us for 32768
+// rows, in 256 threads 183.
+template <class T, class F>
 void with_row(int64_t D, F&& f) {
     using std::integral_constant;
-    auto ept = [&](auto tpr, int64_t per) {
+    constexpr int MOST = sizeof(T) == 4 ? 16 : 32;
+    auto ept = [&](auto tpr) {
+        const int64_t per = (D + tpr.value - 1) / tpr.value;
         if (per <= 8) f(tpr, integral_constant<int, 8>());
         else if (per <= 16) f(tpr, integral_constant<int, 16>());
-        else f(tpr, integral_constant<int, 32>());
+        else f(tpr, integral_constant<int, MOST>());
     };
-    if (D <= 2048) ept(integral_constant<int, 64>(), (D + 63) / 64);
-    else ept(integral_constant<int, 256>(), (D + 255) / 256);
+    if (D <= 64 * MOST) ept(integral_constant<int, 64>());
+    else if (D <= 128 * MOST) ept(integral_constant<int, 128>());
+    else if (D <= 256 * MOST) ept(integral_constant<int, 256>());
+    else if constexpr (256 * MOST < LN_MAX_COLS) ept(integral_constant<int, 512>());
 }
 
-// Workgroups of the backward pass, each with a row of partial sums.
-constexpr int LN_GROUPS = 512;
+// Of a backward workgroup: its threads and the waves a SIMD that its registers are to allow.
+// Accumulators, weights and two rows of 16 elements or more a thread do not fit 128 registers
+// (1024 columns of bfloat16, 16384 rows: 25.6 us with two waves a SIMD, 33.9 with four and
+// spills). Rows of several waves take a smaller workgroup, since their barriers hold up all of it.
+struct LnShape {
+    int threads, per_simd;
+};
+constexpr LnShape ln_shape(int size, int tpr, int ept) {
+    return ept >= 16 ? LnShape{512, 2} : tpr > 64 ? LnShape{512, 4} : LnShape{1024, 4};
+}
 
-// Threads of a backward workgroup: the accumulators of 32 elements a thread need the
-// registers of eight waves a workgroup, smaller rows fit sixteen.
-constexpr int ln_threads(int ept) { return ept == 32 ? 512 : 1024; }
-
-int64_t ln_backward_groups(int64_t rows, int64_t cols) {
+// Workgroups of the backward pass, each with a row of partial sums: as many as run at once.
+int64_t ln_backward_groups(int64_t rows, int64_t cols, int dtype) {
     if (cols > LN_MAX_COLS) return rows < 64 ? rows : 64;
-    int64_t per = 1;
-    with_row(cols, [&](auto tpr, auto ept) { per = ln_threads(ept.value) / tpr.value; });
+    int64_t per = 1, most = 1;
+    with_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        with_row<T>(cols, [&](auto tpr, auto ept) {
+            constexpr LnShape s = ln_shape(sizeof(T), tpr.value, ept.value);
+            per = s.threads / tpr.value;
+            most = 256 * (s.per_simd * 256 / s.threads);
+        });
+        return DRH_OK;
+    });
     const int64_t need = (rows + per - 1) / per;
-    return need < LN_GROUPS ? need : LN_GROUPS;
+    return need < most ? need : most;
 }
 
 int check_ln(drh_ctx* ctx, int64_t rows, int64_t cols, int dtype, int weight_dtype, uint32_t flags) {
@@ -340,18 +381,20 @@ int drh_layer_norm(drh_ctx* ctx, const void* x, const void* weight, const void* 
             ln_forward_wide<T><<<dim3((unsigned)rows), WIDE, 0, s>>>(p);
             return DRH_OK;
         }
-        with_row(cols, [&](auto tpr, auto ept) {
-            constexpr int RPB = 256 / tpr.value;
-            ln_forward<T, ept.value, tpr.value><<<dim3((unsigned)((rows + RPB - 1) / RPB)), 256, 0, s>>>(p);
+        with_row<T>(cols, [&](auto tpr, auto ept) {
+            constexpr int THREADS = tpr.value > 256 ? tpr.value : 256, RPB = THREADS / tpr.value;
+            const dim3 grid((unsigned)((rows + RPB - 1) / RPB));
+            if (cols % (16 / sizeof(T)) == 0) ln_forward<T, ept.value, tpr.value, THREADS, true><<<grid, THREADS, 0, s>>>(p);
+            else ln_forward<T, ept.value, tpr.value, THREADS, false><<<grid, THREADS, 0, s>>>(p);
         });
         return DRH_OK;
     });
     return finish_call(s, flags, "layer norm");
 }
 
-int drh_layer_norm_backward_bytes(int64_t rows, int64_t cols, uint64_t* out_bytes) {
-    if (!out_bytes || rows < 0 || cols <= 0) return fail(DRH_ERR_INVALID_ARG, "bad sizes, or out_bytes is NULL");
-    *out_bytes = up256((size_t)ln_backward_groups(rows, cols) * 2 * (size_t)cols * sizeof(float));
+int drh_layer_norm_backward_bytes(int64_t rows, int64_t cols, int dtype, uint64_t* out_bytes) {
+    if (!out_bytes || !known_type(dtype) || rows < 0 || cols <= 0) return fail(DRH_ERR_INVALID_ARG, "bad sizes, or out_bytes is NULL");
+    *out_bytes = up256((size_t)ln_backward_groups(rows, cols, dtype) * 2 * (size_t)cols * sizeof(float));
     return DRH_OK;
 }
 
@@ -365,13 +408,13 @@ int drh_layer_norm_backward(drh_ctx* ctx, const void* x, const void* weight, con
     if (rows > 0 && (!x || !mean || !rstd || !grad_y)) return fail(DRH_ERR_INVALID_ARG, "an input pointer is NULL");
     if (rows > 1 && (x_stride < 0 || grad_stride < 0)) return fail(DRH_ERR_INVALID_ARG, "strides must not be negative");
     uint64_t need = 0;
-    if (sums) drh_layer_norm_backward_bytes(rows, cols, &need);
+    if (sums) drh_layer_norm_backward_bytes(rows, cols, dtype, &need);
     if (sums && (workspace_bytes < need || (need && !workspace)))
         return fail(DRH_ERR_INVALID_ARG, "the weight's gradient needs " + std::to_string(need) + " bytes of workspace");
     if ((uintptr_t)workspace % 16) return fail(DRH_ERR_INVALID_ARG, "the workspace must be 16-byte aligned");
     DeviceGuard dg(ctx->device);
     hipStream_t s = (hipStream_t)stream;
-    const int64_t groups = ln_backward_groups(rows, cols);
+    const int64_t groups = ln_backward_groups(rows, cols, dtype);
     LnArgs p{};
     p.x = x, p.w = weight, p.g = grad_y, p.dx = grad_x, p.mean = (float*)mean, p.rstd = (float*)rstd;
     p.part = sums ? (float*)workspace : nullptr;
@@ -385,9 +428,13 @@ int drh_layer_norm_backward(drh_ctx* ctx, const void* x, const void* weight, con
                     ln_columns_wide<T><<<dim3((unsigned)((cols + 63) / 64), (unsigned)groups), 64, 0, s>>>(p);
                 return DRH_OK;
             }
-            with_row(cols, [&](auto tpr, auto ept) {
-                constexpr int THREADS = ln_threads(ept.value);
-                ln_backward<T, ept.value, tpr.value, THREADS><<<dim3((unsigned)groups), THREADS, 0, s>>>(p);
+            with_row<T>(cols, [&](auto tpr, auto ept) {
+                constexpr LnShape sh = ln_shape(sizeof(T), tpr.value, ept.value);
+                const dim3 grid((unsigned)groups);
+                if (cols % (16 / sizeof(T)) == 0)
+                    ln_backward<T, ept.value, tpr.value, sh.threads, sh.per_simd, true><<<grid, sh.threads, 0, s>>>(p);
+                else
+                    ln_backward<T, ept.value, tpr.value, sh.threads, sh.per_simd, false><<<grid, sh.threads, 0, s>>>(p);
             });
             return DRH_OK;
         });

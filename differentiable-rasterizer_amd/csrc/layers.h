@@ -46,6 +46,23 @@ __device__ inline void load_some(const T* p, int64_t left, float (&out)[N]) {
     }
 }
 
+// Sixteen bytes of T as they stand in memory. Words and not a vector of T: 16-bit elements that
+// live across branches would each take a register.
+using Raw = vec<uint32_t, 4>;
+template <class T>
+using Elements = vec<T, 16 / sizeof(T)>;
+
+// The 16 bytes at p where WHOLE; else the first `left` elements, zeros behind.
+template <bool WHOLE, class T>
+__device__ inline Raw load_raw(const T* p, int64_t left) {
+    constexpr int N = 16 / sizeof(T);
+    if (WHOLE || left >= N) return __builtin_bit_cast(Raw, (Elements<T>)*reinterpret_cast<const typename Anywhere<T, N>::type*>(p));
+    Elements<T> v;
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = i < left ? p[i] : (T)0.0f;
+    return __builtin_bit_cast(Raw, v);
+}
+
 // Rounds to T once, to nearest even.
 template <int N, class T>
 __device__ inline void store(T* p, const float (&v)[N]) {

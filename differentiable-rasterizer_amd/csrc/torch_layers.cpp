@@ -193,7 +193,7 @@ struct LayerNormBackward : OnceNode {
         if (has_weight && task_should_compute_output(1)) r[1] = at::empty({cols}, w.options());
         if (has_bias && task_should_compute_output(2)) r[2] = at::empty({cols}, b.options());
         uint64_t bytes = 0;
-        if (r[1].defined() || r[2].defined()) check(drh_layer_norm_backward_bytes(rows, cols, &bytes));
+        if (r[1].defined() || r[2].defined()) check(drh_layer_norm_backward_bytes(rows, cols, dtype_code(x), &bytes));
         const Tensor ws = workspace(bytes, x);
         const int code = dtype_code(x), wcode = has_weight ? dtype_code(w) : has_bias ? dtype_code(b) : code;
         const float* mean = stats.const_data_ptr<float>();

@@ -156,7 +156,7 @@ SIGNATURES = {
     "drh_decode_srgb": ([_P, _P, _I64, _P, _P, _U32], ctypes.c_int),
     "drh_resize_lanczos3": ([_P, _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _U32], ctypes.c_int),
     "drh_layer_norm": ([_P, _P, _P, _P, _I64, _I64, _I64, _INT, _INT, _F32, _P, _P, _P, _P, _U32], ctypes.c_int),
-    "drh_layer_norm_backward_bytes": ([_I64, _I64, ctypes.POINTER(_U64)], ctypes.c_int),
+    "drh_layer_norm_backward_bytes": ([_I64, _I64, _INT, ctypes.POINTER(_U64)], ctypes.c_int),
     "drh_layer_norm_backward": ([_P] * 6 + [_I64] * 4 + [_INT, _INT, _P, _P, _P, _P, _U64, _P, _U32], ctypes.c_int),
     "drh_linear": ([_P] * 5 + [_I64] * 5 + [_INT, _INT, _P, _P, _P, _U64, _P, _U32], ctypes.c_int),
     "drh_linear_bytes": ([_I64] * 5 + [_INT, ctypes.POINTER(_U64)], ctypes.c_int),

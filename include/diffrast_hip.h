@@ -356,7 +356,7 @@ int drh_layer_norm(drh_ctx *ctx, const void *x, const void *weight, const void *
                    float *mean, float *rstd, void *stream, uint32_t flags);
 
 /* Workspace of drh_layer_norm_backward; none is needed (NULL, 0) without grad_weight and grad_bias. */
-int drh_layer_norm_backward_bytes(int64_t rows, int64_t cols, uint64_t *out_bytes);
+int drh_layer_norm_backward_bytes(int64_t rows, int64_t cols, int dtype, uint64_t *out_bytes);
 
 /* Gradients of drh_layer_norm from its x, weight, mean and rstd and from grad_y
  * (rows grad_stride elements apart). grad_x (contiguous), grad_weight and grad_bias
