@@ -66,7 +66,7 @@ __global__ __launch_bounds__(THREADS) void ln_forward(LnArgs p) {
     constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC, RPB = THREADS / TPR;
     const int t = threadIdx.x % TPR, D = p.cols;
     const int64_t row = (int64_t)blockIdx.x * RPB + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
-    if (TPR <= 64 && row >= p.rows) return;
+    const bool live = row < p.rows;  // a workgroup's last rows may not be there; their waves keep to its barriers
     const T* x = (const T*)p.x + row * p.xs;
     float v[NV][VEC];
     float s = 0.0f, q = 0.0f;
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(THREADS) void ln_forward(LnArgs p) {
     for (int j = 0; j < NV; j++) {
         const int c = (j * TPR + t) * VEC;
         Raw raw = {};
-        if (c < D) raw = load_raw<WHOLE>(x + c, D - c);
+        if (live && c < D) raw = load_raw<WHOLE>(x + c, D - c);
         const Elements<T> e = __builtin_bit_cast(Elements<T>, raw);
 #pragma unroll
         for (int i = 0; i < VEC; i++) v[j][i] = (float)e[i];
@@ -96,6 +96,7 @@ __global__ __launch_bounds__(THREADS) void ln_forward(LnArgs p) {
     s = 0.0f;
     row_sums<TPR, THREADS>(q, s, 1);
     const float r = 1.0f / sqrtf(q / (float)D + p.eps);
+    if (!live) return;
     if (t == 0 && p.mean) {
         p.mean[row] = mu;
         p.rstd[row] = r;
