@@ -34,6 +34,14 @@ __device__ inline void load(const T* p, float (&out)[N]) {
     for (int i = 0; i < N; i++) out[i] = (float)v[i];
 }
 
+// load, of values that nothing reads again soon.
+template <int N, class T>
+__device__ inline void load_once(const T* p, float (&out)[N]) {
+    const vec<T, N> v = __builtin_nontemporal_load(reinterpret_cast<const typename Anywhere<T, N>::type*>(p));
+#pragma unroll
+    for (int i = 0; i < N; i++) out[i] = (float)v[i];
+}
+
 // The first `left` of N elements at p; the others keep their values.
 template <int N, class T>
 __device__ inline void load_some(const T* p, int64_t left, float (&out)[N]) {

@@ -486,19 +486,32 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * CH;
     float sum[CH] = {};
-    if (c < N)
-        for (int64_t row = (int64_t)blockIdx.y * 4 + w; row < M; row += (int64_t)gridDim.y * 4) {
-            float g[CH] = {};
-            load_some<CH>(dy + row * N + c, N - c, g);
-            if (slope) {
-                float d[CH] = {};
-                load_some<CH>(slope + row * N + c, N - c, d);
+    const int64_t stride = (int64_t)gridDim.y * 4, left = N - c;
+    auto fetch = [&](int64_t row, float (&g)[CH], float (&d)[CH]) {
 #pragma unroll
-                for (int i = 0; i < CH; i++) g[i] *= d[i];
-            }
-            if (dz) store<CH>(dz + row * ldz + c, g);  // ldz is whole chunks
+        for (int i = 0; i < CH; i++) g[i] = 0.0f, d[i] = 1.0f;
+        if (row >= M) return;
+        if (slope && left >= CH) {
+            load_once<CH>(dy + row * N + c, g);
+            load_once<CH>(slope + row * N + c, d);
+            return;
+        }
+        load_some<CH>(dy + row * N + c, left, g);
+        if (slope) load_some<CH>(slope + row * N + c, left, d);
+    };
+    auto finish = [&](int64_t row, float (&g)[CH], const float (&d)[CH]) {
+        if (row >= M) return;
 #pragma unroll
-            for (int i = 0; i < CH; i++) sum[i] += g[i];
+        for (int i = 0; i < CH; i++) sum[i] += g[i] *= d[i];
+        if (dz) store<CH>(dz + row * ldz + c, g);  // ldz is whole chunks
+    };
+    if (left > 0)
+        for (int64_t row = (int64_t)blockIdx.y * 4 + w; row < M; row += 2 * stride) {  // two rows' loads at once
+            float g0[CH], d0[CH], g1[CH], d1[CH];
+            fetch(row, g0, d0);
+            fetch(row + stride, g1, d1);
+            finish(row, g0, d0);
+            finish(row + stride, g1, d1);
         }
     if (!part) return;
     __shared__ float sums[4][64 * CH];
@@ -511,9 +524,11 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
     }
 }
 
-int64_t slope_groups(int64_t M) {
-    const int64_t need = (M + 31) / 32;
-    return need < 256 ? need : 256;
+// Row groups of slope_kernel: two rows a wave at least, and about 2048 workgroups at most.
+int64_t slope_groups(int64_t M, int64_t N, int dtype) {
+    const int64_t cols = 64 * (16 / (int64_t)type_size(dtype)), blocks = (N + cols - 1) / cols;
+    const int64_t need = (M + 7) / 8, most = std::min<int64_t>(512, std::max<int64_t>(64, 2048 / blocks));
+    return std::min(need, most);
 }
 
 struct ForwardPlan {
@@ -567,7 +582,7 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t 
     b.dz_at = off;
     if (b.dz) off += up256((size_t)M * b.ldz * type_size(dtype));
     b.sums_at = off;
-    off += up256((size_t)slope_groups(M) * N * sizeof(float));
+    off += up256((size_t)slope_groups(M, N, dtype) * N * sizeof(float));
     b.part_at = off;
     b.total = off + (b.dx.bytes > b.dw.bytes ? b.dx.bytes : b.dw.bytes);
     return b;
@@ -657,7 +672,7 @@ int drh_linear_backward(drh_ctx* ctx, const void* x, const void* weight, const v
     char* ws = (char*)workspace;
     const bool products = K > 0 && M > 0 && (grad_x || grad_weight), dz_made = plan.dz && products;
     float* sums = grad_bias ? (float*)(ws + plan.sums_at) : nullptr;
-    const int64_t groups = slope_groups(M), ldz = plan.ldz;
+    const int64_t groups = slope_groups(M, N, dtype), ldz = plan.ldz;
     const void* dz = dz_made ? ws + plan.dz_at : grad_y;
     if (M > 0 && (dz_made || grad_bias))
         with_type(dtype, [&](auto t) {
