@@ -61,7 +61,7 @@ struct LnArgs {
 };
 
 // WHOLE: the columns are whole vectors.
-template <class T, int EPT, int TPR, int THREADS, bool WHOLE>
+template <class T, int EPT, int TPR, int THREADS, bool WHOLE, bool ONCE>
 __global__ __launch_bounds__(THREADS) void ln_forward(LnArgs p) {
     constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC, RPB = THREADS / TPR;
     const int t = threadIdx.x % TPR, D = p.cols;
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(THREADS) void ln_forward(LnArgs p) {
     for (int j = 0; j < NV; j++) {
         const int c = (j * TPR + t) * VEC;
         Raw raw = {};
-        if (live && c < D) raw = load_raw<WHOLE>(x + c, D - c);
+        if (live && c < D) raw = load_raw<WHOLE, ONCE>(x + c, D - c);
         const Elements<T> e = __builtin_bit_cast(Elements<T>, raw);
 #pragma unroll
         for (int i = 0; i < VEC; i++) v[j][i] = (float)e[i];
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(THREADS) void ln_forward(LnArgs p) {
 // to the workgroup's own row of p.part, which reduce_columns adds up. A group's next rows are
 // on their way while it works on the present ones: the sums over a row wait for all of it, so
 // without that a wave's loads and its arithmetic would take turns.
-template <class T, int EPT, int TPR, int THREADS, int PER_SIMD, bool WHOLE>
+template <class T, int EPT, int TPR, int THREADS, int PER_SIMD, bool WHOLE, bool ONCE>
 __global__ __launch_bounds__(THREADS, PER_SIMD) void ln_backward(LnArgs p) {
     constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC, GROUPS = THREADS / TPR;
     const int t = threadIdx.x % TPR, D = p.cols;
@@ -157,8 +157,8 @@ __global__ __launch_bounds__(THREADS, PER_SIMD) void ln_backward(LnArgs p) {
             const int c = (j * TPR + t) * VEC;
             to.x[j] = to.g[j] = Raw{};
             if (live && c < D) {
-                to.x[j] = load_raw<WHOLE>((const T*)p.x + row * p.xs + c, D - c);
-                to.g[j] = load_raw<WHOLE>((const T*)p.g + row * p.gs + c, D - c);
+                to.x[j] = load_raw<WHOLE, ONCE>((const T*)p.x + row * p.xs + c, D - c);
+                to.g[j] = load_raw<WHOLE, ONCE>((const T*)p.g + row * p.gs + c, D - c);
             }
         }
     };
@@ -316,6 +316,14 @@ void with_row(int64_t D, F&& f) {
     else if constexpr (256 * MOST < LN_MAX_COLS) ept(integral_constant<int, 512>());
 }
 
+// f(WHOLE, ONCE) as constants.
+template <class T, class F>
+void with_loads(int64_t rows, int64_t cols, F&& f) {
+    if (cols % (16 / (int64_t)sizeof(T))) f(std::false_type(), std::false_type());
+    else if (rows * cols * (int64_t)sizeof(T) < READ_ONCE_BYTES) f(std::true_type(), std::false_type());
+    else f(std::true_type(), std::true_type());
+}
+
 // Of a backward workgroup: its threads and the waves a SIMD that its registers are to allow.
 // Accumulators, weights and two rows of 16 elements or more a thread do not fit 128 registers
 // (1024 columns of bfloat16, 16384 rows: 25.6 us with two waves a SIMD, 33.9 with four and
@@ -385,8 +393,9 @@ int drh_layer_norm(drh_ctx* ctx, const void* x, const void* weight, const void* 
         with_row<T>(cols, [&](auto tpr, auto ept) {
             constexpr int THREADS = tpr.value > 256 ? tpr.value : 256, RPB = THREADS / tpr.value;
             const dim3 grid((unsigned)((rows + RPB - 1) / RPB));
-            if (cols % (16 / sizeof(T)) == 0) ln_forward<T, ept.value, tpr.value, THREADS, true><<<grid, THREADS, 0, s>>>(p);
-            else ln_forward<T, ept.value, tpr.value, THREADS, false><<<grid, THREADS, 0, s>>>(p);
+            with_loads<T>(rows, cols, [&](auto whole, auto once) {
+                ln_forward<T, ept.value, tpr.value, THREADS, whole.value, once.value><<<grid, THREADS, 0, s>>>(p);
+            });
         });
         return DRH_OK;
     });
@@ -432,10 +441,10 @@ int drh_layer_norm_backward(drh_ctx* ctx, const void* x, const void* weight, con
             with_row<T>(cols, [&](auto tpr, auto ept) {
                 constexpr LnShape sh = ln_shape(sizeof(T), tpr.value, ept.value);
                 const dim3 grid((unsigned)groups);
-                if (cols % (16 / sizeof(T)) == 0)
-                    ln_backward<T, ept.value, tpr.value, sh.threads, sh.per_simd, true><<<grid, sh.threads, 0, s>>>(p);
-                else
-                    ln_backward<T, ept.value, tpr.value, sh.threads, sh.per_simd, false><<<grid, sh.threads, 0, s>>>(p);
+                with_loads<T>(rows, cols, [&](auto whole, auto once) {
+                    ln_backward<T, ept.value, tpr.value, sh.threads, sh.per_simd, whole.value, once.value>
+                        <<<grid, sh.threads, 0, s>>>(p);
+                });
             });
             return DRH_OK;
         });

@@ -34,14 +34,6 @@ __device__ inline void load(const T* p, float (&out)[N]) {
     for (int i = 0; i < N; i++) out[i] = (float)v[i];
 }
 
-// load, of values that nothing reads again soon.
-template <int N, class T>
-__device__ inline void load_once(const T* p, float (&out)[N]) {
-    const vec<T, N> v = __builtin_nontemporal_load(reinterpret_cast<const typename Anywhere<T, N>::type*>(p));
-#pragma unroll
-    for (int i = 0; i < N; i++) out[i] = (float)v[i];
-}
-
 // The first `left` of N elements at p; the others keep their values.
 template <int N, class T>
 __device__ inline void load_some(const T* p, int64_t left, float (&out)[N]) {
@@ -60,11 +52,20 @@ using Raw = vec<uint32_t, 4>;
 template <class T>
 using Elements = vec<T, 16 / sizeof(T)>;
 
+// Arrays of this size and more are read past the caches (ONCE below): the last one holds 256
+// MiB, so nothing of them would be there when it is read again, and what else it holds stays.
+// Layer norm 32768 x 4096 in bfloat16 (268 MB) takes 88 us so, 98 with ordinary loads; 16384 x
+// 1024 (34 MB) 16.0 and 13.8.
+constexpr int64_t READ_ONCE_BYTES = 128ll << 20;
+
 // The 16 bytes at p where WHOLE; else the first `left` elements, zeros behind.
-template <bool WHOLE, class T>
+template <bool WHOLE, bool ONCE, class T>
 __device__ inline Raw load_raw(const T* p, int64_t left) {
     constexpr int N = 16 / sizeof(T);
-    if (WHOLE || left >= N) return __builtin_bit_cast(Raw, (Elements<T>)*reinterpret_cast<const typename Anywhere<T, N>::type*>(p));
+    if (WHOLE || left >= N) {
+        const auto q = reinterpret_cast<const typename Anywhere<T, N>::type*>(p);
+        return __builtin_bit_cast(Raw, ONCE ? (Elements<T>)__builtin_nontemporal_load(q) : (Elements<T>)*q);
+    }
     Elements<T> v;
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = i < left ? p[i] : (T)0.0f;

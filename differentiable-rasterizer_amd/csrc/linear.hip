@@ -479,7 +479,7 @@ const void* place_rows(int dtype, const Rows& r, const void* src, int64_t ld, in
 // dz = dy act'(z), rounded to its type for the products, in rows of ldz elements with zeros
 // behind N, and the column sums of the unrounded values: a workgroup owns 64 chunks of every
 // gridDim.y-th slab of rows, its four waves a row each, added in order at the end.
-template <class T>
+template <class T, bool ONCE>
 __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const Kept<T>* __restrict__ slope, int64_t M,
                                                     int64_t N, int64_t ldz, T* __restrict__ dz, float* part) {
     constexpr int CH = 16 / sizeof(T);
@@ -488,16 +488,15 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
     float sum[CH] = {};
     const int64_t stride = (int64_t)gridDim.y * 4, left = N - c;
     auto fetch = [&](int64_t row, float (&g)[CH], float (&d)[CH]) {
-#pragma unroll
-        for (int i = 0; i < CH; i++) g[i] = 0.0f, d[i] = 1.0f;
-        if (row >= M) return;
-        if (slope && left >= CH) {
-            load_once<CH>(dy + row * N + c, g);
-            load_once<CH>(slope + row * N + c, d);
-            return;
+        Raw gr = {}, dr = {};
+        if (row < M) {
+            gr = load_raw<false, ONCE>(dy + row * N + c, left);
+            if (slope) dr = load_raw<false, ONCE>(slope + row * N + c, left);
         }
-        load_some<CH>(dy + row * N + c, left, g);
-        if (slope) load_some<CH>(slope + row * N + c, left, d);
+        const Elements<T> ge = __builtin_bit_cast(Elements<T>, gr);
+        const Elements<Kept<T>> de = __builtin_bit_cast(Elements<Kept<T>>, dr);
+#pragma unroll
+        for (int i = 0; i < CH; i++) g[i] = (float)ge[i], d[i] = slope ? (float)de[i] : 1.0f;
     };
     auto finish = [&](int64_t row, float (&g)[CH], const float (&d)[CH]) {
         if (row >= M) return;
@@ -678,8 +677,13 @@ int drh_linear_backward(drh_ctx* ctx, const void* x, const void* weight, const v
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
             const int64_t cols = 64 * (16 / (int64_t)sizeof(T));
-            slope_kernel<T><<<dim3((unsigned)((N + cols - 1) / cols), (unsigned)groups), 256, 0, s>>>(
-                (const T*)grad_y, slope ? (const Kept<T>*)kept : nullptr, M, N, ldz, dz_made ? (T*)dz : nullptr, sums);
+            auto go = [&](auto once) {
+                slope_kernel<T, once.value><<<dim3((unsigned)((N + cols - 1) / cols), (unsigned)groups), 256, 0, s>>>(
+                    (const T*)grad_y, slope ? (const Kept<T>*)kept : nullptr, M, N, ldz, dz_made ? (T*)dz : nullptr, sums);
+            };
+            // dy is read again where it is dz
+            if (dz_made && M * N * (int64_t)sizeof(T) >= READ_ONCE_BYTES) go(std::true_type());
+            else go(std::false_type());
             return DRH_OK;
         });
     if (grad_bias) reduce_columns(sums, M > 0 ? groups : 0, N, N, grad_bias, nullptr, dtype, s);
