@@ -49,7 +49,7 @@ __device__ inline floatx4 mma(vec<float, 4> a, vec<float, 4> b, floatx4 c) {
     return c;
 }
 
-constexpr int UNIT_BYTES = 16384;
+constexpr int UNIT_BYTES = 16384;  // of 128 rows
 constexpr uint32_t PAST_END = 0x7ffffff0u;  // an offset that no buffer here reaches
 
 using lds_char = __attribute__((address_space(3))) char;
@@ -63,25 +63,26 @@ __device__ inline int frag_row(int f, int r) {
 }
 
 // The chunk permutation: by row where k is contiguous (eight chunks a row), by k where the
-// rows are (sixteen chunks a value of k, 32 in 32 bits).
-template <class T, bool KC, bool B, int NF>
+// rows are (sixteen chunks a value of k for 128 rows, 32 in 32 bits).
+template <class T, bool KC, bool B, int NF, int ROWS>
 __device__ inline int swizzle(int i) {
+    constexpr int PER = ROWS * (int)sizeof(T) / 16;  // chunks a value of k
     if constexpr (KC) {
         return B ? (i & 3) | ((i / (4 * NF)) & 1) << 2 : i & 7;
     } else if constexpr (sizeof(T) == 2) {
-        return B ? 4 * (i & 3) : 2 * ((i & 3) | ((i >> 3) & 1) << 2);
+        return (B ? 4 * (i & 3) : 2 * ((i & 3) | ((i >> 3) & 1) << 2)) & (PER - 1);
     } else {
-        return B ? 8 * ((i >> 2) & 1) + ((i >> 3) & 1) : 4 * ((i >> 2) & 3);
+        return (B ? 8 * ((i >> 2) & 1) + ((i >> 3) & 1) : 4 * ((i >> 2) & 3)) & (PER - 1);
     }
 }
 
-// One operand of a workgroup's tile: UNITS units of 128 rows; row R of unit u is row
-// u * 128 + R of the tile. On B's side with two units and k contiguous it is (R / 32) * 64
+// One operand of a workgroup's tile: UNITS units of ROWS rows; row R of unit u is row
+// u * ROWS + R of the tile. On B's side with two units and k contiguous it is (R / 32) * 64
 // + u * 32 + R % 32 instead, so that a wave's 32 rows of both units are neighbours in the
 // output; with rows contiguous that would read half lines.
-template <class T, bool KC, bool B, int UNITS, int NF, int WAVES>
+template <class T, bool KC, bool B, int UNITS, int NF, int WAVES, int ROWS = 128>
 struct Loader {
-    static constexpr int CH = 16 / sizeof(T), BK = 8 * CH, LOADS = 16 / WAVES;
+    static constexpr int CH = 16 / sizeof(T), BK = 8 * CH, LOADS = ROWS / 8 / WAVES;
     const char* base;
     uint64_t step;          // bytes per tile of k
     uint64_t span;          // KC: bytes from the base to the end of the tile's last row
@@ -94,7 +95,7 @@ struct Loader {
         const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
         K = K_;
         const int64_t ld = o.ld;
-        const int64_t valid = o.rows - row0 < 128 * UNITS ? o.rows - row0 : 128 * UNITS;
+        const int64_t valid = o.rows - row0 < ROWS * UNITS ? o.rows - row0 : ROWS * UNITS;
         if constexpr (KC) {
             base = (const char*)o.ptr + row0 * ld * (int64_t)sizeof(T);
             step = 128;
@@ -113,12 +114,12 @@ struct Loader {
 #pragma unroll
             for (int u = 0; u < UNITS; u++) {
                 if constexpr (KC) {
-                    const int R = pos >> 3, chunk = (pos & 7) ^ swizzle<T, KC, B, NF>(R);
+                    const int R = pos >> 3, chunk = (pos & 7) ^ swizzle<T, KC, B, NF, ROWS>(R);
                     off[u][i] = (uint32_t)(tile_row(u, R) * ld * sizeof(T)) + chunk * 16;
                     kc = chunk * CH;
                 } else {
-                    constexpr int PER = 128 / CH;
-                    const int k = pos / PER, R = ((pos % PER) ^ swizzle<T, KC, B, NF>(k)) * CH;
+                    constexpr int PER = ROWS / CH;
+                    const int k = pos / PER, R = ((pos % PER) ^ swizzle<T, KC, B, NF, ROWS>(k)) * CH;
                     const int64_t row = tile_row(u, R);
                     off[u][i] = row0 + row < o.rows ? (uint32_t)(k * ld * sizeof(T) + row * sizeof(T)) : PAST_END;
                 }
@@ -127,7 +128,7 @@ struct Loader {
     }
 
     static __device__ int64_t tile_row(int u, int R) {
-        return B && KC && UNITS == 2 ? (R / 32) * 64 + u * 32 + R % 32 : u * 128 + R;
+        return B && KC && UNITS == 2 ? (R / 32) * 64 + u * 32 + R % 32 : u * ROWS + R;
     }
 
     // Starts the loads of unit u of k tile kt into LDS at `lds`; past the last tile they
@@ -164,8 +165,8 @@ __device__ inline void wait_vm() {
 }
 __device__ inline void wg_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
-// A wave's fragments of one unit, NFR of 16 rows from row r0 on, both halves of the k tile.
-template <class T, bool KC, bool B, int NF>
+// A wave's fragments of one unit, NF of 16 rows from row r0 on, both halves of the k tile.
+template <class T, bool KC, bool B, int NF, int ROWS = 128>
 struct Frags {
     static constexpr int CH = 16 / sizeof(T);
     using F = vec<T, CH>;
@@ -180,7 +181,7 @@ struct Frags {
             for (int h = 0; h < 2; h++) {
                 if constexpr (KC) {
                     const int R = r0 + frag_row<B, NF>(i, r);
-                    f[i][h] = *(const F*)(unit + R * 128 + (((h * 4 + q) ^ swizzle<T, KC, B, NF>(R)) * 16));
+                    f[i][h] = *(const F*)(unit + R * 128 + (((h * 4 + q) ^ swizzle<T, KC, B, NF, ROWS>(R)) * 16));
                 } else if constexpr (sizeof(T) == 2) {
                     // A transposing read: sixteen lanes give the addresses of four rows' pieces
                     // for four values of k, and each gets its row's four values.
@@ -192,7 +193,7 @@ struct Frags {
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const int k = h * 32 + q * 8 + e * 4 + (r >> 2), R = r0 + frag_row<B, NF>(i, (r & 3) * 4);
-                        const char* p = unit + k * 256 + (((R >> 3) ^ swizzle<T, KC, B, NF>(k)) * 16) + (R & 7) * 2;
+                        const char* p = unit + k * (ROWS * 2) + (((R >> 3) ^ swizzle<T, KC, B, NF, ROWS>(k)) * 16) + (R & 7) * 2;
                         x.s[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)p);
                     }
                     f[i][h] = x.v;
@@ -201,7 +202,7 @@ struct Frags {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int k = h * 16 + q * 4 + e;
-                        f[i][h][e] = *(const float*)(unit + k * 512 + (((R >> 2) ^ swizzle<T, KC, B, NF>(k)) * 16) + (R & 3) * 4);
+                        f[i][h][e] = *(const float*)(unit + k * (ROWS * 4) + (((R >> 2) ^ swizzle<T, KC, B, NF, ROWS>(k)) * 16) + (R & 3) * 4);
                     }
                 }
             }
@@ -212,19 +213,14 @@ struct Frags {
 //
 // Straight: with the instructions of the operands' own type.
 //
-// Thirds, for 32 bits: v = v1 + v2 + v3 in bfloat16, each the nearest to what is left, is
-// exact (3 x 8 bits; signs fill the gaps), and a b is a1 b1 + a1 b2 + a2 b1 + a2 b2 + a1 b3 +
-// a3 b1 to within 2^-23 |a b|, of either sign. Six bfloat16 products take 96 cycles of the
-// matrix core where the 32-bit instructions take 256, and splitting costs 5.5 vector
-// operations an element, which the other wave of the SIMD hides. Values past bfloat16's
-// range and infinities come out as NaN: see gemm_128's second pass.
+// Thirds, for 32 bits: v = v1 + v2 + v3 in bfloat16, each the first eight bits of what is left,
+// is exact (3 x 8 bits), and a b is a1 b1 + a1 b2 + a2 b1 + a2 b2 + a1 b3 + a3 b1 but for less
+// than 2^-21 |a b|, 2^-24 in the mean. Six bfloat16 products take 96 cycles of the matrix core
+// where the 32-bit instructions take 256, and splitting costs 5.5 vector operations an
+// element, which other waves hide. (Rounding each third to the nearest is as many
+// operations, but the conversion is a slow one: 4096^3 took 700 us with it.) Infinities come out
+// as NaN: see gemm_tile's second pass.
 struct Straight {
-    template <class F, int NF>
-    using Held = F;
-    template <class F>
-    static __device__ inline void hold(F& to, const F& from) {
-        to = from;
-    }
     template <class FA, class FB, int NA, int NB>
     static __device__ inline void multiply(const FA& a, const FB& b, floatx4 (&acc)[NA][NB]) {
 #pragma unroll
@@ -237,49 +233,48 @@ struct Straight {
 };
 
 struct Thirds {
-    template <class F, int NF>
-    struct Held {
-        vec<bf16, 8> f[3][NF];
-    };
-    template <class H, class F>
-    static __device__ inline void hold(H& to, const F& from) {
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(from.f) / sizeof(from.f[0])); i++) {
-            split(from.f[i], to.f[0][i], to.f[1][i], to.f[2][i]);
-        }
-    }
-    // Pairs are converted by one instruction; their values come back by a shift and a mask.
-    static __device__ inline void split(const vec<float, 4> (&v)[2], vec<bf16, 8>& t0, vec<bf16, 8>& t1, vec<bf16, 8>& t2) {
-        using F2 = vec<float, 2>;
-        using B2 = vec<bf16, 2>;
+    using Held = vec<bf16, 8>[3];
+    static __device__ inline void split(const vec<float, 4> (&v)[2], Held& to) {
         vec<uint32_t, 4> o[3];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            F2 r = {v[i / 2][2 * (i % 2)], v[i / 2][2 * (i % 2) + 1]};
+            float r[2] = {v[i / 2][2 * (i % 2)], v[i / 2][2 * (i % 2) + 1]};
 #pragma unroll
             for (int third = 0; third < 3; third++) {
-                const uint32_t pair = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, B2));
-                o[third][i] = pair;
+                const uint32_t a = __builtin_bit_cast(uint32_t, r[0]), b = __builtin_bit_cast(uint32_t, r[1]);
+                o[third][i] = __builtin_amdgcn_perm(b, a, 0x07060302);  // the upper halves of both
                 if (third < 2) {
-                    r[0] -= __builtin_bit_cast(float, pair << 16);
-                    r[1] -= __builtin_bit_cast(float, pair & 0xffff0000u);
+                    r[0] -= __builtin_bit_cast(float, a & 0xffff0000u);
+                    r[1] -= __builtin_bit_cast(float, b & 0xffff0000u);
                 }
             }
         }
-        t0 = __builtin_bit_cast(vec<bf16, 8>, o[0]);
-        t1 = __builtin_bit_cast(vec<bf16, 8>, o[1]);
-        t2 = __builtin_bit_cast(vec<bf16, 8>, o[2]);
+#pragma unroll
+        for (int third = 0; third < 3; third++) to[third] = __builtin_bit_cast(vec<bf16, 8>, o[third]);
     }
-    template <class HA, class HB, int NA, int NB>
-    static __device__ inline void multiply(const HA& a, const HB& b, floatx4 (&acc)[NA][NB]) {
-        // the smallest terms first
-        constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+    // A fragment of a is split while the one before it is multiplied: two vector operations
+    // behind each matrix instruction.
+    template <class FA, class FB, int NA, int NB>
+    static __device__ inline void multiply(const FA& a, const FB& b, floatx4 (&acc)[NA][NB]) {
+        constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};  // the smallest terms first
+        Held hb[NB], ha[2];
 #pragma unroll
-        for (int t = 0; t < 6; t++)
+        for (int j = 0; j < NB; j++) split(b.f[j], hb[j]);
+        split(a.f[0], ha[0]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < NA; i++)
+        for (int i = 0; i < NA; i++) {
+            if (i + 1 < NA) split(a.f[i + 1], ha[(i + 1) & 1]);
 #pragma unroll
-                for (int j = 0; j < NB; j++) acc[i][j] = mma(b.f[PB[t]][j], a.f[PA[t]][i], acc[i][j]);
+            for (int t = 0; t < 6; t++)
+#pragma unroll
+                for (int j = 0; j < NB; j++) acc[i][j] = mma(hb[j][PB[t]], ha[i & 1][PA[t]], acc[i][j]);
+#pragma unroll
+            for (int t = 0; t < 6 * NB; t++) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a matrix instruction
+                __builtin_amdgcn_sched_group_barrier(0x2, NB == 4 ? 2 : 4, 0);
+            }
+        }
     }
 };
 
@@ -381,17 +376,20 @@ __device__ inline void gemm_256(const Gemm& p) {
         }
 }
 
-// 128 x 128 by four waves, 64 x 64 each, two k tiles in LDS (64 KiB): two workgroups a CU,
-// each covering the other's waits.
-template <class T, bool AK, bool BK_, class Epilogue, class Math>
-__device__ inline void gemm_128(const Gemm& p) {
-    __shared__ __align__(1024) char lds[4 * UNIT_BYTES];
-    using LA = Loader<T, AK, false, 1, 4, 4>;
-    using LB = Loader<T, BK_, true, 1, 4, 4>;
+// TILE x TILE (128 or 64) by four waves, a quarter each, two k tiles in LDS. A CU takes two
+// workgroups with tiles of 128, five with 64, which cover each other's waits: more k tiles in
+// LDS were slower for both (4096^2 outputs, k = 2048 in bfloat16: 72 us with two of 128, 111 with
+// four; 107 with two of 64, 105 with three, 124 with four).
+template <class T, bool AK, bool BK_, class Epilogue, class Math, int TILE>
+__device__ inline void gemm_tile(const Gemm& p) {
+    constexpr int NF = TILE / 32, UNIT = TILE * 128;
+    __shared__ __align__(1024) char lds[4 * UNIT];
+    using LA = Loader<T, AK, false, 1, NF, 4, TILE>;
+    using LB = Loader<T, BK_, true, 1, NF, 4, TILE>;
     int64_t tm, tn;
-    pick_tile((p.M + 127) / 128, (p.N + 127) / 128, tm, tn);
-    const int64_t m0 = tm * 128, n0 = tn * 128;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w >> 1, wn = w & 1;
+    pick_tile((p.M + TILE - 1) / TILE, (p.N + TILE - 1) / TILE, tm, tn);
+    const int64_t m0 = tm * TILE, n0 = tn * TILE;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = (w >> 1) * (TILE / 2), wn = (w & 1) * (TILE / 2);
     const int64_t tiles = (p.K + LA::BK - 1) / LA::BK, first = (int64_t)blockIdx.y * p.tiles_per_split;
     const int64_t last = first + p.tiles_per_split < tiles ? first + p.tiles_per_split : tiles;
     LA la;
@@ -399,52 +397,49 @@ __device__ inline void gemm_128(const Gemm& p) {
     la.init(p.a, m0, p.K);
     lb.init(p.b, n0, p.K);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)lds;
-    auto load = [&](int64_t kt) {
-        const uint32_t b = (uint32_t)((kt - first) & 1) * 2 * UNIT_BYTES;
+    auto load = [&](int64_t kt, int stage) {
+        const uint32_t b = (uint32_t)stage * 2 * UNIT;
         la.issue(0, kt, lds0 + b);
-        lb.issue(0, kt, lds0 + b + UNIT_BYTES);
+        lb.issue(0, kt, lds0 + b + UNIT);
     };
-    floatx4 acc[4][4];
+    floatx4 acc[NF][NF];
     auto product = [&](auto math) {
         using How = decltype(math);
-        using FA = Frags<T, AK, false, 4>;
-        using FB = Frags<T, BK_, true, 4>;
+        using FA = Frags<T, AK, false, NF, TILE>;
+        using FB = Frags<T, BK_, true, NF, TILE>;
 #pragma unroll
-        for (int i = 0; i < 16; i++) acc[i >> 2][i & 3] = floatx4{};
-        load(first);
+        for (int i = 0; i < NF * NF; i++) acc[i / NF][i % NF] = floatx4{};
+        load(first, 0);
         for (int64_t kt = first; kt < last; kt++) {
-            const char* b = lds + ((kt - first) & 1) * 2 * UNIT_BYTES;
+            const int stage = (int)(kt - first) & 1;
+            const char* b = lds + stage * 2 * UNIT;
             wait_vm<0>();
             wg_barrier();  // this tile is there, and the other buffer read by every wave
-            load(kt + 1);
-            FA ra;
-            FB rb;
-            ra.read(b, wm * 64);
-            rb.read(b + UNIT_BYTES, wn * 64);
-            typename How::template Held<FA, 4> fa;
-            typename How::template Held<FB, 4> fb;
-            How::hold(fa, ra);
-            How::hold(fb, rb);
+            load(kt + 1, stage ^ 1);
+            FA fa;
+            FB fb;
+            fa.read(b, wm);
+            fb.read(b + UNIT, wn);
             How::multiply(fa, fb, acc);
         }
-        wait_vm<0>();
+        wait_vm<0>();  // LDS is given up, or used again, with no load on its way there
     };
     product(Math());
     if constexpr (std::is_same_v<Math, Thirds>) {
         // A result that is not finite comes from an infinity, a NaN or an overflow. The thirds turn
-        // the first and the last into NaN, so the tile is made again with instructions that do not.
+        // the first into NaN, so the tile is made again with instructions that do not.
         float zero = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; i++)
+        for (int i = 0; i < NF * NF; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) zero = fmaf(acc[i >> 2][i & 3][e], 0.0f, zero);
+            for (int e = 0; e < 4; e++) zero = fmaf(acc[i / NF][i % NF][e], 0.0f, zero);
         if (__syncthreads_or(!(zero == 0.0f))) product(Straight());
     }
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     Epilogue epilogue;
-    epilogue.columns(p, n0 + wn * 64 + q * 16);
+    epilogue.columns(p, n0 + wn + q * (4 * NF));
 #pragma unroll
-    for (int i = 0; i < 4; i++) epilogue.row(p, m0 + wm * 64 + i * 16 + r, acc[i]);
+    for (int i = 0; i < NF; i++) epilogue.row(p, m0 + wm + i * 16 + r, acc[i]);
 }
 
 }  // namespace drh_nn

@@ -153,9 +153,9 @@ __global__ __launch_bounds__(512, 2) void gemm_256_kernel(Gemm p) {
     gemm_256<T, AK, BK, Epilogue<T, ACT, 2>>(p);
 }
 
-template <class T, bool AK, bool BK, int ACT, class Math>
-__global__ __launch_bounds__(256, 2) void gemm_128_kernel(Gemm p) {
-    gemm_128<T, AK, BK, Epilogue<T, ACT, 4>, Math>(p);
+template <class T, bool AK, bool BK, int ACT, class Math, int TILE>
+__global__ __launch_bounds__(256, TILE == 128 ? 2 : 3) void gemm_tile_kernel(Gemm p) {
+    gemm_tile<T, AK, BK, Epilogue<T, ACT, TILE / 32>, Math, TILE>(p);
 }
 
 // The parts of a split product added in order, and the epilogue: a thread a 16-byte chunk of
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(Gemm p, bool a_kc, bool b
 enum Layout { KK, KN, MN };  // A's and B's contiguous dimension: forward, dx, dW
 
 struct GemmPlan {
-    int tile = 0;    // 256, 128, or 0: any
+    int tile = 0;    // 256, 128, 64, or 0: any
     bool rows = false;  // gemm_rows_kernel
     int splits = 1;
     size_t bytes = 0;  // of partial sums
@@ -309,8 +309,8 @@ struct GemmPlan {
 
 constexpr int CUS = 256;
 constexpr int64_t ROWS_MOST = 64;  // gemm_rows_kernel
-// Products in 32 bits are split in thirds from this k on: their error, 2^-23 of a term, is
-// then below that of the sum, and shorter products are bound by memory either way.
+// Products in 32 bits are split in thirds from this k on: their error, 2^-21 of a term at the
+// most, is then below that of the sum, and shorter products are bound by memory either way.
 constexpr int64_t THIRDS_LEAST = 64;
 
 // Whether an operand's sizes suit the kernels that load 16-byte chunks through buffers.
@@ -320,22 +320,21 @@ bool chunked(int dtype, bool kc, int64_t ld, int64_t rows, int64_t K) {
     return kc ? 256 * ld * size < PAST_END : 64 * ld * size < PAST_END;
 }
 
-// Microseconds of a product by tiles of 128 or 256 with k in `splits` parts, from what the
-// kernels took on an MI355X at 1024^2 to 8192 x 4096 outputs and k of 256 to 8192: a tile's start
-// and end, and its k tiles of 128 bytes. A CU takes one large tile or two small ones, which
-// are faster alone (the first figures) than two at a time. Joining is bound by the sums' way
-// to memory and back.
+// Microseconds of a product by tiles of 64, 128 or 256 with k in `splits` parts, from what the
+// kernels took on an MI355X at 256^2 to 8192 x 4096 outputs and k of 128 to 8192: with `c`
+// workgroups on the fullest CU, their start and end, and the `steps` k tiles of 128 bytes. Small
+// tiles share a CU at a cost that grows with c, large ones take turns. Joining is bound by the
+// sums' way to memory and back. For 2048 x 1024 outputs and k = 512 in bfloat16 it gives 7, 8 and
+// 19 us for 64, 128 and 256 (measured 6.8, 8.9, 20), for 4096 x 4096 and k = 2048 98, 73, 63 (107,
+// 72, 61).
 double gemm_time(int dtype, int tile, double tiles, int splits, double steps, double outputs) {
-    const double wgs = tiles * splits;
+    const double wgs = tiles * splits, c = std::ceil(wgs / CUS);
     double t;
-    if (tile == 256) {
-        t = std::ceil(wgs / CUS) * (11.0 + steps * (1.12 + 0.45 * std::min(1.0, wgs / CUS)));
-    } else {
-        const bool f32 = dtype == DRH_F32;
-        const double alone = f32 ? 7.0 + 1.7 * steps : 5.5 + 0.62 * steps, both = f32 ? 13.0 + 2.75 * steps : 8.0 + 0.91 * steps;
-        const double full = std::floor(wgs / (2 * CUS)), rest = wgs - full * 2 * CUS;
-        t = full * both + (rest > CUS ? both : rest > 0 ? alone : 0.0);
-    }
+    if (tile == 256) t = c * (11.0 + steps * (1.12 + 0.45 * std::min(1.0, wgs / CUS)));
+    else if (dtype == DRH_F32)
+        t = tile == 128 ? 11.0 + 3.5 * c + steps * (c > 1 ? 1.38 * c : 1.58) : 3.5 + 0.7 * c + steps * (0.25 + 0.42 * c);
+    else
+        t = tile == 128 ? (c > 1 ? 2.0 + 2.4 * c + steps * 0.475 * c : 4.9 + 0.66 * steps) : 4.0 + 0.3 * c + steps * std::max(0.21, 0.18 * c);
     return splits > 1 ? t + 3.0 + splits * outputs * 1.45e-6 : t;
 }
 
@@ -344,7 +343,7 @@ GemmPlan plan_gemm(int dtype, int64_t M, int64_t N, int64_t K, bool fits) {
     if (!fits || K == 0 || M == 0) return g;
     const int64_t bk = 128 / (int64_t)type_size(dtype), kt = (K + bk - 1) / bk;
     double best = 1e30;
-    for (int tile : {256, 128}) {
+    for (int tile : {256, 128, 64}) {
         if (tile == 256 && dtype == DRH_F32) continue;
         const int64_t tiles = (M + tile - 1) / tile * ((N + tile - 1) / tile);
         if (tiles > INT32_MAX) continue;
@@ -378,7 +377,7 @@ int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial,
     const int64_t ch = 16 / (int64_t)type_size(dtype);
     auto aligned = [](const void* q) { return (uintptr_t)q % 16 == 0; };
     const bool fast = plan.tile && aligned(p.a.ptr) && aligned(p.b.ptr);
-    const int tile = fast ? plan.tile : 64;
+    const int tile = fast ? plan.tile : 64;  // gemm_any_kernel's too
     const int64_t tiles = (p.M + tile - 1) / tile * ((p.N + tile - 1) / tile);
     if (tiles > INT32_MAX) return fail(DRH_ERR_TOO_LARGE, "more than 2^31 - 1 tiles of the output");
     p.splits = fast ? plan.splits : 1;
@@ -411,7 +410,8 @@ int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial,
                 constexpr bool AK = ak.value, BK = bk.value;
                 if constexpr (LARGE)
                     if (tile == 256) gemm_256_kernel<T, AK, BK, ACT><<<grid, 512, 0, s>>>(p);
-                if (tile == 128) gemm_128_kernel<T, AK, BK, ACT, Math><<<grid, 256, 0, s>>>(p);
+                if (tile == 128) gemm_tile_kernel<T, AK, BK, ACT, Math, 128><<<grid, 256, 0, s>>>(p);
+                if (tile == 64) gemm_tile_kernel<T, AK, BK, ACT, Math, 64><<<grid, 256, 0, s>>>(p);
             };
             if (layout == KK) launch(std::true_type(), std::true_type());
             else if constexpr (ACT == DRH_ACT_NONE) {
