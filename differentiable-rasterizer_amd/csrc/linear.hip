@@ -435,21 +435,8 @@ int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial,
     });
 }
 
-// An M x K operand copied to rows of K elements rounded up to 16 bytes, zeros behind K.
-template <class T>
-__global__ __launch_bounds__(256) void pad_rows(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t K,
-                                                T* __restrict__ dst) {
-    constexpr int CH = 16 / sizeof(T);
-    const int64_t per = (K + CH - 1) / CH, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * per) return;
-    const int64_t row = i / per, c = i % per * CH;
-    vec<T, CH> v;
-#pragma unroll
-    for (int e = 0; e < CH; e++) v[e] = c + e < K ? src[row * ld + c + e] : (T)0.0f;
-    *(vec<T, CH>*)(dst + row * per * CH + c) = v;
-}
-
-// A row-major operand as the fast kernels take it: as it stands, or copied to `space`.
+// A row-major operand as the fast kernels take it: as it stands, or copied to rows of K
+// elements rounded up to 16 bytes, with zeros behind K.
 struct Rows {
     int64_t ld;
     size_t bytes = 0;  // of the copy, 0: none
@@ -462,16 +449,34 @@ Rows rows_for(int dtype, int64_t rows, int64_t K, int64_t ld) {
     return {padded, up256((size_t)rows * padded * type_size(dtype))};
 }
 
-const void* place_rows(int dtype, const Rows& r, const void* src, int64_t ld, int64_t rows, int64_t K, void* space,
-                       hipStream_t s) {
-    if (!r.bytes) return src;
+struct PadJob {
+    const void* src;
+    void* dst;
+    int64_t ld, rows;  // rows 0: nothing to copy
+};
+
+// Two operands of K columns in one launch, a thread a 16-byte chunk.
+template <class T>
+__global__ __launch_bounds__(256) void pad_rows(PadJob a, PadJob b, int64_t K) {
+    constexpr int CH = 16 / sizeof(T);
+    const int64_t per = (K + CH - 1) / CH;
+    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const bool second = i >= a.rows * per;
+    if (second) i -= a.rows * per;
+    const PadJob& job = second ? b : a;
+    if (i >= job.rows * per) return;
+    const int64_t row = i / per, c = i % per * CH;
+    const Raw v = load_raw<false, false>((const T*)job.src + row * job.ld + c, K - c);
+    *(Raw*)((T*)job.dst + row * per * CH + c) = v;
+}
+
+void pad(int dtype, const PadJob& a, const PadJob& b, int64_t K, hipStream_t s) {
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        const int64_t chunks = rows * (r.ld / (16 / (int64_t)sizeof(T)));
-        pad_rows<T><<<dim3((unsigned)((chunks + 255) / 256)), 256, 0, s>>>((const T*)src, ld, rows, K, (T*)space);
+        const int64_t ch = 16 / (int64_t)sizeof(T), chunks = (a.rows + b.rows) * ((K + ch - 1) / ch);
+        if (chunks) pad_rows<T><<<dim3((unsigned)((chunks + 255) / 256)), 256, 0, s>>>(a, b, K);
         return DRH_OK;
     });
-    return space;
 }
 
 // ---------------------------------------------------------------- dz and the bias gradient
@@ -634,9 +639,11 @@ int drh_linear(drh_ctx* ctx, const void* x, const void* weight, const void* bias
     DeviceGuard dg(ctx->device);
     hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)workspace;
+    pad(dtype, {x, ws + plan.x_at, x_stride, plan.x.bytes ? rows : 0},
+        {weight, ws + plan.w_at, weight_stride, plan.w.bytes ? n_out : 0}, n_in, s);
     Gemm p{};
-    p.a = {place_rows(dtype, plan.x, x, x_stride, rows, n_in, ws + plan.x_at, s), plan.x.ld, rows};
-    p.b = {place_rows(dtype, plan.w, weight, weight_stride, n_out, n_in, ws + plan.w_at, s), plan.w.ld, n_out};
+    p.a = {plan.x.bytes ? ws + plan.x_at : x, plan.x.ld, rows};
+    p.b = {plan.w.bytes ? ws + plan.w_at : weight, plan.w.ld, n_out};
     p.M = rows, p.N = n_out, p.K = n_in;
     p.bias = bias, p.res = residual, p.out = y, p.act = activation;
     p.kept = activation != DRH_ACT_NONE ? kept : nullptr;
@@ -689,18 +696,18 @@ int drh_linear_backward(drh_ctx* ctx, const void* x, const void* weight, const v
     if (grad_bias) reduce_columns(sums, M > 0 ? groups : 0, N, N, grad_bias, nullptr, dtype, s);
     const int64_t ch = 16 / (int64_t)type_size(dtype), N_pad = (N + ch - 1) / ch * ch, K_pad = (K + ch - 1) / ch * ch;
     float* part = (float*)(ws + plan.part_at);
+    const bool pad_x = plan.x.bytes && grad_weight && M > 0 && K > 0, pad_w = plan.w.bytes && grad_x && M > 0 && K > 0;
+    pad(dtype, {x, ws + plan.x_at, x_stride, pad_x ? M : 0}, {weight, ws + plan.w_at, weight_stride, pad_w ? N : 0}, K, s);
     if (grad_x && M > 0 && K > 0) {
         Gemm p{};
-        const void* w = place_rows(dtype, plan.w, weight, weight_stride, N, K, ws + plan.w_at, s);
-        p.a = {dz, ldz, M}, p.b = {w, plan.w.ld, plan.w.bytes ? K_pad : K};
+        p.a = {dz, ldz, M}, p.b = {pad_w ? ws + plan.w_at : weight, plan.w.ld, pad_w ? K_pad : K};
         p.M = M, p.N = K, p.K = N, p.out = grad_x, p.act = DRH_ACT_NONE;
         rc = gemm(dtype, KN, p, plan.dx, part, s);
         if (rc) return rc;
     }
     if (grad_weight && K > 0) {
         Gemm p{};
-        const void* xp = M > 0 ? place_rows(dtype, plan.x, x, x_stride, M, K, ws + plan.x_at, s) : x;
-        p.a = {dz, ldz, dz_made ? N_pad : N}, p.b = {xp, plan.x.ld, plan.x.bytes ? K_pad : K};
+        p.a = {dz, ldz, dz_made ? N_pad : N}, p.b = {pad_x ? ws + plan.x_at : x, plan.x.ld, pad_x ? K_pad : K};
         p.M = N, p.N = K, p.K = M, p.out = grad_weight, p.act = DRH_ACT_NONE;
         rc = gemm(dtype, MN, p, plan.dw, part, s);
         if (rc) return rc;
