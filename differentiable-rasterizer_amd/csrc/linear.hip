@@ -21,24 +21,21 @@ namespace {
 
 // ---------------------------------------------------------------- activations
 
-constexpr float SQRT_HALF = 0.70710678118654752f, INV_SQRT_2PI = 0.39894228040143268f;
+constexpr float LOG2_E = 1.44269504088896341f, SQRT_HALF = 0.70710678118654752f, INV_SQRT_2PI = 0.39894228040143268f;
 constexpr float TANH_C = 0.79788456080286536f, TANH_A = 0.044715f;
 
 // EXACT: for results in 32 bits, with the library's functions; else for values that are
-// rounded to 16 bits afterwards.
-template <bool EXACT>
-__device__ inline float exp_of(float x) {
-    return EXACT ? expf(x) : __expf(x);
-}
+// rounded to 16 bits afterwards, by single instructions.
 
 // 1 / (1 + exp(-v))
 template <bool EXACT>
 __device__ inline float logistic(float v) {
-    return EXACT ? 1.0f / (1.0f + expf(-v)) : __builtin_amdgcn_rcpf(1.0f + __expf(-v));
+    return EXACT ? 1.0f / (1.0f + expf(-v)) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2_E * v));
 }
 
-__device__ inline float not_below(float z, float lo) { return z < lo ? lo : z; }  // NaN passes
-__device__ inline float not_above(float z, float hi) { return z > hi ? hi : z; }
+// One instruction each, which passes NaN.
+__device__ inline float not_below(float z, float lo) { return __builtin_elementwise_maximum(z, lo); }
+__device__ inline float not_above(float z, float hi) { return __builtin_elementwise_minimum(z, hi); }
 
 // act(z), and act'(z) in `slope`. Below -128 every value and slope is 0 in 32 bits, above 64
 // every value z and slope 1; the bounds keep infinity times zero out of the products there.
@@ -62,17 +59,18 @@ __device__ inline float act(float z, float& slope) {
             slope = fmaf(2.0f * TANH_C * c * s * (1.0f - s), fmaf(3.0f, u, 1.0f), s);
             return z * s;
         } else {
-            const float x = c * SQRT_HALF, e = exp_of<EXACT>(-x * x);
-            float erf;
+            float erf, e;  // erf(z / sqrt 2), exp(-z^2 / 2)
             if constexpr (EXACT) {
-                erf = erff(x);
+                erf = erff(c * SQRT_HALF);
+                e = expf(-0.5f * c * c);
             } else {  // Abramowitz and Stegun 7.1.26, within 1.5e-7
-                const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, fabsf(x), 1.0f));
+                e = __builtin_amdgcn_exp2f(c * c * (-0.5f * LOG2_E));
+                const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * SQRT_HALF, fabsf(c), 1.0f));
                 float q = fmaf(t, 1.061405429f, -1.453152027f);
                 q = fmaf(t, q, 1.421413741f);
                 q = fmaf(t, q, -0.284496736f);
                 q = fmaf(t, q, 0.254829592f);
-                erf = copysignf(fmaf(-q * t, e, 1.0f), x);
+                erf = copysignf(fmaf(-q * t, e, 1.0f), c);
             }
             const float phi = fmaf(0.5f, erf, 0.5f);
             slope = fmaf(c * INV_SQRT_2PI, e, phi);
