@@ -306,7 +306,10 @@ struct GemmPlan {
 };
 
 constexpr int CUS = 256;
-constexpr int64_t ROWS_MOST = 64;  // gemm_rows_kernel
+// gemm_rows_kernel's: it reads x from the caches for every 16 outputs, which with more rows and
+// a long k costs more than staging. Microseconds in bfloat16, with it and by tiles: 32 rows
+// 1280 x 1024 4.8 / 6.5, 4096 x 4096 13.2 / 13.9; 64 rows 4096 x 1024 7.2 / 9.1, 4096 x 4096 21.7 / 14.2.
+constexpr int64_t ROWS_FEW = 32, ROWS_MOST = 64, ROWS_MOST_K = 2048;
 // Products in 32 bits are split in thirds from this k on: their error, 2^-21 of a term at the
 // most, is then below that of the sum, and shorter products are bound by memory either way.
 constexpr int64_t THIRDS_LEAST = 64;
@@ -321,8 +324,8 @@ bool chunked(int dtype, bool kc, int64_t ld, int64_t rows, int64_t K) {
 // Microseconds of a product by tiles of 64, 128 or 256 with k in `splits` parts, from what the
 // kernels took on an MI355X at 256^2 to 8192 x 4096 outputs and k of 128 to 8192: with `c`
 // workgroups on the fullest CU, their start and end, and the `steps` k tiles of 128 bytes. Small
-// tiles share a CU at a cost that grows with c, large ones take turns. Joining is bound by the
-// sums' way to memory and back. For 2048 x 1024 outputs and k = 512 in bfloat16 it gives 7, 8 and
+// tiles share a CU at a cost that grows with c, large ones take turns. Joining is a launch more and
+// the sums' way to memory and back. For 2048 x 1024 outputs and k = 512 in bfloat16 it gives 7, 8 and
 // 19 us for 64, 128 and 256 (measured 6.8, 8.9, 20), for 4096 x 4096 and k = 2048 98, 73, 63 (107,
 // 72, 61).
 double gemm_time(int dtype, int tile, double tiles, int splits, double steps, double outputs) {
@@ -333,7 +336,7 @@ double gemm_time(int dtype, int tile, double tiles, int splits, double steps, do
         t = tile == 128 ? 11.0 + 3.5 * c + steps * (c > 1 ? 1.38 * c : 1.58) : 3.5 + 0.7 * c + steps * (0.25 + 0.42 * c);
     else
         t = tile == 128 ? (c > 1 ? 2.0 + 2.4 * c + steps * 0.475 * c : 4.9 + 0.66 * steps) : 4.0 + 0.3 * c + steps * std::max(0.21, 0.18 * c);
-    return splits > 1 ? t + 3.0 + splits * outputs * 1.45e-6 : t;
+    return splits > 1 ? t + 6.0 + splits * outputs * 1.45e-6 : t;
 }
 
 GemmPlan plan_gemm(int dtype, int64_t M, int64_t N, int64_t K, bool fits) {
@@ -541,7 +544,7 @@ struct ForwardPlan {
 
 ForwardPlan forward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype) {
     ForwardPlan f;
-    if (M <= ROWS_MOST && K > 0) {
+    if (K > 0 && (M <= ROWS_FEW || (M <= ROWS_MOST && K <= ROWS_MOST_K))) {
         f.x = {xs}, f.w = {ws}, f.y.rows = true;
         return f;
     }

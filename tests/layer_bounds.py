@@ -126,12 +126,13 @@ def layer_norm(x, w, b, eps, g):
     return out
 
 
-def philox_keep(n, p, seed, offset):
-    """The mask that drh_dropout documents, in Python's own integers and numpy."""
+def philox_keep(n, p, seed, offset, first=0):
+    """The mask that drh_dropout documents for n elements from `first` on, in Python's own
+    integers and numpy."""
     import numpy as np
 
     m32, u = 0xFFFFFFFF, np.uint64
-    blocks = np.arange((n + 7) // 8, dtype=u)
+    blocks = np.arange(first // 8, (first + n + 7) // 8, dtype=u)
     c = [blocks & u(m32), blocks >> u(32), np.full_like(blocks, offset & m32), np.full_like(blocks, offset >> 32)]
     k = [seed & m32, seed >> 32]
     for _ in range(10):
@@ -139,5 +140,5 @@ def philox_keep(n, p, seed, offset):
         c = [(b >> u(32)) ^ c[1] ^ u(k[0]), b & u(m32), (a >> u(32)) ^ c[3] ^ u(k[1]), a & u(m32)]
         k = [(k[0] + 0x9E3779B9) & m32, (k[1] + 0xBB67AE85) & m32]
     words = np.stack(c, 1)
-    bits = np.stack([words & u(0xFFFF), words >> u(16)], 2).reshape(-1)[:n].astype(np.int64)
+    bits = np.stack([words & u(0xFFFF), words >> u(16)], 2).reshape(-1)[first % 8:][:n].astype(np.int64)
     return torch.from_numpy(bits >= int(round(p * 65536)))
