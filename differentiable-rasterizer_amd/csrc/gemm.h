@@ -92,7 +92,7 @@ struct Loader {
     int kc;                 // KC: first k of the lane's chunk in a tile
 
     __device__ void init(const Operand& o, int64_t row0, int64_t K_) {
-        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+        const int lane = threadIdx.x & 63, w = (threadIdx.x >> 6) % WAVES;
         K = K_;
         const int64_t ld = o.ld;
         const int64_t valid = o.rows - row0 < ROWS * UNITS ? o.rows - row0 : ROWS * UNITS;
@@ -134,7 +134,7 @@ struct Loader {
     // Starts the loads of unit u of k tile kt into LDS at `lds`; past the last tile they
     // fill it with zeros and touch no memory, so that every tile has the same loads.
     __device__ void issue(int u, int64_t kt, uint32_t lds) const {
-        const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int w = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % WAVES);
         const int64_t left = K - kt * BK;
         const char* p = base + kt * step;
         uint32_t bytes;
@@ -163,6 +163,8 @@ template <int N>
 __device__ inline void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
 }
+// Nothing of this wave's is on its way to LDS or from it.
+__device__ inline void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 __device__ inline void wg_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // A wave's fragments of one unit, NF of 16 rows from row r0 on, both halves of the k tile.
@@ -217,9 +219,14 @@ struct Frags {
 // is exact (3 x 8 bits), and a b is a1 b1 + a1 b2 + a2 b1 + a2 b2 + a1 b3 + a3 b1 but for less
 // than 2^-21 |a b|, 2^-24 in the mean. Six bfloat16 products take 96 cycles of the matrix core
 // where the 32-bit instructions take 256, and splitting costs 5.5 vector operations an
-// element, which other waves hide. (Rounding each third to the nearest is as many
-// operations, but the conversion is a slow one: 4096^3 took 700 us with it.) Infinities come out
-// as NaN: see gemm_tile's second pass.
+// element, four behind each matrix instruction of a 64 x 64 quarter. (Rounding each third to the
+// nearest is as many operations, but the conversion is a slow one.) Alone, a matrix instruction
+// and four such operations take 12 ns with one wave a SIMD and 10 with two, 8 and 7 without them:
+// the two kinds overlap in part. 4096^3 takes 700 to 760 us (190 TFLOP/s in 32 bits, 1.15 P in
+// bfloat16, where the power limit has the clock) however the splits are placed; with one
+// workgroup a CU, between the next tile's instructions instead of before them, 4096 x 1024
+// outputs and k = 1024 take 60 us instead of 65. Infinities come out as NaN: see gemm_tile's
+// second pass.
 struct Straight {
     template <class FA, class FB, int NA, int NB>
     static __device__ inline void multiply(const FA& a, const FB& b, floatx4 (&acc)[NA][NB]) {
@@ -233,47 +240,60 @@ struct Straight {
 };
 
 struct Thirds {
-    using Held = vec<bf16, 8>[3];
-    static __device__ inline void split(const vec<float, 4> (&v)[2], Held& to) {
-        vec<uint32_t, 4> o[3];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float r[2] = {v[i / 2][2 * (i % 2)], v[i / 2][2 * (i % 2) + 1]};
-#pragma unroll
-            for (int third = 0; third < 3; third++) {
-                const uint32_t a = __builtin_bit_cast(uint32_t, r[0]), b = __builtin_bit_cast(uint32_t, r[1]);
-                o[third][i] = __builtin_amdgcn_perm(b, a, 0x07060302);  // the upper halves of both
-                if (third < 2) {
-                    r[0] -= __builtin_bit_cast(float, a & 0xffff0000u);
-                    r[1] -= __builtin_bit_cast(float, b & 0xffff0000u);
-                }
-            }
+    struct Held {
+        vec<uint32_t, 4> third[3];
+    };
+    // A third of the work of splitting pair i of a fragment's values: three parts in turn, with
+    // `r` and `m` handed on.
+    struct Pair {
+        uint32_t r[2], m[2];
+        __device__ void less(int i) {
+            r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, r[i]) - __builtin_bit_cast(float, m[i]));
         }
+    };
+    template <class F>
+    static __device__ inline void split(const F (&f)[2], Held& to, int i, int part, Pair& p) {
+        if (part == 0)
 #pragma unroll
-        for (int third = 0; third < 3; third++) to[third] = __builtin_bit_cast(vec<bf16, 8>, o[third]);
+            for (int e = 0; e < 2; e++) p.r[e] = __builtin_bit_cast(uint32_t, (float)f[i / 2][2 * (i % 2) + e]);
+        if (part == 1) p.less(1);
+        if (part == 2) p.less(0), p.less(1);
+        uint32_t both = __builtin_amdgcn_perm(p.r[1], p.r[0], 0x07060302);  // the upper halves
+        asm volatile("" : "+v"(both));  // here, not where it is used
+        to.third[part][i] = both;
+        if (part < 2)
+#pragma unroll
+            for (int e = 0; e < 2; e++) p.m[e] = p.r[e] & 0xffff0000u;
+        if (part == 0) p.less(0);
     }
-    // A fragment of a is split while the one before it is multiplied: two vector operations
-    // behind each matrix instruction.
-    template <class FA, class FB, int NA, int NB>
-    static __device__ inline void multiply(const FA& a, const FB& b, floatx4 (&acc)[NA][NB]) {
-        constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};  // the smallest terms first
-        Held hb[NB], ha[2];
+    template <class F>
+    static __device__ inline void split(const F (&f)[2], Held& to) {
+        Pair p;
 #pragma unroll
-        for (int j = 0; j < NB; j++) split(b.f[j], hb[j]);
-        split(a.f[0], ha[0]);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int i = 0; i < NA; i++) {
-            if (i + 1 < NA) split(a.f[i + 1], ha[(i + 1) & 1]);
+            for (int part = 0; part < 3; part++) split(f, to, i, part, p);
+    }
+    static __device__ inline vec<bf16, 8> term(const Held& h, int third) {
+        return __builtin_bit_cast(vec<bf16, 8>, h.third[third]);
+    }
+    // A fragment of A by all of B's, the smallest terms first; between the matrix instructions
+    // the parts of SPLITS splits, v0 to h0 and v1 to h1.
+    template <int SPLITS, int NF, class FA, class FB>
+    static __device__ inline void row(const Held& a, const Held (&b)[NF], floatx4 (&acc)[NF], const FA& v0, Held& h0,
+                                      const FB& v1, Held& h1) {
+        constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0}, PARTS = 4 / NF;
+        Pair p;
 #pragma unroll
-            for (int t = 0; t < 6; t++)
+        for (int m = 0; m < 6 * NF; m++) {
+            acc[m % NF] = mma(term(b[m % NF], PB[m / NF]), term(a, PA[m / NF]), acc[m % NF]);
 #pragma unroll
-                for (int j = 0; j < NB; j++) acc[i][j] = mma(hb[j][PB[t]], ha[i & 1][PA[t]], acc[i][j]);
-#pragma unroll
-            for (int t = 0; t < 6 * NB; t++) {
-                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a matrix instruction
-                __builtin_amdgcn_sched_group_barrier(0x2, NB == 4 ? 2 : 4, 0);
+            for (int e = 0; e < PARTS; e++) {
+                const int n = m * PARTS + e;
+                if (n < 12 && SPLITS > 0) split(v0, h0, n / 3, n % 3, p);
+                if (n >= 12 && SPLITS > 1) split(v1, h1, (n - 12) / 3, n % 3, p);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
@@ -376,56 +396,100 @@ __device__ inline void gemm_256(const Gemm& p) {
         }
 }
 
-// TILE x TILE (128 or 64) by four waves, a quarter each, two k tiles in LDS. A CU takes two
-// workgroups with tiles of 128, five with 64, which cover each other's waits: more k tiles in
-// LDS were slower for both (4096^2 outputs, k = 2048 in bfloat16: 72 us with two of 128, 111 with
-// four; 107 with two of 64, 105 with three, 124 with four).
-template <class T, bool AK, bool BK_, class Epilogue, class Math, int TILE>
+// TILE x TILE (128 or 64) by GROUPS groups of four waves, a quarter of the output each, two k
+// tiles in LDS for each group. With one group a CU takes two workgroups with tiles of 128, five
+// with 64, which cover each other's waits: more k tiles in LDS were slower for both (4096^2
+// outputs, k = 2048 in bfloat16: 72 us with two of 128, 111 with four; 107 with two of 64, 105 with
+// three, 124 with four). A workgroup that is alone on its CU has two groups that cover each
+// other's waits: they take the k tiles in turn, and add their sums through LDS at the end.
+template <class T, bool AK, bool BK_, class Epilogue, class Math, int TILE, int GROUPS>
 __device__ inline void gemm_tile(const Gemm& p) {
     constexpr int NF = TILE / 32, UNIT = TILE * 128;
-    __shared__ __align__(1024) char lds[4 * UNIT];
+    __shared__ __align__(1024) char lds[GROUPS * 4 * UNIT];
     using LA = Loader<T, AK, false, 1, NF, 4, TILE>;
     using LB = Loader<T, BK_, true, 1, NF, 4, TILE>;
+    using FA = Frags<T, AK, false, NF, TILE>;
+    using FB = Frags<T, BK_, true, NF, TILE>;
     int64_t tm, tn;
     pick_tile((p.M + TILE - 1) / TILE, (p.N + TILE - 1) / TILE, tm, tn);
     const int64_t m0 = tm * TILE, n0 = tn * TILE;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = (w >> 1) * (TILE / 2), wn = (w & 1) * (TILE / 2);
-    const int64_t tiles = (p.K + LA::BK - 1) / LA::BK, first = (int64_t)blockIdx.y * p.tiles_per_split;
-    const int64_t last = first + p.tiles_per_split < tiles ? first + p.tiles_per_split : tiles;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3, group = GROUPS == 2 ? wave >> 2 : 0;
+    const int wm = (w >> 1) * (TILE / 2), wn = (w & 1) * (TILE / 2);
+    const int64_t tiles = (p.K + LA::BK - 1) / LA::BK, start = (int64_t)blockIdx.y * p.tiles_per_split;
+    const int64_t last = start + p.tiles_per_split < tiles ? start + p.tiles_per_split : tiles;
+    const int64_t first = start + group, steps = (last - start + GROUPS - 1) / GROUPS;  // the group's tiles
     LA la;
     LB lb;
     la.init(p.a, m0, p.K);
     lb.init(p.b, n0, p.K);
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)lds;
-    auto load = [&](int64_t kt, int stage) {
+    char* mine = lds + group * 4 * UNIT;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)mine;
+    auto load = [&](int64_t step, int stage) {
         const uint32_t b = (uint32_t)stage * 2 * UNIT;
-        la.issue(0, kt, lds0 + b);
-        lb.issue(0, kt, lds0 + b + UNIT);
+        la.issue(0, first + step * GROUPS, lds0 + b);
+        lb.issue(0, first + step * GROUPS, lds0 + b + UNIT);
     };
-    floatx4 acc[NF][NF];
-    auto product = [&](auto math) {
-        using How = decltype(math);
-        using FA = Frags<T, AK, false, NF, TILE>;
-        using FB = Frags<T, BK_, true, NF, TILE>;
-#pragma unroll
-        for (int i = 0; i < NF * NF; i++) acc[i / NF][i % NF] = floatx4{};
-        load(first, 0);
-        for (int64_t kt = first; kt < last; kt++) {
-            const int stage = (int)(kt - first) & 1;
-            const char* b = lds + stage * 2 * UNIT;
-            wait_vm<0>();
+    floatx4 acc[NF][NF] = {};
+    auto straight = [&] {
+        load(0, 0);
+        for (int64_t i = 0; i < steps; i++) {
+            const int stage = (int)i & 1;
+            const char* b = mine + stage * 2 * UNIT;
+            wait_all();
             wg_barrier();  // this tile is there, and the other buffer read by every wave
-            load(kt + 1, stage ^ 1);
-            FA fa;
-            FB fb;
-            fa.read(b, wm);
-            fb.read(b + UNIT, wn);
-            How::multiply(fa, fb, acc);
+            load(i + 1, stage ^ 1);
+            if (GROUPS == 1 || first + i * GROUPS < last) {
+                FA fa;
+                FB fb;
+                fa.read(b, wm);
+                fb.read(b + UNIT, wn);
+                Straight::multiply(fa, fb, acc);
+            }
         }
-        wait_vm<0>();  // LDS is given up, or used again, with no load on its way there
+        wait_all();  // LDS is given up, or used again, with no load on its way there
     };
-    product(Math());
-    if constexpr (std::is_same_v<Math, Thirds>) {
+    if constexpr (std::is_same_v<Math, Straight>) {
+        straight();
+    } else {
+        // While a tile is multiplied, the next one's fragments are read and split. ha[0] holds a
+        // tile's first fragment of A when its turn comes, fa the others as they were read.
+        FA fa;
+        FB fb;
+        Thirds::Held ha[2], even[NF], odd[NF];
+        load(0, 0);
+        load(1, 1);
+        wait_vm<LA::LOADS + LB::LOADS>();
+        wg_barrier();
+        fa.read(mine, wm);
+        fb.read(mine + UNIT, wn);
+#pragma unroll
+        for (int j = 0; j < NF; j++) Thirds::split(fb.f[j], even[j]);
+        Thirds::split(fa.f[0], ha[0]);
+        auto multiply = [&](const char* b, const Thirds::Held (&now)[NF], Thirds::Held (&next)[NF], auto more) {
+            constexpr bool MORE = more.value;
+            if (MORE) fb.read(b + UNIT, wn);
+#pragma unroll
+            for (int r = 0; r < NF - 1; r++)
+                Thirds::row<MORE ? 2 : 1>(ha[r & 1], now, acc[r], fa.f[r + 1], ha[(r + 1) & 1], fb.f[r], next[r]);
+            if (MORE) fa.read(b, wm);
+            Thirds::row<MORE ? 2 : 0>(ha[1], now, acc[NF - 1], fb.f[NF - 1], next[NF - 1], fa.f[0], ha[0]);
+        };
+        auto step = [&](int64_t i, const Thirds::Held (&now)[NF], Thirds::Held (&next)[NF]) {
+            const int stage = (int)i & 1;
+            wait_all();
+            wg_barrier();  // the next tile is there, and this one read by every wave
+            load(i + 2, stage);
+            const char* b = mine + (stage ^ 1) * 2 * UNIT;
+            const int64_t kt = first + i * GROUPS;
+            // The last tile has no next one; where registers are short it takes the code of the others
+            if (kt + GROUPS < last || (NF == 4 && GROUPS == 1)) multiply(b, now, next, std::true_type());
+            else if (GROUPS == 1 || kt < last) multiply(b, now, next, std::false_type());
+        };
+        for (int64_t i = 0; i < steps; i += 2) {
+            step(i, even, odd);
+            if (i + 1 < steps) step(i + 1, odd, even);
+        }
+        wait_all();
         // A result that is not finite comes from an infinity, a NaN or an overflow. The thirds turn
         // the first into NaN, so the tile is made again with instructions that do not.
         float zero = 0.0f;
@@ -433,13 +497,35 @@ __device__ inline void gemm_tile(const Gemm& p) {
         for (int i = 0; i < NF * NF; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) zero = fmaf(acc[i / NF][i % NF][e], 0.0f, zero);
-        if (__syncthreads_or(!(zero == 0.0f))) product(Straight());
+        if (__syncthreads_or(!(zero == 0.0f))) {
+#pragma unroll
+            for (int i = 0; i < NF * NF; i++) acc[i / NF][i % NF] = floatx4{};
+            straight();
+        }
     }
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     Epilogue epilogue;
     epilogue.columns(p, n0 + wn + q * (4 * NF));
+    if constexpr (GROUPS == 1) {
 #pragma unroll
-    for (int i = 0; i < NF; i++) epilogue.row(p, m0 + wm + i * 16 + r, acc[i]);
+        for (int i = 0; i < NF; i++) epilogue.row(p, m0 + wm + i * 16 + r, acc[i]);
+    } else {
+        // Each group finishes half of the rows, with the other's sums of them.
+        constexpr int HALF = NF / 2;
+        floatx4* to = (floatx4*)lds + (wave ^ 4) * (HALF * NF * 64) + lane;
+        const floatx4* from = (const floatx4*)lds + wave * (HALF * NF * 64) + lane;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < HALF * NF; i++) to[i * 64] = group ? acc[i / NF][i % NF] : acc[HALF + i / NF][i % NF];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < HALF; i++) {
+            floatx4 sum[NF];
+#pragma unroll
+            for (int j = 0; j < NF; j++) sum[j] = (group ? acc[HALF + i][j] : acc[i][j]) + from[(i * NF + j) * 64];
+            epilogue.row(p, m0 + wm + (group * HALF + i) * 16 + r, sum);
+        }
+    }
 }
 
 }  // namespace drh_nn

@@ -151,9 +151,9 @@ __global__ __launch_bounds__(512, 2) void gemm_256_kernel(Gemm p) {
     gemm_256<T, AK, BK, Epilogue<T, ACT, 2>>(p);
 }
 
-template <class T, bool AK, bool BK, int ACT, class Math, int TILE>
-__global__ __launch_bounds__(256, TILE == 128 ? 2 : 3) void gemm_tile_kernel(Gemm p) {
-    gemm_tile<T, AK, BK, Epilogue<T, ACT, TILE / 32>, Math, TILE>(p);
+template <class T, bool AK, bool BK, int ACT, class Math, int TILE, int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS, TILE == 64 && GROUPS == 1 ? 3 : 2) void gemm_tile_kernel(Gemm p) {
+    gemm_tile<T, AK, BK, Epilogue<T, ACT, TILE / 32>, Math, TILE, GROUPS>(p);
 }
 
 // The parts of a split product added in order, and the epilogue: a thread a 16-byte chunk of
@@ -325,17 +325,17 @@ bool chunked(int dtype, bool kc, int64_t ld, int64_t rows, int64_t K) {
 // kernels took on an MI355X at 256^2 to 8192 x 4096 outputs and k of 128 to 8192: with `c`
 // workgroups on the fullest CU, their start and end, and the `steps` k tiles of 128 bytes. Small
 // tiles share a CU at a cost that grows with c, large ones take turns. Joining is a launch more and
-// the sums' way to memory and back. For 2048 x 1024 outputs and k = 512 in bfloat16 it gives 7, 8 and
-// 19 us for 64, 128 and 256 (measured 6.8, 8.9, 20), for 4096 x 4096 and k = 2048 98, 73, 63 (107,
-// 72, 61).
+// the sums' way to memory and back. For 2048 x 1024 outputs and k = 1024 in bfloat16 it gives 10 and
+// 15 us for 64 and 128 (measured 10.0, 14.0), for 4096 x 4096 and k = 2048 98, 73 and 63 for 64, 128
+// and 256 (107, 72, 61).
 double gemm_time(int dtype, int tile, double tiles, int splits, double steps, double outputs) {
     const double wgs = tiles * splits, c = std::ceil(wgs / CUS);
     double t;
     if (tile == 256) t = c * (11.0 + steps * (1.12 + 0.45 * std::min(1.0, wgs / CUS)));
-    else if (dtype == DRH_F32)
-        t = tile == 128 ? 11.0 + 3.5 * c + steps * (c > 1 ? 1.38 * c : 1.58) : 3.5 + 0.7 * c + steps * (0.25 + 0.42 * c);
-    else
-        t = tile == 128 ? (c > 1 ? 2.0 + 2.4 * c + steps * 0.475 * c : 4.9 + 0.66 * steps) : 4.0 + 0.3 * c + steps * std::max(0.21, 0.18 * c);
+    else if (dtype == DRH_F32 && tile == 128) t = c > 1 ? 11.0 + 3.5 * c + steps * 1.38 * c : 11.0 + steps * 1.28;
+    else if (dtype == DRH_F32) t = c > 1 ? 3.5 + 0.7 * c + steps * (0.25 + 0.42 * c) : 4.5 + steps * 0.54;
+    else if (tile == 128) t = c > 1 ? 2.0 + 2.4 * c + steps * 0.475 * c : 6.0 + steps * 0.58;
+    else t = c > 1 ? 4.0 + 0.3 * c + steps * std::max(0.21, 0.18 * c) : 3.3 + steps * 0.3;
     return splits > 1 ? t + 6.0 + splits * outputs * 1.45e-6 : t;
 }
 
@@ -411,8 +411,14 @@ int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial,
                 constexpr bool AK = ak.value, BK = bk.value;
                 if constexpr (LARGE)
                     if (tile == 256) gemm_256_kernel<T, AK, BK, ACT><<<grid, 512, 0, s>>>(p);
-                if (tile == 128) gemm_tile_kernel<T, AK, BK, ACT, Math, 128><<<grid, 256, 0, s>>>(p);
-                if (tile == 64) gemm_tile_kernel<T, AK, BK, ACT, Math, 64><<<grid, 256, 0, s>>>(p);
+                // Microseconds with two groups and with one, 256 tiles: 4096 x 1024 outputs and k = 1024
+                // in 32 bits 60 / 65, as k by rows 66 / 74; 1024 x 1024 outputs and k = 4096 in bfloat16
+                // 23.6 / 31. With 512 tiles one is the faster: 2048 x 1024 and k = 1024 10.0 / 10.9
+                const bool alone = tiles * p.splits <= CUS;
+                if (tile == 128 && alone) gemm_tile_kernel<T, AK, BK, ACT, Math, 128, 2><<<grid, 512, 0, s>>>(p);
+                if (tile == 128 && !alone) gemm_tile_kernel<T, AK, BK, ACT, Math, 128, 1><<<grid, 256, 0, s>>>(p);
+                if (tile == 64 && alone) gemm_tile_kernel<T, AK, BK, ACT, Math, 64, 2><<<grid, 512, 0, s>>>(p);
+                if (tile == 64 && !alone) gemm_tile_kernel<T, AK, BK, ACT, Math, 64, 1><<<grid, 256, 0, s>>>(p);
             };
             if (layout == KK) launch(std::true_type(), std::true_type());
             else if constexpr (ACT == DRH_ACT_NONE) {
