@@ -115,32 +115,42 @@ struct Epilogue {
             }
             return;
         }
+        if (n >= p.N) return;
+        float o[W];
 #pragma unroll
-        for (int g = 0; g < W; g += CH) {
-            if (n + g >= p.N) break;
-            float o[CH];
-#pragma unroll
-            for (int i = 0; i < CH; i++) o[i] = v[(g + i) / 4][(g + i) % 4] + bias[g + i];
-            apply<CH>(p, at + g, p.N - n - g, o);
-        }
+        for (int i = 0; i < W; i++) o[i] = v[i / 4][i % 4] + bias[i];
+        apply<W>(p, at, p.N - n, o);
     }
 
-    // From z on: activates, keeps the slope, adds the residual, stores the first `left`.
+    // From z on: activates, keeps the slope, adds the residual, stores the first `left`. The chunks
+    // of a line are stored one right after the other, so that it leaves the L2 whole.
     template <int C>
     static __device__ void apply(const Gemm& p, int64_t at, int64_t left, float (&o)[C]) {
+        constexpr int PART = CH < C ? CH : C;
+        auto store = [&](auto* to, const float (&x)[C]) {
+#pragma unroll
+            for (int g = 0; g < C; g += PART) {
+                float part[PART];
+#pragma unroll
+                for (int i = 0; i < PART; i++) part[i] = x[g + i];
+                if (g < left) store_some<PART>(to + g, left - g, part);
+            }
+        };
         if constexpr (ACT != DRH_ACT_NONE) {
             float slope[C];
 #pragma unroll
             for (int i = 0; i < C; i++) o[i] = act<sizeof(T) == 4, ACT>(o[i], slope[i]);
-            if (p.kept) store_some<C>((Kept<T>*)p.kept + at, left, slope);
+            if (p.kept) store((Kept<T>*)p.kept + at, slope);
         }
-        if (p.res) {
-            float r[C] = {};
-            load_some<C>((const T*)p.res + at, left, r);
+        if (p.res)
 #pragma unroll
-            for (int i = 0; i < C; i++) o[i] += r[i];
-        }
-        store_some<C>((T*)p.out + at, left, o);
+            for (int g = 0; g < C; g += PART) {
+                float r[PART] = {};
+                if (g < left) load_some<PART>((const T*)p.res + at + g, left - g, r);
+#pragma unroll
+                for (int i = 0; i < PART; i++) o[g + i] += r[i];
+            }
+        store((T*)p.out + at, o);
     }
 };
 
