@@ -37,7 +37,8 @@ __device__ inline void philox(uint64_t block, uint64_t offset, uint64_t seed, ui
 
 // A thread takes 16 bytes: the eight elements of a counter, or in 32 bits four of them. Two
 // threads then evaluate the same counter, which costs less than the half-used lines of 32
-// bytes a thread (16384 x 4096 in 32 bits with a residual: 202 us so).
+// bytes a thread (16384 x 4096 in 32 bits with a residual: 116 us so, 202 with those). Bound by
+// memory: in bfloat16 that size takes 63 us with the residual (403 MB, 6.4 TB/s) and 43 without.
 template <class T, bool ONCE>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, const T* __restrict__ res, int64_t n,
                                                       uint32_t threshold, float scale, uint64_t seed, uint64_t offset,

@@ -319,6 +319,12 @@ __device__ inline void pick_tile(int64_t tiles_m, int64_t tiles_n, int64_t& tm, 
 // reading at most one unit's fragments and starting one unit's loads, six steps ahead of
 // their use (five units in flight). A unit is overwritten two steps after both groups have
 // read it at the earliest.
+//
+// 8192^3 in bfloat16 takes 765 us, 1.43 PFLOP/s: the matrix cores are busy for 75% of the cycles
+// at the 1.8 GHz that the power limit leaves, so it is power that bounds it. With k of 1024 and
+// less a tile's start and end, about 10 us that nothing covers, count as well: 16384 x 4096
+// outputs and k = 1024 take 132 us (1.04 PFLOP/s), 16384 x 1024 and k = 4096 103 us (1.33). A CU that
+// is given 128 x 128 tiles instead reads an operand twice as often: 72 and 61 us at 4096^2 and k = 2048.
 template <class T, bool AK, bool BK_, class Epilogue>
 __device__ inline void gemm_256(const Gemm& p) {
     __shared__ __align__(1024) char lds[8 * UNIT_BYTES];

@@ -60,7 +60,8 @@ struct LnArgs {
     float eps;
 };
 
-// WHOLE: the columns are whole vectors.
+// WHOLE: the columns are whole vectors. 16384 x 1024 in bfloat16 (67 MB) take 14 us, 4.7 TB/s;
+// 4099 x 1500 in 32 bits (49 MB) 10.7, 4.6; 32768 x 4096 in bfloat16 (537 MB) 90, 6.0.
 template <class T, int EPT, int TPR, int THREADS, bool WHOLE, bool ONCE>
 __global__ __launch_bounds__(THREADS) void ln_forward(LnArgs p) {
     constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC, RPB = THREADS / TPR;
@@ -127,7 +128,10 @@ __global__ __launch_bounds__(THREADS) void ln_forward(LnArgs p) {
 // of g h and g in registers; at the end its row groups are added through LDS in order and go
 // to the workgroup's own row of p.part, which reduce_columns adds up. A group's next rows are
 // on their way while it works on the present ones: the sums over a row wait for all of it, so
-// without that a wave's loads and its arithmetic would take turns.
+// without that a wave's loads and its arithmetic would take turns. 16384 x 1024 in bfloat16 (101 MB)
+// take 20 us, 5.0 TB/s; 4099 x 1500 in 32 bits (74 MB) 16.8, 4.4; 32768 x 4096 in bfloat16 (805 MB)
+// 171, 4.7: two waves a SIMD with 24 vector operations an element and a sum over LDS a row do not
+// hide all of the loads' latency.
 template <class T, int EPT, int TPR, int THREADS, int PER_SIMD, bool WHOLE, bool ONCE>
 __global__ __launch_bounds__(THREADS, PER_SIMD) void ln_backward(LnArgs p) {
     constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC, GROUPS = THREADS / TPR;

@@ -9,7 +9,8 @@ namespace drh_nn {
 namespace {
 
 // Sixteen waves a workgroup, 64 columns each, so that a wave reads 256 contiguous
-// bytes of a partial row; the waves take every sixteenth row and are added in order.
+// bytes of a partial row; the waves take every sixteenth row and are added in order. The partial
+// sums are 1 to 8 MB and still in the caches: 4 to 5 us, hardly more than a launch.
 constexpr int RC_WAVES = 16;
 template <class T>
 __global__ __launch_bounds__(64 * RC_WAVES) void reduce_columns_kernel(const float* __restrict__ part, int64_t groups,

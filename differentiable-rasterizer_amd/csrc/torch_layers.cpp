@@ -5,7 +5,7 @@
 // Native, because a training step of small layers is bound by the host: the autograd
 // engine runs a backward pass on a thread of its own, where a Python function starts with
 // cold caches and waits for the interpreter's lock. A layer norm's forward and backward
-// (16384 x 1024, 45 us on the GPU) took 146 us as a torch.autograd.Function.
+// (16384 x 1024, 40 us on the GPU) took 146 us as a torch.autograd.Function and take 67 so.
 
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>

@@ -12,6 +12,7 @@ bfloat16 and float16, compute in 32 bits and round each result once. As in `torc
 tensors on the GPU stay there and run on torch's current stream, CPU tensors are moved to
 the current GPU and the results returned on the caller's device, wrong arguments raise
 ValueError, and there is no CPU path. The calls may be captured into a HIP graph.
+`torch_layer.shutdown_gpu` does not concern them: they keep no buffers between calls.
 """
 
 from __future__ import annotations
@@ -67,7 +68,8 @@ def dropout(x: Tensor, p: float, *, seed: int, offset: int = 0, residual: Tensor
     (drh_dropout in include/diffrast_hip.h says which) and is never stored: the backward
     pass draws it again. Call with another offset for another mask, say the step's
     number times the layers plus the layer's. p is applied in steps of 2^-16, and the
-    scale is the inverse of what is applied.
+    scale is the inverse of what is applied. In a captured HIP graph seed and offset are
+    what they were at capture: every replay draws the same mask.
 
     Args:
         x: any shape; p: in [0, 1); seed, offset: integers in [0, 2^64).
