@@ -257,3 +257,35 @@ def test_refusals(layers, change, error):
     t.update(change)
     with pytest.raises(ValueError, match=error):
         layers.linear(t["x"], t["w"], t["b"], t["kind"], t["res"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("K", [64, 72, 96, 128, 136, 160, 192, 224, 320, 328])
+def test_k_tiles_in_turn(layers, K, dtype):
+    """Two groups of waves share an odd or even number of k tiles, whole or not; M in place of K in dW."""
+    t = make(200, 136, K, dtype, res=True)
+    compare(t, "silu", run(layers, t, "silu"), f"200x136x{K}")
+    t = make(K, 136, 200, dtype)
+    compare(t, None, run(layers, t, None), f"{K}x136x200")
+
+
+@pytest.mark.parametrize("M,N", [(200, 136), (2100, 1160)])
+def test_infinities_in_every_k_tile(layers, M, N):
+    """One infinity a row, in any tile of k, alone and against one of the other sign in the next tile."""
+    K = 200
+    t = make(M, N, K, torch.float32, bias=False)
+    x, w = t["x"].detach(), t["w"].detach()
+    inf = float("inf")
+    at = {3: (0,), 70: (31,), 71: (32,), 130: (101,), 190: (199,), 64: (5, 40), 127: (130, 170), M - 1: (64, 96)}
+    for row, ks in at.items():
+        for k in ks:
+            x[row, k] = inf
+    y = run(layers, t, None, train=False)["y"]
+    for row, ks in at.items():
+        sign = w[:, list(ks)].sign()
+        want = torch.where((sign == sign[:, :1]).all(1), sign[:, 0] * inf, float("nan"))
+        assert bool(torch.isclose(y[row], want, rtol=0, atol=0, equal_nan=True).all()), row
+    rest = [i for i in range(M) if i not in at]
+    clean = {k: v for k, v in t.items()}
+    clean["x"] = x[rest].clone()
+    compare(clean, None, {"y": y[rest]}, "other rows")
