@@ -8,7 +8,6 @@
 // (16384 x 1024, 40 us on the GPU) took 146 us as a torch.autograd.Function and take 67 so.
 
 #include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
@@ -131,21 +130,35 @@ bool together(std::initializer_list<Tensor*> ts) {
     return false;
 }
 
-// A node of a layer that is differentiable once: where a graph of the backward pass is
-// asked for, its gradients carry an error for whoever differentiates them again.
+// The history of a gradient that was made with a graph asked for: raises for whoever
+// differentiates it. It leads to all that the gradient depends on (the layer's inputs and the
+// gradient that came in), since the engine skips what is on no path to the inputs asked for.
+struct DifferentiatedAgain : Node {
+    std::string name() const override { return "DiffrastDifferentiatedAgain"; }
+    variable_list apply(variable_list&&) final {
+        throw std::runtime_error("this layer can be differentiated once only");
+    }
+};
+
+// A node of a layer that is differentiable once.
 struct OnceNode : Node {
     variable_list apply(variable_list&& grads) final {
         std::lock_guard<std::mutex> lock(mutex_);
-        const bool again = at::GradMode::is_enabled();
         variable_list r;
         {
             at::NoGradGuard no;
             r = grads[0].defined() ? gradients(grads[0]) : variable_list(num_outputs());
         }
-        if (again) {
-            auto error = std::make_shared<torch::autograd::DelayedError>(
-                "this layer can be differentiated once only", (int64_t)r.size());
-            return (*error)(std::move(r));
+        if (at::GradMode::is_enabled() && grads[0].defined()) {
+            torch::autograd::edge_list edges = next_edges();
+            edges.push_back(torch::autograd::impl::gradient_edge(grads[0]));
+            auto error = std::shared_ptr<Node>(new DifferentiatedAgain(), torch::autograd::deleteNode);
+            error->set_next_edges(std::move(edges));
+            for (Tensor& t : r)
+                if (t.defined()) {
+                    t = t.detach();
+                    torch::autograd::set_history(t, error);
+                }
         }
         return r;
     }
