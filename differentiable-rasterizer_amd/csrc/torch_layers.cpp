@@ -10,10 +10,13 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <mutex>
 #include <optional>
@@ -112,6 +115,26 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     return false;
 }
 
+// The layers are no operators that torch's dispatcher sees: a trace would record the output's
+// allocation alone.
+void refuse_tracing() {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() && !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) &&
+                                    !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE) &&
+                                    !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch),
+                                "the network layers cannot be traced (torch.jit.trace, make_fx, fake tensors)");
+}
+
+// Nor have they tangents: without this a derivative in forward mode would be zero.
+void refuse_transforms(std::initializer_list<const Tensor*> ts) {
+    refuse_tracing();
+    if (!at::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : ts)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
+                                    "the network layers have no forward-mode derivative");
+}
+
 // Whether every tensor is on the GPU that x is on; if not, they are moved there (to the
 // current GPU where x is on none).
 bool together(std::initializer_list<Tensor*> ts) {
@@ -144,6 +167,7 @@ struct DifferentiatedAgain : Node {
 struct OnceNode : Node {
     variable_list apply(variable_list&& grads) final {
         std::lock_guard<std::mutex> lock(mutex_);
+        refuse_transforms({&grads[0]});
         variable_list r;
         {
             at::NoGradGuard no;
@@ -234,6 +258,7 @@ Tensor layer_norm(Tensor x, const Optional& weight, const Optional& bias, double
     vector(b, "bias");
     TORCH_CHECK_VALUE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(), "weight is ", w.scalar_type(),
                       " but bias ", b.scalar_type());
+    refuse_transforms({&x, &w, &b});
     const at::Device home = x.device();
     if (!together({&x, &w, &b})) return layer_norm(x, w.defined() ? Optional(w) : std::nullopt,
                                                    b.defined() ? Optional(b) : std::nullopt, eps).to(home);
@@ -320,6 +345,7 @@ Tensor linear(Tensor x, Tensor w, const Optional& bias, int act, const Optional&
     typed(w, "weight");
     typed(b, "bias");
     typed(res, "residual");
+    refuse_transforms({&x, &w, &b, &res});
     const at::Device home = x.device();
     if (!together({&x, &w, &b, &res}))
         return linear(x, w, b.defined() ? Optional(b) : std::nullopt, act, res.defined() ? Optional(res) : std::nullopt)
@@ -377,6 +403,7 @@ Tensor dropout(Tensor x, double p, uint64_t seed, uint64_t offset, const Optiona
     TORCH_CHECK_VALUE(!res.defined() || (res.sizes() == x.sizes() && res.scalar_type() == x.scalar_type()),
                       "expected a residual of shape ", x.sizes(), " in ", x.scalar_type(), ", got ",
                       res.defined() ? res.sizes() : x.sizes(), " in ", res.defined() ? res.scalar_type() : x.scalar_type());
+    refuse_transforms({&x, &res});
     const at::Device home = x.device();
     if (!together({&x, &res})) return dropout(x, p, seed, offset, res.defined() ? Optional(res) : std::nullopt).to(home);
     const bool grad = wants_grad({&x, &res});

@@ -11,7 +11,9 @@ and has no counterpart of these. All of them are differentiable once, take float
 bfloat16 and float16, compute in 32 bits and round each result once. As in `torch_layer`,
 tensors on the GPU stay there and run on torch's current stream, CPU tensors are moved to
 the current GPU and the results returned on the caller's device, wrong arguments raise
-ValueError, and there is no CPU path. The calls may be captured into a HIP graph.
+ValueError, and there is no CPU path. Differentiating a gradient again raises RuntimeError, and
+forward-mode derivatives and tracers (torch.jit.trace, make_fx, fake tensors) NotImplementedError;
+torch.compile runs the calls outside of its graphs. The calls may be captured into a HIP graph.
 `torch_layer.shutdown_gpu` does not concern them: they keep no buffers between calls.
 """
 
