@@ -152,6 +152,8 @@ struct Loader {
             const uint32_t dst = __builtin_amdgcn_readfirstlane(lds + (i * WAVES + w) * 1024);
             uint32_t o = off[u][i];
             if constexpr (KC) o = kc < left ? o : PAST_END;
+            // m0, the destination, is a reserved register: the compiler keeps nothing in it, and a
+            // clobber list may not name it
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(o),
                          "s"(rsrc)
                          : "memory");
