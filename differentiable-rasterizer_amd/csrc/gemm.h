@@ -218,17 +218,19 @@ struct Frags {
 // Straight: with the instructions of the operands' own type.
 //
 // Thirds, for 32 bits: v = v1 + v2 + v3 in bfloat16, each the first eight bits of what is left,
-// is exact (3 x 8 bits), and a b is a1 b1 + a1 b2 + a2 b1 + a2 b2 + a1 b3 + a3 b1 but for less
-// than 2^-21 |a b|, 2^-24 in the mean. Six bfloat16 products take 96 cycles of the matrix core
-// where the 32-bit instructions take 256, and splitting costs 5.5 vector operations an
-// element, four behind each matrix instruction of a 64 x 64 quarter. (Rounding each third to the
-// nearest is as many operations, but the conversion is a slow one.) Alone, a matrix instruction
-// and four such operations take 12 ns with one wave a SIMD and 10 with two, 8 and 7 without them:
-// the two kinds overlap in part. 4096^3 takes 700 to 760 us (190 TFLOP/s in 32 bits, 1.15 P in
-// bfloat16, where the power limit has the clock) however the splits are placed; with one
-// workgroup a CU, between the next tile's instructions instead of before them, 4096 x 1024
-// outputs and k = 1024 take 60 us instead of 65. Infinities come out as NaN: see gemm_tile's
-// second pass.
+// is exact (3 x 8 bits) from about 2^-111 on, above bfloat16's smallest number, 2^-133, by all of
+// them; a tile with a smaller operand is made again (gemm_tile's second pass). a b is a1 b1 + a1 b2
+// + a2 b1 + a2 b2 + a1 b3 + a3 b1 but for less than 2^-21 |a b|, 2^-24 in the mean; thirds have
+// their value's sign, so what is dropped of a product has the product's. Six bfloat16 products
+// take 96 cycles of the matrix core where the 32-bit instructions take 256, and splitting costs six
+// vector operations an element, four to five behind each matrix instruction of a 64 x 64 quarter.
+// (Rounding each third to the nearest is as many operations, but the conversion is a slow one.)
+// Alone, a matrix instruction and four such operations take 12 ns with one wave a SIMD and 10 with
+// two, 8 and 7 without them: the two kinds overlap in part. 4096^3 takes 700 to 760 us (190
+// TFLOP/s in 32 bits, 1.15 P in bfloat16, where the power limit has the clock) however the splits
+// are placed; with one workgroup a CU, between the next tile's instructions instead of before
+// them, 4096 x 1024 outputs and k = 1024 take 60 us instead of 65. Infinities come out as NaN: see
+// gemm_tile's second pass.
 struct Straight {
     template <class FA, class FB, int NA, int NB>
     static __device__ inline void multiply(const FA& a, const FB& b, floatx4 (&acc)[NA][NB]) {
@@ -253,13 +255,18 @@ struct Thirds {
             r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, r[i]) - __builtin_bit_cast(float, m[i]));
         }
     };
+    // `lost` gathers what the last third leaves in its lower 16 bits.
     template <class F>
-    static __device__ inline void split(const F (&f)[2], Held& to, int i, int part, Pair& p) {
+    static __device__ inline void split(const F (&f)[2], Held& to, int i, int part, Pair& p, uint32_t& lost) {
         if (part == 0)
 #pragma unroll
             for (int e = 0; e < 2; e++) p.r[e] = __builtin_bit_cast(uint32_t, (float)f[i / 2][2 * (i % 2) + e]);
         if (part == 1) p.less(1);
-        if (part == 2) p.less(0), p.less(1);
+        if (part == 2) {
+            p.less(0), p.less(1);
+            lost |= p.r[0] | p.r[1];
+            asm volatile("" : "+v"(lost));  // here, so that nothing of the pairs is kept for it
+        }
         uint32_t both = __builtin_amdgcn_perm(p.r[1], p.r[0], 0x07060302);  // the upper halves
         asm volatile("" : "+v"(both));  // here, not where it is used
         to.third[part][i] = both;
@@ -269,12 +276,12 @@ struct Thirds {
         if (part == 0) p.less(0);
     }
     template <class F>
-    static __device__ inline void split(const F (&f)[2], Held& to) {
+    static __device__ inline void split(const F (&f)[2], Held& to, uint32_t& lost) {
         Pair p;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int part = 0; part < 3; part++) split(f, to, i, part, p);
+            for (int part = 0; part < 3; part++) split(f, to, i, part, p, lost);
     }
     static __device__ inline vec<bf16, 8> term(const Held& h, int third) {
         return __builtin_bit_cast(vec<bf16, 8>, h.third[third]);
@@ -283,7 +290,7 @@ struct Thirds {
     // the parts of SPLITS splits, v0 to h0 and v1 to h1.
     template <int SPLITS, int NF, class FA, class FB>
     static __device__ inline void row(const Held& a, const Held (&b)[NF], floatx4 (&acc)[NF], const FA& v0, Held& h0,
-                                      const FB& v1, Held& h1) {
+                                      const FB& v1, Held& h1, uint32_t& lost) {
         constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0}, PARTS = 4 / NF;
         Pair p;
 #pragma unroll
@@ -292,8 +299,8 @@ struct Thirds {
 #pragma unroll
             for (int e = 0; e < PARTS; e++) {
                 const int n = m * PARTS + e;
-                if (n < 12 && SPLITS > 0) split(v0, h0, n / 3, n % 3, p);
-                if (n >= 12 && SPLITS > 1) split(v1, h1, (n - 12) / 3, n % 3, p);
+                if (n < 12 && SPLITS > 0) split(v0, h0, n / 3, n % 3, p, lost);
+                if (n >= 12 && SPLITS > 1) split(v1, h1, (n - 12) / 3, n % 3, p, lost);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -464,6 +471,7 @@ __device__ inline void gemm_tile(const Gemm& p) {
         FA fa;
         FB fb;
         Thirds::Held ha[2], even[NF], odd[NF];
+        uint32_t lost = 0;
         load(0, 0);
         load(1, 1);
         wait_vm<LA::LOADS + LB::LOADS>();
@@ -471,16 +479,16 @@ __device__ inline void gemm_tile(const Gemm& p) {
         fa.read(mine, wm);
         fb.read(mine + UNIT, wn);
 #pragma unroll
-        for (int j = 0; j < NF; j++) Thirds::split(fb.f[j], even[j]);
-        Thirds::split(fa.f[0], ha[0]);
+        for (int j = 0; j < NF; j++) Thirds::split(fb.f[j], even[j], lost);
+        Thirds::split(fa.f[0], ha[0], lost);
         auto multiply = [&](const char* b, const Thirds::Held (&now)[NF], Thirds::Held (&next)[NF], auto more) {
             constexpr bool MORE = more.value;
             if (MORE) fb.read(b + UNIT, wn);
 #pragma unroll
             for (int r = 0; r < NF - 1; r++)
-                Thirds::row<MORE ? 2 : 1>(ha[r & 1], now, acc[r], fa.f[r + 1], ha[(r + 1) & 1], fb.f[r], next[r]);
+                Thirds::row<MORE ? 2 : 1>(ha[r & 1], now, acc[r], fa.f[r + 1], ha[(r + 1) & 1], fb.f[r], next[r], lost);
             if (MORE) fa.read(b, wm);
-            Thirds::row<MORE ? 2 : 0>(ha[1], now, acc[NF - 1], fb.f[NF - 1], next[NF - 1], fa.f[0], ha[0]);
+            Thirds::row<MORE ? 2 : 0>(ha[1], now, acc[NF - 1], fb.f[NF - 1], next[NF - 1], fa.f[0], ha[0], lost);
         };
         auto step = [&](int64_t i, const Thirds::Held (&now)[NF], Thirds::Held (&next)[NF]) {
             const int stage = (int)i & 1;
@@ -499,13 +507,14 @@ __device__ inline void gemm_tile(const Gemm& p) {
         }
         wait_all();
         // A result that is not finite comes from an infinity, a NaN or an overflow. The thirds turn
-        // the first into NaN, so the tile is made again with instructions that do not.
+        // the first into NaN, and lose bits of what is too small for them: the tile is made again with
+        // instructions that do neither.
         float zero = 0.0f;
 #pragma unroll
         for (int i = 0; i < NF * NF; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) zero = fmaf(acc[i / NF][i % NF][e], 0.0f, zero);
-        if (__syncthreads_or(!(zero == 0.0f))) {
+        if (__syncthreads_or(!(zero == 0.0f) || (lost & 0xffffu))) {
 #pragma unroll
             for (int i = 0; i < NF * NF; i++) acc[i / NF][i % NF] = floatx4{};
             straight();
