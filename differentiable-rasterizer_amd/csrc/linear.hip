@@ -559,6 +559,9 @@ int64_t slope_groups(int64_t M, int64_t N, int dtype) {
     return std::min(need, most);
 }
 
+// A single row has no stride: whatever the caller gives for it must not name rows behind it.
+int64_t stride_of(int64_t rows, int64_t stride, int64_t K) { return rows > 1 ? stride : K; }
+
 struct ForwardPlan {
     Rows x, w;
     GemmPlan y;
@@ -567,6 +570,7 @@ struct ForwardPlan {
 
 ForwardPlan forward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype) {
     ForwardPlan f;
+    xs = stride_of(M, xs, K), ws = stride_of(N, ws, K);
     if (K > 0 && (M <= ROWS_FEW || (M <= ROWS_MOST && K <= ROWS_MOST_K))) {
         f.x = {xs}, f.w = {ws}, f.y.rows = true;
         return f;
@@ -595,6 +599,7 @@ struct BackwardPlan {
 
 BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype, int act) {
     BackwardPlan b;
+    xs = stride_of(M, xs, K), ws = stride_of(N, ws, K);
     const int64_t ch = 16 / (int64_t)type_size(dtype), N_pad = (N + ch - 1) / ch * ch, K_pad = (K + ch - 1) / ch * ch;
     b.x = rows_for(dtype, M, K, xs);
     b.w = rows_for(dtype, N, K, ws);
