@@ -356,6 +356,20 @@ int64_t ln_backward_groups(int64_t rows, int64_t cols, int dtype) {
     return need < most ? need : most;
 }
 
+// f(p) for p's rows, at most `groups` a launch times `per` rows each.
+template <class T, class F>
+void row_launches(const LnArgs& p, int64_t groups, int64_t per, F&& f) {
+    in_launches(p.rows, groups * per, [&](int64_t first, int64_t count) {
+        LnArgs q = p;
+        auto at = [&](auto ptr, int64_t n) { return ptr ? ptr + n : ptr; };
+        q.x = at((const T*)p.x, first * p.xs), q.g = at((const T*)p.g, first * p.gs);
+        q.y = at((T*)p.y, first * p.cols), q.dx = at((T*)p.dx, first * p.cols);
+        q.mean = at(p.mean, first), q.rstd = at(p.rstd, first);
+        q.rows = count;
+        f(q, dim3((unsigned)((count + per - 1) / per)));
+    });
+}
+
 int check_ln(drh_ctx* ctx, int64_t rows, int64_t cols, int dtype, int weight_dtype, uint32_t flags) {
     int rc = check_call(ctx, dtype, flags);
     if (rc) return rc;
@@ -391,14 +405,16 @@ int drh_layer_norm(drh_ctx* ctx, const void* x, const void* weight, const void* 
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
         if (cols > LN_MAX_COLS) {
-            ln_forward_wide<T><<<dim3((unsigned)rows), WIDE, 0, s>>>(p);
+            row_launches<T>(p, most_groups(WIDE), 1,
+                            [&](const LnArgs& q, dim3 grid) { ln_forward_wide<T><<<grid, WIDE, 0, s>>>(q); });
             return DRH_OK;
         }
         with_row<T>(cols, [&](auto tpr, auto ept) {
             constexpr int THREADS = tpr.value > 256 ? tpr.value : 256, RPB = THREADS / tpr.value;
-            const dim3 grid((unsigned)((rows + RPB - 1) / RPB));
             with_loads<T>(rows, cols, [&](auto whole, auto once) {
-                ln_forward<T, ept.value, tpr.value, THREADS, whole.value, once.value><<<grid, THREADS, 0, s>>>(p);
+                row_launches<T>(p, most_groups(THREADS), RPB, [&](const LnArgs& q, dim3 grid) {
+                    ln_forward<T, ept.value, tpr.value, THREADS, whole.value, once.value><<<grid, THREADS, 0, s>>>(q);
+                });
             });
         });
         return DRH_OK;
@@ -437,7 +453,9 @@ int drh_layer_norm_backward(drh_ctx* ctx, const void* x, const void* weight, con
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
             if (cols > LN_MAX_COLS) {
-                if (grad_x) ln_backward_wide<T><<<dim3((unsigned)rows), WIDE, 0, s>>>(p);
+                if (grad_x)
+                    row_launches<T>(p, most_groups(WIDE), 1,
+                                    [&](const LnArgs& q, dim3 grid) { ln_backward_wide<T><<<grid, WIDE, 0, s>>>(q); });
                 if (sums)
                     ln_columns_wide<T><<<dim3((unsigned)((cols + 63) / 64), (unsigned)groups), 64, 0, s>>>(p);
                 return DRH_OK;

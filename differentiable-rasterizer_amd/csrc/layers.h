@@ -110,6 +110,16 @@ inline size_t type_size(int dtype) { return dtype == DRH_F32 ? 4 : 2; }
 inline bool known_type(int dtype) { return dtype == DRH_F32 || dtype == DRH_BF16 || dtype == DRH_F16; }
 inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// A launch has fewer threads than this in x; what needs more takes several launches.
+constexpr int64_t LAUNCH_THREADS = 1ll << 32;
+constexpr int64_t most_groups(int64_t threads) { return (LAUNCH_THREADS - 1) / threads; }
+
+// f(first, count) for n units, `most` at a time.
+template <class F>
+void in_launches(int64_t n, int64_t most, F&& f) {
+    for (int64_t first = 0; first < n; first += most) f(first, n - first < most ? n - first : most);
+}
+
 // Checks that every layer call makes; the flags a layer knows are DRH_SYNC alone.
 int check_call(drh_ctx* ctx, int dtype, uint32_t flags);
 // After the last launch: its error, and DRH_SYNC's wait.

@@ -14,11 +14,11 @@ namespace {
 constexpr int RC_WAVES = 16;
 template <class T>
 __global__ __launch_bounds__(64 * RC_WAVES) void reduce_columns_kernel(const float* __restrict__ part, int64_t groups,
-                                                                       int64_t stride, int64_t cols, T* out_a,
-                                                                       T* out_b) {
+                                                                       int64_t stride, int64_t cols, int64_t first,
+                                                                       T* out_a, T* out_b) {
     __shared__ float sums[RC_WAVES][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.x * 64 + lane, n = out_b ? 2 * cols : cols;
+    const int64_t col = first + (int64_t)blockIdx.x * 64 + lane, n = out_b ? 2 * cols : cols;
     float s = 0.0f;
     if (col < n)
 #pragma unroll 4
@@ -57,8 +57,10 @@ int reduce_columns(const float* part, int64_t groups, int64_t stride, int64_t co
     if (n == 0) return DRH_OK;
     return with_type(out_dtype, [&](auto t) {
         using T = decltype(t);
-        reduce_columns_kernel<T><<<dim3((unsigned)((n + 63) / 64)), 64 * RC_WAVES, 0, s>>>(
-            part, groups, stride, cols, (T*)out_a, (T*)out_b);
+        in_launches((n + 63) / 64, most_groups(64 * RC_WAVES), [&](int64_t first, int64_t count) {
+            reduce_columns_kernel<T><<<dim3((unsigned)count), 64 * RC_WAVES, 0, s>>>(part, groups, stride, cols, first * 64,
+                                                                                     (T*)out_a, (T*)out_b);
+        });
         return DRH_OK;
     });
 }

@@ -362,7 +362,7 @@ GemmPlan plan_gemm(int dtype, int64_t M, int64_t N, int64_t K, bool fits) {
     for (int tile : {256, 128, 64}) {
         if (tile == 256 && dtype == DRH_F32) continue;
         const int64_t tiles = (M + tile - 1) / tile * ((N + tile - 1) / tile);
-        if (tiles > INT32_MAX) continue;
+        if (tiles > most_groups(tile == 256 ? 512 : 256)) continue;
         for (int64_t s = 1; s <= 64 && s <= kt; s++) {
             const int64_t per = (kt + s - 1) / s;
             if ((kt + per - 1) / per != s) continue;
@@ -387,15 +387,23 @@ int with_act(int act, F&& f) {
     }
 }
 
+bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+// Whether a product's launch holds its tiles: a plan's always, gemm_any_kernel's 64 x 64 not
+// from 2^36 outputs on.
+int check_tiles(const GemmPlan& plan, int64_t M, int64_t N, const void* a, const void* b) {
+    if (plan.rows || (plan.tile && aligned(a) && aligned(b))) return DRH_OK;
+    if ((M + 63) / 64 * ((N + 63) / 64) <= most_groups(256)) return DRH_OK;
+    return fail(DRH_ERR_TOO_LARGE, "more tiles of the output than a launch holds");
+}
+
 // p without its plan's fields; `partial` has plan.bytes bytes.
 int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial, hipStream_t s) {
     if (p.M == 0 || p.N == 0) return DRH_OK;
     const int64_t ch = 16 / (int64_t)type_size(dtype);
-    auto aligned = [](const void* q) { return (uintptr_t)q % 16 == 0; };
     const bool fast = plan.tile && aligned(p.a.ptr) && aligned(p.b.ptr);
     const int tile = fast ? plan.tile : 64;  // gemm_any_kernel's too
     const int64_t tiles = (p.M + tile - 1) / tile * ((p.N + tile - 1) / tile);
-    if (tiles > INT32_MAX) return fail(DRH_ERR_TOO_LARGE, "more than 2^31 - 1 tiles of the output");
     p.splits = fast ? plan.splits : 1;
     const int64_t bk = 128 / (int64_t)type_size(dtype), kt = (p.K + bk - 1) / bk;
     p.tiles_per_split = (int)((kt + p.splits - 1) / p.splits);
@@ -479,10 +487,10 @@ struct PadJob {
 
 // Two operands of K columns in one launch, a thread a 16-byte chunk.
 template <class T>
-__global__ __launch_bounds__(256) void pad_rows(PadJob a, PadJob b, int64_t K) {
+__global__ __launch_bounds__(256) void pad_rows(PadJob a, PadJob b, int64_t K, int64_t first) {
     constexpr int CH = 16 / sizeof(T);
     const int64_t per = (K + CH - 1) / CH;
-    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    int64_t i = (first + blockIdx.x) * 256 + threadIdx.x;
     const bool second = i >= a.rows * per;
     if (second) i -= a.rows * per;
     const PadJob& job = second ? b : a;
@@ -496,7 +504,9 @@ void pad(int dtype, const PadJob& a, const PadJob& b, int64_t K, hipStream_t s) 
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
         const int64_t ch = 16 / (int64_t)sizeof(T), chunks = (a.rows + b.rows) * ((K + ch - 1) / ch);
-        if (chunks) pad_rows<T><<<dim3((unsigned)((chunks + 255) / 256)), 256, 0, s>>>(a, b, K);
+        in_launches((chunks + 255) / 256, most_groups(256), [&](int64_t first, int64_t count) {
+            pad_rows<T><<<dim3((unsigned)count), 256, 0, s>>>(a, b, K, first);
+        });
         return DRH_OK;
     });
 }
@@ -571,7 +581,7 @@ struct ForwardPlan {
 ForwardPlan forward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype) {
     ForwardPlan f;
     xs = stride_of(M, xs, K), ws = stride_of(N, ws, K);
-    if (K > 0 && (M <= ROWS_FEW || (M <= ROWS_MOST && K <= ROWS_MOST_K))) {
+    if (K > 0 && (M <= ROWS_FEW || (M <= ROWS_MOST && K <= ROWS_MOST_K)) && (N + 15) / 16 <= most_groups(512)) {
         f.x = {xs}, f.w = {ws}, f.y.rows = true;
         return f;
     }
@@ -665,6 +675,8 @@ int drh_linear(drh_ctx* ctx, const void* x, const void* weight, const void* bias
     const ForwardPlan plan = forward_plan(rows, n_out, n_in, x_stride, weight_stride, dtype);
     rc = check_workspace(plan.total, workspace, workspace_bytes);
     if (rc) return rc;
+    rc = check_tiles(plan.y, rows, n_out, plan.x.bytes ? nullptr : x, plan.w.bytes ? nullptr : weight);
+    if (rc) return rc;
     DeviceGuard dg(ctx->device);
     hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)workspace;
@@ -701,6 +713,10 @@ int drh_linear_backward(drh_ctx* ctx, const void* x, const void* weight, const v
         return fail(DRH_ERR_INVALID_ARG, "an input pointer is NULL");
     const BackwardPlan plan = backward_plan(M, N, K, x_stride, weight_stride, dtype, activation);
     rc = check_workspace(plan.total, workspace, workspace_bytes);
+    if (rc) return rc;
+    const void* own_dz = plan.dz ? nullptr : grad_y;  // what the call copies stands aligned
+    if (grad_x) rc = check_tiles(plan.dx, M, K, own_dz, plan.w.bytes ? nullptr : weight);
+    if (!rc && grad_weight) rc = check_tiles(plan.dw, N, K, own_dz, plan.x.bytes ? nullptr : x);
     if (rc) return rc;
     DeviceGuard dg(ctx->device);
     hipStream_t s = (hipStream_t)stream;
