@@ -207,37 +207,37 @@ std::shared_ptr<N> new_node() {
 
 // ---------------------------------------------------------------- layer norm
 
+// Keeps what the gradients that are wanted need: weight where dx is, never the bias.
 struct LayerNormBackward : OnceNode {
-    SavedVariable x_, weight_, bias_, stats_;
-    bool has_weight = false, has_bias = false;
+    SavedVariable x_, weight_, stats_;
+    at::ScalarType weight_type = at::kFloat;  // and the bias's
+    int weight_code = DRH_F32;
+    bool keeps_weight = false;
 
     std::string name() const override { return "DiffrastLayerNormBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
         x_.reset_data();
         weight_.reset_data();
-        bias_.reset_data();
         stats_.reset_data();
     }
 
     variable_list gradients(const Tensor& g) override {
-        const Tensor x = x_.unpack(), stats = stats_.unpack();
-        const Tensor w = has_weight ? weight_.unpack() : Tensor(), b = has_bias ? bias_.unpack() : Tensor();
+        const Tensor x = x_.unpack(), stats = stats_.unpack(), w = keeps_weight ? weight_.unpack() : Tensor();
         const Tensor xv = as_rows(x), gv = as_rows(g), wv = flat(w);
         const int64_t rows = xv.size(0), cols = xv.size(1);
         variable_list r(3);
         if (task_should_compute_output(0)) r[0] = at::empty(g.sizes(), x.options());
-        if (has_weight && task_should_compute_output(1)) r[1] = at::empty({cols}, w.options());
-        if (has_bias && task_should_compute_output(2)) r[2] = at::empty({cols}, b.options());
+        for (int i : {1, 2})
+            if (task_should_compute_output(i)) r[i] = at::empty({cols}, x.options().dtype(weight_type));
         uint64_t bytes = 0;
         if (r[1].defined() || r[2].defined()) check(drh_layer_norm_backward_bytes(rows, cols, dtype_code(x), &bytes));
         const Tensor ws = workspace(bytes, x);
-        const int code = dtype_code(x), wcode = has_weight ? dtype_code(w) : has_bias ? dtype_code(b) : code;
         const float* mean = stats.const_data_ptr<float>();
         Call call(x);
         check(drh_layer_norm_backward(call.ctx, in(xv), in(wv), mean, mean + rows, in(gv), rows, cols, row_stride(xv),
-                                      row_stride(gv), code, wcode, out(r[0]), out(r[1]), out(r[2]), out(ws), bytes,
-                                      call.stream, 0));
+                                      row_stride(gv), dtype_code(x), weight_code, out(r[0]), out(r[1]), out(r[2]), out(ws),
+                                      bytes, call.stream, 0));
         return r;
     }
 };
@@ -263,6 +263,8 @@ Tensor layer_norm(Tensor x, const Optional& weight, const Optional& bias, double
     if (!together({&x, &w, &b})) return layer_norm(x, w.defined() ? Optional(w) : std::nullopt,
                                                    b.defined() ? Optional(b) : std::nullopt, eps).to(home);
     const bool grad = wants_grad({&x, &w, &b});
+    const at::ScalarType wtype = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : x.scalar_type();
+    const int wcode = w.defined() ? dtype_code(w) : b.defined() ? dtype_code(b) : code;
     Tensor y, stats;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -274,7 +276,6 @@ Tensor layer_norm(Tensor x, const Optional& weight, const Optional& bias, double
             stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
             mean = stats.mutable_data_ptr<float>();
         }
-        const int wcode = w.defined() ? dtype_code(w) : b.defined() ? dtype_code(b) : code;
         Call call(x);
         check(drh_layer_norm(call.ctx, in(xv), in(wv), in(bv), rows, cols, row_stride(xv), code, wcode, (float)eps, out(y),
                              mean, mean ? mean + rows : nullptr, call.stream, 0));
@@ -283,17 +284,23 @@ Tensor layer_norm(Tensor x, const Optional& weight, const Optional& bias, double
     auto node = new_node<LayerNormBackward>();
     node->x_ = SavedVariable(x, false);
     node->stats_ = SavedVariable(stats, false);
-    if ((node->has_weight = w.defined())) node->weight_ = SavedVariable(w, false);
-    if ((node->has_bias = b.defined())) node->bias_ = SavedVariable(b, false);
+    if ((node->keeps_weight = w.defined() && x.requires_grad())) node->weight_ = SavedVariable(w, false);
+    node->weight_type = wtype;
+    node->weight_code = wcode;
     return attach(std::move(y), std::move(node), {&x, &w, &b});
 }
 
 // ---------------------------------------------------------------- linear
 
+// Keeps what the gradients that are wanted need: x where dW is, the weight where dx is, the
+// slopes where any is but the residual's.
 struct LinearBackward : OnceNode {
     SavedVariable x_, weight_, kept_;
-    int act = 0;
-    bool has_kept = false;
+    std::vector<int64_t> x_sizes;
+    at::TensorOptions options;
+    int64_t rows = 0, n_out = 0, n_in = 0;
+    int act = 0, code = 0;
+    bool keeps_x = false, keeps_weight = false, has_kept = false;
 
     std::string name() const override { return "DiffrastLinearBackward"; }
     void release_variables() override {
@@ -304,22 +311,20 @@ struct LinearBackward : OnceNode {
     }
 
     variable_list gradients(const Tensor& grad) override {
-        const Tensor x = x_.unpack(), w = weight_.unpack(), kept = has_kept ? kept_.unpack() : Tensor();
-        const Tensor xv = as_rows(x), wv = as_rows(w);
-        const int64_t rows = xv.size(0), n_in = xv.size(1), n_out = wv.size(0);
+        const Tensor kept = has_kept ? kept_.unpack() : Tensor();
+        const Tensor xv = keeps_x ? as_rows(x_.unpack()) : Tensor(), wv = keeps_weight ? as_rows(weight_.unpack()) : Tensor();
         const Tensor g = flat(grad);
         variable_list r(4);
-        if (task_should_compute_output(0)) r[0] = at::empty(x.sizes(), x.options());
-        if (task_should_compute_output(1)) r[1] = at::empty({n_out, n_in}, x.options());
-        if (task_should_compute_output(2)) r[2] = at::empty({n_out}, x.options());
+        if (task_should_compute_output(0)) r[0] = at::empty(x_sizes, options);
+        if (task_should_compute_output(1)) r[1] = at::empty({n_out, n_in}, options);
+        if (task_should_compute_output(2)) r[2] = at::empty({n_out}, options);
         if (task_should_compute_output(3)) r[3] = grad;
         if (!r[0].defined() && !r[1].defined() && !r[2].defined()) return r;
-        const int code = dtype_code(x);
-        const int64_t xs = row_stride(xv), ws = row_stride(wv);
+        const int64_t xs = xv.defined() ? row_stride(xv) : n_in, ws = wv.defined() ? row_stride(wv) : n_in;
         uint64_t bytes = 0;
         check(drh_linear_backward_bytes(rows, n_out, n_in, xs, ws, code, act, &bytes));
-        const Tensor space = workspace(bytes, x);
-        Call call(x);
+        const Tensor space = workspace(bytes, g);
+        Call call(g);
         check(drh_linear_backward(call.ctx, in(xv), in(wv), in(kept), in(g), rows, n_out, n_in, xs, ws, code, act, out(r[0]),
                                   out(r[1]), out(r[2]), out(space), bytes, call.stream, 0));
         return r;
@@ -350,12 +355,14 @@ Tensor linear(Tensor x, Tensor w, const Optional& bias, int act, const Optional&
     if (!together({&x, &w, &b, &res}))
         return linear(x, w, b.defined() ? Optional(b) : std::nullopt, act, res.defined() ? Optional(res) : std::nullopt)
             .to(home);
-    const bool grad = wants_grad({&x, &w, &b, &res}), keep = grad && act != DRH_ACT_NONE;
+    const bool grad = wants_grad({&x, &w, &b, &res}), keep = act != DRH_ACT_NONE && wants_grad({&x, &w, &b});
     Tensor y, kept;
+    int64_t rows = 0;
     {
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor xv = as_rows(x), wv = as_rows(w), bv = flat(b), rv = flat(res);
-        const int64_t rows = xv.size(0), xs = row_stride(xv), ws = row_stride(wv);
+        rows = xv.size(0);
+        const int64_t xs = row_stride(xv), ws = row_stride(wv);
         y = at::empty(shape, x.options());
         if (keep) kept = at::empty({rows, n_out}, x.options().dtype(code == DRH_F32 ? at::kFloat : at::kHalf));
         uint64_t bytes = 0;
@@ -367,9 +374,12 @@ Tensor linear(Tensor x, Tensor w, const Optional& bias, int act, const Optional&
     }
     if (!grad) return y;
     auto node = new_node<LinearBackward>();
-    node->x_ = SavedVariable(x, false);
-    node->weight_ = SavedVariable(w, false);
-    node->act = act;
+    if ((node->keeps_x = w.requires_grad())) node->x_ = SavedVariable(x, false);
+    if ((node->keeps_weight = x.requires_grad())) node->weight_ = SavedVariable(w, false);
+    node->x_sizes = x.sizes().vec();
+    node->options = x.options();
+    node->rows = rows, node->n_out = n_out, node->n_in = n_in;
+    node->act = act, node->code = code;
     if ((node->has_kept = keep)) node->kept_ = SavedVariable(kept, false);
     return attach(std::move(y), std::move(node), {&x, &w, &b, &res});
 }
