@@ -26,7 +26,7 @@ struct Gemm {
     Operand a, b;
     int64_t M, N, K;
     const void *bias, *res;  // N; M x N
-    void* kept;              // M x N of Kept<T>: the activation's slopes; or null
+    void* kept;              // M x N of Kept<T>: the activation's slopes, scaled; or null
     void* out;               // M x N
     float* partial;          // splits x M x N sums instead of `out`, or null
     int act;

@@ -6,8 +6,9 @@
 // Products run on the matrix cores with 32-bit sums. Each result is rounded to its type
 // once, from 32 bits. The backward pass needs act'(z) alone, so the forward pass, which has
 // act's exponential at hand, keeps that and not z: in 16 bits beside the 16-bit types, in
-// float16 whatever the type is, since slopes are within [-0.13, 1.13] and its 11 bits keep
-// them eight times nearer than bfloat16's 8 would.
+// float16 whatever the type is, since its 11 bits keep a slope eight times nearer than
+// bfloat16's 8 would. Slopes are within [-0.13, 1.13]: kept times 2^15 they fill float16's
+// range, with all 11 bits down to 2e-9, where the gradients of an activation's tail still count.
 
 #include <algorithm>
 #include <cmath>
@@ -82,6 +83,8 @@ __device__ inline float act(float z, float& slope) {
 // The type that slopes are kept in.
 template <class T>
 using Kept = std::conditional_t<sizeof(T) == 4, float, f16>;
+template <class T>
+constexpr float KEPT_SCALE = sizeof(T) == 4 ? 1.0f : 32768.0f;
 
 // ---------------------------------------------------------------- the product's epilogue
 
@@ -139,7 +142,7 @@ struct Epilogue {
         if constexpr (ACT != DRH_ACT_NONE) {
             float slope[C];
 #pragma unroll
-            for (int i = 0; i < C; i++) o[i] = act<sizeof(T) == 4, ACT>(o[i], slope[i]);
+            for (int i = 0; i < C; i++) o[i] = act<sizeof(T) == 4, ACT>(o[i], slope[i]), slope[i] *= KEPT_SCALE<T>;
             if (p.kept) store((Kept<T>*)p.kept + at, slope);
         }
         if (p.res)
@@ -535,7 +538,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
         const Elements<T> ge = __builtin_bit_cast(Elements<T>, gr);
         const Elements<Kept<T>> de = __builtin_bit_cast(Elements<Kept<T>>, dr);
 #pragma unroll
-        for (int i = 0; i < CH; i++) g[i] = (float)ge[i], d[i] = slope ? (float)de[i] : 1.0f;
+        for (int i = 0; i < CH; i++) g[i] = (float)ge[i], d[i] = slope ? (float)de[i] * (1.0f / KEPT_SCALE<T>) : 1.0f;
     };
     auto finish = [&](int64_t row, float (&g)[CH], const float (&d)[CH]) {
         if (row >= M) return;

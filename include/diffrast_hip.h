@@ -375,7 +375,8 @@ enum { DRH_ACT_NONE = 0, DRH_ACT_RELU = 1, DRH_ACT_GELU = 2, DRH_ACT_GELU_TANH =
  * x_stride elements apart), weight n_out x n_in (rows weight_stride apart), y and
  * residual rows x n_out, contiguous. bias (n_out) and residual may be NULL. kept, if
  * not NULL, receives the activation's slopes for the backward pass: rows x n_out floats
- * for DRH_F32, float16 for the other types; nothing is written with DRH_ACT_NONE. */
+ * for DRH_F32, float16 and times 2^15 for the other types; nothing is written with
+ * DRH_ACT_NONE. */
 int drh_linear(drh_ctx *ctx, const void *x, const void *weight, const void *bias, const void *residual,
                int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride,
                int dtype, int activation, void *y, void *kept, void *workspace, uint64_t workspace_bytes,
