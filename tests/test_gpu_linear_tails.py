@@ -48,3 +48,40 @@ def test_slopes_keep_their_precision(layers, kind, low, dtype):
     _, dx = one_each(layers, z, up, kind)
     want = 4096.0 * lb.slope(kind, z.double())
     within(dx, want[:, None].expand_as(dx), 2.01 * lb.U[dtype] + 2.0**-11 + 2.0**-17, kind)
+
+
+# z down to here; beyond 2^-15 (f32: the argument's own rounding counts c^2 times) or 2^-13 (16 bits) of
+# the value there is the rounding to the type alone
+@pytest.mark.parametrize("dtype,low,rel", [(torch.float32, -12.0, 2.0**-15), (torch.bfloat16, -12.0, 2.0**-13),
+                                           (torch.float16, -5.0, 2.0**-13)], ids=["f32", *IDS])
+def test_gelus_tail(layers, dtype, low, rel):
+    z = torch.linspace(low, -1.5, 300, device="cuda").to(dtype)
+    up = torch.full_like(z, 4096.0)
+    y, dx = one_each(layers, z, up, "gelu")
+    want = lb.act("gelu", z.double())[:, None].expand_as(y)
+    lb.check(y, want, rel * want.abs(), dtype, "y")
+    # act' = Phi + z phi, the second term up to z^2 times the first; it is zero nowhere below -0.76
+    want = 4096.0 * lb.slope("gelu", z.double())[:, None].expand_as(dx)
+    within(dx[z >= -6.0], want[z >= -6.0], 2 * rel + (2.01 * lb.U[dtype] + 2.0**-11 if dtype != torch.float32 else 0.0), "dx")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, *DTYPES], ids=["f32", *IDS])
+@pytest.mark.parametrize("kind", lb.ACTS[1:])
+def test_values_over_the_whole_range(layers, kind, dtype):
+    """Every 16-bit number (of float32 as many) as z: between the bends, past them, zeros and infinities."""
+    if dtype == torch.float32:
+        z = (torch.arange(1 << 16, device="cuda", dtype=torch.int32) << 16).view(torch.float32)
+    else:
+        z = torch.arange(-(1 << 15), 1 << 15, device="cuda", dtype=torch.int32).to(torch.int16).view(dtype)
+    z = z[~torch.isnan(z)]
+    x = torch.zeros(z.numel(), 8, dtype=dtype, device="cuda")
+    x[:, 0] = z
+    w = torch.zeros(16, 8, dtype=dtype, device="cuda")
+    w[:, 0] = 1.0
+    bias = torch.zeros(16, dtype=dtype, device="cuda")
+    x = x[torch.isfinite(z)]
+    z = z[torch.isfinite(z)]
+    y = layers.linear(x, w, bias, kind)
+    want = lb.act(kind, z.double())
+    want = torch.where(torch.isnan(want), z.double().clamp(min=0), want)  # the formula's own overflow
+    lb.check(y, want[:, None].expand_as(y), (lb.act_error(kind, dtype)[0] * z.double().abs())[:, None].expand_as(y), dtype, kind)
