@@ -136,9 +136,12 @@ void refuse_transforms(std::initializer_list<const Tensor*> ts) {
 }
 
 // Whether every tensor is on the GPU that x is on; if not, they are moved there (to the
-// current GPU where x is on none).
+// current GPU where x is on none). A tensor that torch negates when it is read (the imaginary
+// part of a conjugate) is negated here: kernels read memory as it stands.
 bool together(std::initializer_list<Tensor*> ts) {
     Tensor& x = **ts.begin();
+    for (Tensor* t : ts)
+        if (t->defined() && t->is_neg()) *t = t->resolve_neg();
     bool same = x.is_cuda();
     for (Tensor* t : ts) same = same && (!t->defined() || t->device() == x.device());
     if (same) return true;
@@ -171,7 +174,7 @@ struct OnceNode : Node {
         variable_list r;
         {
             at::NoGradGuard no;
-            r = grads[0].defined() ? gradients(grads[0]) : variable_list(num_outputs());
+            r = grads[0].defined() ? gradients(grads[0].resolve_neg()) : variable_list(num_outputs());
         }
         if (at::GradMode::is_enabled() && grads[0].defined()) {
             torch::autograd::edge_list edges = next_edges();
