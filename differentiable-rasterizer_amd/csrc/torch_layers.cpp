@@ -156,6 +156,33 @@ bool together(std::initializer_list<Tensor*> ts) {
     return false;
 }
 
+// A tensor kept for the backward pass. What comes back may be a user's (a saved-tensor hook's): a
+// kernel is given nothing but what went in's type, shape and GPU.
+class Kept {
+    SavedVariable saved_;
+    at::TensorOptions options_;
+    c10::DimVector sizes_;
+    bool holds_ = false;
+
+public:
+    void keep(const Tensor& t) {
+        saved_ = SavedVariable(t, false);
+        options_ = t.options();
+        sizes_ = c10::DimVector(t.sizes());
+        holds_ = true;
+    }
+    // Undefined where nothing was kept.
+    Tensor get() const {
+        if (!holds_) return Tensor();
+        const Tensor t = saved_.unpack();
+        TORCH_CHECK(t.defined() && t.sizes() == c10::IntArrayRef(sizes_) && t.scalar_type() == options_.dtype().toScalarType() &&
+                        t.device() == options_.device() && t.layout() == at::kStrided,
+                    "a tensor saved for a layer's backward pass came back as another type, shape or device");
+        return t.resolve_neg();
+    }
+    void release() { saved_.reset_data(); }
+};
+
 // The history of a gradient that was made with a graph asked for: raises for whoever
 // differentiates it. It leads to all that the gradient depends on (the layer's inputs and the
 // gradient that came in), since the engine skips what is on no path to the inputs asked for.
@@ -171,6 +198,12 @@ struct OnceNode : Node {
     variable_list apply(variable_list&& grads) final {
         std::lock_guard<std::mutex> lock(mutex_);
         refuse_transforms({&grads[0]});
+        if (grads[0].defined()) {  // the engine sees to this, but a node's own hooks come after it
+            const auto& meta = input_metadata(0);
+            TORCH_CHECK(meta.is_same_shape(grads[0]) && grads[0].device() == meta.device() && grads[0].layout() == at::kStrided &&
+                            grads[0].scalar_type() == meta.dtype().toScalarType(),
+                        "the gradient of a layer's output is of another type, shape or device than the output");
+        }
         variable_list r;
         {
             at::NoGradGuard no;
@@ -212,21 +245,20 @@ std::shared_ptr<N> new_node() {
 
 // Keeps what the gradients that are wanted need: weight where dx is, never the bias.
 struct LayerNormBackward : OnceNode {
-    SavedVariable x_, weight_, stats_;
+    Kept x_, weight_, stats_;
     at::ScalarType weight_type = at::kFloat;  // and the bias's
     int weight_code = DRH_F32;
-    bool keeps_weight = false;
 
     std::string name() const override { return "DiffrastLayerNormBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
-        x_.reset_data();
-        weight_.reset_data();
-        stats_.reset_data();
+        x_.release();
+        weight_.release();
+        stats_.release();
     }
 
     variable_list gradients(const Tensor& g) override {
-        const Tensor x = x_.unpack(), stats = stats_.unpack(), w = keeps_weight ? weight_.unpack() : Tensor();
+        const Tensor x = x_.get(), stats = stats_.get().contiguous(), w = weight_.get();
         const Tensor xv = as_rows(x), gv = as_rows(g), wv = flat(w);
         const int64_t rows = xv.size(0), cols = xv.size(1);
         variable_list r(3);
@@ -285,9 +317,9 @@ Tensor layer_norm(Tensor x, const Optional& weight, const Optional& bias, double
     }
     if (!grad) return y;
     auto node = new_node<LayerNormBackward>();
-    node->x_ = SavedVariable(x, false);
-    node->stats_ = SavedVariable(stats, false);
-    if ((node->keeps_weight = w.defined() && x.requires_grad())) node->weight_ = SavedVariable(w, false);
+    node->x_.keep(x);
+    node->stats_.keep(stats);
+    if (w.defined() && x.requires_grad()) node->weight_.keep(w);
     node->weight_type = wtype;
     node->weight_code = wcode;
     return attach(std::move(y), std::move(node), {&x, &w, &b});
@@ -298,24 +330,23 @@ Tensor layer_norm(Tensor x, const Optional& weight, const Optional& bias, double
 // Keeps what the gradients that are wanted need: x where dW is, the weight where dx is, the
 // slopes where any is but the residual's.
 struct LinearBackward : OnceNode {
-    SavedVariable x_, weight_, kept_;
+    Kept x_, weight_, slopes_;
     std::vector<int64_t> x_sizes;
     at::TensorOptions options;
     int64_t rows = 0, n_out = 0, n_in = 0;
     int act = 0, code = 0;
-    bool keeps_x = false, keeps_weight = false, has_kept = false;
 
     std::string name() const override { return "DiffrastLinearBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
-        x_.reset_data();
-        weight_.reset_data();
-        kept_.reset_data();
+        x_.release();
+        weight_.release();
+        slopes_.release();
     }
 
     variable_list gradients(const Tensor& grad) override {
-        const Tensor kept = has_kept ? kept_.unpack() : Tensor();
-        const Tensor xv = keeps_x ? as_rows(x_.unpack()) : Tensor(), wv = keeps_weight ? as_rows(weight_.unpack()) : Tensor();
+        const Tensor x = x_.get(), w = weight_.get(), kept = flat(slopes_.get());
+        const Tensor xv = x.defined() ? as_rows(x) : x, wv = w.defined() ? as_rows(w) : w;
         const Tensor g = flat(grad);
         variable_list r(4);
         if (task_should_compute_output(0)) r[0] = at::empty(x_sizes, options);
@@ -377,13 +408,13 @@ Tensor linear(Tensor x, Tensor w, const Optional& bias, int act, const Optional&
     }
     if (!grad) return y;
     auto node = new_node<LinearBackward>();
-    if ((node->keeps_x = w.requires_grad())) node->x_ = SavedVariable(x, false);
-    if ((node->keeps_weight = x.requires_grad())) node->weight_ = SavedVariable(w, false);
+    if (w.requires_grad()) node->x_.keep(x);
+    if (x.requires_grad()) node->weight_.keep(w);
     node->x_sizes = x.sizes().vec();
     node->options = x.options();
     node->rows = rows, node->n_out = n_out, node->n_in = n_in;
     node->act = act, node->code = code;
-    if ((node->has_kept = keep)) node->kept_ = SavedVariable(kept, false);
+    if (keep) node->slopes_.keep(kept);
     return attach(std::move(y), std::move(node), {&x, &w, &b, &res});
 }
 
