@@ -370,14 +370,18 @@ void row_launches(const LnArgs& p, int64_t groups, int64_t per, F&& f) {
     });
 }
 
+int check_sizes(int64_t rows, int64_t cols) {
+    if (rows < 0 || cols <= 0) return fail(DRH_ERR_INVALID_ARG, "rows must not be negative and cols positive");
+    if (rows > INT32_MAX || cols > (1 << 30)) return fail(DRH_ERR_TOO_LARGE, "more than 2^31 - 1 rows or 2^30 columns");
+    return DRH_OK;
+}
+
 int check_ln(drh_ctx* ctx, int64_t rows, int64_t cols, int dtype, int weight_dtype, uint32_t flags) {
     int rc = check_call(ctx, dtype, flags);
     if (rc) return rc;
     if (weight_dtype != dtype && weight_dtype != DRH_F32)
         return fail(DRH_ERR_INVALID_ARG, "weight and bias stand in the input's element type or in 32 bits");
-    if (rows < 0 || cols <= 0) return fail(DRH_ERR_INVALID_ARG, "rows must not be negative and cols positive");
-    if (rows > INT32_MAX || cols > (1 << 30)) return fail(DRH_ERR_TOO_LARGE, "more than 2^31 - 1 rows or 2^30 columns");
-    return DRH_OK;
+    return check_sizes(rows, cols);
 }
 
 }  // namespace
@@ -397,6 +401,7 @@ int drh_layer_norm(drh_ctx* ctx, const void* x, const void* weight, const void* 
     if (!x || !y || !mean != !rstd)
         return fail(DRH_ERR_INVALID_ARG, "x and y must not be NULL; mean and rstd come together");
     if (rows > 1 && x_stride < 0) return fail(DRH_ERR_INVALID_ARG, "x_stride must not be negative");
+    if ((rc = check_span(rows, x_stride))) return rc;
     DeviceGuard dg(ctx->device);
     hipStream_t s = (hipStream_t)stream;
     LnArgs p{};
@@ -423,7 +428,9 @@ int drh_layer_norm(drh_ctx* ctx, const void* x, const void* weight, const void* 
 }
 
 int drh_layer_norm_backward_bytes(int64_t rows, int64_t cols, int dtype, uint64_t* out_bytes) {
-    if (!out_bytes || !known_type(dtype) || rows < 0 || cols <= 0) return fail(DRH_ERR_INVALID_ARG, "bad sizes, or out_bytes is NULL");
+    if (!out_bytes || !known_type(dtype)) return fail(DRH_ERR_INVALID_ARG, "unknown element type, or out_bytes is NULL");
+    int rc = check_sizes(rows, cols);
+    if (rc) return rc;
     *out_bytes = up256((size_t)ln_backward_groups(rows, cols, dtype) * 2 * (size_t)cols * sizeof(float));
     return DRH_OK;
 }
@@ -437,6 +444,7 @@ int drh_layer_norm_backward(drh_ctx* ctx, const void* x, const void* weight, con
     const bool sums = grad_weight || grad_bias;
     if (rows > 0 && (!x || !mean || !rstd || !grad_y)) return fail(DRH_ERR_INVALID_ARG, "an input pointer is NULL");
     if (rows > 1 && (x_stride < 0 || grad_stride < 0)) return fail(DRH_ERR_INVALID_ARG, "strides must not be negative");
+    if ((rc = check_span(rows, x_stride)) || (rc = check_span(rows, grad_stride))) return rc;
     uint64_t need = 0;
     if (sums) drh_layer_norm_backward_bytes(rows, cols, dtype, &need);
     if (sums && (workspace_bytes < need || (need && !workspace)))

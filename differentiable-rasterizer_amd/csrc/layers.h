@@ -122,6 +122,8 @@ void in_launches(int64_t n, int64_t most, F&& f) {
 
 // Checks that every layer call makes; the flags a layer knows are DRH_SYNC alone.
 int check_call(drh_ctx* ctx, int dtype, uint32_t flags);
+// Rows `stride` elements apart: no more than an address space holds, so that no offset passes 64 bits.
+int check_span(int64_t rows, int64_t stride);
 // After the last launch: its error, and DRH_SYNC's wait.
 int finish_call(hipStream_t s, uint32_t flags, const char* what);
 

@@ -46,6 +46,11 @@ int check_call(drh_ctx* ctx, int dtype, uint32_t flags) {
     return DRH_OK;
 }
 
+int check_span(int64_t rows, int64_t stride) {
+    if (rows <= 1 || stride <= (1ll << 48) / rows) return DRH_OK;
+    return fail(DRH_ERR_TOO_LARGE, "an array of more than 2^48 elements");
+}
+
 int finish_call(hipStream_t s, uint32_t flags, const char* what) {
     HIP_TRY(hipGetLastError(), what);
     return (flags & DRH_SYNC) ? wait_stream(s) : DRH_OK;

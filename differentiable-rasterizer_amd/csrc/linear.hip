@@ -639,16 +639,26 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t 
     return b;
 }
 
+int check_sizes(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {
+    if (M < 0 || N <= 0 || K < 0) return fail(DRH_ERR_INVALID_ARG, "rows and inputs must not be negative, outputs positive");
+    if (M > INT32_MAX || N > (1 << 30) || K > (1 << 30))
+        return fail(DRH_ERR_TOO_LARGE, "more than 2^31 - 1 rows or 2^30 features");
+    if ((M > 1 && xs < K) || (N > 1 && ws < K)) return fail(DRH_ERR_INVALID_ARG, "a row stride is less than the row");
+    int rc = check_span(M, xs);
+    return rc ? rc : check_span(N, ws);
+}
+
 int check_linear(drh_ctx* ctx, int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype, int act,
                  uint32_t flags) {
     int rc = check_call(ctx, dtype, flags);
     if (rc) return rc;
     if (act < DRH_ACT_NONE || act > DRH_ACT_SILU) return fail(DRH_ERR_INVALID_ARG, "unknown activation " + std::to_string(act));
-    if (M < 0 || N <= 0 || K < 0) return fail(DRH_ERR_INVALID_ARG, "rows and inputs must not be negative, outputs positive");
-    if (M > INT32_MAX || N > (1 << 30) || K > (1 << 30))
-        return fail(DRH_ERR_TOO_LARGE, "more than 2^31 - 1 rows or 2^30 features");
-    if ((M > 1 && xs < K) || (N > 1 && ws < K)) return fail(DRH_ERR_INVALID_ARG, "a row stride is less than the row");
-    return DRH_OK;
+    return check_sizes(M, N, K, xs, ws);
+}
+
+int check_bytes(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype, const uint64_t* out_bytes) {
+    if (!out_bytes || !known_type(dtype)) return fail(DRH_ERR_INVALID_ARG, "unknown element type, or out_bytes is NULL");
+    return check_sizes(M, N, K, xs, ws);
 }
 
 int check_workspace(size_t need, const void* workspace, uint64_t bytes) {
@@ -667,8 +677,8 @@ extern "C" {
 
 int drh_linear_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride, int dtype,
                      uint64_t* out_bytes) {
-    if (!out_bytes || !known_type(dtype) || rows < 0 || n_out <= 0 || n_in < 0)
-        return fail(DRH_ERR_INVALID_ARG, "bad sizes or type, or out_bytes is NULL");
+    int rc = check_bytes(rows, n_out, n_in, x_stride, weight_stride, dtype, out_bytes);
+    if (rc) return rc;
     *out_bytes = forward_plan(rows, n_out, n_in, x_stride, weight_stride, dtype).total;
     return DRH_OK;
 }
@@ -702,8 +712,8 @@ int drh_linear(drh_ctx* ctx, const void* x, const void* weight, const void* bias
 
 int drh_linear_backward_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride,
                               int dtype, int activation, uint64_t* out_bytes) {
-    if (!out_bytes || !known_type(dtype) || rows < 0 || n_out <= 0 || n_in < 0)
-        return fail(DRH_ERR_INVALID_ARG, "bad sizes or type, or out_bytes is NULL");
+    int rc = check_bytes(rows, n_out, n_in, x_stride, weight_stride, dtype, out_bytes);
+    if (rc) return rc;
     *out_bytes = backward_plan(rows, n_out, n_in, x_stride, weight_stride, dtype, activation).total;
     return DRH_OK;
 }

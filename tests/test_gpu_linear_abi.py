@@ -50,3 +50,17 @@ def test_the_stride_of_a_single_row_counts_for_nothing(L, ctx, stride, dtype):
     # one output: dx = g w
     dx, _, db = backward(L, ctx, rest, one, g.view(many, 1), K, stride, dtype)
     assert bool(torch.equal(dx, g[:, None] * one)) and float(db) == 300
+
+
+def test_strides_past_any_memory_are_refused(L, ctx):
+    f, t = L.lib(), torch.zeros(64, 64, device="cuda")
+    p, h, big = t.data_ptr(), ctx.handle, 1 << 46
+    calls = (lambda: f.drh_linear(h, p, p, None, None, 100, 8, 8, big, 8, 0, 0, p, None, None, 0, None, 0),
+             lambda: f.drh_linear(h, p, p, None, None, 4, 8, 8, 8, big, 0, 0, p, None, None, 0, None, 0),
+             lambda: f.drh_linear_backward(h, p, p, None, p, 100, 8, 8, big, 8, 0, 0, p, p, None, p, 1 << 30, None, 0),
+             lambda: f.drh_layer_norm(h, p, None, None, 100, 8, big, 0, 0, 1e-5, p, None, None, None, 0),
+             lambda: f.drh_layer_norm_backward(h, p, None, p, p, p, 100, 8, 8, big, 0, 0, p, None, None, None, 0, None, 0))
+    for call in calls:
+        assert call() == 5, L.last_error()
+    torch.cuda.synchronize()
+    assert not bool(t.any())
