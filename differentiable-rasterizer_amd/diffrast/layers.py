@@ -38,8 +38,9 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
         weight, bias: `(D,)` each or None, of x's type or both float32.
         eps: added to the variance, which is the mean of squares about the mean.
     """
+    y = _torch_layers.layer_norm(x, weight, bias, eps)
     torch_layer._note_gpu()
-    return _torch_layers.layer_norm(x, weight, bias, eps)
+    return y
 
 
 def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: str | None = None,
@@ -59,8 +60,9 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: st
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r} — expected one of {list(ACTIVATIONS)}")
+    y = _torch_layers.linear(x, weight, bias, act, residual)
     torch_layer._note_gpu()
-    return _torch_layers.linear(x, weight, bias, act, residual)
+    return y
 
 
 def dropout(x: Tensor, p: float, *, seed: int, offset: int = 0, residual: Tensor | None = None) -> Tensor:
@@ -80,5 +82,6 @@ def dropout(x: Tensor, p: float, *, seed: int, offset: int = 0, residual: Tensor
     for name, v in (("seed", seed), ("offset", offset)):
         if not (isinstance(v, int) and 0 <= v < 1 << 64):
             raise ValueError(f"{name} must be an integer in [0, 2^64)")
+    y = _torch_layers.dropout(x, p, seed, offset, residual)
     torch_layer._note_gpu()
-    return _torch_layers.dropout(x, p, seed, offset, residual)
+    return y

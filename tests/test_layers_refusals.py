@@ -1,4 +1,4 @@
-"""The workspace of a call is refused for the sizes that the call refuses, as it does."""
+"""What the network layers refuse, and how: a workspace as its call, a call without a trace."""
 
 import ctypes
 
@@ -32,3 +32,16 @@ def test_a_single_rows_stride_is_free(L):
         L.check(L.lib().drh_linear_backward_bytes(1, 200, 64, xs, 64, 1, 0, ctypes.byref(a)))
         L.check(L.lib().drh_linear_backward_bytes(1, 200, 64, 64, 64, 1, 0, ctypes.byref(b)))
         assert a.value == b.value
+
+
+def test_a_refused_call_ran_on_no_device(monkeypatch):
+    import torch
+    from diffrast import layers, torch_layer
+
+    monkeypatch.setattr(torch_layer, "_last_device", "cpu")
+    x = torch.zeros(3, 8)
+    for call in (lambda: layers.layer_norm(x, torch.zeros(7)), lambda: layers.linear(x, torch.zeros(4, 7)),
+                 lambda: layers.dropout(x, 1.5, seed=0)):
+        with pytest.raises(ValueError):
+            call()
+        assert torch_layer.last_device() == "cpu"
