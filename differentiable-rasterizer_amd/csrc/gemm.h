@@ -219,7 +219,7 @@ struct Frags {
 //
 // Thirds, for 32 bits: v = v1 + v2 + v3 in bfloat16, each the first eight bits of what is left,
 // is exact (3 x 8 bits) from about 2^-111 on, above bfloat16's smallest number, 2^-133, by all of
-// them; a tile with a smaller operand is made again (gemm_tile's second pass). a b is a1 b1 + a1 b2
+// them; a tile where what smaller numbers lose could count is made again (gemm_tile's second pass). a b is a1 b1 + a1 b2
 // + a2 b1 + a2 b2 + a1 b3 + a3 b1 but for less than 2^-21 |a b|, 2^-24 in the mean; thirds have
 // their value's sign, so what is dropped of a product has the product's. Six bfloat16 products
 // take 96 cycles of the matrix core where the 32-bit instructions take 256, and splitting costs six
@@ -445,7 +445,7 @@ __device__ inline void gemm_tile(const Gemm& p) {
         lb.issue(0, first + step * GROUPS, lds0 + b + UNIT);
     };
     floatx4 acc[NF][NF] = {};
-    auto straight = [&] {
+    auto walk = [&](auto use) {  // use(fragments of A, of B) for each tile
         load(0, 0);
         for (int64_t i = 0; i < steps; i++) {
             const int stage = (int)i & 1;
@@ -458,11 +458,12 @@ __device__ inline void gemm_tile(const Gemm& p) {
                 FB fb;
                 fa.read(b, wm);
                 fb.read(b + UNIT, wn);
-                Straight::multiply(fa, fb, acc);
+                use(fa, fb);
             }
         }
         wait_all();  // LDS is given up, or used again, with no load on its way there
     };
+    auto straight = [&] { walk([&](const FA& fa, const FB& fb) { Straight::multiply(fa, fb, acc); }); };
     if constexpr (std::is_same_v<Math, Straight>) {
         straight();
     } else {
@@ -507,14 +508,39 @@ __device__ inline void gemm_tile(const Gemm& p) {
         }
         wait_all();
         // A result that is not finite comes from an infinity, a NaN or an overflow. The thirds turn
-        // the first into NaN, and lose bits of what is too small for them: the tile is made again with
-        // instructions that do neither.
+        // the first into NaN, so the tile is made again with instructions that do not.
         float zero = 0.0f;
 #pragma unroll
         for (int i = 0; i < NF * NF; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) zero = fmaf(acc[i / NF][i % NF][e], 0.0f, zero);
-        if (__syncthreads_or(!(zero == 0.0f) || (lost & 0xffffu))) {
+        bool again = !(zero == 0.0f);
+        // So it is where the thirds lost bits that count. A number loses less than 2^-133, so a sum
+        // is off by that times k times the largest numbers; 2^-21 of the sum is what thirds may cost.
+        // A few numbers of a GELU's tail, say, are no reason: they are found by reading the tiles once
+        // more, a third of the time of making them again.
+        if (__syncthreads_or(lost & 0xffffu)) {
+            float most = 0.0f;
+            auto largest = [&](const auto& f) {
+#pragma unroll
+                for (int i = 0; i < NF; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(f.f[i][e / 4][e % 4]));
+            };
+            walk([&](const FA& fa, const FB& fb) { largest(fa), largest(fb); });
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+            const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+            const float least = most * (float)(steps * LA::BK) * 0x1p-111f;
+#pragma unroll
+            for (int i = 0; i < NF * NF; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const bool there = m0 + wm + i / NF * 16 + r < p.M && n0 + wn + q * (4 * NF) + i % NF * 4 + e < p.N;
+                    again |= there && !(fabsf(acc[i / NF][i % NF][e]) >= least);
+                }
+        }
+        if (__syncthreads_or(again)) {
 #pragma unroll
             for (int i = 0; i < NF * NF; i++) acc[i / NF][i % NF] = floatx4{};
             straight();

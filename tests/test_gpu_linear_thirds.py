@@ -67,3 +67,18 @@ def test_a_small_operand_beside_large_ones(layers):
     x[7, at_k[7]] = 1.2345678 * 2.0**-121
     w[900, 13] = 1.7654321 * 2.0**-119
     check(layers.linear(x, w), x[rows, at_k].double()[:, None] * w.t()[at_k].double(), "y")
+
+
+@pytest.mark.parametrize("M,N,K", [(300, 136, 328), (1000, 1160, 1024), (512, 256, 8192)])
+def test_tails_in_the_operands(layers, M, N, K):
+    """Slopes down to 2^-149 among ordinary ones (GELU far below zero), softmaxes with numbers as small."""
+    import layer_bounds as lb
+    from test_gpu_linear import compare, make, run
+
+    t = make(M, N, K, torch.float32, res=True)
+    t["x"] *= 7.0
+    assert 0 < int(((lb.slope("gelu", t["x"].double() @ t["w"].double().t()).abs() < 2.0**-115)).sum())
+    compare(t, "gelu", run(layers, t, "gelu"), "gelu")
+    t["x"] = torch.softmax(30 * t["x"].detach() / 7, 1)
+    assert 0 < int(((t["x"] > 0) & (t["x"] < 2.0**-115)).sum())
+    compare(t, None, run(layers, t, None), "softmax")
