@@ -26,7 +26,6 @@ ARCH = os.environ.get("DIFFRAST_OFFLOAD_ARCH", "gfx950")
 
 SOURCES = [CSRC / "kernels.hip", CSRC / "runtime.hip", CSRC / "fit.hip", CSRC / "scratch.hip", CSRC / "resize.hip",
            CSRC / "layers.hip", CSRC / "layer_norm.hip", CSRC / "linear.hip", CSRC / "dropout.hip"]
-HEADERS = [CSRC / "kernels.h", CSRC / "runtime.h", CSRC / "layers.h", ROOT / "include" / "diffrast_hip.h"]
 
 # -ffp-contract=off: the kernels state every FMA explicitly; plain a*b+c must
 # round twice, as the reference's arithmetic does.
