@@ -226,11 +226,10 @@ struct Frags {
 // vector operations an element, four to five behind each matrix instruction of a 64 x 64 quarter.
 // (Rounding each third to the nearest is as many operations, but the conversion is a slow one.)
 // Alone, a matrix instruction and four such operations take 12 ns with one wave a SIMD and 10 with
-// two, 8 and 7 without them: the two kinds overlap in part. 4096^3 takes 700 to 760 us (190
+// two, 8 and 7 without them: the two kinds overlap in part. 4096^3 takes 680 to 760 us (190
 // TFLOP/s in 32 bits, 1.15 P in bfloat16, where the power limit has the clock) however the splits
-// are placed; with one workgroup a CU, between the next tile's instructions instead of before
-// them, 4096 x 1024 outputs and k = 1024 take 60 us instead of 65. Infinities come out as NaN: see
-// gemm_tile's second pass.
+// are placed; 4096 x 1024 outputs and k = 1024 64 us, of which gathering what is lost is three.
+// Infinities come out as NaN: see gemm_tile's second pass.
 struct Straight {
     template <class FA, class FB, int NA, int NB>
     static __device__ inline void multiply(const FA& a, const FB& b, floatx4 (&acc)[NA][NB]) {

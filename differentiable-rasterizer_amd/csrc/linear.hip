@@ -334,7 +334,8 @@ constexpr int CUS = 256;
 // 1280 x 1024 4.8 / 6.5, 4096 x 4096 13.2 / 13.9; 64 rows 4096 x 1024 7.2 / 9.1, 4096 x 4096 21.7 / 14.2.
 constexpr int64_t ROWS_FEW = 32, ROWS_MOST = 64, ROWS_MOST_K = 2048;
 // Products in 32 bits are split in thirds from this k on: their error, 2^-21 of a term at the
-// most, is then below that of the sum, and shorter products are bound by memory either way.
+// most (gemm.h says what becomes of terms too small for that), is then below what a 32-bit sum of
+// as many terms may lose, k 2^-24, and shorter products are bound by memory either way.
 constexpr int64_t THIRDS_LEAST = 64;
 
 // Whether an operand's sizes suit the kernels that load 16-byte chunks through buffers.
@@ -443,8 +444,8 @@ int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial,
                 if constexpr (LARGE)
                     if (tile == 256) gemm_256_kernel<T, AK, BK, ACT><<<grid, 512, 0, s>>>(p);
                 // Microseconds with two groups and with one, 256 tiles: 4096 x 1024 outputs and k = 1024
-                // in 32 bits 60 / 65, as k by rows 66 / 74; 1024 x 1024 outputs and k = 4096 in bfloat16
-                // 23.6 / 31. With 512 tiles one is the faster: 2048 x 1024 and k = 1024 10.0 / 10.9
+                // in 32 bits 64 / 64, as k by rows 68 / 72; 1024 x 1024 outputs and k = 4096 in bfloat16
+                // 23.2 / 30.6. With 512 tiles one is the faster: 2048 x 1024 and k = 1024 10.0 / 10.9
                 const bool alone = tiles * p.splits <= CUS;
                 if (tile == 128 && alone) gemm_tile_kernel<T, AK, BK, ACT, Math, 128, 2><<<grid, 512, 0, s>>>(p);
                 if (tile == 128 && !alone) gemm_tile_kernel<T, AK, BK, ACT, Math, 128, 1><<<grid, 256, 0, s>>>(p);
