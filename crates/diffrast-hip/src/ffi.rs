@@ -128,6 +128,19 @@ pub struct drh_fit_status {
     pub stop_reason: i32,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct drh_adamw_tensor {
+    pub param: *mut c_void,
+    pub grad: *const c_void,
+    pub exp_avg: *mut c_void,
+    pub exp_avg_sq: *mut c_void,
+    pub exp_avg_scale: *mut f32,
+    pub exp_avg_sq_scale: *mut f32,
+    pub step: *mut i64,
+    pub n: i64,
+}
+
 extern "C" {
     pub fn drh_create(out: *mut *mut drh_ctx) -> c_int;
     pub fn drh_destroy(ctx: *mut drh_ctx) -> c_int;
@@ -445,6 +458,182 @@ extern "C" {
         seed: u64,
         offset: u64,
         y: *mut c_void,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_rms_norm(
+        ctx: *mut drh_ctx,
+        x: *const c_void,
+        residual: *const c_void,
+        weight: *const c_void,
+        rows: i64,
+        cols: i64,
+        x_stride: i64,
+        residual_stride: i64,
+        dtype: c_int,
+        weight_dtype: c_int,
+        eps: f32,
+        y: *mut c_void,
+        sum: *mut c_void,
+        rstd: *mut f32,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_rms_norm_8bit(
+        ctx: *mut drh_ctx,
+        x: *const c_void,
+        residual: *const c_void,
+        weight: *const c_void,
+        rows: i64,
+        cols: i64,
+        x_stride: i64,
+        residual_stride: i64,
+        dtype: c_int,
+        weight_dtype: c_int,
+        eps: f32,
+        y: *mut c_void,
+        scale: *mut f32,
+        sum: *mut c_void,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_quantize_8bit(
+        ctx: *mut drh_ctx,
+        x: *const c_void,
+        rows: i64,
+        cols: i64,
+        x_stride: i64,
+        dtype: c_int,
+        y: *mut c_void,
+        scale: *mut f32,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_rms_norm_backward_bytes(
+        rows: i64,
+        cols: i64,
+        dtype: c_int,
+        out_bytes: *mut u64,
+    ) -> c_int;
+    pub fn drh_rms_norm_backward(
+        ctx: *mut drh_ctx,
+        sum: *const c_void,
+        weight: *const c_void,
+        rstd: *const f32,
+        grad_y: *const c_void,
+        grad_sum: *const c_void,
+        rows: i64,
+        cols: i64,
+        sum_stride: i64,
+        grad_y_stride: i64,
+        grad_sum_stride: i64,
+        dtype: c_int,
+        weight_dtype: c_int,
+        grad_x: *mut c_void,
+        grad_weight: *mut c_void,
+        workspace: *mut c_void,
+        workspace_bytes: u64,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_linear_8bit(
+        ctx: *mut drh_ctx,
+        x: *const c_void,
+        x_scale: *const f32,
+        weight: *const c_void,
+        weight_scale: *const f32,
+        bias: *const c_void,
+        residual: *const c_void,
+        rows: i64,
+        n_out: i64,
+        n_in: i64,
+        x_stride: i64,
+        weight_stride: i64,
+        dtype: c_int,
+        activation: c_int,
+        y: *mut c_void,
+        workspace: *mut c_void,
+        workspace_bytes: u64,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_linear_8bit_bytes(
+        rows: i64,
+        n_out: i64,
+        n_in: i64,
+        x_stride: i64,
+        weight_stride: i64,
+        out_bytes: *mut u64,
+    ) -> c_int;
+    pub fn drh_gated_linear(
+        ctx: *mut drh_ctx,
+        x: *const c_void,
+        weight: *const c_void,
+        bias: *const c_void,
+        rows: i64,
+        n_out: i64,
+        n_in: i64,
+        x_stride: i64,
+        weight_stride: i64,
+        dtype: c_int,
+        activation: c_int,
+        y: *mut c_void,
+        kept: *mut c_void,
+        workspace: *mut c_void,
+        workspace_bytes: u64,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_gated_linear_bytes(
+        rows: i64,
+        n_out: i64,
+        n_in: i64,
+        x_stride: i64,
+        weight_stride: i64,
+        dtype: c_int,
+        out_bytes: *mut u64,
+    ) -> c_int;
+    pub fn drh_gated_linear_backward_bytes(
+        rows: i64,
+        n_out: i64,
+        n_in: i64,
+        x_stride: i64,
+        weight_stride: i64,
+        dtype: c_int,
+        out_bytes: *mut u64,
+    ) -> c_int;
+    pub fn drh_gated_linear_backward(
+        ctx: *mut drh_ctx,
+        x: *const c_void,
+        weight: *const c_void,
+        kept: *const c_void,
+        grad_y: *const c_void,
+        rows: i64,
+        n_out: i64,
+        n_in: i64,
+        x_stride: i64,
+        weight_stride: i64,
+        dtype: c_int,
+        grad_x: *mut c_void,
+        grad_weight: *mut c_void,
+        grad_bias: *mut c_void,
+        workspace: *mut c_void,
+        workspace_bytes: u64,
+        stream: *mut c_void,
+        flags: u32,
+    ) -> c_int;
+    pub fn drh_adamw(
+        ctx: *mut drh_ctx,
+        tensors: *const drh_adamw_tensor,
+        count: i64,
+        dtype: c_int,
+        state_bits: c_int,
+        lr: f64,
+        beta1: f64,
+        beta2: f64,
+        eps: f64,
+        weight_decay: f64,
+        seed: u64,
         stream: *mut c_void,
         flags: u32,
     ) -> c_int;

@@ -25,7 +25,8 @@ TORCH_LIB = HERE / "diffrast" / "_torch_layers.so"
 ARCH = os.environ.get("DIFFRAST_OFFLOAD_ARCH", "gfx950")
 
 SOURCES = [CSRC / "kernels.hip", CSRC / "runtime.hip", CSRC / "fit.hip", CSRC / "scratch.hip", CSRC / "resize.hip",
-           CSRC / "layers.hip", CSRC / "layer_norm.hip", CSRC / "linear.hip", CSRC / "dropout.hip"]
+           CSRC / "layers.hip", CSRC / "layer_norm.hip", CSRC / "linear.hip", CSRC / "dropout.hip",
+           CSRC / "rms_norm.hip", CSRC / "gated.hip", CSRC / "linear8.hip", CSRC / "adamw.hip"]
 
 # -ffp-contract=off: the kernels state every FMA explicitly; plain a*b+c must
 # round twice, as the reference's arithmetic does.

@@ -12,28 +12,12 @@
 
 #include <cmath>
 
-#include "layers.h"
+#include "philox.h"
 
 using namespace drh_rt;
 
 namespace drh_nn {
 namespace {
-
-__device__ inline void philox(uint64_t block, uint64_t offset, uint64_t seed, uint32_t (&out)[4]) {
-    uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
-    uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
-#pragma unroll
-    for (int i = 0; i < 10; i++) {
-        const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
-        c1 = (uint32_t)b;
-        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
-        c3 = (uint32_t)a;
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
-    }
-    out[0] = c0, out[1] = c1, out[2] = c2, out[3] = c3;
-}
 
 // A thread takes 16 bytes: the eight elements of a counter, or in 32 bits four of them. Two
 // threads then evaluate the same counter, which costs less than the half-used lines of 32

@@ -32,6 +32,7 @@ struct Gemm {
     int act;
     int splits;              // the k range in this many parts, grid.y
     int tiles_per_split;     // tiles of k in each
+    const float *row_scale, *col_scale;  // of 8-bit operands: M; N
 };
 
 // D = A B + C on a wave: lane l gives row l % 16 of A and of B, the 16 bytes of k that
@@ -47,6 +48,17 @@ __device__ inline floatx4 mma(vec<float, 4> a, vec<float, 4> b, floatx4 c) {
 #pragma unroll
     for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
     return c;
+}
+
+// e4m3 in bytes. A k tile's 128 bytes are one instruction's k: lane l gives the chunks l / 16 of both
+// halves of the tile, on both sides, so each k meets its own. The instruction's block scales are 1.
+using e4m3 = uint8_t;
+__device__ inline floatx4 mma(vec<e4m3, 16> a0, vec<e4m3, 16> a1, vec<e4m3, 16> b0, vec<e4m3, 16> b1, floatx4 c) {
+    using int4 = vec<int, 4>;
+    const auto a = __builtin_shufflevector(__builtin_bit_cast(int4, a0), __builtin_bit_cast(int4, a1), 0, 1, 2, 3, 4, 5, 6, 7);
+    const auto b = __builtin_shufflevector(__builtin_bit_cast(int4, b0), __builtin_bit_cast(int4, b1), 0, 1, 2, 3, 4, 5, 6, 7);
+    constexpr int E4M3 = 0, ONE = 0x7f7f7f7f;  // 2^(127 - 127)
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, E4M3, E4M3, 0, ONE, 0, ONE);
 }
 
 constexpr int UNIT_BYTES = 16384;  // of 128 rows
@@ -161,6 +173,67 @@ struct Loader {
     }
 };
 
+// The weights of a gated layer, whose 2 N rows are N of the gate and N of what it gates: a workgroup
+// takes COLS outputs' rows of both, so that a lane has both sums of an output. In LDS a wave's TILE / 2
+// rows are TILE / 4 of the gate and then the same outputs' of the other half.
+template <class T, int NF, int WAVES, int ROWS>
+struct GatedLoader {
+    static constexpr int CH = 16 / sizeof(T), BK = 8 * CH, LOADS = ROWS / 8 / WAVES, HALF = ROWS / 4;
+    static_assert(HALF % 8 == 0, "a load's eight rows are of one half");
+    const char* base;
+    int64_t other;  // bytes from the gate's rows to the others
+    uint64_t span;
+    int64_t K;
+    uint32_t off[LOADS];
+    int kc;
+
+    __device__ void init(const Operand& o, int64_t col0, int64_t K_) {
+        const int lane = threadIdx.x & 63, w = (threadIdx.x >> 6) % WAVES;
+        K = K_;
+        const int64_t ld = o.ld, valid = o.rows - col0 < ROWS / 2 ? o.rows - col0 : ROWS / 2;
+        base = (const char*)o.ptr + col0 * ld * (int64_t)sizeof(T);
+        other = o.rows * ld * (int64_t)sizeof(T);
+        span = ((valid - 1) * ld + (K + CH - 1) / CH * CH) * (int64_t)sizeof(T);  // whole chunks
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int pos = (i * WAVES + w) * 64 + lane, R = pos >> 3;
+            const int chunk = (pos & 7) ^ swizzle<T, true, true, NF / 2, ROWS>(R);
+            off[i] = (uint32_t)((R / (2 * HALF) * HALF + R % HALF) * ld * sizeof(T)) + chunk * 16;
+            kc = chunk * CH;
+        }
+    }
+
+    // As Loader::issue.
+    __device__ void issue(int, int64_t kt, uint32_t lds) const {
+        const int w = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % WAVES);
+        const int64_t left = K - kt * BK;
+        const uint32_t bytes = left > 0 ? (uint32_t)(span - kt * 128) : 0u;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const char* p = base + kt * 128 + (((i * WAVES + w) * 8 / HALF) & 1) * other;
+            vec<uint32_t, 4> rsrc = {(uint32_t)(uintptr_t)p, (uint32_t)((uintptr_t)p >> 32) & 0xffffu, bytes, 0x00020000u};
+#pragma unroll
+            for (int e = 0; e < 4; e++) rsrc[e] = __builtin_amdgcn_readfirstlane(rsrc[e]);
+            const uint32_t dst = __builtin_amdgcn_readfirstlane(lds + (i * WAVES + w) * 1024);
+            const uint32_t o = kc < left ? off[i] : PAST_END;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(o),
+                         "s"(rsrc)
+                         : "memory");
+        }
+    }
+};
+
+// The same for a tile of 256, whose two units of B are the two halves.
+template <class T>
+struct GatedUnits {
+    Loader<T, true, true, 1, 2, 8> half[2];
+    __device__ void init(const Operand& o, int64_t col0, int64_t K) {
+        half[0].init(o, col0, K);
+        half[1].init({(const T*)o.ptr + o.rows * o.ld, o.ld, o.rows}, col0, K);
+    }
+    __device__ void issue(int u, int64_t kt, uint32_t lds) const { half[u].issue(0, kt, lds); }
+};
+
 template <int N>
 __device__ inline void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
@@ -213,6 +286,24 @@ struct Frags {
     }
 };
 
+// NF fragments of a gated layer's weights: the first half are the gate's, the others the same
+// outputs' of what it gates. 2 NF neighbours in the output a lane.
+template <class T, int NF, int ROWS>
+struct GatedFrags {
+    using F = typename Frags<T, true, true, NF / 2, ROWS>::F;
+    F f[NF][2];
+
+    __device__ void read(const char* unit, int r0) {
+        Frags<T, true, true, NF / 2, ROWS> part;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            part.read(unit, r0 + u * (ROWS / 4));
+#pragma unroll
+            for (int i = 0; i < NF; i++) f[u * (NF / 2) + i / 2][i % 2] = part.f[i / 2][i % 2];
+        }
+    }
+};
+
 // How a k tile's fragments are multiplied.
 //
 // Straight: with the instructions of the operands' own type.
@@ -233,12 +324,19 @@ struct Frags {
 struct Straight {
     template <class FA, class FB, int NA, int NB>
     static __device__ inline void multiply(const FA& a, const FB& b, floatx4 (&acc)[NA][NB]) {
-#pragma unroll
-        for (int h = 0; h < 2; h++)
+        if constexpr (sizeof(a.f[0][0][0]) == 1) {
 #pragma unroll
             for (int i = 0; i < NA; i++)
 #pragma unroll
-                for (int j = 0; j < NB; j++) acc[i][j] = mma(b.f[j][h], a.f[i][h], acc[i][j]);
+                for (int j = 0; j < NB; j++) acc[i][j] = mma(b.f[j][0], b.f[j][1], a.f[i][0], a.f[i][1], acc[i][j]);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < NA; i++)
+#pragma unroll
+                    for (int j = 0; j < NB; j++) acc[i][j] = mma(b.f[j][h], a.f[i][h], acc[i][j]);
+        }
     }
 };
 
@@ -333,14 +431,17 @@ __device__ inline void pick_tile(int64_t tiles_m, int64_t tiles_n, int64_t& tm, 
 // less a tile's start and end, about 10 us that nothing covers, count as well: 16384 x 4096
 // outputs and k = 1024 take 132 us (1.04 PFLOP/s), 16384 x 1024 and k = 4096 103 us (1.33). A CU that
 // is given 128 x 128 tiles instead reads an operand twice as often: 72 and 61 us at 4096^2 and k = 2048.
-template <class T, bool AK, bool BK_, class Epilogue>
+//
+// GATED: B is a gated layer's weights, N the outputs, of which a tile has 128.
+template <class T, bool AK, bool BK_, class Epilogue, bool GATED = false>
 __device__ inline void gemm_256(const Gemm& p) {
     __shared__ __align__(1024) char lds[8 * UNIT_BYTES];
     using LA = Loader<T, AK, false, 2, 4, 8>;
-    using LB = Loader<T, BK_, true, 2, 2, 8>;
+    using LB = std::conditional_t<GATED, GatedUnits<T>, Loader<T, BK_, true, 2, 2, 8>>;
+    constexpr int COLS = GATED ? 128 : 256;
     int64_t tm, tn;
-    pick_tile((p.M + 255) / 256, (p.N + 255) / 256, tm, tn);
-    const int64_t m0 = tm * 256, n0 = tn * 256;
+    pick_tile((p.M + 255) / 256, (p.N + COLS - 1) / COLS, tm, tn);
+    const int64_t m0 = tm * 256, n0 = tn * COLS;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w >> 2, wn = w & 3;
     const int64_t tiles = (p.K + LA::BK - 1) / LA::BK, first = (int64_t)blockIdx.y * p.tiles_per_split;
     const int64_t last = first + p.tiles_per_split < tiles ? first + p.tiles_per_split : tiles;
@@ -396,18 +497,30 @@ __device__ inline void gemm_256(const Gemm& p) {
     if (wm == 0) wg_barrier();
     wait_vm<0>();  // LDS is given up with no load on its way there
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-    const int nu = BK_ ? 32 : 128;
-    Epilogue e0, e1;
-    e0.columns(p, n0 + wn * (BK_ ? 64 : 32) + q * 8);
-    e1.columns(p, n0 + wn * (BK_ ? 64 : 32) + nu + q * 8);
+    if constexpr (GATED) {
+        Epilogue e;
+        e.columns(p, n0 + wn * 32 + q * 8);
 #pragma unroll
-    for (int ua = 0; ua < 2; ua++)
+        for (int ua = 0; ua < 2; ua++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int64_t m = m0 + ua * 128 + wm * 64 + i * 16 + r;
-            e0.row(p, m, acc[ua][0][i]);
-            e1.row(p, m, acc[ua][1][i]);
-        }
+            for (int i = 0; i < 4; i++) {
+                const floatx4 both[4] = {acc[ua][0][i][0], acc[ua][0][i][1], acc[ua][1][i][0], acc[ua][1][i][1]};
+                e.row(p, m0 + ua * 128 + wm * 64 + i * 16 + r, both);
+            }
+    } else {
+        const int nu = BK_ ? 32 : 128;
+        Epilogue e0, e1;
+        e0.columns(p, n0 + wn * (BK_ ? 64 : 32) + q * 8);
+        e1.columns(p, n0 + wn * (BK_ ? 64 : 32) + nu + q * 8);
+#pragma unroll
+        for (int ua = 0; ua < 2; ua++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int64_t m = m0 + ua * 128 + wm * 64 + i * 16 + r;
+                e0.row(p, m, acc[ua][0][i]);
+                e1.row(p, m, acc[ua][1][i]);
+            }
+    }
 }
 
 // TILE x TILE (128 or 64) by GROUPS groups of four waves, a quarter of the output each, two k
@@ -416,19 +529,27 @@ __device__ inline void gemm_256(const Gemm& p) {
 // outputs, k = 2048 in bfloat16: 72 us with two of 128, 111 with four; 107 with two of 64, 105 with
 // three, 124 with four). A workgroup that is alone on its CU has two groups that cover each
 // other's waits: they take the k tiles in turn, and add their sums through LDS at the end.
-template <class T, bool AK, bool BK_, class Epilogue, class Math, int TILE, int GROUPS>
+//
+// GATED: B is a gated layer's weights, N the outputs, of which a tile has TILE / 2.
+template <class T, bool AK, bool BK_, class Epilogue, class Math, int TILE, int GROUPS, bool GATED = false>
 __device__ inline void gemm_tile(const Gemm& p) {
     constexpr int NF = TILE / 32, UNIT = TILE * 128;
     __shared__ __align__(1024) char lds[GROUPS * 4 * UNIT];
     using LA = Loader<T, AK, false, 1, NF, 4, TILE>;
-    using LB = Loader<T, BK_, true, 1, NF, 4, TILE>;
+    using LB = std::conditional_t<GATED, GatedLoader<T, NF, 4, TILE>, Loader<T, BK_, true, 1, NF, 4, TILE>>;
     using FA = Frags<T, AK, false, NF, TILE>;
-    using FB = Frags<T, BK_, true, NF, TILE>;
+    using FB = std::conditional_t<GATED, GatedFrags<T, NF, TILE>, Frags<T, BK_, true, NF, TILE>>;
+    constexpr int COLS = GATED ? TILE / 2 : TILE;
     int64_t tm, tn;
-    pick_tile((p.M + TILE - 1) / TILE, (p.N + TILE - 1) / TILE, tm, tn);
-    const int64_t m0 = tm * TILE, n0 = tn * TILE;
+    pick_tile((p.M + TILE - 1) / TILE, (p.N + COLS - 1) / COLS, tm, tn);
+    const int64_t m0 = tm * TILE, n0 = tn * COLS;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3, group = GROUPS == 2 ? wave >> 2 : 0;
-    const int wm = (w >> 1) * (TILE / 2), wn = (w & 1) * (TILE / 2);
+    const int wm = (w >> 1) * (TILE / 2), wn = (w & 1) * (TILE / 2);  // of the output and, for wn, of B's unit
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    // the output column of a lane's fragment j's first number
+    const auto column = [&](int j) {
+        return GATED ? n0 + wn / 2 + q * (2 * NF) + j % (NF / 2) * 4 : n0 + wn + q * (4 * NF) + j * 4;
+    };
     const int64_t tiles = (p.K + LA::BK - 1) / LA::BK, start = (int64_t)blockIdx.y * p.tiles_per_split;
     const int64_t last = start + p.tiles_per_split < tiles ? start + p.tiles_per_split : tiles;
     const int64_t first = start + group, steps = (last - start + GROUPS - 1) / GROUPS;  // the group's tiles
@@ -529,13 +650,12 @@ __device__ inline void gemm_tile(const Gemm& p) {
             walk([&](const FA& fa, const FB& fb) { largest(fa), largest(fb); });
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-            const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
             const float least = most * (float)(steps * LA::BK) * 0x1p-111f;
 #pragma unroll
             for (int i = 0; i < NF * NF; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const bool there = m0 + wm + i / NF * 16 + r < p.M && n0 + wn + q * (4 * NF) + i % NF * 4 + e < p.N;
+                    const bool there = m0 + wm + i / NF * 16 + r < p.M && column(i % NF) + e < p.N;
                     again |= there && !(fabsf(acc[i / NF][i % NF][e]) >= least);
                 }
         }
@@ -545,9 +665,8 @@ __device__ inline void gemm_tile(const Gemm& p) {
             straight();
         }
     }
-    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     Epilogue epilogue;
-    epilogue.columns(p, n0 + wn + q * (4 * NF));
+    epilogue.columns(p, column(0));
     if constexpr (GROUPS == 1) {
 #pragma unroll
         for (int i = 0; i < NF; i++) epilogue.row(p, m0 + wm + i * 16 + r, acc[i]);

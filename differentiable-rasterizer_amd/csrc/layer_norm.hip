@@ -9,7 +9,7 @@
 // the mean is large. All of it is bound by memory: the forward pass reads a row once and
 // writes it once, the backward pass reads two and writes one.
 
-#include "layers.h"
+#include "rows.h"
 
 using namespace drh_rt;
 
@@ -19,37 +19,6 @@ namespace {
 // A row is held in the registers of TPR threads, EPT elements each (with_row), up to
 // LN_MAX_COLS elements. Thread t's vectors are t, t + TPR, ...
 constexpr int LN_MAX_COLS = 256 * 32;
-
-// Weights from column c on; they may stand in 32 bits beside activations in 16.
-template <class T, bool WHOLE, int VEC>
-__device__ inline void load_weight(const void* w, bool wf32, int c, int D, float (&out)[VEC]) {
-    if (wf32)
-        load_some<VEC>((const float*)w + c, WHOLE ? VEC : D - c, out);
-    else
-        load_some<VEC>((const T*)w + c, WHOLE ? VEC : D - c, out);
-}
-
-// Sums of a and b over a row's threads, in all of them. `slot` alternates between
-// calls, so that one barrier a call is enough.
-template <int TPR, int THREADS>
-__device__ inline void row_sums(float& a, float& b, int slot) {
-    a = wave_sum(a);
-    b = wave_sum(b);
-    if constexpr (TPR > 64) {
-        __shared__ float2 part[2][THREADS / 64];
-        const int w = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) part[slot & 1][w] = make_float2(a, b);
-        __syncthreads();
-        const int first = w & ~(TPR / 64 - 1);
-        a = b = 0.0f;
-#pragma unroll
-        for (int i = 0; i < TPR / 64; i++) {
-            const float2 p = part[slot & 1][first + i];
-            a += p.x;
-            b += p.y;
-        }
-    }
-}
 
 struct LnArgs {
     const void *x, *w, *b, *g;
@@ -318,14 +287,6 @@ void with_row(int64_t D, F&& f) {
     else if (D <= 128 * MOST) ept(integral_constant<int, 128>());
     else if (D <= 256 * MOST) ept(integral_constant<int, 256>());
     else if constexpr (256 * MOST < LN_MAX_COLS) ept(integral_constant<int, 512>());
-}
-
-// f(WHOLE, ONCE) as constants.
-template <class T, class F>
-void with_loads(int64_t rows, int64_t cols, F&& f) {
-    if (cols % (16 / (int64_t)sizeof(T))) f(std::false_type(), std::false_type());
-    else if (rows * cols * (int64_t)sizeof(T) < READ_ONCE_BYTES) f(std::true_type(), std::false_type());
-    else f(std::true_type(), std::true_type());
 }
 
 // Of a backward workgroup: its threads and the waves a SIMD that its registers are to allow.

@@ -98,6 +98,12 @@ __device__ inline float wave_sum(float v) {
     return v;
 }
 
+__device__ inline float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
 // f(T()) for the C element type of a DRH_* dtype.
 template <class F>
 int with_type(int dtype, F&& f) {

@@ -13,83 +13,12 @@
 #include <algorithm>
 #include <cmath>
 
-#include "gemm.h"
+#include "products.h"
 
 using namespace drh_rt;
 
 namespace drh_nn {
 namespace {
-
-// ---------------------------------------------------------------- activations
-
-constexpr float LOG2_E = 1.44269504088896341f, SQRT_HALF = 0.70710678118654752f, INV_SQRT_2PI = 0.39894228040143268f;
-constexpr float TANH_C = 0.79788456080286536f, TANH_A = 0.044715f;
-
-// EXACT: for results in 32 bits, with the library's functions; else for values that are
-// rounded to 16 bits afterwards, by single instructions.
-
-// 1 / (1 + exp(-v))
-template <bool EXACT>
-__device__ inline float logistic(float v) {
-    return EXACT ? 1.0f / (1.0f + expf(-v)) : __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2_E * v));
-}
-
-// One instruction each, which passes NaN.
-__device__ inline float not_below(float z, float lo) { return __builtin_elementwise_maximum(z, lo); }
-__device__ inline float not_above(float z, float hi) { return __builtin_elementwise_minimum(z, hi); }
-
-// act(z), and act'(z) in `slope`. Below -128 every value and slope is 0 in 32 bits, above 64
-// every value z and slope 1; the bounds keep infinity times zero out of the products there.
-template <bool EXACT, int ACT>
-__device__ inline float act(float z, float& slope) {
-    if constexpr (ACT == DRH_ACT_NONE) {
-        slope = 1.0f;
-        return z;
-    } else if constexpr (ACT == DRH_ACT_RELU) {
-        slope = z > 0.0f ? 1.0f : 0.0f;
-        return z < 0.0f ? 0.0f : z;
-    } else {
-        z = not_below(z, -128.0f);
-        const float c = not_above(z, 64.0f);
-        if constexpr (ACT == DRH_ACT_SILU) {
-            const float s = logistic<EXACT>(c);
-            slope = s * fmaf(c, 1.0f - s, 1.0f);
-            return z * s;
-        } else if constexpr (ACT == DRH_ACT_GELU_TANH) {
-            const float u = TANH_A * c * c, s = logistic<EXACT>(2.0f * TANH_C * fmaf(u, c, c));  // (1 + tanh) / 2
-            slope = fmaf(2.0f * TANH_C * c * s * (1.0f - s), fmaf(3.0f, u, 1.0f), s);
-            return z * s;
-        } else {
-            // Phi(c) and exp(-c^2 / 2). Phi is made from its own tail and not as (1 + erf) / 2, which
-            // cancels below zero: at -5 that leaves two bits.
-            float phi, e;
-            if constexpr (EXACT) {
-                phi = 0.5f * erfcf(-SQRT_HALF * c);
-                e = expf(-0.5f * c * c);
-            } else {
-                // Phi(-|c|) = e t P(t), t = 1 / (1 + 0.292 |c|), in the manner of Abramowitz and Stegun
-                // 7.1.26, with P fitted to stay within 1e-7 of Phi and 6e-5 of its value down to -13
-                e = __builtin_amdgcn_exp2f(c * c * (-0.5f * LOG2_E));
-                const float t = __builtin_amdgcn_rcpf(fmaf(0.292f, fabsf(c), 1.0f));
-                float q = fmaf(t, -0.0867610723f, 0.27079457f);
-                q = fmaf(t, q, -0.0762883946f);
-                q = fmaf(t, q, 0.170907423f);
-                q = fmaf(t, q, 0.103905939f);
-                q = fmaf(t, q, 0.117441483f);
-                q *= t * e;
-                phi = c < 0.0f ? q : 1.0f - q;
-            }
-            slope = fmaf(c * INV_SQRT_2PI, e, phi);
-            return z * phi;
-        }
-    }
-}
-
-// The type that slopes are kept in.
-template <class T>
-using Kept = std::conditional_t<sizeof(T) == 4, float, f16>;
-template <class T>
-constexpr float KEPT_SCALE = sizeof(T) == 4 ? 1.0f : 32768.0f;
 
 // ---------------------------------------------------------------- the product's epilogue
 
@@ -317,28 +246,10 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(Gemm p, bool a_kc, bool b
     }
 }
 
+}  // namespace
+
 // ---------------------------------------------------------------- which kernel
 
-enum Layout { KK, KN, MN };  // A's and B's contiguous dimension: forward, dx, dW
-
-struct GemmPlan {
-    int tile = 0;    // 256, 128, 64, or 0: any
-    bool rows = false;  // gemm_rows_kernel
-    int splits = 1;
-    size_t bytes = 0;  // of partial sums
-};
-
-constexpr int CUS = 256;
-// gemm_rows_kernel's: it reads x from the caches for every 16 outputs, which with more rows and
-// a long k costs more than staging. Microseconds in bfloat16, with it and by tiles: 32 rows
-// 1280 x 1024 4.8 / 6.5, 4096 x 4096 13.2 / 13.9; 64 rows 4096 x 1024 7.2 / 9.1, 4096 x 4096 21.7 / 14.2.
-constexpr int64_t ROWS_FEW = 32, ROWS_MOST = 64, ROWS_MOST_K = 2048;
-// Products in 32 bits are split in thirds from this k on: their error, 2^-21 of a term at the
-// most (gemm.h says what becomes of terms too small for that), is then below what a 32-bit sum of
-// as many terms may lose, k 2^-24, and shorter products are bound by memory either way.
-constexpr int64_t THIRDS_LEAST = 64;
-
-// Whether an operand's sizes suit the kernels that load 16-byte chunks through buffers.
 bool chunked(int dtype, bool kc, int64_t ld, int64_t rows, int64_t K) {
     const int64_t size = type_size(dtype), ch = 16 / size;
     if (ld % ch || (kc ? K : rows) % ch) return false;
@@ -384,29 +295,13 @@ GemmPlan plan_gemm(int dtype, int64_t M, int64_t N, int64_t K, bool fits) {
     return g;
 }
 
-template <class F>
-int with_act(int act, F&& f) {
-    using std::integral_constant;
-    switch (act) {
-        case DRH_ACT_RELU: return f(integral_constant<int, DRH_ACT_RELU>());
-        case DRH_ACT_GELU: return f(integral_constant<int, DRH_ACT_GELU>());
-        case DRH_ACT_GELU_TANH: return f(integral_constant<int, DRH_ACT_GELU_TANH>());
-        case DRH_ACT_SILU: return f(integral_constant<int, DRH_ACT_SILU>());
-        default: return f(integral_constant<int, DRH_ACT_NONE>());
-    }
-}
 
-bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
-
-// Whether a product's launch holds its tiles: a plan's always, gemm_any_kernel's 64 x 64 not
-// from 2^36 outputs on.
 int check_tiles(const GemmPlan& plan, int64_t M, int64_t N, const void* a, const void* b) {
     if (plan.rows || (plan.tile && aligned(a) && aligned(b))) return DRH_OK;
     if ((M + 63) / 64 * ((N + 63) / 64) <= most_groups(256)) return DRH_OK;
     return fail(DRH_ERR_TOO_LARGE, "more tiles of the output than a launch holds");
 }
 
-// p without its plan's fields; `partial` has plan.bytes bytes.
 int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial, hipStream_t s) {
     if (p.M == 0 || p.N == 0) return DRH_OK;
     const int64_t ch = 16 / (int64_t)type_size(dtype);
@@ -474,13 +369,6 @@ int gemm(int dtype, Layout layout, Gemm p, const GemmPlan& plan, float* partial,
     });
 }
 
-// A row-major operand as the fast kernels take it: as it stands, or copied to rows of K
-// elements rounded up to 16 bytes, with zeros behind K.
-struct Rows {
-    int64_t ld;
-    size_t bytes = 0;  // of the copy, 0: none
-};
-
 Rows rows_for(int dtype, int64_t rows, int64_t K, int64_t ld) {
     const int64_t ch = 16 / (int64_t)type_size(dtype);
     if (K % ch == 0 && ld % ch == 0) return {ld};
@@ -488,11 +376,7 @@ Rows rows_for(int dtype, int64_t rows, int64_t K, int64_t ld) {
     return {padded, up256((size_t)rows * padded * type_size(dtype))};
 }
 
-struct PadJob {
-    const void* src;
-    void* dst;
-    int64_t ld, rows;  // rows 0: nothing to copy
-};
+namespace {
 
 // Two operands of K columns in one launch, a thread a 16-byte chunk.
 template <class T>
@@ -509,6 +393,8 @@ __global__ __launch_bounds__(256) void pad_rows(PadJob a, PadJob b, int64_t K, i
     *(Raw*)((T*)job.dst + row * per * CH + c) = v;
 }
 
+}  // namespace
+
 void pad(int dtype, const PadJob& a, const PadJob& b, int64_t K, hipStream_t s) {
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
@@ -521,6 +407,8 @@ void pad(int dtype, const PadJob& a, const PadJob& b, int64_t K, hipStream_t s) 
 }
 
 // ---------------------------------------------------------------- dz and the bias gradient
+
+namespace {
 
 // dz = dy act'(z), rounded to its type for the products, in rows of ldz elements with zeros
 // behind N, and the column sums of the unrounded values: a workgroup owns 64 chunks of every
@@ -571,15 +459,15 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
     }
 }
 
-// Row groups of slope_kernel: two rows a wave at least, and about 2048 workgroups at most.
+}  // namespace
+
 int64_t slope_groups(int64_t M, int64_t N, int dtype) {
     const int64_t cols = 64 * (16 / (int64_t)type_size(dtype)), blocks = (N + cols - 1) / cols;
     const int64_t need = (M + 7) / 8, most = std::min<int64_t>(512, std::max<int64_t>(64, 2048 / blocks));
     return std::min(need, most);
 }
 
-// A single row has no stride: whatever the caller gives for it must not name rows behind it.
-int64_t stride_of(int64_t rows, int64_t stride, int64_t K) { return rows > 1 ? stride : K; }
+namespace {
 
 struct ForwardPlan {
     Rows x, w;
@@ -590,7 +478,7 @@ struct ForwardPlan {
 ForwardPlan forward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype) {
     ForwardPlan f;
     xs = stride_of(M, xs, K), ws = stride_of(N, ws, K);
-    if (K > 0 && (M <= ROWS_FEW || (M <= ROWS_MOST && K <= ROWS_MOST_K)) && (N + 15) / 16 <= most_groups(512)) {
+    if (few_rows(M, N, K)) {
         f.x = {xs}, f.w = {ws}, f.y.rows = true;
         return f;
     }
@@ -606,15 +494,7 @@ ForwardPlan forward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws
     return f;
 }
 
-// x and W padded where dW and dx need them, dz where it is not dy itself or dy needs
-// padding, the bias gradient's partial sums, and the larger of the products' partial sums.
-struct BackwardPlan {
-    Rows x, w;
-    bool dz = false;
-    int64_t ldz = 0;
-    GemmPlan dx, dw;
-    size_t x_at = 0, w_at = 0, dz_at = 0, sums_at = 0, part_at = 0, total = 0;
-};
+}  // namespace
 
 BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype, int act) {
     BackwardPlan b;
@@ -640,7 +520,7 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t 
     return b;
 }
 
-int check_sizes(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {
+int check_product_sizes(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {
     if (M < 0 || N <= 0 || K < 0) return fail(DRH_ERR_INVALID_ARG, "rows and inputs must not be negative, outputs positive");
     if (M > INT32_MAX || N > (1 << 30) || K > (1 << 30))
         return fail(DRH_ERR_TOO_LARGE, "more than 2^31 - 1 rows or 2^30 features");
@@ -649,18 +529,22 @@ int check_sizes(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws) {
     return rc ? rc : check_span(N, ws);
 }
 
+namespace {
+
 int check_linear(drh_ctx* ctx, int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype, int act,
                  uint32_t flags) {
     int rc = check_call(ctx, dtype, flags);
     if (rc) return rc;
     if (act < DRH_ACT_NONE || act > DRH_ACT_SILU) return fail(DRH_ERR_INVALID_ARG, "unknown activation " + std::to_string(act));
-    return check_sizes(M, N, K, xs, ws);
+    return check_product_sizes(M, N, K, xs, ws);
 }
 
 int check_bytes(int64_t M, int64_t N, int64_t K, int64_t xs, int64_t ws, int dtype, const uint64_t* out_bytes) {
     if (!out_bytes || !known_type(dtype)) return fail(DRH_ERR_INVALID_ARG, "unknown element type, or out_bytes is NULL");
-    return check_sizes(M, N, K, xs, ws);
+    return check_product_sizes(M, N, K, xs, ws);
 }
+
+}  // namespace
 
 int check_workspace(size_t need, const void* workspace, uint64_t bytes) {
     if (bytes < need || (need && !workspace))
@@ -669,7 +553,6 @@ int check_workspace(size_t need, const void* workspace, uint64_t bytes) {
     return DRH_OK;
 }
 
-}  // namespace
 }  // namespace drh_nn
 
 using namespace drh_nn;

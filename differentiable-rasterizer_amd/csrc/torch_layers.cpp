@@ -197,21 +197,29 @@ struct DifferentiatedAgain : Node {
 struct OnceNode : Node {
     variable_list apply(variable_list&& grads) final {
         std::lock_guard<std::mutex> lock(mutex_);
-        refuse_transforms({&grads[0]});
-        if (grads[0].defined()) {  // the engine sees to this, but a node's own hooks come after it
-            const auto& meta = input_metadata(0);
-            TORCH_CHECK(meta.is_same_shape(grads[0]) && grads[0].device() == meta.device() && grads[0].layout() == at::kStrided &&
-                            grads[0].scalar_type() == meta.dtype().toScalarType(),
+        bool any = false;
+        for (size_t i = 0; i < grads.size(); i++) {
+            refuse_transforms({&grads[i]});
+            if (!grads[i].defined()) continue;
+            any = true;  // the engine sees to what follows, but a node's own hooks come after it
+            const auto& meta = input_metadata(i);
+            TORCH_CHECK(meta.is_same_shape(grads[i]) && grads[i].device() == meta.device() && grads[i].layout() == at::kStrided &&
+                            grads[i].scalar_type() == meta.dtype().toScalarType(),
                         "the gradient of a layer's output is of another type, shape or device than the output");
         }
+        if (!any) return variable_list(num_outputs());
         variable_list r;
         {
             at::NoGradGuard no;
-            r = grads[0].defined() ? gradients(grads[0].resolve_neg()) : variable_list(num_outputs());
+            variable_list resolved(grads.size());
+            for (size_t i = 0; i < grads.size(); i++)
+                if (grads[i].defined()) resolved[i] = grads[i].resolve_neg();
+            r = gradients_of(resolved);
         }
-        if (at::GradMode::is_enabled() && grads[0].defined()) {
+        if (at::GradMode::is_enabled()) {
             torch::autograd::edge_list edges = next_edges();
-            edges.push_back(torch::autograd::impl::gradient_edge(grads[0]));
+            for (const Tensor& g : grads)
+                if (g.defined()) edges.push_back(torch::autograd::impl::gradient_edge(g));
             auto error = std::shared_ptr<Node>(new DifferentiatedAgain(), torch::autograd::deleteNode);
             error->set_next_edges(std::move(edges));
             for (Tensor& t : r)
@@ -222,16 +230,24 @@ struct OnceNode : Node {
         }
         return r;
     }
-    virtual variable_list gradients(const Tensor& g) = 0;
+    // From the gradients of all outputs, one of which at least is defined; a layer of one output has the other.
+    virtual variable_list gradients_of(const variable_list& g) { return gradients(g[0]); }
+    virtual variable_list gradients(const Tensor&) { return variable_list(num_outputs()); }
 };
 
-// y as the output of `node`, whose inputs are `inputs` in the order of its gradients.
+// The node's edges to `inputs`, in the order of its gradients.
 template <class N>
-Tensor attach(Tensor y, std::shared_ptr<N> node, std::initializer_list<const Tensor*> inputs) {
+void lead_to(const std::shared_ptr<N>& node, std::initializer_list<const Tensor*> inputs) {
     torch::autograd::edge_list edges;
     for (const Tensor* t : inputs)
         edges.push_back(t->defined() ? torch::autograd::impl::gradient_edge(*t) : torch::autograd::Edge());
     node->set_next_edges(std::move(edges));
+}
+
+// y as the output of `node`, whose inputs are `inputs` in the order of its gradients.
+template <class N>
+Tensor attach(Tensor y, std::shared_ptr<N> node, std::initializer_list<const Tensor*> inputs) {
+    lead_to(node, inputs);
     torch::autograd::set_history(y, node);
     return y;
 }
@@ -464,10 +480,367 @@ Tensor dropout(Tensor x, double p, uint64_t seed, uint64_t offset, const Optiona
     return attach(std::move(y), std::move(node), {&x, &res});
 }
 
+// ---------------------------------------------------------------- rms norm
+
+// Keeps what the gradients that are wanted need: the sum, of which the backward pass makes h; the
+// weight where dx (which is the residual's gradient too) is.
+struct RmsNormBackward : OnceNode {
+    Kept sum_, weight_, rstd_;
+    at::ScalarType weight_type = at::kFloat;
+    int weight_code = DRH_F32;
+
+    std::string name() const override { return "DiffrastRmsNormBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        sum_.release();
+        weight_.release();
+        rstd_.release();
+    }
+
+    // x, weight, residual from y (and the sum)
+    variable_list gradients_of(const variable_list& g) override {
+        const Tensor gs = g.size() > 1 ? g[1] : undefined();
+        const bool data = task_should_compute_output(0) || task_should_compute_output(2);
+        const Tensor s = sum_.get(), rstd = flat(rstd_.get()), w = weight_.get();
+        const Tensor sv = as_rows(s), wv = flat(w);
+        const int64_t rows = sv.size(0), cols = sv.size(1);
+        variable_list r(3);
+        if (!g[0].defined()) {  // y was not used
+            if (task_should_compute_output(1)) r[1] = at::zeros({cols}, s.options().dtype(weight_type));
+            for (int i : {0, 2})
+                if (task_should_compute_output(i)) r[i] = gs;
+            return r;
+        }
+        const Tensor gv = as_rows(g[0]), gsv = gs.defined() ? as_rows(gs) : gs;
+        Tensor dx;
+        if (data) dx = at::empty(g[0].sizes(), s.options());
+        if (task_should_compute_output(1)) r[1] = at::empty({cols}, s.options().dtype(weight_type));
+        uint64_t bytes = 0;
+        if (r[1].defined()) check(drh_rms_norm_backward_bytes(rows, cols, dtype_code(s), &bytes));
+        const Tensor ws = workspace(bytes, s);
+        Call call(s);
+        check(drh_rms_norm_backward(call.ctx, in(sv), in(wv), (const float*)in(rstd), in(gv), in(gsv), rows, cols, row_stride(sv),
+                                    row_stride(gv), gsv.defined() ? row_stride(gsv) : cols, dtype_code(s), weight_code, out(dx),
+                                    out(r[1]), out(ws), bytes, call.stream, 0));
+        for (int i : {0, 2})
+            if (task_should_compute_output(i)) r[i] = dx;
+        return r;
+    }
+};
+
+void check_rms(const Tensor& x, const Tensor& w, const Tensor& res, double eps) {
+    dtype_code(x);
+    const int64_t cols = x.dim() ? x.size(-1) : 0;
+    TORCH_CHECK_VALUE(cols > 0, "expected x of shape (..., D), got ", x.sizes());
+    TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative");
+    TORCH_CHECK_VALUE(!w.defined() || (w.dim() == 1 && w.size(0) == cols), "expected weight of shape (", cols, ",), got ",
+                      w.defined() ? w.sizes() : x.sizes());
+    TORCH_CHECK_VALUE(!w.defined() || w.scalar_type() == x.scalar_type() || w.scalar_type() == at::kFloat, "expected weight in ",
+                      x.scalar_type(), " or float32, got ", w.defined() ? w.scalar_type() : x.scalar_type());
+    TORCH_CHECK_VALUE(!res.defined() || (res.sizes() == x.sizes() && res.scalar_type() == x.scalar_type()),
+                      "expected a residual of shape ", x.sizes(), " in ", x.scalar_type(), ", got ",
+                      res.defined() ? res.sizes() : x.sizes(), " in ", res.defined() ? res.scalar_type() : x.scalar_type());
+}
+
+Optional maybe(const Tensor& t) { return t.defined() ? Optional(t) : std::nullopt; }
+
+std::vector<Tensor> to(std::vector<Tensor> ts, at::Device home) {
+    for (Tensor& t : ts) t = t.to(home);
+    return ts;
+}
+
+// y, and with a residual the sum.
+std::vector<Tensor> rms_norm(Tensor x, const Optional& weight, const Optional& residual, double eps) {
+    Tensor w = of(weight), res = of(residual);
+    check_rms(x, w, res, eps);
+    refuse_transforms({&x, &w, &res});
+    const at::Device home = x.device();
+    if (!together({&x, &w, &res})) return to(rms_norm(x, maybe(w), maybe(res), eps), home);
+    const bool grad = wants_grad({&x, &w, &res});
+    const int code = dtype_code(x), wcode = w.defined() ? dtype_code(w) : code;
+    Tensor y, sum, rstd;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Tensor xv = as_rows(x), wv = flat(w), rv = res.defined() ? as_rows(res) : res;
+        const int64_t rows = xv.size(0);
+        y = at::empty(x.sizes(), x.options());
+        if (res.defined()) sum = at::empty(x.sizes(), x.options());
+        if (grad) rstd = at::empty({rows}, x.options().dtype(at::kFloat));
+        Call call(x);
+        check(drh_rms_norm(call.ctx, in(xv), in(rv), in(wv), rows, xv.size(1), row_stride(xv), rv.defined() ? row_stride(rv) : 0,
+                           code, wcode, (float)eps, out(y), out(sum), (float*)out(rstd), call.stream, 0));
+    }
+    if (grad) {
+        auto node = new_node<RmsNormBackward>();
+        // the sum itself leads to this node: its values are kept without that
+        node->sum_.keep(sum.defined() ? sum.detach() : x);
+        node->rstd_.keep(rstd);
+        if (w.defined() && (x.requires_grad() || (res.defined() && res.requires_grad()))) node->weight_.keep(w);
+        node->weight_type = w.defined() ? w.scalar_type() : x.scalar_type();
+        node->weight_code = wcode;
+        y = attach(std::move(y), node, {&x, &w, &res});
+        if (sum.defined()) torch::autograd::set_history(sum, node);
+    }
+    if (!sum.defined()) return {y};
+    return {y, sum};
+}
+
+void refuse_gradients(std::initializer_list<const Tensor*> ts, const char* what) {
+    TORCH_CHECK(!wants_grad(ts), what, " has no gradient: call it under torch.no_grad(), or on tensors that need none");
+}
+
+// The codes, their rows' scales, and with a residual the sum.
+std::vector<Tensor> rms_norm_8bit(Tensor x, const Optional& weight, const Optional& residual, double eps) {
+    Tensor w = of(weight), res = of(residual);
+    check_rms(x, w, res, eps);
+    refuse_transforms({&x, &w, &res});
+    refuse_gradients({&x, &w, &res}, "rms_norm_8bit");
+    const at::Device home = x.device();
+    if (!together({&x, &w, &res})) return to(rms_norm_8bit(x, maybe(w), maybe(res), eps), home);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor xv = as_rows(x), wv = flat(w), rv = res.defined() ? as_rows(res) : res;
+    const Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+    const Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    Tensor sum;
+    if (res.defined()) sum = at::empty(x.sizes(), x.options());
+    Call call(x);
+    check(drh_rms_norm_8bit(call.ctx, in(xv), in(rv), in(wv), xv.size(0), xv.size(1), row_stride(xv),
+                            rv.defined() ? row_stride(rv) : 0, dtype_code(x), w.defined() ? dtype_code(w) : dtype_code(x),
+                            (float)eps, out(q), (float*)out(scale), out(sum), call.stream, 0));
+    if (!sum.defined()) return {q, scale};
+    return {q, scale, sum};
+}
+
+std::vector<Tensor> quantize_8bit(Tensor x) {
+    check_rms(x, undefined(), undefined(), 0.0);
+    refuse_transforms({&x});
+    refuse_gradients({&x}, "quantize_8bit");
+    const at::Device home = x.device();
+    if (!together({&x})) return to(quantize_8bit(x), home);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor xv = as_rows(x);
+    const Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+    const Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    Call call(x);
+    check(drh_quantize_8bit(call.ctx, in(xv), xv.size(0), xv.size(1), row_stride(xv), dtype_code(x), out(q), (float*)out(scale),
+                            call.stream, 0));
+    return {q, scale};
+}
+
+// ---------------------------------------------------------------- 8-bit linear
+
+// t as (rows, K) of bytes as drh_linear_8bit takes them: 16-byte rows at 16-byte addresses.
+Tensor as_byte_rows(const Tensor& t) {
+    Tensor v = as_rows(t);
+    if ((v.size(0) > 1 && v.stride(0) % 16) || (uintptr_t)in(v) % 16) v = v.clone(at::MemoryFormat::Contiguous);
+    return v;
+}
+
+Tensor linear_8bit(Tensor x, Tensor xs, Tensor w, Tensor ws, const Optional& bias, int act, const Optional& residual,
+                   at::ScalarType dtype) {
+    Tensor b = of(bias), res = of(residual);
+    TORCH_CHECK_VALUE(x.scalar_type() == at::kFloat8_e4m3fn && w.scalar_type() == at::kFloat8_e4m3fn,
+                      "expected x and weight in float8_e4m3fn, got ", x.scalar_type(), " and ", w.scalar_type());
+    TORCH_CHECK_VALUE(xs.scalar_type() == at::kFloat && ws.scalar_type() == at::kFloat, "expected scales in float32, got ",
+                      xs.scalar_type(), " and ", ws.scalar_type());
+    TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1) && w.size(0) > 0,
+                      "expected x (..., K) and weight (N, K), got ", x.sizes(), " and ", w.sizes());
+    const int64_t n_out = w.size(0), n_in = w.size(1);
+    TORCH_CHECK_VALUE(n_in > 0 && n_in % 16 == 0, "the inputs of 8-bit products are multiples of 16, got ", n_in);
+    TORCH_CHECK_VALUE(xs.sizes() == x.sizes().slice(0, x.dim() - 1) && ws.dim() == 1 && ws.size(0) == n_out,
+                      "expected a scale for each row of x and of weight, got ", xs.sizes(), " and ", ws.sizes());
+    TORCH_CHECK_VALUE(dtype == at::kFloat || dtype == at::kBFloat16 || dtype == at::kHalf,
+                      "expected an output in float32, bfloat16 or float16, got ", dtype);
+    c10::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = n_out;
+    TORCH_CHECK_VALUE(!b.defined() || (b.dim() == 1 && b.size(0) == n_out && b.scalar_type() == dtype),
+                      "expected bias of shape (", n_out, ",) in ", dtype);
+    TORCH_CHECK_VALUE(!res.defined() || (res.sizes() == c10::IntArrayRef(shape) && res.scalar_type() == dtype),
+                      "expected residual of shape ", c10::IntArrayRef(shape), " in ", dtype);
+    refuse_transforms({&x, &xs, &w, &ws, &b, &res});
+    refuse_gradients({&x, &xs, &w, &ws, &b, &res}, "linear_8bit");
+    const at::Device home = x.device();
+    if (!together({&x, &xs, &w, &ws, &b, &res})) return linear_8bit(x, xs, w, ws, maybe(b), act, maybe(res), dtype).to(home);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor y = at::empty(shape, x.options().dtype(dtype));
+    const Tensor xv = as_byte_rows(x), wv = as_byte_rows(w), xsv = flat(xs), wsv = flat(ws), bv = flat(b), rv = flat(res);
+    uint64_t bytes = 0;
+    check(drh_linear_8bit_bytes(xv.size(0), n_out, n_in, row_stride(xv), row_stride(wv), &bytes));
+    const Tensor space = workspace(bytes, x);
+    Call call(x);
+    check(drh_linear_8bit(call.ctx, in(xv), (const float*)in(xsv), in(wv), (const float*)in(wsv), in(bv), in(rv), xv.size(0), n_out,
+                          n_in, row_stride(xv), row_stride(wv), dtype_code(y), act, out(y), out(space), bytes, call.stream, 0));
+    return y;
+}
+
+// ---------------------------------------------------------------- gated linear
+
+// Keeps what the gradients that are wanted need: x where dW is, the weight where dx is, the pairs
+// that make dz.
+struct GatedLinearBackward : OnceNode {
+    Kept x_, weight_, pairs_;
+    std::vector<int64_t> x_sizes;
+    at::TensorOptions options;
+    int64_t rows = 0, n_out = 0, n_in = 0;
+    int code = 0;
+
+    std::string name() const override { return "DiffrastGatedLinearBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        x_.release();
+        weight_.release();
+        pairs_.release();
+    }
+
+    variable_list gradients(const Tensor& grad) override {
+        const Tensor x = x_.get(), w = weight_.get(), kept = flat(pairs_.get());
+        const Tensor xv = x.defined() ? as_rows(x) : x, wv = w.defined() ? as_rows(w) : w;
+        const Tensor g = flat(grad);
+        variable_list r(3);
+        if (task_should_compute_output(0)) r[0] = at::empty(x_sizes, options);
+        if (task_should_compute_output(1)) r[1] = at::empty({2 * n_out, n_in}, options);
+        if (task_should_compute_output(2)) r[2] = at::empty({2 * n_out}, options);
+        const int64_t xs = xv.defined() ? row_stride(xv) : n_in, ws = wv.defined() ? row_stride(wv) : n_in;
+        uint64_t bytes = 0;
+        check(drh_gated_linear_backward_bytes(rows, n_out, n_in, xs, ws, code, &bytes));
+        const Tensor space = workspace(bytes, g);
+        Call call(g);
+        check(drh_gated_linear_backward(call.ctx, in(xv), in(wv), in(kept), in(g), rows, n_out, n_in, xs, ws, code, out(r[0]),
+                                        out(r[1]), out(r[2]), out(space), bytes, call.stream, 0));
+        return r;
+    }
+};
+
+Tensor gated_linear(Tensor x, Tensor w, const Optional& bias, int act) {
+    Tensor b = of(bias);
+    const int code = dtype_code(x);
+    TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1) && w.size(0) > 0 && w.size(0) % 2 == 0,
+                      "expected x (..., K) and weight (2 N, K), got ", x.sizes(), " and ", w.sizes());
+    const int64_t n_out = w.size(0) / 2, n_in = w.size(1);
+    c10::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = n_out;
+    TORCH_CHECK_VALUE(!b.defined() || (b.dim() == 1 && b.size(0) == 2 * n_out), "expected bias of shape (", 2 * n_out,
+                      ",), got ", b.defined() ? b.sizes() : x.sizes());
+    for (const Tensor* t : {&w, &b})
+        TORCH_CHECK_VALUE(!t->defined() || t->scalar_type() == x.scalar_type(), "x is ", x.scalar_type(), " but ",
+                          t == &w ? "weight " : "bias ", t->defined() ? t->scalar_type() : x.scalar_type());
+    refuse_transforms({&x, &w, &b});
+    const at::Device home = x.device();
+    if (!together({&x, &w, &b})) return gated_linear(x, w, maybe(b), act).to(home);
+    const bool grad = wants_grad({&x, &w, &b});
+    Tensor y, kept;
+    int64_t rows = 0;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Tensor xv = as_rows(x), wv = as_rows(w), bv = flat(b);
+        rows = xv.size(0);
+        const int64_t xs = row_stride(xv), ws = row_stride(wv);
+        y = at::empty(shape, x.options());
+        if (grad) kept = at::empty({rows * n_out * (code == DRH_F32 ? 8 : 6)}, x.options().dtype(at::kByte));
+        uint64_t bytes = 0;
+        check(drh_gated_linear_bytes(rows, n_out, n_in, xs, ws, code, &bytes));
+        const Tensor space = workspace(bytes, x);
+        Call call(x);
+        check(drh_gated_linear(call.ctx, in(xv), in(wv), in(bv), rows, n_out, n_in, xs, ws, code, act, out(y), out(kept),
+                               out(space), bytes, call.stream, 0));
+    }
+    if (!grad) return y;
+    auto node = new_node<GatedLinearBackward>();
+    if (w.requires_grad()) node->x_.keep(x);
+    if (x.requires_grad()) node->weight_.keep(w);
+    node->x_sizes = x.sizes().vec();
+    node->options = x.options();
+    node->rows = rows, node->n_out = n_out, node->n_in = n_in;
+    node->code = code;
+    node->pairs_.keep(kept);
+    return attach(std::move(y), std::move(node), {&x, &w, &b});
+}
+
+// ---------------------------------------------------------------- AdamW
+
+using Tensors = std::vector<Tensor>;
+
+// One step over all tensors, in place. steps: one tensor of all counts, or one a parameter.
+void adamw(const Tensors& params, const Tensors& grads, const Tensors& avgs, const Tensors& sqs,
+           const std::optional<Tensors>& avg_scales, const std::optional<Tensors>& sq_scales, const Optional& flat_steps,
+           const std::optional<Tensors>& steps, double lr, double beta1, double beta2, double eps, double weight_decay,
+           uint64_t seed) {
+    const size_t n = params.size();
+    TORCH_CHECK_VALUE(avg_scales.has_value() == sq_scales.has_value(), "the scales of both states come together");
+    const bool small = avg_scales.has_value();
+    TORCH_CHECK_VALUE(grads.size() == n && avgs.size() == n && sqs.size() == n && (!steps || steps->size() == n) &&
+                          (!small || (avg_scales->size() == n && sq_scales->size() == n)),
+                      "expected a gradient, both states and a step count for each of ", n, " parameters");
+    refuse_tracing();
+    if (n == 0) return;
+    const int code = dtype_code(params[0]);
+    const at::Device device = params[0].device();
+    TORCH_CHECK_VALUE(device.is_cuda(), "the step is made in place: the parameters must be on the GPU");
+    const auto state_type = small ? at::kFloat8_e4m3fn : at::kFloat;
+    auto like = [&](const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const char* what, size_t i) {
+        TORCH_CHECK_VALUE(t.device() == device && t.layout() == at::kStrided && t.scalar_type() == type && t.sizes() == sizes &&
+                              t.is_contiguous() && !t.is_neg(),
+                          "expected ", what, " ", i, " contiguous, of shape ", sizes, " in ", type, " on ", device, ", got ",
+                          t.sizes(), " in ", t.scalar_type(), " on ", t.device(),
+                          t.layout() == at::kStrided && t.is_contiguous() ? "" : ", not contiguous");
+    };
+    if (flat_steps) like(*flat_steps, {(int64_t)n}, at::kLong, "step counts", 0);
+    std::vector<drh_adamw_tensor> table(n);
+    Tensors held;  // gradients that had to be copied
+    for (size_t i = 0; i < n; i++) {
+        const Tensor& p = params[i];
+        like(p, p.sizes(), params[0].scalar_type(), "parameter", i);
+        TORCH_CHECK_VALUE(grads[i].device() == device && grads[i].layout() == at::kStrided &&
+                              grads[i].scalar_type() == p.scalar_type() && grads[i].sizes() == p.sizes(),
+                          "expected gradient ", i, " of shape ", p.sizes(), " in ", p.scalar_type(), " on ", device);
+        refuse_transforms({&p, &grads[i]});
+        like(avgs[i], p.sizes(), state_type, "exp_avg", i);
+        like(sqs[i], p.sizes(), state_type, "exp_avg_sq", i);
+        const int64_t count = p.numel(), blocks = (count + 255) / 256;
+        if (small) {
+            like((*avg_scales)[i], {blocks}, at::kFloat, "exp_avg_scale", i);
+            like((*sq_scales)[i], {blocks}, at::kFloat, "exp_avg_sq_scale", i);
+        }
+        if (steps) like((*steps)[i], {}, at::kLong, "step count", i);
+    }
+    for (size_t i = 0; i < n; i++) {  // nothing is written before everything is checked
+        Tensor g = grads[i].is_neg() ? grads[i].resolve_neg() : grads[i];
+        if (!g.is_contiguous()) {
+            at::NoGradGuard no;
+            g = g.contiguous();
+        }
+        if (!g.is_same(grads[i])) held.push_back(g);
+        drh_adamw_tensor& t = table[i];
+        t.param = out(params[i]), t.grad = in(g), t.exp_avg = out(avgs[i]), t.exp_avg_sq = out(sqs[i]);
+        t.exp_avg_scale = small ? (float*)out((*avg_scales)[i]) : nullptr;
+        t.exp_avg_sq_scale = small ? (float*)out((*sq_scales)[i]) : nullptr;
+        t.step = (int64_t*)(steps ? out((*steps)[i]) : out(*flat_steps)) + (steps ? 0 : i);
+        t.n = params[i].numel();
+    }
+    Call call(params[0]);
+    check(drh_adamw(call.ctx, table.data(), (int64_t)n, code, small ? 8 : 32, lr, beta1, beta2, eps, weight_decay, seed, call.stream,
+                    0));
+    auto written = [](const Tensor& t) {  // what saved it for a backward pass is to know
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    };
+    for (const Tensors* ts : {&params, &avgs, &sqs})
+        for (const Tensor& t : *ts) written(t);
+    for (const auto* ts : {&avg_scales, &sq_scales, &steps})
+        if (ts->has_value())
+            for (const Tensor& t : **ts) written(t);
+    if (flat_steps) written(*flat_steps);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("layer_norm", &layer_norm);
     m.def("linear", &linear);
     m.def("dropout", &dropout);
+    m.def("rms_norm", &rms_norm);
+    m.def("rms_norm_8bit", &rms_norm_8bit);
+    m.def("quantize_8bit", &quantize_8bit);
+    m.def("linear_8bit", &linear_8bit);
+    m.def("gated_linear", &gated_linear);
+    m.def("adamw", &adamw);
 }

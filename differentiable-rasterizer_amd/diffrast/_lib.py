@@ -112,6 +112,11 @@ class FitStatus(ctypes.Structure):
     ]
 
 
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in
+                ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step")] + [("n", _I64)]
+
+
 # Every symbol include/diffrast_hip.h declares, with its ctypes signature.
 SIGNATURES = {
     "drh_timing_enable": ([_P, ctypes.c_int], ctypes.c_int),
@@ -163,6 +168,23 @@ SIGNATURES = {
     "drh_linear_backward_bytes": ([_I64] * 5 + [_INT, _INT, ctypes.POINTER(_U64)], ctypes.c_int),
     "drh_linear_backward": ([_P] * 5 + [_I64] * 5 + [_INT, _INT, _P, _P, _P, _P, _U64, _P, _U32], ctypes.c_int),
     "drh_dropout": ([_P, _P, _P, _I64, _INT, ctypes.c_double, _U64, _U64, _P, _P, _U32], ctypes.c_int),
+    "drh_rms_norm": ([_P, _P, _P, _P, _I64, _I64, _I64, _I64, _INT, _INT, _F32, _P, _P, _P, _P, _U32], ctypes.c_int),
+    "drh_rms_norm_8bit": ([_P, _P, _P, _P, _I64, _I64, _I64, _I64, _INT, _INT, _F32, _P, _P, _P, _P, _U32], ctypes.c_int),
+    "drh_quantize_8bit": ([_P, _P, _I64, _I64, _I64, _INT, _P, _P, _P, _U32], ctypes.c_int),
+    "drh_rms_norm_backward_bytes": ([_I64, _I64, _INT, ctypes.POINTER(_U64)], ctypes.c_int),
+    "drh_rms_norm_backward": ([_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _INT, _P, _P, _P, _U64,
+        _P, _U32], ctypes.c_int),
+    "drh_linear_8bit": ([_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _INT, _P, _P, _U64, _P,
+        _U32], ctypes.c_int),
+    "drh_linear_8bit_bytes": ([_I64, _I64, _I64, _I64, _I64, ctypes.POINTER(_U64)], ctypes.c_int),
+    "drh_gated_linear": ([_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _INT, _P, _P, _P, _U64, _P, _U32],
+        ctypes.c_int),
+    "drh_gated_linear_bytes": ([_I64, _I64, _I64, _I64, _I64, _INT, ctypes.POINTER(_U64)], ctypes.c_int),
+    "drh_gated_linear_backward_bytes": ([_I64, _I64, _I64, _I64, _I64, _INT, ctypes.POINTER(_U64)], ctypes.c_int),
+    "drh_gated_linear_backward": ([_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _P, _P, _P, _P, _U64, _P,
+        _U32], ctypes.c_int),
+    "drh_adamw": ([_P, ctypes.POINTER(AdamWTensor), _I64, _INT, _INT, ctypes.c_double, ctypes.c_double,
+        ctypes.c_double, ctypes.c_double, ctypes.c_double, _U64, _P, _U32], ctypes.c_int),
 }
 
 _lib = None

@@ -6,9 +6,19 @@
     x = dropout(h, 0.1, seed=seed, offset=step, residual=x)      # a residual block
     params = linear(x, w3, c3).float().view(B, T, 10)            # -> torch_layer.rasterize
 
+or, with gated blocks (and `optim.AdamW` to train them),
+
+    y, x = rms_norm(h, g1, residual=x)                           # x: the stream with h added
+    h = linear(gated_linear(y, w1), w2)
+
+and, to answer in 8 bits,
+
+    q, t, x = rms_norm_8bit(h, g1, residual=x)
+    h = linear_8bit(q, t, *w1_in_8_bits, activation="gelu")      # weights: quantize_8bit(w1)
+
 The reference builds such a network from PyTorch's own layers (python/diffrast/model.py)
-and has no counterpart of these. All of them are differentiable once, take float32,
-bfloat16 and float16, compute in 32 bits and round each result once. As in `torch_layer`,
+and has no counterpart of these. All of them but those in 8 bits are differentiable once; they take
+float32, bfloat16 and float16, compute in 32 bits and round each result once. As in `torch_layer`,
 tensors on the GPU stay there and run on torch's current stream, CPU tensors are moved to
 the current GPU and the results returned on the caller's device, wrong arguments raise
 ValueError, and there is no CPU path. Differentiating a gradient again raises RuntimeError, and
@@ -19,6 +29,7 @@ torch.compile runs the calls outside of its graphs. The calls may be captured in
 
 from __future__ import annotations
 
+import torch
 from torch import Tensor
 
 from . import _lib, torch_layer
@@ -28,6 +39,13 @@ _lib.lib()  # the native module links against it
 from . import _torch_layers  # noqa: E402
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _act(activation: str | None) -> int:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"unknown activation {activation!r} — expected one of {list(ACTIVATIONS)}")
+    return act
 
 
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5) -> Tensor:
@@ -57,10 +75,79 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: st
     The backward pass rounds dz = dy act'(z) to x's type for its two products; act'(z) is kept
     for it in float16 beside 16-bit types (in float32 otherwise), where there is an activation.
     """
-    act = ACTIVATIONS.get(activation)
-    if act is None:
-        raise ValueError(f"unknown activation {activation!r} — expected one of {list(ACTIVATIONS)}")
-    y = _torch_layers.linear(x, weight, bias, act, residual)
+    y = _torch_layers.linear(x, weight, bias, _act(activation), residual)
+    torch_layer._note_gpu()
+    return y
+
+
+def gated_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation: str | None = "silu") -> Tensor:
+    """activation(z[..., :N]) * z[..., N:] with z = x @ weight.T + bias, in one kernel.
+
+    Args:
+        x: `(..., K)`.
+        weight: `(2 N, K)`, the gate's rows first, of x's type, as is bias.
+        bias: `(2 N,)` or None.
+        activation: of the gate: None, "relu", "gelu" (z Phi(z)), "gelu_tanh" or "silu".
+
+    The backward pass rounds the gradient of z to x's type for its two products. For it the forward
+    pass keeps the gate's value and slope times the other half, in 24 bits each beside 16-bit types
+    (in float32 otherwise): 6 or 8 bytes an output.
+    """
+    y = _torch_layers.gated_linear(x, weight, bias, _act(activation))
+    torch_layer._note_gpu()
+    return y
+
+
+def rms_norm(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = None, eps: float = 1e-5):
+    """s / sqrt(mean(s^2) + eps) * weight over the last dimension, with s = x + residual.
+
+    Returns y, or with a residual (y, s): the norm and the stream that it was taken of, both
+    differentiable. y is made from s in 32 bits; s is rounded to its type where it is stored, and
+    the backward pass starts from that. The mean of squares is held in float32, which ends at 3e38.
+
+    Args:
+        x: `(..., D)`.
+        weight: `(D,)` or None, of x's type or float32.
+        residual: x's shape and type, or None.
+    """
+    r = _torch_layers.rms_norm(x, weight, residual, eps)
+    torch_layer._note_gpu()
+    return r[0] if residual is None else (r[0], r[1])
+
+
+def rms_norm_8bit(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = None, eps: float = 1e-5):
+    """`rms_norm` with y in 8 bits, for `linear_8bit`: (q, scale), or with a residual (q, scale, s).
+
+    q is float8_e4m3fn, y / scale rounded to nearest even, and scale `(...)` in float32 has
+    max(max |y| / 448, 2^-126) for each row. No gradients: raises RuntimeError where they are wanted.
+    """
+    r = _torch_layers.rms_norm_8bit(x, weight, residual, eps)
+    torch_layer._note_gpu()
+    return tuple(r)
+
+
+def quantize_8bit(x: Tensor) -> tuple[Tensor, Tensor]:
+    """x `(..., D)` as (q, scale) of `rms_norm_8bit`, without the norm: activations, or a `(N, K)` weight."""
+    r = _torch_layers.quantize_8bit(x)
+    torch_layer._note_gpu()
+    return r[0], r[1]
+
+
+def linear_8bit(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor, bias: Tensor | None = None,
+                activation: str | None = None, residual: Tensor | None = None,
+                dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """activation((x * x_scale) @ (weight * weight_scale).T + bias) + residual, in one kernel.
+
+    Args:
+        x: `(..., K)` and weight: `(N, K)`, float8_e4m3fn, K a multiple of 16.
+        x_scale: `(...)` and weight_scale: `(N,)`, float32: a factor for each row.
+        bias: `(N,)` or None; residual: `(..., N)` or None; of type dtype.
+        activation: as in `linear`, within 2^-20 of its argument in every type.
+        dtype: of the output: float32, bfloat16 or float16.
+
+    No gradients: raises RuntimeError where they are wanted.
+    """
+    y = _torch_layers.linear_8bit(x, x_scale, weight, weight_scale, bias, _act(activation), residual, dtype)
     torch_layer._note_gpu()
     return y
 

@@ -408,6 +408,116 @@ int drh_linear_backward(drh_ctx *ctx, const void *x, const void *weight, const v
 int drh_dropout(drh_ctx *ctx, const void *x, const void *residual, int64_t n, int dtype, double p,
                 uint64_t seed, uint64_t offset, void *y, void *stream, uint32_t flags);
 
+/* Root-mean-square norm of `rows` rows of `cols` elements, of the sum with a residual:
+ *   s = x + residual (NULL: 0),  y = s / sqrt(mean(s^2) + eps) * weight (NULL: 1)
+ * x_stride and residual_stride elements lie between the rows of x and residual; y and
+ * sum are contiguous. y is made from s in 32 bits; sum (may be NULL; only with a
+ * residual) receives s in its type. weight: cols elements of weight_dtype (dtype or
+ * DRH_F32). rstd (rows floats, may be NULL) keeps the reciprocal roots for the backward
+ * pass. */
+int drh_rms_norm(drh_ctx *ctx, const void *x, const void *residual, const void *weight, int64_t rows,
+                 int64_t cols, int64_t x_stride, int64_t residual_stride, int dtype, int weight_dtype,
+                 float eps, void *y, void *sum, float *rstd, void *stream, uint32_t flags);
+
+/* The same with y in 8 bits, for drh_linear_8bit: bytes of e4m3 (a sign, four bits of
+ * exponent, three of mantissa, up to 448), y / scale rounded to nearest even, with a scale
+ * for each row, max(max |y| / 448, 2^-126). An element that is not finite becomes NaN. */
+int drh_rms_norm_8bit(drh_ctx *ctx, const void *x, const void *residual, const void *weight,
+                      int64_t rows, int64_t cols, int64_t x_stride, int64_t residual_stride, int dtype,
+                      int weight_dtype, float eps, void *y, float *scale, void *sum, void *stream,
+                      uint32_t flags);
+
+/* Rows to 8 bits without the norm: y and scale of drh_rms_norm_8bit for y = x. */
+int drh_quantize_8bit(drh_ctx *ctx, const void *x, int64_t rows, int64_t cols, int64_t x_stride,
+                      int dtype, void *y, float *scale, void *stream, uint32_t flags);
+
+/* Workspace of drh_rms_norm_backward; none is needed (NULL, 0) without grad_weight. */
+int drh_rms_norm_backward_bytes(int64_t rows, int64_t cols, int dtype, uint64_t *out_bytes);
+
+/* Gradients of drh_rms_norm from its sum (x, where there was no residual), weight and rstd,
+ * from grad_y and from grad_sum (NULL: 0), each with its rows' stride. grad_x (contiguous;
+ * the residual's gradient is the same) and grad_weight (of weight_dtype) may each be
+ * NULL: not computed. */
+int drh_rms_norm_backward(drh_ctx *ctx, const void *sum, const void *weight, const float *rstd,
+                          const void *grad_y, const void *grad_sum, int64_t rows, int64_t cols,
+                          int64_t sum_stride, int64_t grad_y_stride, int64_t grad_sum_stride, int dtype,
+                          int weight_dtype, void *grad_x, void *grad_weight, void *workspace,
+                          uint64_t workspace_bytes, void *stream, uint32_t flags);
+
+/* Linear layer of 8-bit operands: y = activation((x weight^T) x_scale weight_scale + bias)
+ * + residual, x rows x n_in and weight n_out x n_in in bytes of e4m3, with a scale for each
+ * row of both (drh_rms_norm_8bit, drh_quantize_8bit). bias, residual and y are of
+ * dtype. n_in, x_stride and weight_stride are multiples of 16, both operands 16-byte
+ * aligned. */
+int drh_linear_8bit(drh_ctx *ctx, const void *x, const float *x_scale, const void *weight,
+                    const float *weight_scale, const void *bias, const void *residual, int64_t rows,
+                    int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride, int dtype,
+                    int activation, void *y, void *workspace, uint64_t workspace_bytes, void *stream,
+                    uint32_t flags);
+
+/* Workspace of drh_linear_8bit (0 for many sizes). */
+int drh_linear_8bit_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride,
+                          int64_t weight_stride, uint64_t *out_bytes);
+
+/* Gated linear layer: z = x weight^T + bias, y = activation(z[:, :n_out]) z[:, n_out:], x rows
+ * x n_in (rows x_stride elements apart), weight 2 n_out x n_in (rows weight_stride apart, the
+ * gate's first), bias 2 n_out or NULL, y rows x n_out, contiguous. kept, if not NULL,
+ * receives what the backward pass needs, activation(zg) and zu activation'(zg): rows x
+ * n_out x 8 bytes for DRH_F32 (float32), x 6 for the other types (24 bits each). */
+int drh_gated_linear(drh_ctx *ctx, const void *x, const void *weight, const void *bias, int64_t rows,
+                     int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride, int dtype,
+                     int activation, void *y, void *kept, void *workspace, uint64_t workspace_bytes,
+                     void *stream, uint32_t flags);
+
+/* Workspace of drh_gated_linear (0 for many sizes) and of drh_gated_linear_backward. */
+int drh_gated_linear_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride,
+                           int64_t weight_stride, int dtype, uint64_t *out_bytes);
+int drh_gated_linear_backward_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride,
+                                    int64_t weight_stride, int dtype, uint64_t *out_bytes);
+
+/* Gradients of drh_gated_linear from grad_y (rows x n_out, contiguous), its x, weight and
+ * kept. grad_x (rows x n_in), grad_weight (2 n_out x n_in) and grad_bias (2 n_out),
+ * contiguous, may each be NULL: not computed. */
+int drh_gated_linear_backward(drh_ctx *ctx, const void *x, const void *weight, const void *kept,
+                              const void *grad_y, int64_t rows, int64_t n_out, int64_t n_in,
+                              int64_t x_stride, int64_t weight_stride, int dtype, void *grad_x,
+                              void *grad_weight, void *grad_bias, void *workspace,
+                              uint64_t workspace_bytes, void *stream, uint32_t flags);
+
+/* A tensor of drh_adamw: n parameters and their gradients of the call's dtype, the
+ * averages of the gradients and of their squares, and the number of steps done so far.
+ * Each is contiguous; no two tensors share any of what is written. With 8-bit states
+ * exp_avg and exp_avg_sq are bytes of e4m3, the second of the root, each times its
+ * block's scale: (n + 255) / 256 scales, one for 256 elements in order. Zeros are the
+ * states of a new parameter. The scales are NULL with 32-bit states, which are floats. */
+typedef struct {
+    void * param;
+    const void * grad;
+    void * exp_avg;
+    void * exp_avg_sq;
+    float * exp_avg_scale;
+    float * exp_avg_sq_scale;
+    int64_t * step;
+    int64_t n;
+} drh_adamw_tensor;
+
+/* One AdamW step over `count` tensors (a host array of device pointers), each with
+ * t = *step + 1, from 1 to 2^32 - 1, which *step becomes:
+ *   exp_avg = beta1 exp_avg + (1 - beta1) grad
+ *   exp_avg_sq = beta2 exp_avg_sq + (1 - beta2) grad^2
+ *   param = param (1 - lr weight_decay)
+ *           - lr / (1 - beta1^t) exp_avg / (sqrt(exp_avg_sq / (1 - beta2^t)) + eps)
+ * in 32 bits. state_bits is 32 or 8. 8-bit states are stored with scales of
+ * max(the block's largest magnitude / 448, 2^-126) and rounded at random: up where 16
+ * random bits, as a fraction, added to the place between its neighbours reach the upper one.
+ * Element i of tensor j has the bits of drh_dropout for the key `seed` and the offset t +
+ * j 2^32, for exp_avg_sq with their bytes swapped; a root that is not zero is 2^-9 of
+ * its scale at least. `step` is read on the device, so a captured call counts on
+ * when it is replayed; the other numbers are those of the capture. */
+int drh_adamw(drh_ctx *ctx, const drh_adamw_tensor *tensors, int64_t count, int dtype, int state_bits,
+              double lr, double beta1, double beta2, double eps, double weight_decay, uint64_t seed,
+              void *stream, uint32_t flags);
+
 #ifdef __cplusplus
 }
 #endif
