@@ -13,7 +13,9 @@
 // or m would be divided by eps alone. p is made from the m and v before they are rounded.
 //
 // Bound by memory: an element in 32 bits is read as 16 bytes and written as 12, with 8-bit states
-// as 10 and 6.
+// as 10 and 6. 203 M float32 parameters with 8-bit states (3.3 GB) take 569 us, 5.7 TB/s; 25 M bfloat16
+// with 32-bit states, odd and unaligned (555 MB), 110 us, 5.0. ONCE, for arrays past the caches' size: loads and
+// stores that leave the caches alone (609 and 119 us without).
 
 #include <algorithm>
 #include <cmath>
@@ -37,9 +39,9 @@ struct Tensor {
     const void* g;
     void *m, *v;
     float *ms, *vs;
-    int64_t* step;
+    const int64_t* step;
     int64_t n;
-    uint32_t first, blocks;  // of the launch's workgroups, those that work on it
+    uint32_t first;  // of the launch's workgroups, the first that works on it
 };
 
 struct StepArgs {
@@ -63,33 +65,91 @@ __device__ inline double power(double b, uint32_t t) {
     return r;
 }
 
-// |x| <= 448 rounded to e4m3's grid, up where the 16 random bits, as a fraction, pass what is
-// missing; not below `least` unless x is zero.
-__device__ inline float round_at_random(float x, uint32_t bits, float least) {
-    const float a = fabsf(x);
-    // the step of the grid at a: 2^(exponent - 3), 2^-9 from 2^-6 down
-    const int e = (int)((__builtin_bit_cast(uint32_t, a) >> 23) & 0xff);
-    const int es = e < 121 ? 118 : e > 135 ? 132 : e - 3;
-    const float step = __builtin_bit_cast(float, (uint32_t)es << 23), inv = __builtin_bit_cast(float, (uint32_t)(254 - es) << 23);
-    float q = fminf(floorf(fmaf(a, inv, (float)bits * 0x1p-16f)) * step, E4M3_MOST);
-    if (a > 0.0f) q = fmaxf(q, least);
-    return a != a ? x : copysignf(q, x);
+// |x| rounded to e4m3's grid, up where the 16 random bits `r`, as a fraction, and what the grid leaves of
+// |x| make a whole step. In a float's bits three of its mantissa stay and r is added right below them;
+// under 2^-6, where the grid's steps are 2^-9 throughout, 2^-6 is added first. What r rounds past 448
+// (|x| may pass it by a rounding) is 448, and NaN stays NaN.
+__device__ inline float round_at_random(float x, uint32_t r) {
+    const float a = fabsf(x), base = a < 0x1p-6f ? 0x1p-6f : 0.0f;
+    const uint32_t up = __builtin_bit_cast(uint32_t, a + base) + (r << 4);
+    const float q = fminf(__builtin_bit_cast(float, up & 0xfff00000u) - base, E4M3_MOST);
+    return a == a ? q : a;
 }
 
-// A workgroup takes a tensor's next `rounds` rounds; a wave's vector is the 256 elements of one
+// Quotients by one divisor, as a division rounds them: the random bits decide by the last bit now
+// and then, and a state is what its formula says.
+struct Divisor {
+    float d, r;
+    __device__ explicit Divisor(float by) : d(by) {
+        const float e = __builtin_amdgcn_rcpf(by);
+        r = fmaf(fmaf(-by, e, 1.0f), e, e);
+    }
+    __device__ float of(float x) const {
+        const float q = x * r;
+        return fmaf(fmaf(-q, d, x), r, q);
+    }
+};
+
+// The largest v >= 0 of the wave, in a scalar register; NaN is passed over.
+__device__ inline float wave_most(float v) {
+    int x = __builtin_bit_cast(int, v);
+    auto step = [&](auto ctrl) {
+        const float y = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, x, ctrl.value, 0xf, 0xf, false));
+        x = __builtin_bit_cast(int, fmaxf(__builtin_bit_cast(float, x), y));
+    };
+    // one, two, four and eight lanes down within 16, then lane 15's to the next 16 and 31's to the
+    // upper half: lane 63 has all
+    step(std::integral_constant<int, 0x111>());
+    step(std::integral_constant<int, 0x112>());
+    step(std::integral_constant<int, 0x114>());
+    step(std::integral_constant<int, 0x118>());
+    step(std::integral_constant<int, 0x142>());
+    step(std::integral_constant<int, 0x143>());
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 63));
+}
+
+// The first `left` of N elements at p, in a state's or a parameter's type; zeros behind.
+template <int N, bool ONCE, class T>
+__device__ inline void fetch(const T* p, int64_t left, float (&out)[N]) {
+    if (left >= N) {
+        const auto q = reinterpret_cast<const typename Anywhere<T, N>::type*>(p);
+        const vec<T, N> v = ONCE ? (vec<T, N>)__builtin_nontemporal_load(q) : (vec<T, N>)*q;
+#pragma unroll
+        for (int i = 0; i < N; i++) out[i] = (float)v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) out[i] = i < left ? (float)p[i] : 0.0f;
+    }
+}
+
+// Rounds the first `left` of VEC elements to T.
+template <bool ONCE, class T>
+__device__ inline void put(T* p, int64_t left, const float (&v)[VEC]) {
+    if (ONCE && left >= VEC) {
+        vec<T, VEC> r;
+#pragma unroll
+        for (int i = 0; i < VEC; i++) r[i] = (T)v[i];
+        __builtin_nontemporal_store(r, reinterpret_cast<typename Anywhere<T, VEC>::type*>(p));
+    } else {
+        store_some<VEC>(p, left, v);
+    }
+}
+
+// A workgroup takes a tensor's next `rounds` rounds (one, but for tensors that a launch would not hold);
+// a wave's vector is the 256 elements of one
 // 8-bit block. Neighbouring lanes share a counter's eight draws: each evaluates the counter of one
 // of its two vectors and hands the neighbour its half.
-template <class T, bool SMALL>
+template <class T, bool SMALL, bool ONCE>
 __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
     const int lane = threadIdx.x & 63;
-    // the tensor: the last one whose first workgroup is not past this one
+    // the tensor: the last one whose first workgroup is not past this one (one of no elements has none, and
+    // stands before the tensor with the same first)
     const bool reached = lane < a.count && a.t[lane < a.count ? lane : 0].first <= blockIdx.x;
     const int id = __builtin_amdgcn_readfirstlane(__popcll(__ballot(reached)) - 1);
     const Tensor& t = a.t[id];
-    const uint32_t step = (uint32_t)__hip_atomic_load(t.step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
-    const float rate = a.lr / (float)(1.0 - power(a.beta1, step));
-    const float root = 1.0f / (float)sqrt(1.0 - power(a.beta2, step));
+    const uint32_t step = (uint32_t)*t.step + 1;
     const int64_t n = t.n, begin = (int64_t)(blockIdx.x - t.first) * a.rounds * ROUND;
+    float rate = 0.0f, root = 0.0f;
     for (int round = 0; round < a.rounds; round++) {
         const int64_t at0 = begin + (int64_t)round * ROUND;
         if (at0 >= n) break;
@@ -105,16 +165,20 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
 #pragma unroll
             for (int e = 0; e < VEC; e++) g[k][e] = p[k][e] = m[k][e] = v[k][e] = 0.0f;
             if (left[k] <= 0) continue;
-            load_some<VEC>((const T*)t.g + i, left[k], g[k]);
-            load_some<VEC>((const T*)t.p + i, left[k], p[k]);
+            fetch<VEC, ONCE>((const T*)t.g + i, left[k], g[k]);
+            fetch<VEC, ONCE>((const T*)t.p + i, left[k], p[k]);
             if constexpr (SMALL) {
                 mc[k] = load_codes((const uint8_t*)t.m + i, left[k]);
                 vc[k] = load_codes((const uint8_t*)t.v + i, left[k]);
                 ms[k] = t.ms[i / STATE_BLOCK], vs[k] = t.vs[i / STATE_BLOCK];
             } else {
-                load_some<VEC>((const float*)t.m + i, left[k], m[k]);
-                load_some<VEC>((const float*)t.v + i, left[k], v[k]);
+                fetch<VEC, ONCE>((const float*)t.m + i, left[k], m[k]);
+                fetch<VEC, ONCE>((const float*)t.v + i, left[k], v[k]);
             }
+        }
+        if (round == 0) {  // while the first loads are on their way
+            rate = a.lr / (float)(1.0 - power(a.beta1, step));
+            root = 1.0f / (float)sqrt(1.0 - power(a.beta2, step));
         }
         uint32_t draws[GROUPS][2];  // four 16-bit draws a vector
         if constexpr (SMALL) {
@@ -124,7 +188,9 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
             philox((uint64_t)i >> 3, (uint64_t)step | (uint64_t)(a.base + id) << 32, a.seed, w);
             // lane 2j has its first vector's counter, lane 2j + 1 its second's: words 0 and 1 are the even lane's
             const uint32_t s0 = odd ? w[0] : w[2], s1 = odd ? w[1] : w[3];
-            const uint32_t r0 = __shfl_xor(s0, 1, 64), r1 = __shfl_xor(s1, 1, 64);
+            constexpr int SWAP = 0xb1;  // lanes 1, 0, 3, 2 of each four
+            const uint32_t r0 = __builtin_amdgcn_update_dpp(0, s0, SWAP, 0xf, 0xf, false),
+                           r1 = __builtin_amdgcn_update_dpp(0, s1, SWAP, 0xf, 0xf, false);
             draws[0][0] = odd ? r0 : w[0], draws[0][1] = odd ? r1 : w[1];
             draws[1][0] = odd ? w[2] : r0, draws[1][1] = odd ? w[3] : r1;
         }
@@ -140,27 +206,29 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
             }
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                m[k][e] = fmaf(a.b1, m[k][e], a.c1 * g[k][e]);
-                v[k][e] = fmaf(a.b2, v[k][e], a.c2 * g[k][e] * g[k][e]);
+                m[k][e] = a.b1 * m[k][e] + a.c1 * g[k][e];
+                v[k][e] = a.b2 * v[k][e] + a.c2 * g[k][e] * g[k][e];
                 r[e] = sqrtf(v[k][e]);
-                p[k][e] = fmaf(p[k][e], a.keep, -rate * (m[k][e] / fmaf(r[e], root, a.eps)));
+                p[k][e] = fmaf(p[k][e], a.keep, -rate * (m[k][e] * __builtin_amdgcn_rcpf(fmaf(r[e], root, a.eps))));
             }
             if constexpr (SMALL) {
-                float mm = 0.0f, mv = 0.0f;
+                float mm = 0.0f, mv = 0.0f;  // zeros past the tensor's end: g and the codes are
 #pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    if (e < left[k]) mm = fmaxf(mm, fabsf(m[k][e])), mv = fmaxf(mv, r[e]);
-                mm = fmaxf(wave_max(mm) / E4M3_MOST, LEAST_SCALE);
-                mv = fmaxf(wave_max(mv) / E4M3_MOST, LEAST_SCALE);
+                for (int e = 0; e < VEC; e++) mm = fmaxf(mm, fabsf(m[k][e])), mv = fmaxf(mv, r[e]);
+                mm = fmaxf(wave_most(mm) * (1.0f / E4M3_MOST), LEAST_SCALE);
+                mv = fmaxf(wave_most(mv) * (1.0f / E4M3_MOST), LEAST_SCALE);
                 if (left[k] <= 0) continue;
                 if (lane == 0) t.ms[i / STATE_BLOCK] = mm, t.vs[i / STATE_BLOCK] = mv;
-                const float im = 1.0f / mm, iv = 1.0f / mv;
+                const Divisor dm(mm), dv(mv);
                 float qm[VEC], qv[VEC];
 #pragma unroll
                 for (int e = 0; e < VEC; e++) {
-                    const uint32_t bits = (e & 1) ? draws[k][e >> 1] >> 16 : draws[k][e >> 1] & 0xffffu;
-                    qm[e] = round_at_random(m[k][e] * im, bits, 0.0f);
-                    qv[e] = round_at_random(r[e] * iv, (bits >> 8) | (bits & 0xffu) << 8, 0x1p-9f);
+                    const uint32_t word = draws[k][e >> 1];
+                    const uint32_t bits = (e & 1) ? word >> 16 : word & 0xffffu;
+                    const uint32_t swapped = __builtin_amdgcn_perm(0, word, (e & 1) ? 0x0c0c0203 : 0x0c0c0001);
+                    qm[e] = copysignf(round_at_random(dm.of(m[k][e]), bits), m[k][e]);
+                    qv[e] = round_at_random(dv.of(r[e]), swapped);
+                    if (r[e] > 0.0f) qv[e] = fmaxf(qv[e], 0x1p-9f);
                 }
                 uint32_t cm[1], cv[1];
                 to_e4m3<VEC>(qm, cm);
@@ -169,20 +237,24 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
                 store_codes<false, VEC>((uint8_t*)t.v + i, left[k], cv);
             } else {
                 if (left[k] <= 0) continue;
-                store_some<VEC>((float*)t.m + i, left[k], m[k]);
-                store_some<VEC>((float*)t.v + i, left[k], v[k]);
+                put<ONCE>((float*)t.m + i, left[k], m[k]);
+                put<ONCE>((float*)t.v + i, left[k], v[k]);
             }
-            store_some<VEC>((T*)t.p + i, left[k], p[k]);
+            put<ONCE>((T*)t.p + i, left[k], p[k]);
         }
     }
-    // The tensor's last workgroup counts the step. Until then the upper half of the number counts
-    // the workgroups that are done, each of which has read the lower half.
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const int64_t before = __hip_atomic_fetch_add(t.step, (int64_t)1 << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if ((uint32_t)(before >> 32) == t.blocks - 1)
-            __hip_atomic_store(t.step, (int64_t)step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+}
+
+// The steps are counted behind the kernels that read them. (By each tensor's last workgroup, found by
+// an atomic count, 12000 workgroups took 460 us to be counted: one address takes an atomic every 37 ns.)
+constexpr int COUNTS = 448;
+struct CountArgs {
+    int64_t* step[COUNTS];
+    int count;
+};
+__global__ __launch_bounds__(64) void count_steps(CountArgs a) {
+    const int i = blockIdx.x * 64 + threadIdx.x;
+    if (i < a.count) *a.step[i] += 1;
 }
 
 int check_tensors(const drh_adamw_tensor* tensors, int64_t count, int dtype, bool small) {
@@ -241,24 +313,33 @@ extern "C" int drh_adamw(drh_ctx* ctx, const drh_adamw_tensor* tensors, int64_t 
         a.base = (uint32_t)from;
         int64_t rounds = 0;
         for (int i = 0; i < a.count; i++) rounds += (tensors[from + i].n + ROUND - 1) / ROUND;
-        // Eight rounds a workgroup where that leaves some for every CU's waves, and more where a
-        // launch would not hold their number
-        const int64_t per = std::max(std::min<int64_t>(8, std::max<int64_t>(1, rounds / 2048)), (rounds >> 22) + 1);
+        // One round a workgroup, more only where a launch would not hold their number: with eight, 203 M
+        // parameters with 8-bit states took 672 us, with one 609 (and 569 past the caches)
+        const int64_t per = (rounds >> 23) + 1;
         a.rounds = (int)per;
         uint32_t first = 0;
         for (int i = 0; i < a.count; i++) {
             const drh_adamw_tensor& t = tensors[from + i];
-            const int64_t need = (t.n + per * ROUND - 1) / (per * ROUND);
-            const uint32_t blocks = (uint32_t)std::max<int64_t>(1, need);  // one to count the step
-            a.t[i] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.step, t.n, first, blocks};
-            first += blocks;
+            a.t[i] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.step, t.n, first};
+            first += (uint32_t)((t.n + per * ROUND - 1) / (per * ROUND));
         }
+        if (first == 0) continue;
         with_type(dtype, [&](auto ty) {
             using T = decltype(ty);
-            if (small) adamw_kernel<T, true><<<dim3(first), THREADS, 0, s>>>(a);
-            else adamw_kernel<T, false><<<dim3(first), THREADS, 0, s>>>(a);
+            auto go = [&](auto once) {
+                if (small) adamw_kernel<T, true, once.value><<<dim3(first), THREADS, 0, s>>>(a);
+                else adamw_kernel<T, false, once.value><<<dim3(first), THREADS, 0, s>>>(a);
+            };
+            if (rounds * ROUND * (int64_t)(2 * sizeof(T) + (small ? 2 : 8)) >= READ_ONCE_BYTES) go(std::true_type());
+            else go(std::false_type());
             return DRH_OK;
         });
+    }
+    for (int64_t from = 0; from < count; from += COUNTS) {
+        CountArgs c;
+        c.count = (int)std::min<int64_t>(COUNTS, count - from);
+        for (int i = 0; i < c.count; i++) c.step[i] = tensors[from + i].step;
+        count_steps<<<dim3((unsigned)((c.count + 63) / 64)), 64, 0, s>>>(c);
     }
     return finish_call(s, flags, "AdamW");
 }

@@ -10,8 +10,8 @@
 // once. The backward pass needs act(zg) and zu act'(zg); the forward pass has both at hand and keeps
 // them, not z, which would have to be activated again. They are unbounded, so float16 will not do,
 // and bfloat16's 8 bits would cost the gradients as much again as the rounding of dz does (which is
-// an operand of two products): beside the 16-bit types they are kept in 24 bits, float32 rounded to
-// 16 bits of precision, 2^-16, in three planes of 16 bits (the upper halves of both and a byte of each).
+// an operand of two products): beside bfloat16 they are kept in 20 bits, beside float16 in 24, float32
+// cut off to 12 and 16 bits of precision, 16 times finer than dz is rounded.
 
 #include "products.h"
 
@@ -22,42 +22,101 @@ namespace {
 
 // ---------------------------------------------------------------- what is kept
 
-// M x N pairs (act(zg), zu act'(zg)) in planes of M x N.
+// M x N pairs (act(zg), zu act'(zg)) in planes of M x N. For 16-bit types the upper 16 bits of the
+// first and of the second, and then what is left of both: for float16 16 bits, a byte each, the first's
+// below, for bfloat16 8, four each. The rest is cut off and not rounded, which would take twice the
+// instructions; a NaN has its mantissa's upper bit.
+template <class T>
+constexpr int PAIR_BYTES = sizeof(T) == 4 ? 8 : std::is_same_v<T, bf16> ? 5 : 6;
+
+// N bytes at any address.
+template <int N>
+struct AnyWords {
+    typedef vec<uint32_t, N / 4> type __attribute__((aligned(1)));
+};
+
 template <class T, int C>
 struct Pairs {
-    static constexpr bool SHORT = sizeof(T) == 2;
-
-    static __device__ uint32_t rounded(float v) {
-        const uint32_t b = __builtin_bit_cast(uint32_t, v);
-        return v == v ? b + 0x80u : b;  // not a NaN into a number; the largest become infinity
-    }
     static __device__ void keep(void* kept, int64_t size, int64_t at, int64_t left, const float (&a)[C], const float (&b)[C]) {
-        if constexpr (SHORT) {
-            uint16_t* p = (uint16_t*)kept;
-            uint16_t ha[C], hb[C], lo[C];
+        if constexpr (sizeof(T) == 2) {
+            using Words = vec<uint32_t, C / 2>;
+            constexpr bool NIBBLES = PAIR_BYTES<T> == 5;
+            Words ha, hb;
+            vec<uint32_t, NIBBLES ? C / 4 : C / 2> lo;
 #pragma unroll
-            for (int i = 0; i < C; i++) {
-                const uint32_t ra = rounded(a[i]), rb = rounded(b[i]);
-                ha[i] = (uint16_t)(ra >> 16), hb[i] = (uint16_t)(rb >> 16);
-                lo[i] = (uint16_t)(((ra >> 8) & 0xffu) | (rb & 0xff00u));
+            for (int i = 0; i < C; i += 2) {
+                const uint32_t a0 = __builtin_bit_cast(uint32_t, a[i]), a1 = __builtin_bit_cast(uint32_t, a[i + 1]);
+                const uint32_t b0 = __builtin_bit_cast(uint32_t, b[i]), b1 = __builtin_bit_cast(uint32_t, b[i + 1]);
+                ha[i / 2] = __builtin_amdgcn_perm(a1, a0, 0x07060302);
+                hb[i / 2] = __builtin_amdgcn_perm(b1, b0, 0x07060302);
+                // bytes 1 of both numbers, of the first's and the second's
+                const uint32_t la = __builtin_amdgcn_perm(a1, a0, 0x0c0c0501), lb = __builtin_amdgcn_perm(b1, b0, 0x0c0c0501);
+                if constexpr (NIBBLES) {
+                    const uint32_t two = ((la >> 4) & 0x0f0fu) | (lb & 0xf0f0u);
+                    lo[i / 4] = i % 4 ? lo[i / 4] | two << 16 : two;
+                } else {
+                    lo[i / 2] = __builtin_amdgcn_perm(lb, la, 0x05010400);
+                }
             }
-            put(p + at, left, ha), put(p + size + at, left, hb), put(p + 2 * size + at, left, lo);
+            char* p = (char*)kept;
+            put<2 * C>(p + at * 2, left, ha), put<2 * C>(p + (size + at) * 2, left, hb);
+            put<(NIBBLES ? 1 : 2) * C>(p + size * 4 + at * (NIBBLES ? 1 : 2), left, lo);
         } else {
             store_some<C>((float*)kept + at, left, a);
             store_some<C>((float*)kept + size + at, left, b);
         }
     }
-    static __device__ void put(uint16_t* p, int64_t left, const uint16_t (&v)[C]) {
+    // The first `left` of C parts of v's N bytes.
+    template <int N>
+    static __device__ void put(char* p, int64_t left, const vec<uint32_t, N / 4>& v) {
         if (left >= C) {
-            vec<uint16_t, C> r;
-#pragma unroll
-            for (int i = 0; i < C; i++) r[i] = v[i];
-            *reinterpret_cast<typename Anywhere<uint16_t, C>::type*>(p) = r;
+            *reinterpret_cast<typename AnyWords<N>::type*>(p) = v;
         } else {
+            constexpr int PER = N / C;
 #pragma unroll
-            for (int i = 0; i < C; i++)
-                if (i < left) p[i] = v[i];
+            for (int i = 0; i < N; i++)
+                if (i / PER < left) p[i] = (char)(v[i / 4] >> (8 * (i % 4)));
         }
+    }
+    // C pairs as they were read: a, b.
+    static __device__ void open(const Raw& ha, const Raw& hb, const Raw& lo, float (&a)[C], float (&b)[C]) {
+        static_assert(C == 16 / sizeof(T), "16 bytes of a plane");
+#pragma unroll
+        for (int i = 0; i < C; i++) {
+            if constexpr (sizeof(T) == 4) {
+                a[i] = __builtin_bit_cast(vec<float, 4>, ha)[i], b[i] = __builtin_bit_cast(vec<float, 4>, hb)[i];
+            } else {
+                const uint32_t ua = i % 2 ? ha[i / 2] & 0xffff0000u : ha[i / 2] << 16,
+                               ub = i % 2 ? hb[i / 2] & 0xffff0000u : hb[i / 2] << 16;
+                if constexpr (PAIR_BYTES<T> == 5) {
+                    const uint32_t byte = lo[i / 4] >> (8 * (i % 4));
+                    a[i] = __builtin_bit_cast(float, ua | (byte & 0x0fu) << 12);
+                    b[i] = __builtin_bit_cast(float, ub | (byte & 0xf0u) << 8);
+                } else {
+                    const uint32_t half = lo[i / 2] >> (16 * (i % 2));
+                    a[i] = __builtin_bit_cast(float, ua | (half & 0xffu) << 8);
+                    b[i] = __builtin_bit_cast(float, ub | (half & 0xff00u));
+                }
+            }
+        }
+    }
+    // The plane of what is left, the first `left` of C parts; zeros behind.
+    static __device__ Raw rest(const void* kept, int64_t size, int64_t at, int64_t left) {
+        Raw r = {};
+        if constexpr (sizeof(T) == 2) {
+            constexpr int PER = PAIR_BYTES<T> - 4, N = PER * C;
+            const char* p = (const char*)kept + size * 4 + at * PER;
+            if (left >= C) {
+                const vec<uint32_t, N / 4> v = *reinterpret_cast<const typename AnyWords<N>::type*>(p);
+#pragma unroll
+                for (int i = 0; i < N / 4; i++) r[i] = v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                    if (i / PER < left) r[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
+            }
+        }
+        return r;
     }
 };
 
@@ -75,10 +134,10 @@ struct GatedEpilogue {
         n = n_;
 #pragma unroll
         for (int i = 0; i < W; i++) bg[i] = bu[i] = 0.0f;
-        if (p.bias && !p.partial)
-#pragma unroll
-            for (int i = 0; i < W; i++)
-                if (n + i < p.N) bg[i] = (float)((const T*)p.bias)[n + i], bu[i] = (float)((const T*)p.bias)[p.N + n + i];
+        if (p.bias && !p.partial && n < p.N) {
+            load_some<W>((const T*)p.bias + n, p.N - n, bg);
+            load_some<W>((const T*)p.bias + p.N + n, p.N - n, bu);
+        }
     }
 
     __device__ void row(const Gemm& p, int64_t m, const floatx4 (&v)[NV]) const {
@@ -95,7 +154,10 @@ struct GatedEpilogue {
         }
         float g[W], u[W];
 #pragma unroll
-        for (int i = 0; i < W; i++) g[i] = v[i / 4][i % 4] + bg[i], u[i] = v[NV / 2 + i / 4][i % 4] + bu[i];
+        for (int i = 0; i < W; i++) g[i] = v[i / 4][i % 4], u[i] = v[NV / 2 + i / 4][i % 4];
+        if (p.bias)
+#pragma unroll
+            for (int i = 0; i < W; i++) g[i] += bg[i], u[i] += bu[i];
         apply<W>(p, m * p.N + n, p.N - n, g, u);
     }
 
@@ -329,38 +391,31 @@ int gated_gemm(int dtype, Gemm p, const GemmPlan& plan, float* partial, hipStrea
 template <class T, bool ONCE>
 __global__ __launch_bounds__(256) void gate_slopes(const T* __restrict__ dy, const void* __restrict__ kept, int64_t M, int64_t N,
                                                    int64_t ldz, T* __restrict__ dz, float* part) {
-    constexpr int CH = 16 / sizeof(T), PLANES = sizeof(T) == 2 ? 3 : 2;
+    constexpr int CH = 16 / sizeof(T);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * CH;
     float sum[2][CH] = {};
     const int64_t stride = (int64_t)gridDim.y * 4, left = N - c;
     struct Row {
-        Raw g, k[PLANES];
+        Raw g, a, b, lo;
     };
     auto fetch = [&](int64_t row, Row& to) {
         to = Row{};
         if (row >= M) return;
-        to.g = load_raw<false, ONCE>(dy + row * N + c, left);
-#pragma unroll
-        for (int i = 0; i < PLANES; i++) to.k[i] = load_raw<false, ONCE>((const T*)kept + i * M * N + row * N + c, left);
+        const int64_t at = row * N + c;
+        to.g = load_raw<false, ONCE>(dy + at, left);
+        to.a = load_raw<false, ONCE>((const T*)kept + at, left);
+        to.b = load_raw<false, ONCE>((const T*)kept + M * N + at, left);
+        to.lo = Pairs<T, CH>::rest(kept, M * N, at, left);
     };
     auto finish = [&](int64_t row, const Row& from) {
         if (row >= M) return;
         const Elements<T> ge = __builtin_bit_cast(Elements<T>, from.g);
-        float dg[CH], du[CH];
+        float dg[CH], du[CH], a[CH], b[CH];
+        Pairs<T, CH>::open(from.a, from.b, from.lo, a, b);
 #pragma unroll
         for (int i = 0; i < CH; i++) {
-            float a, b;
-            if constexpr (sizeof(T) == 2) {
-                using S = vec<uint16_t, 8>;
-                const uint32_t ha = __builtin_bit_cast(S, from.k[0])[i], hb = __builtin_bit_cast(S, from.k[1])[i],
-                               lo = __builtin_bit_cast(S, from.k[2])[i];
-                a = __builtin_bit_cast(float, ha << 16 | (lo & 0xffu) << 8);
-                b = __builtin_bit_cast(float, hb << 16 | (lo & 0xff00u));
-            } else {
-                a = __builtin_bit_cast(vec<float, 4>, from.k[0])[i], b = __builtin_bit_cast(vec<float, 4>, from.k[1])[i];
-            }
-            du[i] = (float)ge[i] * a, dg[i] = (float)ge[i] * b;
+            du[i] = (float)ge[i] * a[i], dg[i] = (float)ge[i] * b[i];
             sum[0][i] += dg[i], sum[1][i] += du[i];
         }
         if (dz) {
@@ -463,6 +518,7 @@ int drh_gated_linear(drh_ctx* ctx, const void* x, const void* weight, const void
         return fail(DRH_ERR_INVALID_ARG, "unknown activation " + std::to_string(activation));
     if (rows == 0) return DRH_OK;
     if (!y || (n_in > 0 && (!x || !weight))) return fail(DRH_ERR_INVALID_ARG, "x, weight and y must not be NULL");
+    if (!aligned(kept)) return fail(DRH_ERR_INVALID_ARG, "kept must be 16-byte aligned");
     const ForwardPlan plan = forward_plan(rows, n_out, n_in, x_stride, weight_stride, dtype);
     rc = check_workspace(plan.total, workspace, workspace_bytes);
     if (rc) return rc;
@@ -498,6 +554,7 @@ int drh_gated_linear_backward(drh_ctx* ctx, const void* x, const void* weight, c
     if (rc) return rc;
     const int64_t M = rows, N = n_out, K = n_in;
     if (M > 0 && (!grad_y || !kept)) return fail(DRH_ERR_INVALID_ARG, "grad_y and kept must not be NULL");
+    if (!aligned(kept)) return fail(DRH_ERR_INVALID_ARG, "kept must be 16-byte aligned");
     if (M > 0 && K > 0 && ((grad_x && !weight) || (grad_weight && !x)))
         return fail(DRH_ERR_INVALID_ARG, "an input pointer is NULL");
     const BackwardPlan plan = gated_backward_plan(M, N, K, x_stride, weight_stride, dtype);

@@ -16,9 +16,19 @@ using namespace drh_rt;
 namespace drh_nn {
 namespace {
 
+// Kernels of 16-bit outputs hold every activation; those of float32, whose functions are long, one each.
+constexpr int ANY_ACT = -1;
+
+// f(activation) as a constant.
+template <class T, class F>
+void with_kernel_act(int kind, F&& f) {
+    if constexpr (sizeof(T) == 2) f(std::integral_constant<int, ANY_ACT>());
+    else with_act(kind, [&](auto a) { return f(a), DRH_OK; });
+}
+
 // One lane's 4 NV neighbouring outputs of a row: columns() is called before the rows that
 // share them.
-template <class T, int NV>
+template <class T, int NV, int ACT>
 struct Epilogue8 {
     static constexpr int W = 4 * NV, CH = 16 / sizeof(T) < W ? 16 / sizeof(T) : W;
     int64_t n = 0;
@@ -53,13 +63,12 @@ struct Epilogue8 {
         apply<W>(p, at, p.N - n, o);
     }
 
-    // From z on: activates, adds the residual, stores the first `left`. The activations are those of the
-    // 16-bit types (2^-20 of z) for a float32 output too, whose operands have four bits.
+    // From z on: activates, adds the residual, stores the first `left`.
     template <int C>
     static __device__ void apply(const Gemm& p, int64_t at, int64_t left, float (&o)[C]) {
         float slope;
 #pragma unroll
-        for (int i = 0; i < C; i++) o[i] = act_of<false>(p.act, o[i], slope);
+        for (int i = 0; i < C; i++) o[i] = ACT == ANY_ACT ? act_of<false>(p.act, o[i], slope) : act<true, ACT == ANY_ACT ? 0 : ACT>(o[i], slope);
         constexpr int PART = CH < C ? CH : C;
 #pragma unroll
         for (int g = 0; g < C; g += PART) {
@@ -73,18 +82,18 @@ struct Epilogue8 {
     }
 };
 
-template <class T>
+template <class T, int ACT>
 __global__ __launch_bounds__(512, 2) void linear8_256_kernel(Gemm p) {
-    gemm_256<e4m3, true, true, Epilogue8<T, 2>>(p);
+    gemm_256<e4m3, true, true, Epilogue8<T, 2, ACT>>(p);
 }
 
-template <class T, int TILE, int GROUPS>
+template <class T, int ACT, int TILE, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS, TILE == 64 && GROUPS == 1 ? 3 : 2) void linear8_tile_kernel(Gemm p) {
-    gemm_tile<e4m3, true, true, Epilogue8<T, TILE / 32>, Straight, TILE, GROUPS>(p);
+    gemm_tile<e4m3, true, true, Epilogue8<T, TILE / 32, ACT>, Straight, TILE, GROUPS>(p);
 }
 
 // The parts of a split product added in order, and the epilogue: a thread 16 bytes of a row of y.
-template <class T>
+template <class T, int ACT>
 __global__ __launch_bounds__(256) void linear8_join(Gemm p, int64_t first) {
     constexpr int CH = 16 / sizeof(T);
     const int64_t per = (p.N + CH - 1) / CH, id = (first + blockIdx.x) * 256 + threadIdx.x;
@@ -103,14 +112,14 @@ __global__ __launch_bounds__(256) void linear8_join(Gemm p, int64_t first) {
     const float s = p.row_scale[m];
 #pragma unroll
     for (int i = 0; i < CH; i++) o[i] = fmaf(o[i] * s, c[i], b[i]);
-    Epilogue8<T, 2>::template apply<CH>(p, at, left, o);
+    Epilogue8<T, 2, ACT>::template apply<CH>(p, at, left, o);
 }
 
 // Few rows of x (up to 16 MT): the weights are read once and that is what it costs, so nothing is
 // staged. A workgroup takes 16 outputs; its eight waves take an eighth of k each, straight from memory
 // to the matrix cores (a lane 16 bytes of row l % 16, four lanes 64 contiguous bytes), and are added
 // through LDS in order.
-template <class T, int MT>
+template <class T, int ACT, int MT>
 __global__ __launch_bounds__(512) void linear8_rows_kernel(Gemm p) {
     constexpr int CH = 16, WAVES = 8, AT_ONCE = MT == 1 ? 4 : 2;  // pairs of steps
     using F = vec<e4m3, CH>;
@@ -168,7 +177,7 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(Gemm p) {
     floatx4 v[1] = {part[0][w][lane]};
 #pragma unroll
     for (int i = 1; i < WAVES; i++) v[0] += part[i][w][lane];
-    Epilogue8<T, 1> e;
+    Epilogue8<T, 1, ACT> e;
     e.columns(p, n0 + 4 * q);
     e.row(p, 16 * w + r, v);
 }
@@ -255,27 +264,30 @@ int drh_linear_8bit(drh_ctx* ctx, const void* x, const float* x_scale, const voi
     p.partial = p.splits > 1 ? (float*)workspace : nullptr;
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        if (plan.rows) {
-            const dim3 groups((unsigned)((n_out + 15) / 16));
-            if (rows <= 16) linear8_rows_kernel<T, 1><<<groups, 512, 0, s>>>(p);
-            else if (rows <= 32) linear8_rows_kernel<T, 2><<<groups, 512, 0, s>>>(p);
-            else linear8_rows_kernel<T, 4><<<groups, 512, 0, s>>>(p);
-            return DRH_OK;
-        }
-        const int64_t tiles = (rows + plan.tile - 1) / plan.tile * ((n_out + plan.tile - 1) / plan.tile);
-        const dim3 grid((unsigned)tiles, (unsigned)p.splits);
-        const bool alone = tiles * p.splits <= CUS;
-        if (plan.tile == 256) linear8_256_kernel<T><<<grid, 512, 0, s>>>(p);
-        if (plan.tile == 128 && alone) linear8_tile_kernel<T, 128, 2><<<grid, 512, 0, s>>>(p);
-        if (plan.tile == 128 && !alone) linear8_tile_kernel<T, 128, 1><<<grid, 256, 0, s>>>(p);
-        if (plan.tile == 64 && alone) linear8_tile_kernel<T, 64, 2><<<grid, 512, 0, s>>>(p);
-        if (plan.tile == 64 && !alone) linear8_tile_kernel<T, 64, 1><<<grid, 256, 0, s>>>(p);
-        if (p.partial) {
-            const int64_t ch = 16 / (int64_t)sizeof(T);
-            in_launches((rows * ((n_out + ch - 1) / ch) + 255) / 256, most_groups(256), [&](int64_t first, int64_t count) {
-                linear8_join<T><<<dim3((unsigned)count), 256, 0, s>>>(p, first);
-            });
-        }
+        with_kernel_act<T>(activation, [&](auto kind) {
+            constexpr int ACT = kind.value;
+            if (plan.rows) {
+                const dim3 groups((unsigned)((n_out + 15) / 16));
+                if (rows <= 16) linear8_rows_kernel<T, ACT, 1><<<groups, 512, 0, s>>>(p);
+                else if (rows <= 32) linear8_rows_kernel<T, ACT, 2><<<groups, 512, 0, s>>>(p);
+                else linear8_rows_kernel<T, ACT, 4><<<groups, 512, 0, s>>>(p);
+                return;
+            }
+            const int64_t tiles = (rows + plan.tile - 1) / plan.tile * ((n_out + plan.tile - 1) / plan.tile);
+            const dim3 grid((unsigned)tiles, (unsigned)p.splits);
+            const bool alone = tiles * p.splits <= CUS;
+            if (plan.tile == 256) linear8_256_kernel<T, ACT><<<grid, 512, 0, s>>>(p);
+            if (plan.tile == 128 && alone) linear8_tile_kernel<T, ACT, 128, 2><<<grid, 512, 0, s>>>(p);
+            if (plan.tile == 128 && !alone) linear8_tile_kernel<T, ACT, 128, 1><<<grid, 256, 0, s>>>(p);
+            if (plan.tile == 64 && alone) linear8_tile_kernel<T, ACT, 64, 2><<<grid, 512, 0, s>>>(p);
+            if (plan.tile == 64 && !alone) linear8_tile_kernel<T, ACT, 64, 1><<<grid, 256, 0, s>>>(p);
+            if (p.partial) {
+                const int64_t ch = 16 / (int64_t)sizeof(T);
+                in_launches((rows * ((n_out + ch - 1) / ch) + 255) / 256, most_groups(256), [&](int64_t first, int64_t count) {
+                    linear8_join<T, ACT><<<dim3((unsigned)count), 256, 0, s>>>(p, first);
+                });
+            }
+        });
         return DRH_OK;
     });
     return finish_call(s, flags, "8-bit linear");

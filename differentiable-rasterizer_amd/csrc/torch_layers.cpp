@@ -693,7 +693,9 @@ struct GatedLinearBackward : OnceNode {
     }
 
     variable_list gradients(const Tensor& grad) override {
-        const Tensor x = x_.get(), w = weight_.get(), kept = flat(pairs_.get());
+        const Tensor x = x_.get(), w = weight_.get();
+        Tensor kept = flat(pairs_.get());
+        if ((uintptr_t)in(kept) % 16) kept = kept.clone();  // a hook's
         const Tensor xv = x.defined() ? as_rows(x) : x, wv = w.defined() ? as_rows(w) : w;
         const Tensor g = flat(grad);
         variable_list r(3);
@@ -736,7 +738,7 @@ Tensor gated_linear(Tensor x, Tensor w, const Optional& bias, int act) {
         rows = xv.size(0);
         const int64_t xs = row_stride(xv), ws = row_stride(wv);
         y = at::empty(shape, x.options());
-        if (grad) kept = at::empty({rows * n_out * (code == DRH_F32 ? 8 : 6)}, x.options().dtype(at::kByte));
+        if (grad) kept = at::empty({rows * n_out * (code == DRH_F32 ? 8 : code == DRH_BF16 ? 5 : 6)}, x.options().dtype(at::kByte));
         uint64_t bytes = 0;
         check(drh_gated_linear_bytes(rows, n_out, n_in, xs, ws, code, &bytes));
         const Tensor space = workspace(bytes, x);

@@ -90,8 +90,8 @@ def gated_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activati
         activation: of the gate: None, "relu", "gelu" (z Phi(z)), "gelu_tanh" or "silu".
 
     The backward pass rounds the gradient of z to x's type for its two products. For it the forward
-    pass keeps the gate's value and slope times the other half, in 24 bits each beside 16-bit types
-    (in float32 otherwise): 6 or 8 bytes an output.
+    pass keeps the gate's value, and its slope times the other half: 5 bytes an output beside bfloat16
+    (20 bits each), 6 beside float16 (24 bits) and 8 beside float32.
     """
     y = _torch_layers.gated_linear(x, weight, bias, _act(activation))
     torch_layer._note_gpu()
@@ -142,7 +142,7 @@ def linear_8bit(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor
         x: `(..., K)` and weight: `(N, K)`, float8_e4m3fn, K a multiple of 16.
         x_scale: `(...)` and weight_scale: `(N,)`, float32: a factor for each row.
         bias: `(N,)` or None; residual: `(..., N)` or None; of type dtype.
-        activation: as in `linear`, within 2^-20 of its argument in every type.
+        activation: as in `linear`.
         dtype: of the output: float32, bfloat16 or float16.
 
     No gradients: raises RuntimeError where they are wanted.

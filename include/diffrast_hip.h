@@ -463,7 +463,8 @@ int drh_linear_8bit_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_s
  * x n_in (rows x_stride elements apart), weight 2 n_out x n_in (rows weight_stride apart, the
  * gate's first), bias 2 n_out or NULL, y rows x n_out, contiguous. kept, if not NULL,
  * receives what the backward pass needs, activation(zg) and zu activation'(zg): rows x
- * n_out x 8 bytes for DRH_F32 (float32), x 6 for the other types (24 bits each). */
+ * n_out x 8 bytes for DRH_F32 (float32), x 5 for DRH_BF16 (20 bits each) and x 6 for
+ * DRH_F16 (24 bits); 16-byte aligned. */
 int drh_gated_linear(drh_ctx *ctx, const void *x, const void *weight, const void *bias, int64_t rows,
                      int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride, int dtype,
                      int activation, void *y, void *kept, void *workspace, uint64_t workspace_bytes,
