@@ -563,6 +563,7 @@ extern "C" {
         n_in: i64,
         x_stride: i64,
         weight_stride: i64,
+        dtype: c_int,
         out_bytes: *mut u64,
     ) -> c_int;
     pub fn drh_gated_linear(

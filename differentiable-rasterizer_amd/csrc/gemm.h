@@ -52,6 +52,10 @@ __device__ inline floatx4 mma(vec<float, 4> a, vec<float, 4> b, floatx4 c) {
 
 // e4m3 in bytes. A k tile's 128 bytes are one instruction's k: lane l gives the chunks l / 16 of both
 // halves of the tile, on both sides, so each k meets its own. The instruction's block scales are 1.
+// What it adds is not quite what 32 bits hold: of each eight products (measured: a large one among
+// small ones) it cuts off what is below 2^-13 of the largest, so that a sum may be off by 7 2^-13, less
+// than 2^-10, of its terms' magnitudes, where normal numbers leave it 8e-6 of the result's norm off. Results in
+// 16 bits, rounded by 2^-9 and 2^-12 themselves, do not show that; those in 32 are made by Widened.
 using e4m3 = uint8_t;
 __device__ inline floatx4 mma(vec<e4m3, 16> a0, vec<e4m3, 16> a1, vec<e4m3, 16> b0, vec<e4m3, 16> b1, floatx4 c) {
     using int4 = vec<int, 4>;
@@ -340,6 +344,50 @@ struct Straight {
     }
 };
 
+// e4m3 as bfloat16, which holds it exactly, as do 32 bits a product of two: half the rate of the 8-bit
+// instructions, for sums in 32 bits.
+struct Widened {
+    using F8 = vec<e4m3, 16>;
+    static __device__ inline void widen(F8 f, vec<bf16, 8> (&to)[2]) {
+        const auto words = __builtin_bit_cast(vec<uint32_t, 4>, f);
+        vec<uint32_t, 8> both;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t w = words[i];
+            const auto lo = __builtin_bit_cast(vec<uint32_t, 2>, __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false));
+            const auto hi = __builtin_bit_cast(vec<uint32_t, 2>, __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true));
+            both[2 * i] = __builtin_amdgcn_perm(lo[1], lo[0], 0x07060302);  // the upper halves
+            both[2 * i + 1] = __builtin_amdgcn_perm(hi[1], hi[0], 0x07060302);
+        }
+        const auto all = __builtin_bit_cast(vec<bf16, 16>, both);
+        to[0] = __builtin_shufflevector(all, all, 0, 1, 2, 3, 4, 5, 6, 7);
+        to[1] = __builtin_shufflevector(all, all, 8, 9, 10, 11, 12, 13, 14, 15);
+    }
+    static __device__ inline floatx4 product(F8 a, F8 b, floatx4 c) {
+        vec<bf16, 8> wa[2], wb[2];
+        widen(a, wa), widen(b, wb);
+        return mma(wa[1], wb[1], mma(wa[0], wb[0], c));
+    }
+    template <class FA, class FB, int NA, int NB>
+    static __device__ inline void multiply(const FA& a, const FB& b, floatx4 (&acc)[NA][NB]) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            vec<bf16, 8> wb[NB][2];
+#pragma unroll
+            for (int j = 0; j < NB; j++) widen(b.f[j][h], wb[j]);
+#pragma unroll
+            for (int i = 0; i < NA; i++) {
+                vec<bf16, 8> wa[2];
+                widen(a.f[i][h], wa);
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int j = 0; j < NB; j++) acc[i][j] = mma(wb[j][e], wa[e], acc[i][j]);
+            }
+        }
+    }
+};
+
 struct Thirds {
     struct Held {
         vec<uint32_t, 4> third[3];
@@ -583,8 +631,9 @@ __device__ inline void gemm_tile(const Gemm& p) {
         }
         wait_all();  // LDS is given up, or used again, with no load on its way there
     };
-    auto straight = [&] { walk([&](const FA& fa, const FB& fb) { Straight::multiply(fa, fb, acc); }); };
-    if constexpr (std::is_same_v<Math, Straight>) {
+    using Plain = std::conditional_t<std::is_same_v<Math, Thirds>, Straight, Math>;
+    auto straight = [&] { walk([&](const FA& fa, const FB& fb) { Plain::multiply(fa, fb, acc); }); };
+    if constexpr (std::is_same_v<Math, Plain>) {
         straight();
     } else {
         // While a tile is multiplied, the next one's fragments are read and split. ha[0] holds a

@@ -3,8 +3,9 @@
 //   y = act((xq wq^T) s_x s_w + bias) + residual      xq: M x K, s_x: M;  wq: N x K, s_w: N
 //
 // with e4m3 values and a float32 scale for each row of both (rms_norm.hip makes them). The product
-// runs on the matrix cores' 8-bit instructions, twice the rate of bfloat16 and half the bytes, with
-// 32-bit sums; scales, bias, activation and residual follow in 32 bits, and y is rounded once.
+// runs on the matrix cores' 8-bit instructions, twice the rate of bfloat16 and half the bytes, where y
+// has 16 bits, and for y in 32 bits, which would show how those instructions add, on the bfloat16 ones
+// (Widened in gemm.h); scales, bias, activation and residual follow in 32 bits, and y is rounded once.
 
 #include <algorithm>
 #include <cmath>
@@ -82,14 +83,14 @@ struct Epilogue8 {
     }
 };
 
-template <class T, int ACT>
+template <class T, int ACT>  // 16-bit outputs alone
 __global__ __launch_bounds__(512, 2) void linear8_256_kernel(Gemm p) {
     gemm_256<e4m3, true, true, Epilogue8<T, 2, ACT>>(p);
 }
 
 template <class T, int ACT, int TILE, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS, TILE == 64 && GROUPS == 1 ? 3 : 2) void linear8_tile_kernel(Gemm p) {
-    gemm_tile<e4m3, true, true, Epilogue8<T, TILE / 32, ACT>, Straight, TILE, GROUPS>(p);
+    gemm_tile<e4m3, true, true, Epilogue8<T, TILE / 32, ACT>, std::conditional_t<sizeof(T) == 4, Widened, Straight>, TILE, GROUPS>(p);
 }
 
 // The parts of a split product added in order, and the epilogue: a thread 16 bytes of a row of y.
@@ -135,6 +136,10 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(Gemm p) {
     const e4m3* ap[MT];
 #pragma unroll
     for (int t = 0; t < MT; t++) ap[t] = (const e4m3*)p.a.ptr + (16 * t + r < p.M ? 16 * t + r : p.M - 1) * p.a.ld;
+    auto product = [](const F(&b)[2], const F(&a)[2], floatx4 c) {
+        if constexpr (sizeof(T) == 4) return Widened::product(b[1], a[1], Widened::product(b[0], a[0], c));
+        else return mma(b[0], b[1], a[0], a[1], c);
+    };
     floatx4 acc[MT] = {};
     const int whole = (int)(K / 128) < s1 ? (int)(K / 128) : s1;
     int s = s0;
@@ -152,7 +157,7 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(Gemm p) {
 #pragma unroll
         for (int u = 0; u < AT_ONCE; u++)
 #pragma unroll
-            for (int t = 0; t < MT; t++) acc[t] = mma(b[u][0], b[u][1], a[u][t][0], a[u][t][1], acc[t]);
+            for (int t = 0; t < MT; t++) acc[t] = product(b[u], a[u][t], acc[t]);
     }
     auto chunk = [&](const e4m3* row, int64_t k) {
         F v;
@@ -166,9 +171,12 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(Gemm p) {
     };
     for (; s < s1; s++) {
         const int64_t k = (int64_t)s * 128 + q * CH;
-        const F b0 = chunk(bp, k), b1 = chunk(bp, k + 64);
+        const F b[2] = {chunk(bp, k), chunk(bp, k + 64)};
 #pragma unroll
-        for (int t = 0; t < MT; t++) acc[t] = mma(b0, b1, chunk(ap[t], k), chunk(ap[t], k + 64), acc[t]);
+        for (int t = 0; t < MT; t++) {
+            const F a[2] = {chunk(ap[t], k), chunk(ap[t], k + 64)};
+            acc[t] = product(b, a, acc[t]);
+        }
     }
 #pragma unroll
     for (int t = 0; t < MT; t++) part[w][t][lane] = acc[t];
@@ -188,7 +196,7 @@ double linear8_time(int tile, double tiles, int splits, double steps, double out
     return gemm_time(DRH_BF16, tile, tiles, splits, steps, outputs);
 }
 
-GemmPlan plan8(int64_t M, int64_t N, int64_t K) {
+GemmPlan plan8(int64_t M, int64_t N, int64_t K, int dtype) {
     GemmPlan g;
     if (few_rows(M, N, K / 2)) {  // half of the bytes that its bound on k means
         g.rows = true;
@@ -197,6 +205,7 @@ GemmPlan plan8(int64_t M, int64_t N, int64_t K) {
     const int64_t kt = (K + 127) / 128;
     double best = 1e30;
     for (int tile : {256, 128, 64}) {
+        if (tile == 256 && dtype == DRH_F32) continue;
         const int64_t tiles = (M + tile - 1) / tile * ((N + tile - 1) / tile);
         if (tiles > most_groups(tile == 256 ? 512 : 256)) continue;
         for (int64_t s = 1; s <= 64 && s <= kt; s++) {
@@ -229,11 +238,11 @@ using namespace drh_nn;
 extern "C" {
 
 int drh_linear_8bit_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride,
-                          uint64_t* out_bytes) {
-    if (!out_bytes) return fail(DRH_ERR_INVALID_ARG, "out_bytes is NULL");
+                          int dtype, uint64_t* out_bytes) {
+    if (!out_bytes || !known_type(dtype)) return fail(DRH_ERR_INVALID_ARG, "unknown element type, or out_bytes is NULL");
     int rc = check_sizes8(rows, n_out, n_in, x_stride, weight_stride);
     if (rc) return rc;
-    *out_bytes = rows > 0 ? plan8(rows, n_out, n_in).bytes : 0;
+    *out_bytes = rows > 0 ? plan8(rows, n_out, n_in, dtype).bytes : 0;
     return DRH_OK;
 }
 
@@ -249,7 +258,7 @@ int drh_linear_8bit(drh_ctx* ctx, const void* x, const float* x_scale, const voi
     if (!x || !x_scale || !weight || !weight_scale || !y)
         return fail(DRH_ERR_INVALID_ARG, "x, weight, their scales and y must not be NULL");
     if (!aligned(x) || !aligned(weight)) return fail(DRH_ERR_INVALID_ARG, "8-bit operands must be 16-byte aligned");
-    const GemmPlan plan = plan8(rows, n_out, n_in);
+    const GemmPlan plan = plan8(rows, n_out, n_in, dtype);
     if ((rc = check_workspace(plan.bytes, workspace, workspace_bytes))) return rc;
     if (!plan.rows && !plan.tile) return fail(DRH_ERR_TOO_LARGE, "more tiles of the output than a launch holds");
     DeviceGuard dg(ctx->device);
@@ -276,7 +285,8 @@ int drh_linear_8bit(drh_ctx* ctx, const void* x, const float* x_scale, const voi
             const int64_t tiles = (rows + plan.tile - 1) / plan.tile * ((n_out + plan.tile - 1) / plan.tile);
             const dim3 grid((unsigned)tiles, (unsigned)p.splits);
             const bool alone = tiles * p.splits <= CUS;
-            if (plan.tile == 256) linear8_256_kernel<T, ACT><<<grid, 512, 0, s>>>(p);
+            if constexpr (sizeof(T) == 2)
+                if (plan.tile == 256) linear8_256_kernel<T, ACT><<<grid, 512, 0, s>>>(p);
             if (plan.tile == 128 && alone) linear8_tile_kernel<T, ACT, 128, 2><<<grid, 512, 0, s>>>(p);
             if (plan.tile == 128 && !alone) linear8_tile_kernel<T, ACT, 128, 1><<<grid, 256, 0, s>>>(p);
             if (plan.tile == 64 && alone) linear8_tile_kernel<T, ACT, 64, 2><<<grid, 512, 0, s>>>(p);

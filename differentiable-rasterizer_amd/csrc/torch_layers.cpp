@@ -665,7 +665,7 @@ Tensor linear_8bit(Tensor x, Tensor xs, Tensor w, Tensor ws, const Optional& bia
     const Tensor y = at::empty(shape, x.options().dtype(dtype));
     const Tensor xv = as_byte_rows(x), wv = as_byte_rows(w), xsv = flat(xs), wsv = flat(ws), bv = flat(b), rv = flat(res);
     uint64_t bytes = 0;
-    check(drh_linear_8bit_bytes(xv.size(0), n_out, n_in, row_stride(xv), row_stride(wv), &bytes));
+    check(drh_linear_8bit_bytes(xv.size(0), n_out, n_in, row_stride(xv), row_stride(wv), dtype_code(y), &bytes));
     const Tensor space = workspace(bytes, x);
     Call call(x);
     check(drh_linear_8bit(call.ctx, in(xv), (const float*)in(xsv), in(wv), (const float*)in(wsv), in(bv), in(rv), xv.size(0), n_out,

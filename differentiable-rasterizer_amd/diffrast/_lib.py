@@ -176,7 +176,7 @@ SIGNATURES = {
         _P, _U32], ctypes.c_int),
     "drh_linear_8bit": ([_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _INT, _P, _P, _U64, _P,
         _U32], ctypes.c_int),
-    "drh_linear_8bit_bytes": ([_I64, _I64, _I64, _I64, _I64, ctypes.POINTER(_U64)], ctypes.c_int),
+    "drh_linear_8bit_bytes": ([_I64, _I64, _I64, _I64, _I64, _INT, ctypes.POINTER(_U64)], ctypes.c_int),
     "drh_gated_linear": ([_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _INT, _INT, _P, _P, _P, _U64, _P, _U32],
         ctypes.c_int),
     "drh_gated_linear_bytes": ([_I64, _I64, _I64, _I64, _I64, _INT, ctypes.POINTER(_U64)], ctypes.c_int),

@@ -447,8 +447,10 @@ int drh_rms_norm_backward(drh_ctx *ctx, const void *sum, const void *weight, con
 /* Linear layer of 8-bit operands: y = activation((x weight^T) x_scale weight_scale + bias)
  * + residual, x rows x n_in and weight n_out x n_in in bytes of e4m3, with a scale for each
  * row of both (drh_rms_norm_8bit, drh_quantize_8bit). bias, residual and y are of
- * dtype. n_in, x_stride and weight_stride are multiples of 16, both operands 16-byte
- * aligned. */
+ * dtype. With a 16-bit dtype the sums over n_in are the 8-bit matrix instructions',
+ * within 2^-10 of their terms' magnitudes (8e-6 of the result for normal numbers); for
+ * DRH_F32 they are held in 32 bits. n_in, x_stride and weight_stride are multiples of
+ * 16, both operands 16-byte aligned. */
 int drh_linear_8bit(drh_ctx *ctx, const void *x, const float *x_scale, const void *weight,
                     const float *weight_scale, const void *bias, const void *residual, int64_t rows,
                     int64_t n_out, int64_t n_in, int64_t x_stride, int64_t weight_stride, int dtype,
@@ -457,7 +459,7 @@ int drh_linear_8bit(drh_ctx *ctx, const void *x, const float *x_scale, const voi
 
 /* Workspace of drh_linear_8bit (0 for many sizes). */
 int drh_linear_8bit_bytes(int64_t rows, int64_t n_out, int64_t n_in, int64_t x_stride,
-                          int64_t weight_stride, uint64_t *out_bytes);
+                          int64_t weight_stride, int dtype, uint64_t *out_bytes);
 
 /* Gated linear layer: z = x weight^T + bias, y = activation(z[:, :n_out]) z[:, n_out:], x rows
  * x n_in (rows x_stride elements apart), weight 2 n_out x n_in (rows weight_stride apart, the
