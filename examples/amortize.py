@@ -11,6 +11,11 @@ and pooled; a last linear layer gives 10 numbers per triangle, squashed to their
 Every product, norm and dropout is a layer of `diffrast.layers`, the loss is
 `torch_layer.fused_mse`, so a training step stays on the GPU throughout. Weights are kept
 in 32 bits and used in bfloat16; the images are renders of random scenes.
+
+With --block rms the norm is rms_norm, which adds the residual itself, and with --block gated
+the widening product is gated_linear too; --states 32 or 8 trains by diffrast.optim.AdamW
+with states of so many bits instead of torch's Adam. A network of rms blocks can answer in 8 bits
+(`answer_8bit`).
 """
 
 from __future__ import annotations
@@ -24,15 +29,18 @@ from torch import Tensor, nn
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "differentiable-rasterizer_amd"))
 
-from diffrast import layers, torch_layer  # noqa: E402
+from diffrast import layers, optim, torch_layer  # noqa: E402
 
 
 class TriangleMLP(nn.Module):
     """(B, 3, S, S) images -> (B, T, 10) scenes."""
 
     def __init__(self, size: int = 64, patch: int = 8, width: int = 256, blocks: int = 3, triangles: int = 32,
-                 p: float = 0.1, seed: int = 0, dtype: torch.dtype = torch.bfloat16):
+                 p: float = 0.1, seed: int = 0, dtype: torch.dtype = torch.bfloat16, block: str = "mlp"):
         super().__init__()
+        if block not in ("mlp", "rms", "gated"):
+            raise ValueError(f"unknown block {block!r}")
+        self.block = block
         self.patch, self.triangles, self.p, self.seed, self.dtype = patch, triangles, p, seed, dtype
         self.calls = 0  # names this call's dropout masks
         n = (size // patch) ** 2
@@ -45,12 +53,15 @@ class TriangleMLP(nn.Module):
             return nn.ParameterList([weight(out, inp), nn.Parameter(torch.zeros(out))])
 
         def norm():
-            return nn.ParameterList([nn.Parameter(torch.ones(width)), nn.Parameter(torch.zeros(width))])
+            biases = [nn.Parameter(torch.zeros(width))] if block == "mlp" else []
+            return nn.ParameterList([nn.Parameter(torch.ones(width)), *biases])
+
+        wide = 8 * width if block == "gated" else 4 * width  # both halves
 
         self.embed = pair(width, 3 * patch * patch)
         self.place = nn.Parameter(0.02 * torch.randn(n, width, generator=g))
         self.blocks = nn.ModuleList(
-            nn.ModuleDict({"norm": norm(), "wide": pair(4 * width, width), "narrow": pair(width, 4 * width)})
+            nn.ModuleDict({"norm": norm(), "wide": pair(wide, width), "narrow": pair(width, 4 * width)})
             for _ in range(blocks))
         self.norm = norm()
         self.head = pair(triangles * torch_layer.N_PARAMS, width)
@@ -58,11 +69,21 @@ class TriangleMLP(nn.Module):
     def _linear(self, x: Tensor, wb: nn.ParameterList, **more) -> Tensor:
         return layers.linear(x, wb[0].to(x.dtype), wb[1].to(x.dtype), **more)
 
-    def forward(self, images: Tensor) -> Tensor:
+    def _patches(self, images: Tensor) -> Tensor:
         B, _, S, _ = images.shape
         q, n = self.patch, S // self.patch
-        patches = images.to(self.dtype).reshape(B, 3, n, q, n, q).permute(0, 2, 4, 1, 3, 5).reshape(B, n * n, 3 * q * q)
-        x = self._linear(patches, self.embed, residual=self.place.to(self.dtype).expand(B, -1, -1))
+        return images.to(self.dtype).reshape(B, 3, n, q, n, q).permute(0, 2, 4, 1, 3, 5).reshape(B, n * n, 3 * q * q)
+
+    def _scenes(self, raw: Tensor) -> Tensor:
+        raw = raw.float().view(-1, self.triangles, torch_layer.N_PARAMS)
+        verts = 1.5 * torch.sigmoid(raw[..., :6]) - 0.25
+        rest = torch.sigmoid(raw[..., 6:])
+        return torch.cat([verts, rest[..., :3], 0.1 + 0.8 * rest[..., 3:]], -1)
+
+    def forward(self, images: Tensor) -> Tensor:
+        x = self._linear(self._patches(images), self.embed, residual=self.place.to(self.dtype).expand(len(images), -1, -1))
+        if self.block != "mlp":
+            return self._scenes(self._linear(self._rms_blocks(x).mean(1), self.head))
         for i, b in enumerate(self.blocks):
             h = layers.layer_norm(x, b["norm"][0], b["norm"][1])
             h = self._linear(h, b["wide"], activation="gelu")
@@ -74,10 +95,45 @@ class TriangleMLP(nn.Module):
         if self.training:
             self.calls += 1
         x = layers.layer_norm(x, self.norm[0], self.norm[1]).mean(1)
-        raw = self._linear(x, self.head).float().view(B, self.triangles, torch_layer.N_PARAMS)
-        verts = 1.5 * torch.sigmoid(raw[..., :6]) - 0.25
-        rest = torch.sigmoid(raw[..., 6:])
-        return torch.cat([verts, rest[..., :3], 0.1 + 0.8 * rest[..., 3:]], -1)
+        return self._scenes(self._linear(x, self.head))
+
+    def _rms_blocks(self, x: Tensor) -> Tensor:
+        """The stream through the blocks and the last norm: what a block adds is added by the next norm."""
+        h = None
+        for i, b in enumerate(self.blocks):
+            g = b["norm"][0]
+            y, x = (layers.rms_norm(x, g), x) if h is None else layers.rms_norm(h, g, residual=x)
+            if self.block == "gated":
+                h = layers.gated_linear(y, b["wide"][0].to(y.dtype), b["wide"][1].to(y.dtype))
+            else:
+                h = self._linear(y, b["wide"], activation="gelu")
+            h = self._linear(h, b["narrow"])
+            if self.training:
+                h = layers.dropout(h, self.p, seed=self.seed, offset=self.calls * len(self.blocks) + i)
+        if self.training:
+            self.calls += 1
+        return layers.rms_norm(x, self.norm[0]) if h is None else layers.rms_norm(h, self.norm[0], residual=x)[0]
+
+    @torch.no_grad()
+    def weights_8bit(self) -> list[tuple[Tensor, ...]]:
+        """The blocks' weights in 8 bits with their biases, made once for `answer_8bit`."""
+        return [(*layers.quantize_8bit(b[k][0]), b[k][1].to(self.dtype)) for b in self.blocks for k in ("wide", "narrow")]
+
+    @torch.no_grad()
+    def answer_8bit(self, images: Tensor, weights: list[tuple[Tensor, ...]]) -> Tensor:
+        """forward of rms blocks whose products run in 8 bits."""
+        if self.block != "rms":
+            raise ValueError("rms blocks alone answer in 8 bits")
+        x = self._linear(self._patches(images), self.embed, residual=self.place.to(self.dtype).expand(len(images), -1, -1))
+        h = None
+        for i, b in enumerate(self.blocks):
+            wide, narrow = weights[2 * i], weights[2 * i + 1]
+            q, t, *s = layers.rms_norm_8bit(x if h is None else h, b["norm"][0], residual=None if h is None else x)
+            x = s[0] if s else x
+            h = layers.linear_8bit(q, t, *wide, activation="gelu", dtype=self.dtype)
+            h = layers.linear_8bit(*layers.quantize_8bit(h), *narrow, dtype=self.dtype)
+        x = layers.rms_norm(x, self.norm[0]) if h is None else layers.rms_norm(h, self.norm[0], residual=x)[0]
+        return self._scenes(self._linear(x.mean(1), self.head))
 
 
 def random_images(batch: int, size: int, triangles: int, generator: torch.Generator) -> Tensor:
@@ -87,10 +143,11 @@ def random_images(batch: int, size: int, triangles: int, generator: torch.Genera
 
 
 def train(steps: int, batch: int = 16, size: int = 64, lr: float = 1e-3, sigma: float = 0.01, report: int = 0,
-          pool: int = 64, **model) -> list[float]:
-    """The losses of `steps` steps of Adam on batches drawn from a pool of random images."""
+          pool: int = 64, states: int | None = None, **model) -> list[float]:
+    """The losses of `steps` steps of Adam, or of AdamW with states of so many bits, on batches
+    drawn from a pool of random images."""
     net = TriangleMLP(size=size, **model).cuda().train()
-    opt = torch.optim.Adam(net.parameters(), lr=lr)
+    opt = optim.AdamW(net.parameters(), lr=lr, state_bits=states) if states else torch.optim.Adam(net.parameters(), lr=lr)
     g = torch.Generator("cuda").manual_seed(1)
     seen = random_images(pool, size, 8, g)
     losses = []
@@ -112,5 +169,7 @@ if __name__ == "__main__":
     ap.add_argument("--steps", type=int, default=200)
     ap.add_argument("--batch", type=int, default=16)
     ap.add_argument("--triangles", type=int, default=32)
+    ap.add_argument("--block", choices=("mlp", "rms", "gated"), default="mlp")
+    ap.add_argument("--states", type=int, choices=(32, 8))
     a = ap.parse_args()
-    train(a.steps, a.batch, triangles=a.triangles, report=max(1, a.steps // 10))
+    train(a.steps, a.batch, triangles=a.triangles, block=a.block, states=a.states, report=max(1, a.steps // 10))
