@@ -506,41 +506,79 @@ __device__ inline void gemm_256(const Gemm& p) {
     floatx4 acc[2][2][4][2] = {};
     Frags<T, AK, false, 4> fa;
     Frags<T, BK_, true, 2> fb[2];
-    load_b(0, first);
-    load_a(0, first);
-    load_b(1, first);
-    load_a(1, first);
-    load_b(0, first + 1);
-    load_a(0, first + 1);
-    load_b(1, first + 1);
-    wait_vm<10>();
-    wg_barrier();
-    fb[0].read(lds + at(first, 2), wn * 32);
-    if (wm == 1) wg_barrier();
-
-    auto step = [&](int ua, int ub) {
-        wait_vm<10>();
+    auto meet = [&](auto work) {
         __builtin_amdgcn_sched_barrier(0);
         wg_barrier();
         __builtin_amdgcn_s_setprio(1);
-        Straight::multiply(fa, fb[ub], acc[ua][ub]);
+        work();
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
         wg_barrier();
     };
-    for (int64_t kt = first; kt < last; kt++) {
-        fa.read(lds + at(kt, 0), wm * 64);
-        load_a(1, kt + 1);
-        step(0, 0);
-        fb[1].read(lds + at(kt, 3), wn * 32);
-        load_b(0, kt + 2);
-        step(0, 1);
-        fa.read(lds + at(kt, 1), wm * 64);
-        load_a(0, kt + 2);
-        step(1, 0);
-        fb[0].read(lds + at(kt + 1, 2), wn * 32);
-        load_b(1, kt + 2);
-        step(1, 1);
+    if constexpr (sizeof(T) == 1) {
+        // Of 8 bits a quarter's products take half as long, and the barriers about them would cost more
+        // than they: two steps a k tile, of A0 and of A1 with all of B. What a step has read may be
+        // overwritten in the next one, so a step waits for its reads before the other group may start it.
+        // 16384 x 1024 outputs and k = 4096 with a residual: XXX.
+        auto issue = [&](int64_t kt) {
+            load_a(0, kt);
+            load_b(0, kt);
+            load_b(1, kt);
+        };
+        auto step = [&](int ua) {
+            asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+            meet([&] {
+                Straight::multiply(fa, fb[0], acc[ua][0]);
+                Straight::multiply(fa, fb[1], acc[ua][1]);
+            });
+        };
+        issue(first);
+        load_a(1, first);
+        issue(first + 1);
+        wait_vm<8>();
+        wg_barrier();
+        if (wm == 1) wg_barrier();
+        for (int64_t kt = first; kt < last; kt++) {
+            fa.read(lds + at(kt, 0), wm * 64);
+            fb[0].read(lds + at(kt, 2), wn * 32);
+            fb[1].read(lds + at(kt, 3), wn * 32);
+            load_a(1, kt + 1);
+            step(0);
+            fa.read(lds + at(kt, 1), wm * 64);
+            issue(kt + 2);
+            step(1);
+        }
+    } else {
+        load_b(0, first);
+        load_a(0, first);
+        load_b(1, first);
+        load_a(1, first);
+        load_b(0, first + 1);
+        load_a(0, first + 1);
+        load_b(1, first + 1);
+        wait_vm<10>();
+        wg_barrier();
+        fb[0].read(lds + at(first, 2), wn * 32);
+        if (wm == 1) wg_barrier();
+
+        auto step = [&](int ua, int ub) {
+            wait_vm<10>();
+            meet([&] { Straight::multiply(fa, fb[ub], acc[ua][ub]); });
+        };
+        for (int64_t kt = first; kt < last; kt++) {
+            fa.read(lds + at(kt, 0), wm * 64);
+            load_a(1, kt + 1);
+            step(0, 0);
+            fb[1].read(lds + at(kt, 3), wn * 32);
+            load_b(0, kt + 2);
+            step(0, 1);
+            fa.read(lds + at(kt, 1), wm * 64);
+            load_a(0, kt + 2);
+            step(1, 0);
+            fb[0].read(lds + at(kt + 1, 2), wn * 32);
+            load_b(1, kt + 2);
+            step(1, 1);
+        }
     }
     if (wm == 0) wg_barrier();
     wait_vm<0>();  // LDS is given up with no load on its way there
@@ -560,14 +598,29 @@ __device__ inline void gemm_256(const Gemm& p) {
         Epilogue e0, e1;
         e0.columns(p, n0 + wn * (BK_ ? 64 : 32) + q * 8);
         e1.columns(p, n0 + wn * (BK_ ? 64 : 32) + nu + q * 8);
+        if constexpr (sizeof(T) == 1) {
 #pragma unroll
-        for (int ua = 0; ua < 2; ua++)
+            for (int ua = 0; ua < 2; ua++) {
+                typename Epilogue::Ahead ahead[4][2];
+                const int64_t m = m0 + ua * 128 + wm * 64 + r;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int64_t m = m0 + ua * 128 + wm * 64 + i * 16 + r;
-                e0.row(p, m, acc[ua][0][i]);
-                e1.row(p, m, acc[ua][1][i]);
+                for (int i = 0; i < 4; i++) ahead[i][0] = e0.ahead(p, m + i * 16), ahead[i][1] = e1.ahead(p, m + i * 16);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    e0.row(p, m + i * 16, acc[ua][0][i], ahead[i][0]);
+                    e1.row(p, m + i * 16, acc[ua][1][i], ahead[i][1]);
+                }
             }
+        } else {
+#pragma unroll
+            for (int ua = 0; ua < 2; ua++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int64_t m = m0 + ua * 128 + wm * 64 + i * 16 + r;
+                    e0.row(p, m, acc[ua][0][i]);
+                    e1.row(p, m, acc[ua][1][i]);
+                }
+        }
     }
 }
 
@@ -716,7 +769,13 @@ __device__ inline void gemm_tile(const Gemm& p) {
     }
     Epilogue epilogue;
     epilogue.columns(p, column(0));
-    if constexpr (GROUPS == 1) {
+    if constexpr (GROUPS == 1 && sizeof(T) == 1) {
+        typename Epilogue::Ahead ahead[NF];
+#pragma unroll
+        for (int i = 0; i < NF; i++) ahead[i] = epilogue.ahead(p, m0 + wm + i * 16 + r);
+#pragma unroll
+        for (int i = 0; i < NF; i++) epilogue.row(p, m0 + wm + i * 16 + r, acc[i], ahead[i]);
+    } else if constexpr (GROUPS == 1) {
 #pragma unroll
         for (int i = 0; i < NF; i++) epilogue.row(p, m0 + wm + i * 16 + r, acc[i]);
     } else {

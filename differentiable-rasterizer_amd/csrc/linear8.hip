@@ -38,14 +38,32 @@ struct Epilogue8 {
     __device__ void columns(const Gemm& p, int64_t n_) {
         n = n_;
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            const bool there = n + i < p.N && !p.partial;
-            scale[i] = there ? p.col_scale[n + i] : 0.0f;
-            bias[i] = there && p.bias ? (float)((const T*)p.bias)[n + i] : 0.0f;
-        }
+        for (int i = 0; i < W; i++) scale[i] = bias[i] = 0.0f;
+        if (p.partial || n >= p.N) return;
+        load_some<W>(p.col_scale + n, p.N - n, scale);
+        if (p.bias) load_some<W>((const T*)p.bias + n, p.N - n, bias);
     }
 
-    __device__ void row(const Gemm& p, int64_t m, const floatx4 (&v)[NV]) const {
+    // What a row adds at the end, and its scale, loaded ahead: one after the other the rows of a tile would
+    // wait for memory each.
+    static constexpr bool EARLY = sizeof(T) == 2 && W >= 8;
+    struct Ahead {
+        Raw res[EARLY ? W / 8 : 1];
+        float scale;
+    };
+    __device__ Ahead ahead(const Gemm& p, int64_t m) const {
+        Ahead a = {};
+        if (p.partial || m >= p.M || n >= p.N) return a;
+        a.scale = p.row_scale[m];
+        if (EARLY && p.res)
+#pragma unroll
+            for (int g = 0; g < W / 8; g++)
+                if (n + 8 * g < p.N) a.res[g] = load_raw<false, false>((const T*)p.res + m * p.N + n + 8 * g, p.N - n - 8 * g);
+        return a;
+    }
+
+    __device__ void row(const Gemm& p, int64_t m, const floatx4 (&v)[NV]) const { row(p, m, v, ahead(p, m)); }
+    __device__ void row(const Gemm& p, int64_t m, const floatx4 (&v)[NV], const Ahead& a) const {
         if (m >= p.M || n >= p.N) return;
         const int64_t at = m * p.N + n;
         if (p.partial) {
@@ -57,27 +75,34 @@ struct Epilogue8 {
             }
             return;
         }
-        const float s = p.row_scale[m];
-        float o[W];
+        float o[W], r[W] = {};
 #pragma unroll
-        for (int i = 0; i < W; i++) o[i] = fmaf(v[i / 4][i % 4] * s, scale[i], bias[i]);
-        apply<W>(p, at, p.N - n, o);
+        for (int i = 0; i < W; i++) o[i] = fmaf(v[i / 4][i % 4] * a.scale, scale[i], bias[i]);
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int i = 0; i < W; i++) r[i] = (float)__builtin_bit_cast(Elements<T>, a.res[i / 8])[i % 8];
+        } else if (p.res) {
+            load_some<W>((const T*)p.res + at, p.N - n, r);
+        }
+        apply<W>(p, at, p.N - n, o, r);
     }
 
     // From z on: activates, adds the residual, stores the first `left`.
     template <int C>
-    static __device__ void apply(const Gemm& p, int64_t at, int64_t left, float (&o)[C]) {
+    static __device__ void apply(const Gemm& p, int64_t at, int64_t left, float (&o)[C], const float (&r)[C]) {
         float slope;
 #pragma unroll
         for (int i = 0; i < C; i++) o[i] = ACT == ANY_ACT ? act_of<false>(p.act, o[i], slope) : act<true, ACT == ANY_ACT ? 0 : ACT>(o[i], slope);
+        if (p.res)
+#pragma unroll
+            for (int i = 0; i < C; i++) o[i] += r[i];
         constexpr int PART = CH < C ? CH : C;
 #pragma unroll
         for (int g = 0; g < C; g += PART) {
             if (g >= left) break;
-            float part[PART], r[PART] = {};
-            if (p.res) load_some<PART>((const T*)p.res + at + g, left - g, r);
+            float part[PART];
 #pragma unroll
-            for (int i = 0; i < PART; i++) part[i] = p.res ? o[g + i] + r[i] : o[g + i];
+            for (int i = 0; i < PART; i++) part[i] = o[g + i];
             store_some<PART>((T*)p.out + at + g, left - g, part);
         }
     }
@@ -107,13 +132,14 @@ __global__ __launch_bounds__(256) void linear8_join(Gemm p, int64_t first) {
 #pragma unroll
         for (int i = 0; i < CH; i++) o[i] += v[i];
     }
-    float b[CH] = {}, c[CH] = {};
+    float b[CH] = {}, c[CH] = {}, r[CH] = {};
     if (p.bias) load_some<CH>((const T*)p.bias + n, left, b);
+    if (p.res) load_some<CH>((const T*)p.res + at, left, r);
     load_some<CH>(p.col_scale + n, left, c);
     const float s = p.row_scale[m];
 #pragma unroll
     for (int i = 0; i < CH; i++) o[i] = fmaf(o[i] * s, c[i], b[i]);
-    Epilogue8<T, 2, ACT>::template apply<CH>(p, at, left, o);
+    Epilogue8<T, 2, ACT>::template apply<CH>(p, at, left, o, r);
 }
 
 // Few rows of x (up to 16 MT): the weights are read once and that is what it costs, so nothing is
