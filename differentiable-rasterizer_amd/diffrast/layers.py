@@ -89,8 +89,8 @@ def gated_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, activati
         bias: `(2 N,)` or None.
         activation: of the gate: None, "relu", "gelu" (z Phi(z)), "gelu_tanh" or "silu".
 
-    The backward pass rounds the gradient of z to x's type for its two products. For it the forward
-    pass keeps the gate's value, and its slope times the other half: 5 bytes an output beside bfloat16
+    The backward pass rounds the gradient of z to x's type for its two products (in float16 it ends at
+    65504, as y does). For it the forward pass keeps the gate's value, and its slope times the other half: 5 bytes an output beside bfloat16
     (20 bits each), 6 beside float16 (24 bits) and 8 beside float32.
     """
     y = _torch_layers.gated_linear(x, weight, bias, _act(activation))

@@ -73,10 +73,11 @@ def test_activations(layers, act, bias, dtype):
         compare(t, run(layers, t, act), act, f"{M}x{K}x{N}")
 
 
-@pytest.mark.parametrize("dtype", DTYPES[:2], ids=IDS[:2])
-def test_large_tiles(layers, dtype):
-    """What takes tiles of 256 (16 bits), with rows, outputs and k that end inside of them."""
-    t = make(4100, 1032, 2056, dtype)
+# tiles of 256 (16 bits), as many as the card has CUs, with rows, outputs and k that end inside of them
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("K,N,bias", [(1032, 1980, True), (512, 1979, False), (75, 1976, True)])
+def test_large_tiles(layers, K, N, bias, dtype):
+    t = make(3900, K, N, dtype, bias)
     compare(t, run(layers, t, "silu"), "silu", "large")
 
 

@@ -67,10 +67,25 @@ def test_activations_bias_residual(layers, act, dtype):
                 compare(t, run(layers, t, act, dtype), act, dtype, f"{M}x{K}x{N} {bias} {res}")
 
 
+# tiles of 256 (16-bit outputs), as many as the card has CUs: one k tile, two and three, whole and not, an odd
+# and an even number of them; widths of whole chunks and not
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
-def test_large_tiles(layers, dtype):
-    t = make(8200, 1040, 2056, dtype)
-    compare(t, run(layers, t, None, dtype), None, dtype, "large")
+@pytest.mark.parametrize("K,N", [(16, 3960), (128, 3960), (144, 3960), (256, 3960), (272, 3962), (384, 3960), (1040, 3960), (1152, 3961),
+                                 (1280, 3848)])
+def test_large_tiles(layers, K, N, dtype):
+    for res in (True, False):
+        t = make(3900, K, N, dtype, res=res)
+        compare(t, run(layers, t, None, dtype), None, dtype, f"large {res}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_a_residual_at_any_address(layers, dtype):
+    for M, K, N in ((3900, 512, 3960), (300, 512, 64), (20, 64, 40)):
+        t = make(M, K, N, dtype)
+        want = run(layers, t, "relu", dtype)
+        room = torch.empty(M * N + 1, dtype=dtype, device="cuda")
+        room[1:] = t["res"].view(-1)
+        assert same(run(layers, {**t, "res": room[1:].view(M, N)}, "relu", dtype), want)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
