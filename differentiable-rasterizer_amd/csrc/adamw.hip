@@ -122,19 +122,6 @@ __device__ inline void fetch(const T* p, int64_t left, float (&out)[N]) {
     }
 }
 
-// Rounds the first `left` of VEC elements to T.
-template <bool ONCE, class T>
-__device__ inline void put(T* p, int64_t left, const float (&v)[VEC]) {
-    if (ONCE && left >= VEC) {
-        vec<T, VEC> r;
-#pragma unroll
-        for (int i = 0; i < VEC; i++) r[i] = (T)v[i];
-        __builtin_nontemporal_store(r, reinterpret_cast<typename Anywhere<T, VEC>::type*>(p));
-    } else {
-        store_some<VEC>(p, left, v);
-    }
-}
-
 // A workgroup takes a tensor's next `rounds` rounds (one, but for tensors that a launch would not hold);
 // a wave's vector is the 256 elements of one
 // 8-bit block. Neighbouring lanes share a counter's eight draws: each evaluates the counter of one
@@ -237,10 +224,10 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
                 store_codes<false, VEC>((uint8_t*)t.v + i, left[k], cv);
             } else {
                 if (left[k] <= 0) continue;
-                put<ONCE>((float*)t.m + i, left[k], m[k]);
-                put<ONCE>((float*)t.v + i, left[k], v[k]);
+                store_once<ONCE, VEC>((float*)t.m + i, left[k], m[k]);
+                store_once<ONCE, VEC>((float*)t.v + i, left[k], v[k]);
             }
-            put<ONCE>((T*)t.p + i, left[k], p[k]);
+            store_once<ONCE, VEC>((T*)t.p + i, left[k], p[k]);
         }
     }
 }

@@ -92,6 +92,19 @@ __device__ inline void store_some(T* p, int64_t left, const float (&v)[N]) {
     }
 }
 
+// store_some, past the caches where ONCE.
+template <bool ONCE, int N, class T>
+__device__ inline void store_once(T* p, int64_t left, const float (&v)[N]) {
+    if (ONCE && left >= N) {
+        vec<T, N> r;
+#pragma unroll
+        for (int i = 0; i < N; i++) r[i] = (T)v[i];
+        __builtin_nontemporal_store(r, reinterpret_cast<typename Anywhere<T, N>::type*>(p));
+    } else {
+        store_some<N>(p, left, v);
+    }
+}
+
 __device__ inline float wave_sum(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
