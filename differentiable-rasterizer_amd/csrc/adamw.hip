@@ -13,9 +13,11 @@
 // or m would be divided by eps alone. p is made from the m and v before they are rounded.
 //
 // Bound by memory: an element in 32 bits is read as 16 bytes and written as 12, with 8-bit states
-// as 10 and 6. 203 M float32 parameters with 8-bit states (3.3 GB) take 569 us, 5.7 TB/s; 25 M bfloat16
-// with 32-bit states, odd and unaligned (555 MB), 110 us, 5.0. ONCE, for arrays past the caches' size: loads and
-// stores that leave the caches alone (609 and 119 us without).
+// as 10 and 6. 203 M float32 parameters with 8-bit states (3.3 GB) take 553 us, 5.9 TB/s; 25 M bfloat16
+// with 32-bit states, odd and unaligned (555 MB), 106 us, 5.2. The 8-bit states' arithmetic comes next, a hundred
+// instructions an element at first and 581 us: the rounding instruction, roots by one correction, the blocks'
+// maxima side by side and whole rounds without their ends brought it below the memory's time. ONCE, for arrays
+// past the caches' size: loads and stores that leave the caches alone (609 and 119 us without, of 569 and 110).
 
 #include <algorithm>
 #include <cmath>
@@ -65,15 +67,33 @@ __device__ inline double power(double b, uint32_t t) {
     return r;
 }
 
-// |x| rounded to e4m3's grid, up where the 16 random bits `r`, as a fraction, and what the grid leaves of
-// |x| make a whole step. In a float's bits three of its mantissa stay and r is added right below them;
-// under 2^-6, where the grid's steps are 2^-9 throughout, 2^-6 is added first. What r rounds past 448
-// (|x| may pass it by a rounding) is 448, and NaN stays NaN.
-__device__ inline float round_at_random(float x, uint32_t r) {
-    const float a = fabsf(x), base = a < 0x1p-6f ? 0x1p-6f : 0.0f;
-    const uint32_t up = __builtin_bit_cast(uint32_t, a + base) + (r << 4);
-    const float q = fminf(__builtin_bit_cast(float, up & 0xfff00000u) - base, E4M3_MOST);
-    return a == a ? q : a;
+// The square roots of a vector's values, rounded right: with the reciprocal root's unit in the last place one
+// correction does (checked for each value from 2^-100 to 2^102), beyond that sqrtf's dozen instructions more.
+template <int N>
+__device__ inline void roots(const float (&v)[N], float (&r)[N]) {
+    float least = v[0], most = v[0];
+#pragma unroll
+    for (int i = 1; i < N; i++) least = fminf(least, v[i]), most = fmaxf(most, v[i]);
+    if (least >= 0x1p-100f && most <= 0x1p100f) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float y = __builtin_amdgcn_rsqf(v[i]), s = v[i] * y;
+            r[i] = fmaf(fmaf(-s, s, v[i]), 0.5f * y, s);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) r[i] = sqrtf(v[i]);
+    }
+}
+
+// Four values as e4m3 codes, each rounded up where its draw, 16 random bits in its word's upper half, as a
+// fraction, and what the grid leaves of the magnitude make a whole step. The instruction adds the word's upper
+// 20 bits to the 20 that it cuts: what a rounding put past 448, by less than 16 units in the last place, stays 448.
+__device__ inline uint32_t to_e4m3_at_random(const float (&v)[4], uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    int w = __builtin_amdgcn_cvt_sr_fp8_f32(v[0], (int)r0, 0, 0);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(v[1], (int)r1, w, 1);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(v[2], (int)r2, w, 2);
+    return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(v[3], (int)r3, w, 3);
 }
 
 // Quotients by one divisor, as a division rounds them: the random bits decide by the last bit now
@@ -90,12 +110,16 @@ struct Divisor {
     }
 };
 
-// The largest v >= 0 of the wave, in a scalar register; NaN is passed over.
-__device__ inline float wave_most(float v) {
-    int x = __builtin_bit_cast(int, v);
+// The largest v >= 0 of the wave, of N at once (a step waits for the one before it); none is NaN, so that
+// their bits have their order.
+template <int N>
+__device__ inline void wave_most(float (&v)[N]) {
+    uint32_t x[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = __builtin_bit_cast(uint32_t, v[i]);
     auto step = [&](auto ctrl) {
-        const float y = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, x, ctrl.value, 0xf, 0xf, false));
-        x = __builtin_bit_cast(int, fmaxf(__builtin_bit_cast(float, x), y));
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = std::max(x[i], (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x[i], ctrl.value, 0xf, 0xf, true));
     };
     // one, two, four and eight lanes down within 16, then lane 15's to the next 16 and 31's to the
     // upper half: lane 63 has all
@@ -105,7 +129,8 @@ __device__ inline float wave_most(float v) {
     step(std::integral_constant<int, 0x118>());
     step(std::integral_constant<int, 0x142>());
     step(std::integral_constant<int, 0x143>());
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, 63));
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane((int)x[i], 63));
 }
 
 // The first `left` of N elements at p, in a state's or a parameter's type; zeros behind.
@@ -137,9 +162,8 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
     const uint32_t step = (uint32_t)*t.step + 1;
     const int64_t n = t.n, begin = (int64_t)(blockIdx.x - t.first) * a.rounds * ROUND;
     float rate = 0.0f, root = 0.0f;
-    for (int round = 0; round < a.rounds; round++) {
-        const int64_t at0 = begin + (int64_t)round * ROUND;
-        if (at0 >= n) break;
+    // a round that the tensor fills has no ends to look for
+    auto update = [&](auto whole, int64_t at0, bool first) {
         float g[GROUPS][VEC], p[GROUPS][VEC], m[GROUPS][VEC], v[GROUPS][VEC];
         uint32_t mc[GROUPS], vc[GROUPS];
         float ms[GROUPS], vs[GROUPS];
@@ -147,7 +171,7 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
 #pragma unroll
         for (int k = 0; k < GROUPS; k++) {
             const int64_t i = at0 + (int64_t)k * THREADS * VEC + threadIdx.x * VEC;
-            left[k] = n - i;
+            left[k] = whole ? VEC : n - i;
             mc[k] = vc[k] = 0, ms[k] = vs[k] = 0.0f;
 #pragma unroll
             for (int e = 0; e < VEC; e++) g[k][e] = p[k][e] = m[k][e] = v[k][e] = 0.0f;
@@ -163,7 +187,7 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
                 fetch<VEC, ONCE>((const float*)t.v + i, left[k], v[k]);
             }
         }
-        if (round == 0) {  // while the first loads are on their way
+        if (first) {  // while the first loads are on their way
             rate = a.lr / (float)(1.0 - power(a.beta1, step));
             root = 1.0f / (float)sqrt(1.0 - power(a.beta2, step));
         }
@@ -181,10 +205,9 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
             draws[0][0] = odd ? r0 : w[0], draws[0][1] = odd ? r1 : w[1];
             draws[1][0] = odd ? w[2] : r0, draws[1][1] = odd ? w[3] : r1;
         }
+float r[GROUPS][VEC], scale[2 * GROUPS];
 #pragma unroll
         for (int k = 0; k < GROUPS; k++) {
-            const int64_t i = at0 + (int64_t)k * THREADS * VEC + threadIdx.x * VEC;
-            float r[VEC];
             if constexpr (SMALL) {
                 from_e4m3(mc[k], m[k]);
                 from_e4m3(vc[k], v[k]);
@@ -195,40 +218,54 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(StepArgs a) {
             for (int e = 0; e < VEC; e++) {
                 m[k][e] = a.b1 * m[k][e] + a.c1 * g[k][e];
                 v[k][e] = a.b2 * v[k][e] + a.c2 * g[k][e] * g[k][e];
-                r[e] = sqrtf(v[k][e]);
-                p[k][e] = fmaf(p[k][e], a.keep, -rate * (m[k][e] * __builtin_amdgcn_rcpf(fmaf(r[e], root, a.eps))));
             }
-            if constexpr (SMALL) {
-                float mm = 0.0f, mv = 0.0f;  // zeros past the tensor's end: g and the codes are
+            roots<VEC>(v[k], r[k]);
 #pragma unroll
-                for (int e = 0; e < VEC; e++) mm = fmaxf(mm, fabsf(m[k][e])), mv = fmaxf(mv, r[e]);
-                mm = fmaxf(wave_most(mm) * (1.0f / E4M3_MOST), LEAST_SCALE);
-                mv = fmaxf(wave_most(mv) * (1.0f / E4M3_MOST), LEAST_SCALE);
-                if (left[k] <= 0) continue;
-                if (lane == 0) t.ms[i / STATE_BLOCK] = mm, t.vs[i / STATE_BLOCK] = mv;
-                const Divisor dm(mm), dv(mv);
+            for (int e = 0; e < VEC; e++)
+                p[k][e] = fmaf(p[k][e], a.keep, -rate * (m[k][e] * __builtin_amdgcn_rcpf(fmaf(r[k][e], root, a.eps))));
+            float mm = 0.0f, mv = 0.0f;  // zeros past the tensor's end: g and the codes are
+#pragma unroll
+            for (int e = 0; e < VEC; e++) mm = fmaxf(mm, fabsf(m[k][e])), mv = fmaxf(mv, r[k][e]);
+            scale[2 * k] = mm, scale[2 * k + 1] = mv;
+        }
+        if constexpr (SMALL) {
+            wave_most<2 * GROUPS>(scale);
+#pragma unroll
+            for (int k = 0; k < 2 * GROUPS; k++) scale[k] = fmaxf(scale[k] * (1.0f / E4M3_MOST), LEAST_SCALE);
+        }
+#pragma unroll
+        for (int k = 0; k < GROUPS; k++) {
+            const int64_t i = at0 + (int64_t)k * THREADS * VEC + threadIdx.x * VEC;
+            if (left[k] <= 0) break;
+            if constexpr (SMALL) {
+                if (lane == 0) t.ms[i / STATE_BLOCK] = scale[2 * k], t.vs[i / STATE_BLOCK] = scale[2 * k + 1];
+                const Divisor dm(scale[2 * k]), dv(scale[2 * k + 1]);
                 float qm[VEC], qv[VEC];
 #pragma unroll
                 for (int e = 0; e < VEC; e++) {
-                    const uint32_t word = draws[k][e >> 1];
-                    const uint32_t bits = (e & 1) ? word >> 16 : word & 0xffffu;
-                    const uint32_t swapped = __builtin_amdgcn_perm(0, word, (e & 1) ? 0x0c0c0203 : 0x0c0c0001);
-                    qm[e] = copysignf(round_at_random(dm.of(m[k][e]), bits), m[k][e]);
-                    qv[e] = round_at_random(dv.of(r[e]), swapped);
-                    if (r[e] > 0.0f) qv[e] = fmaxf(qv[e], 0x1p-9f);
+                    qm[e] = dm.of(m[k][e]), qv[e] = dv.of(r[k][e]);
+                    if (r[k][e] > 0.0f) qv[e] = fmaxf(qv[e], 0x1p-9f);
                 }
                 uint32_t cm[1], cv[1];
-                to_e4m3<VEC>(qm, cm);
-                to_e4m3<VEC>(qv, cv);
+                cm[0] = to_e4m3_at_random(qm, draws[k][0] << 16, draws[k][0] & 0xffff0000u, draws[k][1] << 16, draws[k][1] & 0xffff0000u);
+                // v takes its draws' two bytes the other way round
+                const uint32_t w0 = draws[k][0], w1 = draws[k][1];
+                cv[0] = to_e4m3_at_random(qv, __builtin_amdgcn_perm(0, w0, 0x00010c0c), __builtin_amdgcn_perm(0, w0, 0x02030c0c),
+                                          __builtin_amdgcn_perm(0, w1, 0x00010c0c), __builtin_amdgcn_perm(0, w1, 0x02030c0c));
                 store_codes<false, VEC>((uint8_t*)t.m + i, left[k], cm);
                 store_codes<false, VEC>((uint8_t*)t.v + i, left[k], cv);
             } else {
-                if (left[k] <= 0) continue;
                 store_once<ONCE, VEC>((float*)t.m + i, left[k], m[k]);
                 store_once<ONCE, VEC>((float*)t.v + i, left[k], v[k]);
             }
             store_once<ONCE, VEC>((T*)t.p + i, left[k], p[k]);
         }
+    };
+    for (int round = 0; round < a.rounds; round++) {
+        const int64_t at0 = begin + (int64_t)round * ROUND;
+        if (at0 >= n) break;
+        if (n - at0 >= ROUND) update(std::true_type(), at0, round == 0);
+        else update(std::false_type(), at0, round == 0);
     }
 }
 
@@ -301,7 +338,7 @@ extern "C" int drh_adamw(drh_ctx* ctx, const drh_adamw_tensor* tensors, int64_t 
         int64_t rounds = 0;
         for (int i = 0; i < a.count; i++) rounds += (tensors[from + i].n + ROUND - 1) / ROUND;
         // One round a workgroup, more only where a launch would not hold their number: with eight, 203 M
-        // parameters with 8-bit states took 672 us, with one 609 (and 569 past the caches)
+        // parameters with 8-bit states took 672 us, with one 609
         const int64_t per = (rounds >> 23) + 1;
         a.rounds = (int)per;
         uint32_t first = 0;
