@@ -108,7 +108,9 @@ struct Epilogue8 {
     }
 };
 
-template <class T, int ACT>  // 16-bit outputs alone
+// 16-bit outputs alone. 16384 x 4096 -> 1024 with bias and residual takes 65 us (2.1 PFLOP/s), one tile a
+// CU: 42% of the matrix cores' time, its start and its end are covered by nothing.
+template <class T, int ACT>
 __global__ __launch_bounds__(512, 2) void linear8_256_kernel(Gemm p) {
     gemm_256<e4m3, true, true, Epilogue8<T, 2, ACT>>(p);
 }
@@ -145,7 +147,8 @@ __global__ __launch_bounds__(256) void linear8_join(Gemm p, int64_t first) {
 // Few rows of x (up to 16 MT): the weights are read once and that is what it costs, so nothing is
 // staged. A workgroup takes 16 outputs; its eight waves take an eighth of k each, straight from memory
 // to the matrix cores (a lane 16 bytes of row l % 16, four lanes 64 contiguous bytes), and are added
-// through LDS in order.
+// through LDS in order. One row of 1024 -> 4096 with GELU (4.2 MB of weights) takes 3.9 us, of which a
+// launch and one wave's chain of loads are most.
 template <class T, int ACT, int MT>
 __global__ __launch_bounds__(512) void linear8_rows_kernel(Gemm p) {
     constexpr int CH = 16, WAVES = 8, AT_ONCE = MT == 1 ? 4 : 2;  // pairs of steps

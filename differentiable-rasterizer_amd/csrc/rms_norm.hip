@@ -125,8 +125,8 @@ __global__ __launch_bounds__(THREADS) void rms_forward(RmsArgs p) {
 // A workgroup takes every gridDim-th group of THREADS / TPR rows and keeps its columns' sums of g h
 // in registers; at the end its row groups are added through LDS in order and go to the workgroup's
 // own row of p.part, which reduce_columns adds up. A group's next rows are on their way while it
-// works on the present ones. With a residual's gradient 32768 x 4096 in bfloat16 (1.07 GB) take 183 us,
-// 5.9 TB/s with the column sums' second step, 32768 x 1500 in 32 bits, without, 104, 5.7.
+// works on the present ones. With a residual's gradient 32768 x 4096 in bfloat16 (1.07 GB) take 178 us,
+// 6.1 TB/s with the column sums' second step, 32768 x 1500 in 32 bits, without, 104, 5.7.
 template <class T, int EPT, int TPR, int THREADS, int PER_SIMD, bool WHOLE, bool ONCE>
 __global__ __launch_bounds__(THREADS, PER_SIMD) void rms_backward(RmsArgs p) {
     constexpr int VEC = 16 / sizeof(T), NV = EPT / VEC, GROUPS = THREADS / TPR;
