@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 #include <vector>
 
 #include "e4m3.h"
@@ -282,7 +283,8 @@ __global__ __launch_bounds__(64) void count_steps(CountArgs a) {
 }
 
 int check_tensors(const drh_adamw_tensor* tensors, int64_t count, int dtype, bool small) {
-    std::vector<const void*> params, steps;
+    std::vector<std::pair<uintptr_t, uintptr_t>> written;  // each array's first byte and the one behind its last
+    auto writes = [&](const void* p, int64_t bytes) { written.emplace_back((uintptr_t)p, (uintptr_t)p + (uint64_t)bytes); };
     for (int64_t i = 0; i < count; i++) {
         const drh_adamw_tensor& t = tensors[i];
         if (t.n < 0) return fail(DRH_ERR_INVALID_ARG, "a tensor has a negative number of elements");
@@ -296,14 +298,17 @@ int check_tensors(const drh_adamw_tensor* tensors, int64_t count, int dtype, boo
             (!small && ((uintptr_t)t.exp_avg % 4 || (uintptr_t)t.exp_avg_sq % 4)) ||
             (small && ((uintptr_t)t.exp_avg_scale % 4 || (uintptr_t)t.exp_avg_sq_scale % 4)))
             return fail(DRH_ERR_INVALID_ARG, "a pointer of a tensor is not aligned to its elements");
-        if (t.n > 0) params.push_back(t.param);
-        steps.push_back(t.step);
+        writes(t.step, 8);
+        if (t.n == 0) continue;
+        writes(t.param, t.n * (int64_t)e);
+        for (const void* state : {t.exp_avg, t.exp_avg_sq}) writes(state, t.n * (small ? 1 : 4));
+        if (small)
+            for (const void* scale : {t.exp_avg_scale, t.exp_avg_sq_scale}) writes(scale, (t.n + STATE_BLOCK - 1) / STATE_BLOCK * 4);
     }
-    for (auto* v : {&params, &steps}) {
-        std::sort(v->begin(), v->end());
-        if (std::adjacent_find(v->begin(), v->end()) != v->end())
-            return fail(DRH_ERR_INVALID_ARG, "two tensors share a parameter or a step count");
-    }
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); i++)
+        if (written[i].first < written[i - 1].second)
+            return fail(DRH_ERR_INVALID_ARG, "two parameters, states, scales or step counts share memory");
     return DRH_OK;
 }
 

@@ -39,8 +39,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
                 - lr / (1 - beta1^t) exp_avg / (sqrt(exp_avg_sq / (1 - beta2^t)) + eps)
 
     Args:
-        params, grads: of one type (float32, bfloat16 or float16), on one GPU, no parameter twice.
-            Parameters are contiguous; gradients that are not are copied.
+        params, grads: of one type (float32, bfloat16 or float16), on one GPU. Parameters
+            are contiguous; gradients that are not are copied. Of what is written no two share memory.
         exp_avgs, exp_avg_sqs: float32 of the parameters' shapes; or, with scales, float8_e4m3fn, the
             second of the root.
         steps: an int64 tensor with a count for each parameter, or one tensor of shape () each, on

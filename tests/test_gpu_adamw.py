@@ -429,3 +429,20 @@ def test_refusals(optim):
     p.grad = torch.ones(3)
     with pytest.raises(ValueError, match="on the GPU"):
         optim.AdamW([p]).step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_what_is_written_shares_no_memory(optim, bits):
+    s = make([200, 200], torch.float32, bits)
+    before = copied(s)
+    both = torch.zeros(300, device="cuda")
+    twice = [dict(p=[both[:200], both[100:]]), dict(m=[s["m"][0]] * 2), dict(v=[s["v"][1]] * 2), dict(v=s["m"])]
+    twice += [dict(ms=[s["ms"][0]] * 2), dict(vs=s["ms"])] if bits == 8 else []
+    for bad in twice:
+        with pytest.raises(RuntimeError, match="share"):
+            call(optim, {**s, **bad})
+    for k in s:
+        for a, b in zip(s[k], before[k]):
+            assert same(a, b), k
+    call(optim, {**s, "p": [both[:150], both[150:]], **{k: [t[:150] for t in s[k]] for k in ("g", "m", "v")}})  # neighbours do not
+    call(optim, {**s, "g": [s["g"][0]] * 2})  # nor what is read
