@@ -395,7 +395,7 @@ int gated_gemm(int dtype, Gemm p, const GemmPlan& plan, float* partial, hipStrea
 // dz = [dy zu act'(zg), dy act(zg)], rounded to its type for the products, in rows of ldz elements
 // with zeros behind 2 N, and the column sums of the unrounded values: a workgroup owns 64 chunks of
 // every gridDim.y-th slab of rows, its four waves a row each, added in order at the end. Bound by memory:
-// 16384 x 4096 in bfloat16 (740 MB) take 132 us, 5.6 TB/s; ONCE: loads and stores past the caches, without
+// 16384 x 4096 in bfloat16 (740 MB) take 130 us, 5.7 TB/s; ONCE: loads and stores past the caches, without
 // which forward and backward of that size take 34 us more.
 template <class T, bool ONCE>
 __global__ __launch_bounds__(256) void gate_slopes(const T* __restrict__ dy, const void* __restrict__ kept, int64_t M, int64_t N,
