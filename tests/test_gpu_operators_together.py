@@ -113,3 +113,71 @@ def test_a_captured_training_step(amortize):  # noqa: F811
         step(*b)
         for p, q in zip(a[0], b[0]):
             assert bool(torch.equal(p, q)), i
+
+
+def chain(seed):
+    """Inputs of a chain of all layers whose products are split (workspaces of partial sums), and the chain."""
+    from diffrast import layers
+
+    g = torch.Generator("cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g, dtype=torch.bfloat16)  # noqa: E731
+    x, res, w, w8 = r(100, 2048), r(100, 2048), 0.02 * r(256, 2048), 0.1 * r(96, 128)
+    q8, s8 = layers.quantize_8bit(w8)
+    for t in (x, w):
+        t.requires_grad_(True)
+
+    def run():
+        y, s = layers.rms_norm(x, None, residual=res)
+        h = layers.gated_linear(y, w)
+        gx, gw = torch.autograd.grad((h.float().square().sum() + s.float().sum()), (x, w))
+        with torch.no_grad():
+            a, t = layers.rms_norm_8bit(h)
+            return h.detach(), gx, gw, layers.linear_8bit(a, t, q8, s8, activation="gelu")
+
+    return run
+
+
+def test_two_threads_on_two_streams():
+    import threading
+
+    runs = [chain(1), chain(2)]
+    want = [f() for f in runs]
+    torch.cuda.synchronize()
+    wrong = [[], []]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for k in range(10):
+                got = runs[i]()
+                stream.synchronize()
+                wrong[i] += [(k, j) for j, (a, b) in enumerate(zip(got, want[i])) if not torch.equal(a.view(torch.int16), b.view(torch.int16))]
+        wrong[i].append("done")
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [["done"], ["done"]]
+
+
+def test_two_captured_chains_of_one_memory_pool():
+    runs = [chain(1), chain(2)]
+    want = [f() for f in runs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for f in runs:
+            f()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, got = [torch.cuda.CUDAGraph() for _ in runs], []
+    for k, f in enumerate(runs):
+        with torch.cuda.graph(graphs[k], pool=graphs[0].pool() if k else None):
+            got.append(f())
+    for i in range(4):
+        for graph, out, ref in zip(graphs, got, want):  # a graph's workspaces may be the other's outputs: one at a time
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(bool(torch.equal(a.view(torch.int16), b.view(torch.int16))) for a, b in zip(out, ref)), i
+        runs[i % 2]()
