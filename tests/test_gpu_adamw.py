@@ -446,3 +446,25 @@ def test_what_is_written_shares_no_memory(optim, bits):
             assert same(a, b), k
     call(optim, {**s, "p": [both[:150], both[150:]], **{k: [t[:150] for t in s[k]] for k in ("g", "m", "v")}})  # neighbours do not
     call(optim, {**s, "g": [s["g"][0]] * 2})  # nor what is read
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("step", [0, 3])
+def test_roots_of_tiny_and_huge_numbers(optim, dtype, step):
+    """Gradients from 1e-25, whose squares are nothing in 32 bits, to 1e18, side by side and in runs of
+    neighbours; exact zeros between them. Their squares' roots are taken in two ways by their size."""
+    n = 8192
+    s = make([n], dtype, step=step)
+    e = torch.linspace(-25, 18, n, device="cuda")
+    mixed = torch.cat([e[: n // 2], e[n // 2:][torch.randperm(n // 2, device="cuda", generator=torch.Generator("cuda").manual_seed(1))]])
+    s["g"][0].copy_((10.0 ** mixed.double() * torch.where(torch.arange(n, device="cuda") % 3 == 0, -1, 1)).to(dtype))
+    s["g"][0][::7] = 0
+    if step:
+        s["v"][0].copy_((0.1 * s["g"][0].double() ** 2).float())
+        s["m"][0].copy_((0.3 * s["g"][0].double()).float())
+    old = copied(s)
+    call(optim, s)
+    want = ob.adamw(old["p"][0], old["g"][0], old["m"][0], old["v"][0], step + 1, 1e-3, 0.9, 0.999, 1e-8, 0.01)
+    ob.check(s["p"][0], *want["p"], dtype, "p")
+    ob.check(s["m"][0], *want["m"], torch.float32, "m")
+    ob.check(s["v"][0], *want["v"], torch.float32, "v")
