@@ -79,7 +79,8 @@ class AdamW(torch.optim.Optimizer):
         params, lr, betas, eps, weight_decay: as torch.optim.AdamW's.
         state_bits: 32, or 8: a byte for each state and a float for 256 of them, 2.03 bytes a
             parameter instead of 8, rounded at random.
-        seed: of that rounding; the i-th call of a step takes seed + i.
+        seed: of that rounding; the i-th call of a step takes its group's seed + i. It stands in the groups,
+            and so in copies and state dicts: a run that loads one goes on with the seed it was saved with.
 
     A step may be captured into a HIP graph once every parameter has had one outside of it.
     """
@@ -91,8 +92,16 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
         if not (isinstance(seed, int) and 0 <= seed < 1 << 63):
             raise ValueError("seed must be an integer in [0, 2^63)")
-        self.seed = seed
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed))
+
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__(state)
+        for group in self.param_groups:  # of a state dict without a seed
+            group.setdefault("seed", self.defaults.get("seed", 0))
+
+    @property
+    def seed(self) -> int:
+        return self.param_groups[0]["seed"]
 
     def _state_of(self, p: Tensor, bits: int) -> dict:
         state = self.state[p]
@@ -129,7 +138,7 @@ class AdamW(torch.optim.Optimizer):
                            [s["exp_avg_sq"] for s in states], [s["step"] for s in states],
                            exp_avg_scales=[s["exp_avg_scale"] for s in states] if small else None,
                            exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in states] if small else None, lr=group["lr"],
-                           betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], seed=self.seed + call)
+                           betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], seed=group["seed"] + call)
                 call += 1
         return loss
 

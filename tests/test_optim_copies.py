@@ -1,0 +1,69 @@
+"""What a copied, pickled or loaded diffrast.optim.AdamW goes on with."""
+
+import copy
+import pickle
+
+import pytest
+import torch
+
+
+def seeds(opt):
+    return [g["seed"] for g in opt.param_groups]
+
+
+def make(seed, second=None):
+    from diffrast import optim
+
+    a, b = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.ones(4))
+    return optim.AdamW([dict(params=[a]), dict(params=[b]) if second is None else dict(params=[b], seed=second)], state_bits=8, seed=seed)
+
+
+@pytest.mark.parametrize("copied", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))], ids=["copied", "pickled"])
+def test_a_copy_has_the_seed(copied):
+    opt = copied(make(7, 9))
+    assert opt.seed == 7 and seeds(opt) == [7, 9]
+    assert opt.step() is None  # no gradients: nothing
+
+
+def test_a_state_dict_has_the_seed():
+    opt = make(5)
+    opt.load_state_dict(make(7, 9).state_dict())
+    assert seeds(opt) == [7, 9]
+    saved = make(7).state_dict()
+    for g in saved["param_groups"]:
+        del g["seed"]  # one that was saved without
+    opt = make(5)
+    opt.load_state_dict(saved)
+    assert seeds(opt) == [5, 5]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("copied", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o)), None], ids=["copied", "pickled", "loaded"])
+def test_a_copy_steps_as_the_original(copied):
+    from diffrast import optim
+
+    g = torch.Generator("cuda").manual_seed(0)
+    net = torch.nn.Linear(70, 30).cuda()
+
+    def step(net, opt, g):
+        for p in net.parameters():
+            p.grad = torch.randn(p.shape, device="cuda", generator=g)
+        opt.step()
+
+    opt = optim.AdamW(net.parameters(), lr=0.1, state_bits=8, seed=3)
+    step(net, opt, g)
+    if copied:
+        net2, opt2 = copied((net, opt))
+    else:
+        net2 = copy.deepcopy(net)
+        opt2 = optim.AdamW(net2.parameters(), lr=0.1, state_bits=8, seed=4)
+        opt2.load_state_dict(opt.state_dict())
+    for _ in range(3):
+        same = torch.Generator("cuda")
+        same.set_state(g.get_state())
+        step(net, opt, g)
+        step(net2, opt2, same)
+    for p, q in zip(net.parameters(), net2.parameters()):
+        assert p.data_ptr() != q.data_ptr() and bool(torch.equal(p, q))
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert bool(torch.equal(opt.state[p][k].view(torch.uint8), opt2.state[q][k].view(torch.uint8)))
