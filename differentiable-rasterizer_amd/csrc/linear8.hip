@@ -2,10 +2,11 @@
 //
 //   y = act((xq wq^T) s_x s_w + bias) + residual      xq: M x K, s_x: M;  wq: N x K, s_w: N
 //
-// with e4m3 values and a float32 scale for each row of both (rms_norm.hip makes them). The product
-// runs on the matrix cores' 8-bit instructions, twice the rate of bfloat16 and half the bytes, where y
-// has 16 bits, and for y in 32 bits, which would show how those instructions add, on the bfloat16 ones
-// (Widened in gemm.h); scales, bias, activation and residual follow in 32 bits, and y is rounded once.
+// with e4m3 values and a float32 scale for each row of both (rms_norm.hip makes them). Where y has 16
+// bits the product runs on the matrix cores' 8-bit instructions, twice the rate of bfloat16 and half the
+// bytes, which lose up to 2^-10 of the terms (mma in gemm.h says how, and why that is taken); for y in 32
+// bits, which is how a caller asks for sums in 32 bits, on the bfloat16 ones (Widened in gemm.h). Scales,
+// bias, activation and residual follow in 32 bits, and y is rounded once.
 
 #include <algorithm>
 #include <cmath>

@@ -144,8 +144,9 @@ def linear_8bit(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor
         bias: `(N,)` or None; residual: `(..., N)` or None; of type dtype.
         activation: as in `linear`.
         dtype: of the output: float32, bfloat16 or float16. Sums of products are held in 32 bits for
-            float32, and for the others as the matrix cores' 8-bit instructions hold them, within 2^-10
-            of their terms' magnitudes (8e-6 for normal numbers).
+            float32, and for the others, at twice the speed, as the matrix cores' 8-bit instructions hold
+            them: within 2^-10 of their terms' magnitudes. For normal numbers that is 8e-6 of the result; in rows
+            with outliers it may pass float16's own rounding, and bfloat16's where large terms cancel.
 
     No gradients: raises RuntimeError where they are wanted.
     """
