@@ -97,20 +97,6 @@ __device__ inline uint32_t to_e4m3_at_random(const float (&v)[4], uint32_t r0, u
     return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(v[3], (int)r3, w, 3);
 }
 
-// Quotients by one divisor, as a division rounds them: the random bits decide by the last bit now
-// and then, and a state is what its formula says.
-struct Divisor {
-    float d, r;
-    __device__ explicit Divisor(float by) : d(by) {
-        const float e = __builtin_amdgcn_rcpf(by);
-        r = fmaf(fmaf(-by, e, 1.0f), e, e);
-    }
-    __device__ float of(float x) const {
-        const float q = x * r;
-        return fmaf(fmaf(-q, d, x), r, q);
-    }
-};
-
 // The largest v >= 0 of the wave, of N at once (a step waits for the one before it); none is NaN, so that
 // their bits have their order.
 template <int N>

@@ -100,16 +100,17 @@ __global__ __launch_bounds__(THREADS) void rms_forward(RmsArgs p) {
 #pragma unroll
             for (int i = 0; i < VEC; i++) most = fmaxf(most, fabsf(v[j][i]));  // zeros past the row's end
         most = row_max<TPR, THREADS>(most);
-        const float scale = fmaxf(most / E4M3_MOST, LEAST_SCALE), inv = 1.0f / scale;
+        const float scale = fmaxf(most / E4M3_MOST, LEAST_SCALE);
         if (!live) return;
         if (t == 0) p.scale[row] = scale;
+        const RowDivisor by(scale);
         uint8_t* y = (uint8_t*)p.y + row * D;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const int c = (j * TPR + t) * VEC;
             uint32_t codes[VEC / 4];
 #pragma unroll
-            for (int i = 0; i < VEC; i++) v[j][i] *= inv;
+            for (int i = 0; i < VEC; i++) v[j][i] = by.of(v[j][i]);
             to_e4m3<VEC>(v[j], codes);
             if (c < D) store_codes<WHOLE, VEC>(y + c, D - c, codes);
         }
@@ -246,18 +247,18 @@ __global__ __launch_bounds__(WIDE) void rms_forward_wide(RmsArgs p) {
         if (p.w) load_weight<T, true>(p.w, p.wf32, c, D, w);
         return at(c) * (r * w[0]);
     };
-    float inv = 0.0f;
+    float scale = 1.0f;
     if constexpr (CODES) {
         float most = 0.0f;
         for (int c = threadIdx.x; c < D; c += WIDE) most = fmaxf(most, fabsf(value(c)));
-        const float scale = fmaxf(row_max<WIDE, WIDE>(most) / E4M3_MOST, LEAST_SCALE);
-        inv = 1.0f / scale;
+        scale = fmaxf(row_max<WIDE, WIDE>(most) / E4M3_MOST, LEAST_SCALE);
         if (threadIdx.x == 0) p.scale[row] = scale;
     }
+    const RowDivisor by(scale);
     for (int c = threadIdx.x; c < D; c += WIDE) {
         const float s = at(c), y = value(c);
         if constexpr (CODES)
-            ((uint8_t*)p.y)[row * D + c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y * inv, 0.0f, 0, false);
+            ((uint8_t*)p.y)[row * D + c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(by.of(y), 0.0f, 0, false);
         else
             ((T*)p.y)[row * D + c] = (T)y;
         if (p.sum) ((T*)p.sum)[row * D + c] = (T)s;
