@@ -575,15 +575,16 @@ std::vector<Tensor> rms_norm(Tensor x, const Optional& weight, const Optional& r
                            code, wcode, (float)eps, out(y), out(sum), (float*)out(rstd), call.stream, 0));
     }
     if (grad) {
+        const bool data = x.requires_grad() || (res.defined() && res.requires_grad());
         auto node = new_node<RmsNormBackward>();
         // the sum itself leads to this node: its values are kept without that
         node->sum_.keep(sum.defined() ? sum.detach() : x);
         node->rstd_.keep(rstd);
-        if (w.defined() && (x.requires_grad() || (res.defined() && res.requires_grad()))) node->weight_.keep(w);
+        if (w.defined() && data) node->weight_.keep(w);
         node->weight_type = w.defined() ? w.scalar_type() : x.scalar_type();
         node->weight_code = wcode;
         y = attach(std::move(y), node, {&x, &w, &res});
-        if (sum.defined()) torch::autograd::set_history(sum, node);
+        if (sum.defined() && data) torch::autograd::set_history(sum, node);  // of the weight it is no function
     }
     if (!sum.defined()) return {y};
     return {y, sum};

@@ -102,7 +102,7 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = 
     """s / sqrt(mean(s^2) + eps) * weight over the last dimension, with s = x + residual.
 
     Returns y, or with a residual (y, s): the norm and the stream that it was taken of, both
-    differentiable. y is made from s in 32 bits; s is rounded to its type where it is stored, and
+    differentiable (of s the weight's gradient is zero, where s alone is used too). y is made from s in 32 bits; s is rounded to its type where it is stored, and
     the backward pass starts from that. The mean of squares is held in float32, which ends at 3e38.
 
     Args:
