@@ -143,10 +143,17 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict) -> None:
-        super().load_state_dict(state_dict)
-        # as they were saved: the base class gives states the parameters' type
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
-            if i in state_dict["state"]:
-                self.state[p] = {k: v.to(device=p.device, copy=True) if isinstance(v, Tensor) else v
-                                 for k, v in state_dict["state"][i].items()}
+        loaded = []
+
+        def keep(_, d):  # behind the caller's own hooks: the dictionary as they leave it
+            loaded.append(d)
+
+        def restore(_):  # before theirs; as they were saved: the base class gives states the parameters' type
+            saved = [i for g in loaded[-1]["param_groups"] for i in g["params"]]
+            for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
+                if i in loaded[-1]["state"]:
+                    self.state[p] = {k: v.to(device=p.device, copy=True) if isinstance(v, Tensor) else v
+                                     for k, v in loaded[-1]["state"][i].items()}
+
+        with self.register_load_state_dict_pre_hook(keep), self.register_load_state_dict_post_hook(restore, prepend=True):
+            super().load_state_dict(state_dict)

@@ -76,3 +76,38 @@ def test_a_copy_steps_as_the_original(copied):
         assert p.data_ptr() != q.data_ptr() and bool(torch.equal(p, q))
         for k in ("exp_avg", "exp_avg_sq"):
             assert bool(torch.equal(opt.state[p][k].view(torch.uint8), opt2.state[q][k].view(torch.uint8)))
+
+
+def test_load_hooks_see_and_change_what_is_loaded():
+    """Pre-hooks' dictionary is what is loaded, in the states' own types, before post-hooks run."""
+    from diffrast import optim
+
+    def opt_of(value):
+        p = torch.nn.Parameter(torch.zeros(5, dtype=torch.bfloat16))
+        opt = optim.AdamW([p])
+        opt.state[p] = dict(step=torch.tensor(3), exp_avg=torch.full((5,), value), exp_avg_sq=torch.full((5,), value))
+        return opt, p
+
+    source, q = opt_of(1 + 2.0**-20)
+    opt, p = opt_of(7.0)
+    seen = []
+
+    def doubled(o, d):
+        d = copy.deepcopy(d)
+        d["state"][0]["exp_avg"] *= 2
+        d["param_groups"][0]["lr"] = 0.5
+        return d
+
+    opt.register_load_state_dict_pre_hook(doubled)
+    opt.register_load_state_dict_post_hook(lambda o: seen.append(o.state[p]["exp_avg"].clone()))
+    for _ in range(2):  # nothing of the first load is left for the second
+        opt.load_state_dict(source.state_dict())
+        s = opt.state[p]
+        assert opt.param_groups[0]["lr"] == 0.5 and s["exp_avg"].dtype == torch.float32 and int(s["step"]) == 3
+        assert torch.equal(s["exp_avg"], 2 * source.state[q]["exp_avg"]) and torch.equal(s["exp_avg_sq"], source.state[q]["exp_avg_sq"])
+        assert s["exp_avg_sq"].data_ptr() != source.state[q]["exp_avg_sq"].data_ptr()
+        assert torch.equal(seen.pop(), s["exp_avg"])
+    bad = source.state_dict()
+    bad["param_groups"][0]["params"] = [0, 1]
+    with pytest.raises(ValueError):
+        opt.load_state_dict(bad)
