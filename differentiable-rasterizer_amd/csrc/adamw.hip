@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <iterator>
 #include <utility>
 #include <vector>
 
@@ -295,6 +296,12 @@ int check_tensors(const drh_adamw_tensor* tensors, int64_t count, int dtype, boo
     for (size_t i = 1; i < written.size(); i++)
         if (written[i].first < written[i - 1].second)
             return fail(DRH_ERR_INVALID_ARG, "two parameters, states, scales or step counts share memory");
+    for (int64_t i = 0; i < count; i++) {  // a workgroup must not read as a gradient what another one writes
+        const uintptr_t begin = (uintptr_t)tensors[i].grad, end = begin + (uint64_t)tensors[i].n * type_size(dtype);
+        const auto next = std::lower_bound(written.begin(), written.end(), std::make_pair(end, (uintptr_t)0));
+        if (tensors[i].n > 0 && next != written.begin() && std::prev(next)->second > begin)
+            return fail(DRH_ERR_INVALID_ARG, "a gradient and a parameter, state, scale or step count share memory");
+    }
     return DRH_OK;
 }
 

@@ -40,7 +40,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
 
     Args:
         params, grads: of one type (float32, bfloat16 or float16), on one GPU. Parameters
-            are contiguous; gradients that are not are copied. Of what is written no two share memory.
+            are contiguous; gradients that are not are copied. Of what is written no two share memory, nor
+            does a gradient share any of it.
         exp_avgs, exp_avg_sqs: float32 of the parameters' shapes; or, with scales, float8_e4m3fn, the
             second of the root.
         steps: an int64 tensor with a count for each parameter, or one tensor of shape () each, on

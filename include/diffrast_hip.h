@@ -489,7 +489,8 @@ int drh_gated_linear_backward(drh_ctx *ctx, const void *x, const void *weight, c
 
 /* A tensor of drh_adamw: n parameters and their gradients of the call's dtype, the
  * averages of the gradients and of their squares, and the number of steps done so far.
- * Each is contiguous; no two tensors share any of what is written. With 8-bit states
+ * Each is contiguous; no two tensors share any of what is written, nor does a gradient
+ * share any of it (two gradients may share theirs). With 8-bit states
  * exp_avg and exp_avg_sq are bytes of e4m3, the second of the root, each times its
  * block's scale: (n + 255) / 256 scales, one for 256 elements in order. Zeros are the
  * states of a new parameter. The scales are NULL with 32-bit states, which are floats. */
