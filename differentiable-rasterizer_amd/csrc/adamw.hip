@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cmath>
 #include <iterator>
+#include <new>
 #include <utility>
 #include <vector>
 
@@ -323,7 +324,12 @@ extern "C" int drh_adamw(drh_ctx* ctx, const drh_adamw_tensor* tensors, int64_t 
     if (count < 0 || (count > 0 && !tensors)) return fail(DRH_ERR_INVALID_ARG, "tensors must not be NULL, nor count negative");
     if (count > INT32_MAX) return fail(DRH_ERR_TOO_LARGE, "more than 2^31 - 1 tensors");
     const bool small = state_bits == 8;
-    if ((rc = check_tensors(tensors, count, dtype, small))) return rc;
+    try {
+        rc = check_tensors(tensors, count, dtype, small);
+    } catch (const std::bad_alloc&) {
+        return fail(DRH_ERR_TOO_LARGE, "no memory to check so many tensors");
+    }
+    if (rc) return rc;
     if (count == 0) return DRH_OK;
     DeviceGuard dg(ctx->device);
     hipStream_t s = (hipStream_t)stream;

@@ -37,3 +37,22 @@ def test_a_gradient_that_is_written_is_refused(program):  # noqa: F811
     assert call(tensor(0, n=200), tensor(1, grad=t[0].param + 200), dtype=1) == 6
     assert call(tensor(0, n=200), tensor(1, grad=t[0].param + 400), dtype=1) == 0
     """)
+
+
+def test_no_memory_to_check_the_tensors(program):  # noqa: F811
+    """An error, and no exception through the C entry."""
+    program("""
+    import resource
+    n = 1 << 20
+    table = (_lib.AdamWTensor * n)()
+    steps = np.zeros(n, np.int64)
+    np.frombuffer(table, np.int64).reshape(n, 8)[:, 6] = addr(steps) + 8 * np.arange(n)  # tensors of nothing
+    call = lambda: code(lambda: _lib.check(_lib.lib().drh_adamw(ctx.handle, table, n, 0, 32, .1, .9, .99, 0., 0., 0, None, 0)))
+    assert call() == 0
+    used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+    resource.setrlimit(resource.RLIMIT_AS, (used + 4 * MIB, resource.RLIM_INFINITY))
+    rc = call()
+    resource.setrlimit(resource.RLIMIT_AS, (resource.RLIM_INFINITY, resource.RLIM_INFINITY))
+    assert rc == 5 and "memory" in _lib.last_error(), rc
+    assert call() == 0
+    """)
