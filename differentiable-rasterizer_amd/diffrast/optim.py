@@ -72,6 +72,14 @@ def _check_numbers(lr: float, beta1: float, beta2: float, eps: float, weight_dec
             raise ValueError(f"betas must be in [0, 1), got {v}")
 
 
+def _check_group(g: dict) -> None:
+    _check_numbers(float(g["lr"]), *g["betas"], g["eps"], g["weight_decay"])
+    if g["state_bits"] not in (32, 8):
+        raise ValueError(f"state_bits must be 32 or 8, got {g['state_bits']}")
+    if not (isinstance(g["seed"], int) and 0 <= g["seed"] < 1 << 63):
+        raise ValueError("seed must be an integer in [0, 2^63)")
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW by `adamw_step`: one call for all parameters of a group that are of one type
     and on one GPU, one kernel for 48 of them.
@@ -88,12 +96,13 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, seed: int = 0):
-        _check_numbers(float(lr), *betas, eps, weight_decay)
-        if state_bits not in (32, 8):
-            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
-        if not (isinstance(seed, int) and 0 <= seed < 1 << 63):
-            raise ValueError("seed must be an integer in [0, 2^63)")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed))
+        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed)
+        _check_group(defaults)
+        super().__init__(params, defaults)
+
+    def add_param_group(self, param_group: dict) -> None:
+        _check_group({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def __setstate__(self, state: dict) -> None:
         super().__setstate__(state)

@@ -111,3 +111,20 @@ def test_load_hooks_see_and_change_what_is_loaded():
     bad["param_groups"][0]["params"] = [0, 1]
     with pytest.raises(ValueError):
         opt.load_state_dict(bad)
+
+
+@pytest.mark.parametrize("bad", [dict(state_bits=16), dict(seed=-1), dict(seed=1 << 63), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0),
+                                 dict(weight_decay=float("nan"))])
+def test_a_groups_own_numbers_are_checked(bad):
+    """As the optimizer's are, before there are states by them."""
+    from diffrast import optim
+
+    t = lambda: torch.nn.Parameter(torch.zeros(3))  # noqa: E731
+    with pytest.raises(ValueError):
+        optim.AdamW([dict(params=[t()]), dict(params=[t()], **bad)])
+    opt = optim.AdamW([t()])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[t()], **bad))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[t()], state_bits=8, lr=torch.tensor(0.5)))
+    assert len(opt.param_groups) == 2 and seeds(opt) == [0, 0]
