@@ -516,7 +516,8 @@ typedef struct {
  * random bits, as a fraction, added to the place between its neighbours reach the upper one.
  * Element i of tensor j has the bits of drh_dropout for the key `seed` and the offset t +
  * j 2^32, for exp_avg_sq with their bytes swapped; a root that is not zero is 2^-9 of
- * its scale at least. `step` is read on the device, so a captured call counts on
+ * its scale at least. The root keeps its mean, exp_avg_sq gains the rounding's variance: 3
+ * to 5% for normal gradients and beta2 = 0.999. `step` is read on the device, so a captured call counts on
  * when it is replayed; the other numbers are those of the capture. */
 int drh_adamw(drh_ctx *ctx, const drh_adamw_tensor *tensors, int64_t count, int dtype, int state_bits,
               double lr, double beta1, double beta2, double eps, double weight_decay, uint64_t seed,
