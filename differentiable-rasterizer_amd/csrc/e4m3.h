@@ -68,13 +68,13 @@ struct Divisor {
 };
 
 // The same by a row's scale, which may be tiny (remainders lose bits below 2^-126) or infinite (finite
-// numbers are nothing of it, others NaN).
+// numbers are nothing of it, others NaN). A zero keeps its sign, which the correction would drop.
 struct RowDivisor {
     float up;
     Divisor by;
     __device__ explicit RowDivisor(float scale)
         : up(scale < 0x1p-64f ? 0x1p64f : scale < __builtin_inff() ? 1.0f : 0.0f), by(up > 0.0f ? scale * up : 1.0f) {}
-    __device__ float of(float x) const { return by.of(x * up); }
+    __device__ float of(float x) const { return __builtin_copysignf(by.of(x * up), x); }
 };
 
 }  // namespace drh_nn

@@ -53,3 +53,15 @@ def test_any_numbers():
     x *= torch.exp2(torch.linspace(-130, 110, 20000, device="cuda"))[:, None]
     q, s = layers.quantize_8bit(x)
     assert torch.equal(q.view(torch.uint8), (x / s[:, None]).to(ob.E4M3).view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_zeros_keep_their_signs(dtype):
+    from diffrast import layers
+
+    for D in (300, 40000):
+        x = torch.zeros(3, D, dtype=dtype, device="cuda")
+        x[:, ::3] = -0.0
+        x[1, 1], x[2, 1] = 3.0, -1e-4
+        q, s = layers.quantize_8bit(x)
+        assert torch.equal(q.view(torch.uint8), (x.float() / s[:, None]).to(ob.E4M3).view(torch.uint8))
