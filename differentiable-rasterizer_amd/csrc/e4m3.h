@@ -54,7 +54,7 @@ __device__ inline void from_e4m3(uint32_t w, float (&out)[4]) {
 // Quotients by one divisor, as a division rounds them: a reciprocal corrected once, and each quotient by its own
 // remainder (Markstein, 1990). What is rounded to few bits afterwards goes by the last one now and then: a value
 // half way between two codes, or random bits that just reach the upper one. 32768 x 4096 bfloat16 numbers take
-// 62 us to their codes so, 76 with a division for each, 61 with a product (whose ties are wrong).
+// 63 us to their codes so, 76 with a division for each, 61 with a product (whose ties are wrong).
 struct Divisor {
     float d, r;
     __device__ explicit Divisor(float by) : d(by) {

@@ -186,7 +186,7 @@ struct GatedEpilogue {
 
 // ---------------------------------------------------------------- the products
 
-// 16384 x 1024 -> 4096 in bfloat16 takes 240 us without the pairs (1.15 PFLOP/s), 316 with them: 335 MB
+// 16384 x 1024 -> 4096 in bfloat16 takes 258 us without the pairs (1.06 PFLOP/s), 314 with them: 335 MB
 // more that are written at the rate of memory, beside products that run at the power limit. So neither
 // starting CUs one after the other nor starting the next tile's loads before a tile's end (312) nor two
 // workgroups of 128 a CU (379) covers them, and stores past the caches, half lines each, take 44 more.

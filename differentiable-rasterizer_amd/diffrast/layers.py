@@ -116,7 +116,7 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = 
 
 
 def rms_norm_8bit(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = None, eps: float = 1e-5):
-    """`rms_norm` with y in 8 bits, for `linear_8bit`: (q, scale), or with a residual (q, scale, s).
+    """`rms_norm` with y in 8 bits, for `linear_8bit` (where D is a multiple of 16): (q, scale), or with a residual (q, scale, s).
 
     q is float8_e4m3fn, y / scale rounded to nearest even, and scale `(...)` in float32 has
     max(max |y| / 448, 2^-126) for each row. No gradients: raises RuntimeError where they are wanted.
@@ -127,7 +127,10 @@ def rms_norm_8bit(x: Tensor, weight: Tensor | None = None, residual: Tensor | No
 
 
 def quantize_8bit(x: Tensor) -> tuple[Tensor, Tensor]:
-    """x `(..., D)` as (q, scale) of `rms_norm_8bit`, without the norm: activations, or a `(N, K)` weight."""
+    """x `(..., D)` as (q, scale) of `rms_norm_8bit`, without the norm: activations, or a `(N, K)` weight.
+
+    D may be any width; `linear_8bit` takes multiples of 16.
+    """
     r = _torch_layers.quantize_8bit(x)
     torch_layer._note_gpu()
     return r[0], r[1]
