@@ -128,7 +128,7 @@ class AdamW(torch.optim.Optimizer):
             for name in ("exp_avg", "exp_avg_sq"):
                 state[name] = torch.zeros(p.shape, dtype=kind, device=p.device)
                 if bits == 8:
-                    state[name + "_scale"] = torch.zeros(-(-p.numel() // BLOCK), device=p.device)
+                    state[name + "_scale"] = torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32, device=p.device)
         return state
 
     @torch.no_grad()

@@ -128,3 +128,23 @@ def test_a_groups_own_numbers_are_checked(bad):
     assert len(opt.param_groups) == 1
     opt.add_param_group(dict(params=[t()], state_bits=8, lr=torch.tensor(0.5)))
     assert len(opt.param_groups) == 2 and seeds(opt) == [0, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_under_another_default_type(bits, default):
+    from diffrast import optim
+
+    p = torch.nn.Parameter(torch.ones(300, device="cuda", dtype=torch.float32))
+    p.grad = torch.ones_like(p)
+    opt = optim.AdamW([p], state_bits=bits)
+    was = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        opt.step()
+    finally:
+        torch.set_default_dtype(was)
+    kinds = {k: v.dtype for k, v in opt.state[p].items()}
+    assert kinds.pop("step") == torch.int64 and bool((p < 1).all())
+    assert set(kinds.values()) == ({torch.float32} if bits == 32 else {torch.float32, torch.float8_e4m3fn})
