@@ -13,7 +13,8 @@
 // or m would be divided by eps alone. It is the root that keeps its mean: v gains the rounding's variance at
 // each step, so that with normal gradients and b2 = 0.999 it is 3 to 5% above that of 32 bits and deviates by a
 // third of itself (its root by a sixth). In a block of unlike elements a v whose root is below 2^-15 of the largest is
-// 15% high and more, and no root falls below 2^-18 of it: such elements take shorter steps. p is made from the m and v before they are rounded.
+// 15% high and more, and no root falls below 2^-18 of it: such elements take shorter steps. p is made from the m
+// and v before they are rounded.
 //
 // Bound by memory: an element in 32 bits is read as 16 bytes and written as 12, with 8-bit states
 // as 10 and 6. 203 M float32 parameters with 8-bit states (3.3 GB) take 553 us, 5.9 TB/s; 25 M bfloat16

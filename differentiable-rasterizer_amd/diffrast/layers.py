@@ -102,8 +102,8 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = 
     """s / sqrt(mean(s^2) + eps) * weight over the last dimension, with s = x + residual.
 
     Returns y, or with a residual (y, s): the norm and the stream that it was taken of, both
-    differentiable (of s the weight's gradient is zero, where s alone is used too). y is made from s in 32 bits; s is rounded to its type where it is stored, and
-    the backward pass starts from that. The mean of squares is held in float32, which ends at 3e38.
+    differentiable (of s the weight's gradient is zero, where s alone is used too). y is made
+    from s in 32 bits; s is rounded to its type where it is stored, and the backward pass starts from that. The mean of squares is held in float32, which ends at 3e38.
 
     Args:
         x: `(..., D)`.
@@ -116,7 +116,8 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = 
 
 
 def rms_norm_8bit(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = None, eps: float = 1e-5):
-    """`rms_norm` with y in 8 bits, for `linear_8bit` (where D is a multiple of 16): (q, scale), or with a residual (q, scale, s).
+    """`rms_norm` with y in 8 bits: (q, scale), or with a residual (q, scale, s); for `linear_8bit`
+    where D is a multiple of 16.
 
     q is float8_e4m3fn, y / scale rounded to nearest even, and scale `(...)` in float32 has
     max(max |y| / 448, 2^-126) for each row. No gradients: raises RuntimeError where they are wanted.
