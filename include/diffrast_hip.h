@@ -448,9 +448,9 @@ int drh_rms_norm_backward(drh_ctx *ctx, const void *sum, const void *weight, con
  * + residual, x rows x n_in and weight n_out x n_in in bytes of e4m3, with a scale for each
  * row of both (drh_rms_norm_8bit, drh_quantize_8bit). bias, residual and y are of
  * dtype. With a 16-bit dtype the sums over n_in are the 8-bit matrix instructions',
- * within 2^-10 of their terms' magnitudes (8e-6 of the result for normal numbers, more
- * than the dtype's rounding where large terms cancel); for DRH_F32 they are held in 32
- * bits. n_in, x_stride and weight_stride are multiples of 16, both operands 16-byte
+ * within 2^-10 of their terms' magnitudes (8e-6 of the result for normal numbers; beside
+ * outliers, or where large terms cancel, that may pass the dtype's rounding); for DRH_F32
+ * they are held in 32 bits. n_in, x_stride and weight_stride are multiples of 16, both operands 16-byte
  * aligned. */
 int drh_linear_8bit(drh_ctx *ctx, const void *x, const float *x_scale, const void *weight,
                     const float *weight_scale, const void *bias, const void *residual, int64_t rows,
